@@ -47,6 +47,7 @@ KERNEL_SOURCES = [
     "conv_f32_umma", "conv_f32_taps",
     "gemm_w8a16_umma",
     "dequant_w8",
+    "add_rms_norm",
     "selftest",
 ]
 
@@ -185,7 +186,8 @@ def build_libs(verbose=False, force=False):
     kernels = OUT / "libhc-b200-kernels.so"
     host_src = CSRC / "launch" / "host_api.cpp"
     spec_src = CSRC / "launch" / "specialise.cpp"
-    srcs = [CSRC / "launch" / "kernels_api.cpp", host_src, spec_src,
+    serving_src = CSRC / "launch" / "serving_api.cpp"
+    srcs = [CSRC / "launch" / "kernels_api.cpp", host_src, spec_src, serving_src,
             CSRC / "launch" / "context.hpp",
             *(CSRC / "kernels" / name for name in EMBEDDED_SOURCES),
             INCLUDE / "hc_b200_kernels.h",
@@ -205,7 +207,7 @@ def build_libs(verbose=False, force=False):
         _run([cuda / "bin" / "nvcc", *NVCC_FLAGS, "-Xcompiler", "-fPIC,-fvisibility=hidden",
               "-cudart", "static", *inc, "-c", "-o", static_obj, static_src], verbose)
         _run([cxx, *CXX_FLAGS, *inc, "-I", OUT, "-I", CSRC / "kernels", "-o", kernels, srcs[0],
-              host_src, spec_src, asm, static_obj,
+              host_src, spec_src, serving_src, asm, static_obj,
               "-L", OUT, "-lhc-gpu-runtime-loader", "-L", cuda / "lib64", "-lcudart_static",
               "-lrt", "-lpthread", "-ldl"], verbose)
 

@@ -19,7 +19,7 @@ NATIVE_DIR = Path(__file__).resolve().parent / "_native"
 OlErrorCallback = C.CFUNCTYPE(None, C.c_void_p, C.c_int, C.c_char_p)
 
 # hc_b200_kernels.h: enum HcDType
-HC_F32, HC_F64, HC_BF16, HC_I8, HC_I32, HC_I64 = 0, 1, 2, 3, 4, 5
+HC_F32, HC_F64, HC_BF16, HC_I8, HC_I32, HC_I64, HC_E4M3 = 0, 1, 2, 3, 4, 5, 6
 
 # offload_api.h: OLX_DEVICE_*
 OLX_DEVICE_SM_COUNT = 1
@@ -123,6 +123,7 @@ OL_PROTOTYPES = {
 }
 OLX_PROTOTYPES = {
     "olxQueueNativeHandle": (_vp, [_vp]),
+    "olxCreateQueueOnStream": (_vp, [_vp, _vp]),
     "olxMemcpyHtoD": (C.c_int, [_vp, _vp, _vp, _sz]),
     "olxMemcpyDtoH": (C.c_int, [_vp, _vp, _vp, _sz]),
     "olxMemsetD8": (C.c_int, [_vp, _vp, C.c_int, _sz]),
@@ -167,6 +168,8 @@ KERNELS_PROTOTYPES = {
     "hcContextQueue": (_vp, [_vp]),
     "hcContextStream": (_vp, [_vp]),
     "hcSynchronize": (C.c_int, [_vp]),
+    "hcUseStream": (C.c_int, [_vp, _vp]),
+    "hcUseOwnStream": (C.c_int, [_vp]),
     "hcLastError": (C.c_char_p, [_vp]),
     "hcLaunchCount": (_ll, [_vp]),
     "hcKernelStatus": (C.c_int, [_vp, C.POINTER(C.c_int)]),
@@ -232,6 +235,10 @@ KERNELS_PROTOTYPES = {
     "hcDequantW8": (C.c_int, [_vp, _vp, _vp, _ll, _ll, _ll, _ll]),
     "hcGemmW8A16StaticMaxBytes": (_sz, []),
     "hcGemmW8A16Static": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _ll, _ll]),
+    "hcAddRmsNorm": (
+        C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
+                  C.c_float, C.c_int, C.c_int]
+    ),
     "hcReportError": (C.c_int, [_vp, C.c_char_p]),
     "hcHostPin": (C.c_int, [_vp, _vp, _sz]),
     "hcHostUnpin": (C.c_int, [_vp, _vp]),
@@ -539,6 +546,23 @@ class Context:
         self._check(
             self.lib.hcGemmW8A16Static(self.handle, a, w, scale, out, m, n, k, lda, ldw, ldc),
             "hcGemmW8A16Static",
+        )
+
+    def use_stream(self, stream: int):
+        """Launches go to this CUstream (0: the legacy default stream) from here on."""
+        self._check(self.lib.hcUseStream(self.handle, stream), "hcUseStream")
+
+    def use_own_stream(self):
+        self._check(self.lib.hcUseOwnStream(self.handle), "hcUseOwnStream")
+
+    def add_rms_norm(self, x, residual, summed, gain, out, scale_out, rows, cols, x_pitch,
+                     residual_pitch, summed_pitch, out_pitch, scale_pitch, group, eps,
+                     dtype=HC_BF16, out_dtype=HC_BF16):
+        self._check(
+            self.lib.hcAddRmsNorm(self.handle, x, residual, summed, gain, out, scale_out, rows,
+                                  cols, x_pitch, residual_pitch, summed_pitch, out_pitch,
+                                  scale_pitch, group, eps, dtype, out_dtype),
+            "hcAddRmsNorm",
         )
 
     def host_pin(self, ptr, nbytes):

@@ -657,6 +657,88 @@ void gemmW8A16(Context &ctx, py::handle a, py::handle w, py::handle scale, py::h
             "gemm_w8a16");
 }
 
+// ---- serving operators ------------------------------------------------------------------
+// Launches go to `stream` (a raw CUstream, 0 = the legacy default stream) for the
+// length of the scope, then to the context's own stream again; None: the own one.
+class StreamScope {
+public:
+  StreamScope(Context &ctx, py::handle stream) {
+    if (stream.is_none())
+      return;
+    ctx.check(hcUseStream(ctx.get(), reinterpret_cast<void *>(stream.cast<uintptr_t>())),
+              "use_stream");
+    held = ctx.get();
+  }
+  ~StreamScope() {
+    if (held)
+      hcUseOwnStream(held);
+  }
+  StreamScope(const StreamScope &) = delete;
+  StreamScope &operator=(const StreamScope &) = delete;
+
+private:
+  HcContext held = nullptr;
+};
+
+int storedDType(const ArrayArg &a, const char *name) {
+  if (a.kind == ElemKind::I8)
+    return HC_I8;
+  if (a.kind == ElemKind::E4M3)
+    return HC_E4M3;
+  throw py::type_error(std::string(name) + ": int8 or float8_e4m3fn expected, got " +
+                       hc::kindName(a.kind));
+}
+
+void vectorOf(const ArrayArg &a, ElemKind kind, long long n, const char *name) {
+  if (a.kind != kind)
+    throw py::type_error(std::string(name) + ": " + hc::kindName(kind) + " expected, got " +
+                         hc::kindName(a.kind));
+  if (a.shape[0] != n || (n > 1 && a.strides[0] != 1))
+    throw py::value_error(std::string(name) + ": expected " + std::to_string(n) +
+                          " contiguous elements");
+}
+
+void addRmsNorm(Context &ctx, py::handle x, py::handle gain, py::handle residual,
+                py::handle summed, py::handle out, py::handle scale, long long group, float eps,
+                py::handle stream) {
+  ArrayArg X = deviceArray(ctx, x, "x", 2), G = deviceArray(ctx, gain, "gain", 1),
+           O = deviceArray(ctx, out, "out", 2);
+  if (X.kind != ElemKind::BF16 && X.kind != ElemKind::F32)
+    throw py::type_error(std::string("x: bfloat16 or float32 expected, got ") +
+                         hc::kindName(X.kind));
+  vectorOf(G, X.kind, X.shape[1], "gain");
+  sameShape(X, O, "x", "out");
+  ArrayArg R, S, C;
+  if (!residual.is_none()) {
+    R = deviceArray(ctx, residual, "residual", 2);
+    sameKind(X, R, "x", "residual");
+    sameShape(X, R, "x", "residual");
+  }
+  if (!summed.is_none()) {
+    S = deviceArray(ctx, summed, "summed", 2);
+    sameKind(X, S, "x", "summed");
+    sameShape(X, S, "x", "summed");
+  }
+  const int dtype = X.kind == ElemKind::BF16 ? HC_BF16 : HC_F32;
+  const int outDtype = O.kind == X.kind ? dtype : storedDType(O, "out");
+  if (outDtype != dtype) {
+    C = deviceArray(ctx, scale, "scale", 2);
+    const long long cols = X.shape[1];
+    const long long groups = group > 0 && group < cols ? (cols + group - 1) / group : 1;
+    if (C.kind != ElemKind::F32)
+      throw py::type_error("scale: float32 expected");
+    if (C.shape[0] != X.shape[0] || C.shape[1] != groups)
+      throw py::value_error("scale: expected one row per row of x and " +
+                            std::to_string(groups) + " columns");
+  }
+  StreamScope scope(ctx, stream);
+  ctx.check(hcAddRmsNorm(ctx.get(), X.data, R.data, S.data, G.data, O.data,
+                         static_cast<float *>(C.data), X.shape[0], X.shape[1], pitch(X),
+                         R.data ? pitch(R) : 0, S.data ? pitch(S) : 0, pitch(O),
+                         C.data ? pitch(C) : 0, group, eps, dtype, outDtype),
+            "add_rms_norm");
+}
+
 } // namespace
 
 PYBIND11_MODULE(_dispatcher, m) {
@@ -733,6 +815,9 @@ PYBIND11_MODULE(_dispatcher, m) {
   m.def("gemm_w8a16", &gemmW8A16, py::arg("ctx"), py::arg("a"), py::arg("w"),
         py::arg("scale"), py::arg("out"), py::arg("workspace") = py::none());
   m.def("w8a16_workspace_bytes", &w8a16WorkspaceBytes, py::arg("n"), py::arg("k"));
+  m.def("add_rms_norm", &addRmsNorm, py::arg("ctx"), py::arg("x"), py::arg("gain"),
+        py::arg("residual"), py::arg("summed"), py::arg("out"), py::arg("scale"),
+        py::arg("group") = 0, py::arg("eps") = 1e-5f, py::arg("stream") = py::none());
   m.def("image_names", [] {
     std::vector<std::string> names;
     for (int i = 0; i < hcImageCount(); ++i)

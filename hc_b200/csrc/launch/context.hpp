@@ -15,7 +15,9 @@ struct HcContextImpl {
   OlErrorCallback callback = nullptr;
   void *callbackCtx = nullptr;
   OlDevice device = nullptr;
-  OlQueue queue = nullptr;
+  OlQueue queue = nullptr;    // where launches go: ownQueue, or a borrowed one (hcUseStream)
+  OlQueue ownQueue = nullptr;
+  std::map<void *, OlQueue> borrowedQueues; // by the caller's stream handle
   std::vector<OlModule> modules; // one slot per image, loaded on first use
   std::map<std::string, OlKernel> kernels;
   int *statusWord = nullptr; // device
@@ -77,6 +79,9 @@ struct HcContextImpl {
 
 // Frees what the host-buffer entry points keep in a context (host_api.cpp).
 void hcReleaseHostPipeline(HcContextImpl *c);
+
+// Image of a serving kernel by its name, or null (serving_api.cpp).
+const char *hcServingImageOf(const char *kernel);
 
 // Run-time specialisation (specialise.cpp).
 struct HcMapProgramDev;

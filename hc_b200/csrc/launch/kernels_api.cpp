@@ -140,7 +140,7 @@ const char *imageOfKernel(const char *kernel) {
                                     : std::strcmp(e.kernel, kernel) == 0)
       return e.image;
   }
-  return nullptr;
+  return hcServingImageOf(kernel);
 }
 
 int findImage(const char *name) {
@@ -291,7 +291,7 @@ HcContext hcCreateContext(const char *deviceDesc, OlErrorCallback errCallback,
   c->device = olCreateDevice(deviceDesc, &HcContextImpl::onBackendMessage, c.get());
   if (!c->device)
     return nullptr;
-  c->queue = olCreateQueue(c->device);
+  c->queue = c->ownQueue = olCreateQueue(c->device);
   if (!c->queue) {
     olReleaseDevice(c->device);
     return nullptr;
@@ -313,8 +313,11 @@ HcContext hcCreateContext(const char *deviceDesc, OlErrorCallback errCallback,
 void hcReleaseContext(HcContext c) {
   if (!c)
     return;
+  c->queue = c->ownQueue;
   if (c->queue)
     olSyncQueue(c->queue);
+  for (auto &kv : c->borrowedQueues)
+    olReleaseQueue(kv.second);
   for (auto &kv : c->kernels)
     olReleaseKernel(kv.second);
   for (OlModule m : c->modules)
@@ -332,10 +335,32 @@ void hcReleaseContext(HcContext c) {
 }
 
 OlDevice hcContextDevice(HcContext c) { return c ? c->device : nullptr; }
-OlQueue hcContextQueue(HcContext c) { return c ? c->queue : nullptr; }
+OlQueue hcContextQueue(HcContext c) { return c ? c->ownQueue : nullptr; }
 void *hcContextStream(HcContext c) {
-  return c ? olxQueueNativeHandle(c->queue) : nullptr;
+  return c ? olxQueueNativeHandle(c->ownQueue) : nullptr;
 }
+
+int hcUseStream(HcContext c, void *stream) {
+  if (!c)
+    return 1;
+  OlQueue &q = c->borrowedQueues[stream];
+  if (!q)
+    q = olxCreateQueueOnStream(c->device, stream);
+  if (!q) {
+    c->borrowedQueues.erase(stream);
+    return c->fail("hcUseStream: no queue on that stream: %s", c->lastError.c_str());
+  }
+  c->queue = q;
+  return 0;
+}
+
+int hcUseOwnStream(HcContext c) {
+  if (!c)
+    return 1;
+  c->queue = c->ownQueue;
+  return 0;
+}
+
 int hcSynchronize(HcContext c) { return c ? olSyncQueue(c->queue) : 1; }
 const char *hcLastError(HcContext c) { return c ? c->lastError.c_str() : ""; }
 long long hcLaunchCount(HcContext c) { return c ? c->launches : 0; }

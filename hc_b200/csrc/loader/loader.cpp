@@ -86,6 +86,7 @@ struct Backend {
   decltype(&olLaunchKernel) LaunchKernel = nullptr;
   // Optional additions; null when the backend does not have them.
   decltype(&olxQueueNativeHandle) QueueNativeHandle = nullptr;
+  decltype(&olxCreateQueueOnStream) CreateQueueOnStream = nullptr;
   decltype(&olxMemcpyHtoD) MemcpyHtoD = nullptr;
   decltype(&olxMemcpyDtoH) MemcpyDtoH = nullptr;
   decltype(&olxMemsetD8) MemsetD8 = nullptr;
@@ -167,6 +168,7 @@ std::unique_ptr<Backend> openBackend(const std::string &path,
   }
 #define HC_BIND_OPT(fn) bindSymbol(lib, b->fn, "olx" #fn, nullptr)
   HC_BIND_OPT(QueueNativeHandle);
+  HC_BIND_OPT(CreateQueueOnStream);
   HC_BIND_OPT(MemcpyHtoD);
   HC_BIND_OPT(MemcpyDtoH);
   HC_BIND_OPT(MemsetD8);
@@ -395,6 +397,19 @@ static int missing(const DeviceHandle *dev, const char *what) {
   dev->report(OlSeverity::Error,
               std::string("Backend does not export ") + what);
   return 1;
+}
+
+OlQueue olxCreateQueueOnStream(OlDevice d, void *stream) noexcept {
+  Trace t(__func__);
+  auto *dev = static_cast<DeviceHandle *>(d);
+  if (!dev)
+    return nullptr;
+  if (!dev->api->CreateQueueOnStream) {
+    missing(dev, "olxCreateQueueOnStream");
+    return nullptr;
+  }
+  OlQueue inner = dev->api->CreateQueueOnStream(dev->inner, stream);
+  return inner ? new QueueHandle{dev, inner} : nullptr;
 }
 
 void *olxQueueNativeHandle(OlQueue q) noexcept {

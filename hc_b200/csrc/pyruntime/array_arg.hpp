@@ -17,13 +17,14 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 namespace hc {
 
 namespace py = pybind11;
 
-enum class ElemKind { F32, F64, BF16, F16, I8, U8, I16, I32, I64, Other };
+enum class ElemKind { F32, F64, BF16, F16, I8, U8, I16, I32, I64, E4M3, Other };
 
 struct ArrayArg {
   void *data = nullptr;
@@ -50,6 +51,7 @@ inline const char *kindName(ElemKind k) {
   case ElemKind::I16: return "int16";
   case ElemKind::I32: return "int32";
   case ElemKind::I64: return "int64";
+  case ElemKind::E4M3: return "float8_e4m3fn";
   default: return "other";
   }
 }
@@ -67,6 +69,7 @@ inline ElemKind kindFromTorchName(const std::string &name) {
   if (n == "int16" || n == "short") return ElemKind::I16;
   if (n == "int32" || n == "int") return ElemKind::I32;
   if (n == "int64" || n == "long") return ElemKind::I64;
+  if (n == "float8_e4m3fn") return ElemKind::E4M3;
   return ElemKind::Other;
 }
 
@@ -109,16 +112,46 @@ inline ArrayArg arrayFromInterface(const py::dict &iface, bool onDevice) {
   return a;
 }
 
+// The kind of a dtype object.  torch's dtypes are singletons that live as long as
+// torch does; naming one costs more than the rest of a tensor's reading, so each is
+// named once (the table holds a reference).
+inline ElemKind kindFromTorchDtype(const py::object &dtype) {
+  static std::vector<std::pair<PyObject *, ElemKind>> known;
+  for (const auto &k : known)
+    if (k.first == dtype.ptr())
+      return k.second;
+  const ElemKind kind = kindFromTorchName(py::str(dtype).cast<std::string>());
+  if (known.size() < 64) { // (an array type that makes dtype objects anew is not kept)
+    Py_INCREF(dtype.ptr());
+    known.emplace_back(dtype.ptr(), kind);
+  }
+  return kind;
+}
+
 inline ArrayArg arrayFromPython(py::handle obj) {
   if (py::hasattr(obj, "data_ptr") && py::hasattr(obj, "element_size")) {
     ArrayArg a;
     a.data = reinterpret_cast<void *>(obj.attr("data_ptr")().cast<uintptr_t>());
-    for (auto d : obj.attr("shape"))
-      a.shape.push_back(d.cast<int64_t>());
-    for (auto s : obj.attr("stride")())
-      a.strides.push_back(s.cast<int64_t>());
+    const py::object shape = obj.attr("shape"), strides = obj.attr("stride")();
+    if (PyTuple_Check(shape.ptr()) && PyTuple_Check(strides.ptr())) {
+      // torch.Size and the strides are tuples of ints: read them without iterators.
+      const Py_ssize_t rank = PyTuple_GET_SIZE(shape.ptr());
+      a.shape.reserve(size_t(rank));
+      a.strides.reserve(size_t(rank));
+      for (Py_ssize_t d = 0; d < rank; ++d)
+        a.shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), d)));
+      for (Py_ssize_t d = 0; d < PyTuple_GET_SIZE(strides.ptr()); ++d)
+        a.strides.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(strides.ptr(), d)));
+      if (PyErr_Occurred())
+        throw py::error_already_set();
+    } else {
+      for (auto d : shape)
+        a.shape.push_back(d.cast<int64_t>());
+      for (auto s : strides)
+        a.strides.push_back(s.cast<int64_t>());
+    }
     a.itemsize = obj.attr("element_size")().cast<int64_t>();
-    a.kind = kindFromTorchName(py::str(obj.attr("dtype")).cast<std::string>());
+    a.kind = kindFromTorchDtype(obj.attr("dtype"));
     a.onDevice = obj.attr("is_cuda").cast<bool>();
     if (a.onDevice) {
       py::object idx = obj.attr("device").attr("index");

@@ -101,6 +101,7 @@ struct KernelState {
 struct QueueState {
   DeviceState *device = nullptr;
   CUstream stream = nullptr;
+  bool borrowed = false; // the stream is the caller's: never destroyed here
 };
 
 // A blob is accepted when it is a complete ELF image (cubin), a fatbin
@@ -275,7 +276,7 @@ void olReleaseQueue(OlQueue queue) noexcept {
   auto *q = static_cast<QueueState *>(queue);
   if (!q)
     return;
-  if (q->stream) {
+  if (q->stream && !q->borrowed) {
     ContextScope scope(q->device);
     if (scope)
       q->device->check("cuStreamDestroy",
@@ -380,6 +381,17 @@ int olLaunchKernel(OlQueue queue, OlKernel kernel, const size_t *gridSizes,
 }
 
 // ---- additions -----------------------------------------------------------
+
+OlQueue olxCreateQueueOnStream(OlDevice d, void *stream) noexcept {
+  auto *dev = static_cast<DeviceState *>(d);
+  if (!dev)
+    return nullptr;
+  auto q = std::make_unique<QueueState>();
+  q->device = dev;
+  q->stream = static_cast<CUstream>(stream);
+  q->borrowed = true;
+  return q.release();
+}
 
 void *olxQueueNativeHandle(OlQueue queue) noexcept {
   auto *q = static_cast<QueueState *>(queue);

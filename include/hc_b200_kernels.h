@@ -35,7 +35,8 @@ enum HcDType {
   HC_BF16 = 2,
   HC_I8 = 3,
   HC_I32 = 4,
-  HC_I64 = 5
+  HC_I64 = 5,
+  HC_E4M3 = 6 /* 8-bit float, 4 exponent and 3 fraction bits, no infinities */
 };
 
 /* ---- kernel images -------------------------------------------------------
@@ -63,6 +64,15 @@ HC_B200_API OlQueue hcContextQueue(HcContext c);
 /* The CUstream behind the context's queue. */
 HC_B200_API void *hcContextStream(HcContext c);
 HC_B200_API int hcSynchronize(HcContext c);
+/* Sends what follows to a stream of the caller's (a CUstream of the device's
+ * primary context; null: its legacy default stream) instead of the context's
+ * own, and back.  Work launched this way is ordered with the caller's by the
+ * stream alone and can be captured into a CUDA graph (launch each kernel once
+ * before the capture: its image is loaded at the first launch).  The stream has
+ * to outlive its work; hcContextQueue and hcContextStream stay the context's
+ * own; hcSynchronize and hcKernelStatus wait for the stream in use. */
+HC_B200_API int hcUseStream(HcContext c, void *stream);
+HC_B200_API int hcUseOwnStream(HcContext c);
 HC_B200_API const char *hcLastError(HcContext c);
 /* Kernel launches issued through this context so far. */
 HC_B200_API long long hcLaunchCount(HcContext c);
@@ -482,6 +492,28 @@ HC_B200_API int hcGemmW8A16Static(HcContext c, const void *a, const void *w,
                                   const float *scale, void *out, long long M,
                                   long long N, long long K, long long lda,
                                   long long ldw, long long ldc);
+
+/* ---- serving operators ---------------------------------------------------------
+ * What a decoding step needs beside the GEMMs above, with weights of 4 bits and a
+ * key/value cache of 8: they have no counterpart in the reference.  Python reaches
+ * them through hc_b200/serving.py, on torch's current stream.
+ *
+ * Root-mean-square norm of rows, with the residual's addition:
+ *   s = x + residual          (s = x where residual is null)
+ *   y = s / sqrt(mean over the row of s^2 + eps) * gain
+ * x, residual, summed and gain are HC_BF16 or HC_F32 (`dtype`); gain has `cols`
+ * elements.  `summed` receives s, rounded to that type; it may be null, and it may be
+ * `residual` itself.  The norm uses s before that rounding.  outDtype == dtype: out
+ * receives y (it may be x itself).  outDtype HC_I8 or HC_E4M3: per row and `group`
+ * columns (0: the whole row; the last group may be shorter)
+ *   scale = max |y| / peak (127 or 448),  out = round(y / scale)
+ * with scaleOut float [rows, groups]; a group of zeros has scale 0.  A group that
+ * holds NaN or an infinity gets a scale that is not finite. */
+HC_B200_API int hcAddRmsNorm(HcContext c, const void *x, const void *residual, void *summed,
+                             const void *gain, void *out, float *scaleOut, long long rows,
+                             long long cols, long long xPitch, long long residualPitch,
+                             long long summedPitch, long long outPitch, long long scalePitch,
+                             long long group, float eps, int dtype, int outDtype);
 
 /* ---- host buffers ------------------------------------------------------------
  * The row-wise workloads and the bf16 GEMM on matrices that live in HOST

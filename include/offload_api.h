@@ -99,6 +99,12 @@ OFFLOAD_API_EXPORT int olLaunchKernel(OlQueue q, OlKernel k,
  * it or hand it to another library (e.g. wrap it as a torch ExternalStream). */
 OFFLOAD_API_EXPORT void *olxQueueNativeHandle(OlQueue q) HC_NOEXCEPT;
 
+/* A queue whose work goes to a stream that the caller owns (a CUstream of this
+ * device's primary context; null: its legacy default stream).  The stream has to
+ * outlive the work put on the queue; olReleaseQueue leaves it alone. */
+OFFLOAD_API_EXPORT OlQueue olxCreateQueueOnStream(OlDevice dev,
+                                                  void *stream) HC_NOEXCEPT;
+
 /* Asynchronous copies on the queue's stream.  The reference ABI has no copy
  * call because its callers always pass device-resident torch tensors. */
 OFFLOAD_API_EXPORT int olxMemcpyHtoD(OlQueue q, void *dst, const void *src,
