@@ -124,6 +124,9 @@ OL_PROTOTYPES = {
 OLX_PROTOTYPES = {
     "olxQueueNativeHandle": (_vp, [_vp]),
     "olxCreateQueueOnStream": (_vp, [_vp, _vp]),
+    "olxLaunchCluster": (
+        C.c_int, [_vp, _vp, C.POINTER(_sz), _sz, C.POINTER(_sz), C.POINTER(_vp), _sz]
+    ),
     "olxMemcpyHtoD": (C.c_int, [_vp, _vp, _vp, _sz]),
     "olxMemcpyDtoH": (C.c_int, [_vp, _vp, _vp, _sz]),
     "olxMemsetD8": (C.c_int, [_vp, _vp, C.c_int, _sz]),
@@ -238,6 +241,12 @@ KERNELS_PROTOTYPES = {
     "hcAddRmsNorm": (
         C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
                   C.c_float, C.c_int, C.c_int]
+    ),
+    "hcGemmW4FewRows": (_ll, []),
+    "hcGemmW4WorkspaceBytes": (_sz, [_ll, _ll, _ll, C.c_int]),
+    "hcGemmW4": (
+        C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
+                  _ll, _ll, _ll, _ll, C.c_int, C.c_int]
     ),
     "hcReportError": (C.c_int, [_vp, C.c_char_p]),
     "hcHostPin": (C.c_int, [_vp, _vp, _sz]),
@@ -563,6 +572,15 @@ class Context:
                                   cols, x_pitch, residual_pitch, summed_pitch, out_pitch,
                                   scale_pitch, group, eps, dtype, out_dtype),
             "hcAddRmsNorm",
+        )
+
+    def gemm_w4(self, a, a_scale, w, scale, zero, out, workspace, workspace_bytes, m, n, k, group,
+                a_group, lda, ldas, ldw, lds, ldz, ldc, a_dtype=HC_BF16, scale_dtype=HC_BF16):
+        self._check(
+            self.lib.hcGemmW4(self.handle, a, a_scale, w, scale, zero, out, workspace,
+                              workspace_bytes, m, n, k, group, a_group, lda, ldas, ldw, lds, ldz,
+                              ldc, a_dtype, scale_dtype),
+            "hcGemmW4",
         )
 
     def host_pin(self, ptr, nbytes):

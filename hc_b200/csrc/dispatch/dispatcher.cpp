@@ -739,6 +739,64 @@ void addRmsNorm(Context &ctx, py::handle x, py::handle gain, py::handle residual
             "add_rms_norm");
 }
 
+// `group`: columns of K per scale of the weights; a bf16, or int8 with `aScale`
+// [M, groups] (one column: per row) of `aGroup` columns each.
+void gemmW4(Context &ctx, py::handle a, py::handle w, py::handle scale, py::handle zero,
+            py::handle out, long long group, py::handle aScale, long long aGroup,
+            py::handle workspace, py::handle stream) {
+  ArrayArg A = deviceArray(ctx, a, "a", 2), W = deviceArray(ctx, w, "w", 2),
+           S = deviceArray(ctx, scale, "scale", 2), O = deviceArray(ctx, out, "out", 2);
+  if (O.kind != ElemKind::BF16)
+    throw py::type_error("gemm_w4: out must be bfloat16");
+  if (A.kind != ElemKind::BF16 && A.kind != ElemKind::I8)
+    throw py::type_error(std::string("gemm_w4: a must be bfloat16 or int8, got ") +
+                         hc::kindName(A.kind));
+  if (W.kind != ElemKind::U8)
+    throw py::type_error(std::string("gemm_w4: w must be uint8, got ") + hc::kindName(W.kind));
+  if (S.kind != ElemKind::BF16 && S.kind != ElemKind::F32)
+    throw py::type_error("gemm_w4: scale must be bfloat16 or float32");
+  const long long M = A.shape[0], K = A.shape[1], N = W.shape[0];
+  if (group <= 0 || group % 32)
+    throw py::value_error("gemm_w4: group must be a multiple of 32");
+  const long long groups = (K + group - 1) / group;
+  if (W.shape[1] != (K + 1) / 2 || O.shape[0] != M || O.shape[1] != N)
+    throw py::value_error("gemm_w4: shapes do not form [M,K] @ [N,K/2] -> [M,N]");
+  if (S.shape[0] != N || S.shape[1] != groups)
+    throw py::value_error("gemm_w4: scale must be [N, " + std::to_string(groups) + "]");
+  ArrayArg Z, AS, WS;
+  if (!zero.is_none()) {
+    Z = deviceArray(ctx, zero, "zero", 2);
+    if (Z.kind != ElemKind::U8)
+      throw py::type_error("gemm_w4: zero must be uint8");
+    sameShape(S, Z, "scale", "zero");
+  }
+  const bool narrow = A.kind == ElemKind::I8;
+  if (narrow) {
+    if (aScale.is_none())
+      throw py::value_error("gemm_w4: int8 activations need their scales");
+    AS = deviceArray(ctx, aScale, "a_scale", 2);
+    if (AS.kind != ElemKind::F32)
+      throw py::type_error("gemm_w4: a_scale must be float32");
+    const long long want = aGroup > 0 && aGroup < K ? (K + aGroup - 1) / aGroup : 1;
+    if (AS.shape[0] != M || AS.shape[1] != want)
+      throw py::value_error("gemm_w4: a_scale must be [M, " + std::to_string(want) + "]");
+  } else if (!aScale.is_none()) {
+    throw py::value_error("gemm_w4: a_scale belongs to int8 activations");
+  }
+  size_t wsBytes = 0;
+  if (!workspace.is_none()) {
+    WS = deviceArray(ctx, workspace, "workspace", 1);
+    wsBytes = size_t(WS.shape[0]) * size_t(WS.itemsize);
+  }
+  StreamScope scope(ctx, stream);
+  ctx.check(hcGemmW4(ctx.get(), A.data, static_cast<const float *>(AS.data), W.data, S.data,
+                     Z.data, O.data, WS.data, wsBytes, M, N, K, group, narrow ? aGroup : 0,
+                     pitch(A), AS.data ? pitch(AS) : 0, pitch(W), pitch(S),
+                     Z.data ? pitch(Z) : 0, pitch(O), narrow ? HC_I8 : HC_BF16,
+                     S.kind == ElemKind::F32 ? HC_F32 : HC_BF16),
+            "gemm_w4");
+}
+
 } // namespace
 
 PYBIND11_MODULE(_dispatcher, m) {
@@ -818,6 +876,15 @@ PYBIND11_MODULE(_dispatcher, m) {
   m.def("add_rms_norm", &addRmsNorm, py::arg("ctx"), py::arg("x"), py::arg("gain"),
         py::arg("residual"), py::arg("summed"), py::arg("out"), py::arg("scale"),
         py::arg("group") = 0, py::arg("eps") = 1e-5f, py::arg("stream") = py::none());
+  m.def("gemm_w4", &gemmW4, py::arg("ctx"), py::arg("a"), py::arg("w"), py::arg("scale"),
+        py::arg("zero"), py::arg("out"), py::arg("group"), py::arg("a_scale") = py::none(),
+        py::arg("a_group") = 0, py::arg("workspace") = py::none(), py::arg("stream") = py::none());
+  m.def("w4_few_rows", [] { return hcGemmW4FewRows(); });
+  m.def("w4_workspace_bytes",
+        [](long long rows, long long n, long long k, bool int8) {
+          return hcGemmW4WorkspaceBytes(rows, n, k, int8 ? HC_I8 : HC_BF16);
+        },
+        py::arg("m"), py::arg("n"), py::arg("k"), py::arg("int8") = false);
   m.def("image_names", [] {
     std::vector<std::string> names;
     for (int i = 0; i < hcImageCount(); ++i)

@@ -41,6 +41,7 @@ struct HcContextImpl {
   int pairSlotsF32 = 0; // the same for the float32 tensor-core kernel
   int pairSlotsBanded = 0; // the same for the dequant GEMM that converts band by band
   int pairSlotsW8 = 0;  // the same for the dequant GEMM that converts in its pipeline
+  long long w4Splits = 0;  // CTAs along K of the 4-bit products for few rows (0: chosen)
   long long w8Variant = 0; // 1: convert the weights in a pass of its own, 2: never
   // Programs without a precompiled body: 0 interpret them, 1 compile them at their
   // first launch and interpret where that is not possible, 2 fail where it is not.
@@ -73,6 +74,9 @@ struct HcContextImpl {
   // Launches `name` with a one-dimensional block on the context's queue.
   int launch(const char *name, size_t gx, size_t gy, size_t gz, size_t threads, void **args,
              size_t nArgs, size_t smem);
+  // The same in clusters of `cluster` CTAs along y (1..8; gy is a multiple of it).
+  int launchCluster(const char *name, size_t gx, size_t gy, size_t cluster, size_t threads,
+                    void **args, size_t smem);
   // Scratch of the host-buffer entry points (host_api.cpp), released with the context.
   struct HostPipeline *hostPipeline = nullptr;
 };

@@ -237,6 +237,19 @@ int HcContextImpl::launch(const char *name, size_t gx, size_t gy, size_t gz, siz
   return 0;
 }
 
+int HcContextImpl::launchCluster(const char *name, size_t gx, size_t gy, size_t cluster,
+                                 size_t threads, void **args, size_t smem) {
+  OlKernel k = kernel(name);
+  if (!k)
+    return 1;
+  const size_t grid[3] = {gx, gy, 1};
+  const size_t clusters[3] = {1, cluster, 1};
+  if (olxLaunchCluster(queue, k, grid, threads, clusters, args, smem))
+    return fail("olxLaunchCluster failed for %s: %s", name, lastError.c_str());
+  ++launches;
+  return 0;
+}
+
 namespace {
 
 // Directory this shared library was loaded from; the backend library lives
@@ -464,6 +477,11 @@ int hcSetOption(HcContext c, const char *name, long long value) {
     // the GEMM kernel band by band, by warps of their own (the first
     // hcGemmW8A16BandedBytes of the workspace; fails where the layout does not allow it).
     c->w8Variant = value;
+    return 0;
+  }
+  if (std::strcmp(name, "w4_splits") == 0 &&
+      (value == 0 || value == 1 || value == 2 || value == 4 || value == 8)) {
+    c->w4Splits = value; // hcGemmW4, few rows: CTAs that share a tile's K (0: chosen)
     return 0;
   }
   if (std::strcmp(name, "conv_stacked") == 0 && value >= 0 && value <= 1) {

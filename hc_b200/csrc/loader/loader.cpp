@@ -87,6 +87,7 @@ struct Backend {
   // Optional additions; null when the backend does not have them.
   decltype(&olxQueueNativeHandle) QueueNativeHandle = nullptr;
   decltype(&olxCreateQueueOnStream) CreateQueueOnStream = nullptr;
+  decltype(&olxLaunchCluster) LaunchCluster = nullptr;
   decltype(&olxMemcpyHtoD) MemcpyHtoD = nullptr;
   decltype(&olxMemcpyDtoH) MemcpyDtoH = nullptr;
   decltype(&olxMemsetD8) MemsetD8 = nullptr;
@@ -169,6 +170,7 @@ std::unique_ptr<Backend> openBackend(const std::string &path,
 #define HC_BIND_OPT(fn) bindSymbol(lib, b->fn, "olx" #fn, nullptr)
   HC_BIND_OPT(QueueNativeHandle);
   HC_BIND_OPT(CreateQueueOnStream);
+  HC_BIND_OPT(LaunchCluster);
   HC_BIND_OPT(MemcpyHtoD);
   HC_BIND_OPT(MemcpyDtoH);
   HC_BIND_OPT(MemsetD8);
@@ -397,6 +399,24 @@ static int missing(const DeviceHandle *dev, const char *what) {
   dev->report(OlSeverity::Error,
               std::string("Backend does not export ") + what);
   return 1;
+}
+
+int olxLaunchCluster(OlQueue q, OlKernel k, const size_t *gridSizes, size_t blockThreads,
+                     const size_t *clusterSizes, void **args, size_t sharedMemSize) noexcept {
+  Trace t(__func__);
+  auto *queue = static_cast<QueueHandle *>(q);
+  auto *kernel = static_cast<KernelHandle *>(k);
+  if (!queue)
+    return 1;
+  auto fn = queue->device->api->LaunchCluster;
+  if (!fn)
+    return missing(queue->device, "olxLaunchCluster");
+  if (!kernel) {
+    queue->device->report(OlSeverity::Error, "Invalid kernel handle");
+    return 1;
+  }
+  return fn(queue->inner, kernel->inner, gridSizes, blockThreads, clusterSizes, args,
+            sharedMemSize);
 }
 
 OlQueue olxCreateQueueOnStream(OlDevice d, void *stream) noexcept {

@@ -382,6 +382,47 @@ int olLaunchKernel(OlQueue queue, OlKernel kernel, const size_t *gridSizes,
 
 // ---- additions -----------------------------------------------------------
 
+int olxLaunchCluster(OlQueue queue, OlKernel kernel, const size_t *gridSizes, size_t blockThreads,
+                     const size_t *clusterSizes, void **args, size_t sharedMemSize) noexcept {
+  auto *q = static_cast<QueueState *>(queue);
+  auto *k = static_cast<KernelState *>(kernel);
+  if (!q)
+    return 1;
+  DeviceState *dev = q->device;
+  if (!k || !gridSizes || !clusterSizes) {
+    dev->report(OlSeverity::Error, "Invalid launch arguments");
+    return 1;
+  }
+  const DriverApi &cu = DriverApi::get();
+  ContextScope scope(dev);
+  if (!scope)
+    return 1;
+  if (sharedMemSize > size_t(k->dynSmemLimit)) {
+    if (dev->check("cuFuncSetAttribute",
+                   cu.FuncSetAttribute(k->function,
+                                       CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                                       static_cast<int>(sharedMemSize))))
+      return 1;
+    k->dynSmemLimit = static_cast<int>(sharedMemSize);
+  }
+  CUlaunchAttribute attr{};
+  attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+  attr.value.clusterDim.x = static_cast<unsigned>(clusterSizes[0]);
+  attr.value.clusterDim.y = static_cast<unsigned>(clusterSizes[1]);
+  attr.value.clusterDim.z = static_cast<unsigned>(clusterSizes[2]);
+  CUlaunchConfig config{};
+  config.gridDimX = static_cast<unsigned>(gridSizes[0]);
+  config.gridDimY = static_cast<unsigned>(gridSizes[1]);
+  config.gridDimZ = static_cast<unsigned>(gridSizes[2]);
+  config.blockDimX = static_cast<unsigned>(blockThreads);
+  config.blockDimY = config.blockDimZ = 1;
+  config.sharedMemBytes = static_cast<unsigned>(sharedMemSize);
+  config.hStream = q->stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return dev->check("cuLaunchKernelEx", cu.LaunchKernelEx(&config, k->function, args, nullptr));
+}
+
 OlQueue olxCreateQueueOnStream(OlDevice d, void *stream) noexcept {
   auto *dev = static_cast<DeviceState *>(d);
   if (!dev)

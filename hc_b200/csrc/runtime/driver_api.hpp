@@ -42,6 +42,7 @@ struct DriverApi {
   CUresult (*LaunchKernel)(CUfunction, unsigned, unsigned, unsigned, unsigned,
                            unsigned, unsigned, unsigned, CUstream, void **,
                            void **) = nullptr;
+  CUresult (*LaunchKernelEx)(const CUlaunchConfig *, CUfunction, void **, void **) = nullptr;
   CUresult (*TensorMapEncodeTiled)(
       CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
       const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -116,6 +117,7 @@ private:
          bind(MemcpyDtoHAsync, "cuMemcpyDtoHAsync_v2") &&
          bind(MemsetD8Async, "cuMemsetD8Async") &&
          bind(LaunchKernel, "cuLaunchKernel") &&
+         bind(LaunchKernelEx, "cuLaunchKernelEx") &&
          bind(TensorMapEncodeTiled, "cuTensorMapEncodeTiled") &&
          bind(OccupancyMaxActiveClusters, "cuOccupancyMaxActiveClusters") &&
          bind(PointerGetAttribute, "cuPointerGetAttribute") &&

@@ -64,3 +64,30 @@ def add_rms_norm(x, gain, residual=None, *, eps=1e-5, out_dtype=None, group=0, o
         summed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     native.add_rms_norm(ctx, x, gain, residual, summed, out, scale, group, eps, stream)
     return out, scale, summed
+
+
+def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None):
+    """``out[m, n] = sum_k a[m, k] (u[n, k] - z[n, k // group]) s[n, k // group]``.
+
+    ``w`` uint8 [N, ceil(K / 2)] holds u, two 4-bit numbers per byte along K
+    (even k in the low half); ``scale`` bfloat16 or float32 and ``zero`` uint8
+    (None: 8 throughout) are [N, ceil(K / group)], ``group`` a multiple of 32.
+    ``a`` is bfloat16 [M, K], or int8 with ``a_scale`` float32 as
+    :func:`add_rms_norm` returns them (``a_group``: its ``group``).  Returns
+    ``out`` bfloat16 [M, N].
+
+    Up to 64 rows stream the weights as they are.  More rows convert them to
+    bfloat16 first, into scratch memory taken from torch's allocator for the
+    length of the call, and run the bf16 GEMM.
+    """
+    native, ctx, stream = _launcher(a)
+    m, k = a.shape
+    n = w.shape[0]
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+    workspace = None
+    if m > 64:
+        need = native.w4_workspace_bytes(m, n, k, a.dtype == torch.int8)
+        workspace = torch.empty(need, dtype=torch.uint8, device=a.device)
+    native.gemm_w4(ctx, a, w, scale, zero, out, group, a_scale, a_group, workspace, stream)
+    return out

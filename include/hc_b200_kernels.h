@@ -125,7 +125,8 @@ HC_B200_API int hcSelfTestWaitTimeout(HcContext c, unsigned long long limitNs,
  * the workspace, 2 = inside the GEMM's pipeline (no workspace), 3 = inside the
  * GEMM kernel band by band into a ring of three bands (hcGemmW8A16BandedBytes of
  * workspace); 2 and 3 fail where the layout does not allow them, and all give
- * the same result bit for bit. */
+ * the same result bit for bit.  "w4_splits" (hcGemmW4 with few rows): 0 = the
+ * library's choice, 1, 2, 4 or 8 CTAs share the K of a tile. */
 HC_B200_API int hcSetOption(HcContext c, const char *name, long long value);
 
 /* Run-time specialisation.  The reference compiles every kernel body at its
@@ -514,6 +515,27 @@ HC_B200_API int hcAddRmsNorm(HcContext c, const void *x, const void *residual, v
                              long long cols, long long xPitch, long long residualPitch,
                              long long summedPitch, long long outPitch, long long scalePitch,
                              long long group, float eps, int dtype, int outDtype);
+
+/* Product with 4-bit weights:
+ *   out[m,n] = bf16( sum_k a[m,k] * as[m,k/aGroup] * (u[n,k] - z[n,k/group]) * s[n,k/group] )
+ * w holds u, numbers 0..15, two per byte along K, even k in the low half: [N, ceil(K/2)]
+ * bytes with row pitch ldw; scale s and zero z are [N, ceil(K/group)] with pitches
+ * lds and ldz in elements: HC_BF16 or HC_F32 scales, zero one byte each (0..15) or null
+ * (z = 8 throughout).  `group` is a multiple of 32.  a is HC_BF16 (aScale null, as = 1)
+ * or HC_I8 with float aScale [M, ceil(K/aGroup)], pitch ldas - what hcAddRmsNorm
+ * writes; aGroup is 0 (one scale per row) or a multiple of `group`.  out is bf16.
+ * Up to hcGemmW4FewRows() rows run on the kernel that streams the weights as they are
+ * and need no workspace; more rows convert the weights to bf16 first (each rounded
+ * once) and run hcGemmBf16: workspace of hcGemmW4WorkspaceBytes(M, N, K, aDtype)
+ * bytes, 16-byte aligned, written by every call. */
+HC_B200_API long long hcGemmW4FewRows(void);
+HC_B200_API size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, int aDtype);
+HC_B200_API int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w,
+                         const void *scale, const void *zero, void *out, void *workspace,
+                         size_t workspaceBytes, long long M, long long N, long long K,
+                         long long group, long long aGroup, long long lda, long long ldas,
+                         long long ldw, long long lds, long long ldz, long long ldc, int aDtype,
+                         int scaleDtype);
 
 /* ---- host buffers ------------------------------------------------------------
  * The row-wise workloads and the bf16 GEMM on matrices that live in HOST

@@ -99,6 +99,15 @@ OFFLOAD_API_EXPORT int olLaunchKernel(OlQueue q, OlKernel k,
  * it or hand it to another library (e.g. wrap it as a torch ExternalStream). */
 OFFLOAD_API_EXPORT void *olxQueueNativeHandle(OlQueue q) HC_NOEXCEPT;
 
+/* A launch whose CTAs form clusters of clusterSizes[3] (the grid's sizes are
+ * multiples of them; at most 8 CTAs).  Otherwise as olLaunchKernel, with one-
+ * dimensional blocks of blockThreads.  Returns 0 on success. */
+OFFLOAD_API_EXPORT int olxLaunchCluster(OlQueue q, OlKernel k,
+                                        const size_t *gridSizes,
+                                        size_t blockThreads,
+                                        const size_t *clusterSizes, void **args,
+                                        size_t sharedMemSize) HC_NOEXCEPT;
+
 /* A queue whose work goes to a stream that the caller owns (a CUstream of this
  * device's primary context; null: its legacy default stream).  The stream has to
  * outlive the work put on the queue; olReleaseQueue leaves it alone. */

@@ -91,3 +91,13 @@ int cuLaunchKernel(void *f, unsigned gx, unsigned gy, unsigned gz, unsigned bx, 
   l->block = bx * by * bz, l->smem = smem, l->stream = (unsigned long long)(uintptr_t)stream;
   return 0;
 }
+
+/* The head of CUlaunchConfig. */
+struct config {
+  unsigned grid[3], block[3], smem;
+  void *stream;
+};
+int cuLaunchKernelEx(const struct config *c, void *f, void **params, void **extra) {
+  return cuLaunchKernel(f, c->grid[0], c->grid[1], c->grid[2], c->block[0], c->block[1],
+                        c->block[2], c->smem, c->stream, params, extra);
+}

@@ -51,3 +51,14 @@ def stored_values(raw, store):
     if store == "int8":
         return raw.view(np.int8).astype(np.float64)
     return e4m3_values()[raw.view(np.uint8)]
+
+
+def unpack_w4(w, scale, zero, k, group):
+    """Weights [N, K] in float64 of the packed bytes w [N, ceil(K / 2)]."""
+    n = w.shape[0]
+    u = np.empty((n, 2 * w.shape[1]))
+    u[:, 0::2] = w & 15
+    u[:, 1::2] = w >> 4
+    u = u[:, :k]
+    z = np.full(scale.shape, 8.0) if zero is None else zero.astype(np.float64)
+    return (u - np.repeat(z, group, axis=1)[:, :k]) * np.repeat(scale, group, axis=1)[:, :k]
