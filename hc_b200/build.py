@@ -49,6 +49,8 @@ KERNEL_SOURCES = [
     "dequant_w8",
     "add_rms_norm",
     "gemm_w4",
+    "kv_append",
+    "kv_attention",
     "selftest",
 ]
 
@@ -194,7 +196,8 @@ def build_libs(verbose=False, force=False):
             INCLUDE / "hc_b200_kernels.h",
             INCLUDE / "offload_api.h", CSRC / "kernels" / "mapped_params.h",
             CSRC / "kernels" / "map_params.h", CSRC / "kernels" / "fused_programs.h",
-            CSRC / "kernels" / "items_params.h", CSRC / "kernels" / "conv_params.h", loader,
+            CSRC / "kernels" / "items_params.h", CSRC / "kernels" / "conv_params.h",
+            CSRC / "kernels" / "kv_params.h", loader,
             *cubins]
     static_src = CSRC / "launch" / "w8a16_static.cu"
     srcs.append(static_src)

@@ -102,6 +102,26 @@ class HcItemProgram(C.Structure):
     ]
 
 
+class HcKvCache(C.Structure):
+    """include/hc_b200_kernels.h: the paged 8-bit key/value cache."""
+
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("kScale", _vp), ("vScale", _vp),
+        ("pageStride", _ll), ("headStride", _ll), ("tokenStride", _ll), ("scalePitch", _ll),
+        ("pages", C.c_int), ("block", C.c_int), ("heads", C.c_int), ("dim", C.c_int),
+        ("dtype", C.c_int),
+    ]
+
+
+class HcKvPlace(C.Structure):
+    """include/hc_b200_kernels.h: which rows of a call belong where in the cache."""
+
+    _fields_ = [
+        ("table", _vp), ("lengths", _vp), ("starts", _vp), ("tablePitch", _ll),
+        ("seqs", C.c_int), ("width", C.c_int), ("tokens", C.c_int), ("maxNew", C.c_int),
+    ]
+
+
 # name -> (restype, argtypes), exactly as declared in include/offload_api.h
 OL_PROTOTYPES = {
     "olCreateDevice": (_vp, [C.c_char_p, OlErrorCallback, _vp]),
@@ -247,6 +267,14 @@ KERNELS_PROTOTYPES = {
     "hcGemmW4": (
         C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
                   _ll, _ll, _ll, _ll, C.c_int, C.c_int]
+    ),
+    "hcKvAppend": (
+        C.c_int, [_vp, C.POINTER(HcKvCache), C.POINTER(HcKvPlace), _vp, _vp, _ll, _ll, _ll, _ll]
+    ),
+    "hcKvAttentionWorkspaceBytes": (_sz, [_vp]),
+    "hcKvAttention": (
+        C.c_int, [_vp, C.POINTER(HcKvCache), C.POINTER(HcKvPlace), _vp, _vp, _vp, C.c_int,
+                  C.c_float, C.c_int, _ll, _ll, _ll, _ll, _ll, _vp, _sz]
     ),
     "hcReportError": (C.c_int, [_vp, C.c_char_p]),
     "hcHostPin": (C.c_int, [_vp, _vp, _sz]),
@@ -581,6 +609,28 @@ class Context:
                               workspace_bytes, m, n, k, group, a_group, lda, ldas, ldw, lds, ldz,
                               ldc, a_dtype, scale_dtype),
             "hcGemmW4",
+        )
+
+    def kv_append(self, cache, place, k, v, k_token_stride, k_head_stride, v_token_stride,
+                  v_head_stride):
+        """``cache``: :class:`HcKvCache`, ``place``: :class:`HcKvPlace`."""
+        self._check(
+            self.lib.hcKvAppend(self.handle, C.byref(cache), C.byref(place), k, v, k_token_stride,
+                                k_head_stride, v_token_stride, v_head_stride),
+            "hcKvAppend",
+        )
+
+    def kv_attention_workspace_bytes(self) -> int:
+        return self.lib.hcKvAttentionWorkspaceBytes(self.handle)
+
+    def kv_attention(self, cache, place, q, out, lse, share, scale, window, q_token_stride,
+                     q_head_stride, out_token_stride, out_head_stride, lse_stride, workspace,
+                     workspace_bytes):
+        self._check(
+            self.lib.hcKvAttention(self.handle, C.byref(cache), C.byref(place), q, out, lse, share,
+                                   scale, window, q_token_stride, q_head_stride, out_token_stride,
+                                   out_head_stride, lse_stride, workspace, workspace_bytes),
+            "hcKvAttention",
         )
 
     def host_pin(self, ptr, nbytes):

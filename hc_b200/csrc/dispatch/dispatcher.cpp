@@ -797,6 +797,127 @@ void gemmW4(Context &ctx, py::handle a, py::handle w, py::handle scale, py::hand
             "gemm_w4");
 }
 
+// The paged 8-bit cache: four arrays checked once and kept (with a reference to each).
+class KvCache {
+public:
+  KvCache(Context &ctx, py::object k, py::object v, py::object kScale, py::object vScale)
+      : arrays{k, v, kScale, vScale}, ordinal(ctx.ordinal) {
+    ArrayArg K = deviceArray(ctx, k, "k", 4), V = deviceArray(ctx, v, "v", 4),
+             KS = deviceArray(ctx, kScale, "k_scale", 2),
+             VS = deviceArray(ctx, vScale, "v_scale", 2);
+    cache.dtype = storedDType(K, "k");
+    sameKind(K, V, "k", "v");
+    sameShape(K, V, "k", "v");
+    sameShape(KS, VS, "k_scale", "v_scale");
+    if (K.strides != V.strides)
+      throw py::value_error("k and v differ in layout");
+    if (KS.kind != ElemKind::F32 || VS.kind != ElemKind::F32)
+      throw py::type_error("k_scale and v_scale must be float32");
+    if (KS.shape[0] != K.shape[0] || KS.shape[1] != K.shape[1] || pitch(KS) != pitch(VS))
+      throw py::value_error("k_scale and v_scale must be [pages, heads], in one layout");
+    for (long long n : K.shape)
+      if (n > 0x7fffffffLL)
+        throw py::value_error("k: an extent above 2^31");
+    cache.k = K.data, cache.v = V.data;
+    cache.kScale = static_cast<float *>(KS.data);
+    cache.vScale = static_cast<float *>(VS.data);
+    cache.pages = int(K.shape[0]), cache.heads = int(K.shape[1]);
+    cache.block = int(K.shape[2]), cache.dim = int(K.shape[3]);
+    // An axis of extent 1 may report any stride.
+    cache.tokenStride = cache.block > 1 ? K.strides[2] : cache.dim;
+    cache.headStride = cache.heads > 1 ? K.strides[1] : 0;
+    cache.pageStride = cache.pages > 1 ? K.strides[0] : 0;
+    cache.scalePitch = pitch(KS);
+  }
+  void on(const Context &ctx) const {
+    if (ctx.ordinal != ordinal)
+      throw py::value_error("the cache lives on another GPU than " + ctx.description);
+  }
+  HcKvCache cache{};
+
+private:
+  std::array<py::object, 4> arrays;
+  int ordinal;
+};
+
+HcKvPlace kvPlace(Context &ctx, py::handle table, py::handle lengths, py::handle starts,
+                  long long tokens, long long maxNew) {
+  ArrayArg T = deviceArray(ctx, table, "table", 2), L = deviceArray(ctx, lengths, "lengths", 1);
+  if (T.kind != ElemKind::I32)
+    throw py::type_error("table: int32 expected");
+  const long long seqs = T.shape[0];
+  vectorOf(L, ElemKind::I32, seqs, "lengths");
+  HcKvPlace p{};
+  if (!starts.is_none()) {
+    ArrayArg S = deviceArray(ctx, starts, "starts", 1);
+    vectorOf(S, ElemKind::I32, seqs + 1, "starts");
+    p.starts = static_cast<const int *>(S.data);
+    if (maxNew < 0)
+      throw py::value_error("max_new: the most new tokens of a sequence are needed with starts");
+  } else if (tokens < seqs) {
+    throw py::value_error("one row per sequence expected (or starts)");
+  }
+  if (seqs > 0x7fffffffLL || T.shape[1] > 0x7fffffffLL || tokens > 0x7fffffffLL ||
+      maxNew > 0x7fffffffLL)
+    throw py::value_error("an extent above 2^31");
+  p.table = static_cast<const int *>(T.data);
+  p.lengths = static_cast<const int *>(L.data);
+  p.tablePitch = pitch(T);
+  p.seqs = int(seqs), p.width = int(T.shape[1]), p.tokens = int(tokens);
+  p.maxNew = maxNew < 0 ? 1 : int(maxNew);
+  return p;
+}
+
+long long stride3(const ArrayArg &a, int d) { return a.shape[d] > 1 ? a.strides[d] : 0; }
+
+void rowsOfHeads(const ArrayArg &a, long long tokens, long long heads, long long dim,
+                 const char *name) {
+  if (a.kind != ElemKind::BF16)
+    throw py::type_error(std::string(name) + ": bfloat16 expected, got " + hc::kindName(a.kind));
+  if (a.shape[0] != tokens || a.shape[1] != heads || a.shape[2] != dim)
+    throw py::value_error(std::string(name) + ": expected [" + std::to_string(tokens) + ", " +
+                          std::to_string(heads) + ", " + std::to_string(dim) + "]");
+}
+
+void kvAppend(Context &ctx, KvCache &cache, py::handle k, py::handle v, py::handle table,
+              py::handle lengths, py::handle starts, long long maxNew, py::handle stream) {
+  cache.on(ctx);
+  ArrayArg K = deviceArray(ctx, k, "k", 3), V = deviceArray(ctx, v, "v", 3);
+  rowsOfHeads(K, K.shape[0], cache.cache.heads, cache.cache.dim, "k");
+  rowsOfHeads(V, K.shape[0], cache.cache.heads, cache.cache.dim, "v");
+  HcKvPlace place = kvPlace(ctx, table, lengths, starts, K.shape[0], maxNew);
+  StreamScope scope(ctx, stream);
+  ctx.check(hcKvAppend(ctx.get(), &cache.cache, &place, K.data, V.data, stride3(K, 0),
+                       stride3(K, 1), stride3(V, 0), stride3(V, 1)),
+            "kv_append");
+}
+
+void kvAttention(Context &ctx, KvCache &cache, py::handle q, py::handle out, py::handle lse,
+                 py::handle table, py::handle lengths, py::handle starts, long long maxNew,
+                 float scale, int window, py::handle workspace, py::handle stream) {
+  cache.on(ctx);
+  ArrayArg Q = deviceArray(ctx, q, "q", 3), O = deviceArray(ctx, out, "out", 3);
+  const long long heads = Q.shape[1];
+  if (heads < 1 || heads % cache.cache.heads)
+    throw py::value_error("q: " + std::to_string(heads) + " heads are not a multiple of the " +
+                          std::to_string(cache.cache.heads) + " of the cache");
+  rowsOfHeads(Q, Q.shape[0], heads, cache.cache.dim, "q");
+  rowsOfHeads(O, Q.shape[0], heads, cache.cache.dim, "out");
+  ArrayArg L, W = deviceArray(ctx, workspace, "workspace", 1);
+  if (!lse.is_none()) {
+    L = deviceArray(ctx, lse, "lse", 2);
+    if (L.kind != ElemKind::F32 || L.shape[0] != Q.shape[0] || L.shape[1] != heads)
+      throw py::value_error("lse: float32 [tokens, heads] expected");
+  }
+  HcKvPlace place = kvPlace(ctx, table, lengths, starts, Q.shape[0], maxNew);
+  StreamScope scope(ctx, stream);
+  ctx.check(hcKvAttention(ctx.get(), &cache.cache, &place, Q.data, O.data,
+                          static_cast<float *>(L.data), int(heads / cache.cache.heads), scale,
+                          window, stride3(Q, 0), stride3(Q, 1), stride3(O, 0), stride3(O, 1),
+                          L.data ? pitch(L) : 0, W.data, size_t(W.shape[0]) * size_t(W.itemsize)),
+            "kv_attention");
+}
+
 } // namespace
 
 PYBIND11_MODULE(_dispatcher, m) {
@@ -885,6 +1006,18 @@ PYBIND11_MODULE(_dispatcher, m) {
           return hcGemmW4WorkspaceBytes(rows, n, k, int8 ? HC_I8 : HC_BF16);
         },
         py::arg("m"), py::arg("n"), py::arg("k"), py::arg("int8") = false);
+  py::class_<KvCache>(m, "KvCache")
+      .def(py::init<Context &, py::object, py::object, py::object, py::object>(), py::arg("ctx"),
+           py::arg("k"), py::arg("v"), py::arg("k_scale"), py::arg("v_scale"));
+  m.def("kv_append", &kvAppend, py::arg("ctx"), py::arg("cache"), py::arg("k"), py::arg("v"),
+        py::arg("table"), py::arg("lengths"), py::arg("starts") = py::none(),
+        py::arg("max_new") = -1, py::arg("stream") = py::none());
+  m.def("kv_attention", &kvAttention, py::arg("ctx"), py::arg("cache"), py::arg("q"),
+        py::arg("out"), py::arg("lse"), py::arg("table"), py::arg("lengths"), py::arg("starts"),
+        py::arg("max_new"), py::arg("scale"), py::arg("window"), py::arg("workspace"),
+        py::arg("stream") = py::none());
+  m.def("kv_attention_workspace_bytes",
+        [](Context &c) { return hcKvAttentionWorkspaceBytes(c.get()); }, py::arg("ctx"));
   m.def("image_names", [] {
     std::vector<std::string> names;
     for (int i = 0; i < hcImageCount(); ++i)

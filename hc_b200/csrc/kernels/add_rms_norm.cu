@@ -88,10 +88,11 @@ __device__ __forceinline__ void storePacket(float *p, const float (&v)[8]) {
                                   __float_as_uint(v[6]), __float_as_uint(v[7])));
 }
 
-// 1 / scale, or 0 where that would not be a finite number: such values (below
-// 127 * 2^-126 or not finite) are stored as 0.
-__device__ __forceinline__ float inverse(float scale) {
-  return scale >= 1.17549435e-38f && scale < __int_as_float(0x7f800000) ? 1.0f / scale : 0.0f;
+// What y is multiplied with to be stored, peak / most (one rounding, where 1 / scale
+// would take two); 0 where that is not a finite number: the values of such groups
+// (below 2^-118, or not finite) are stored as 0 or NaN.
+template <class Out> __device__ __forceinline__ float inverse(float most) {
+  return most >= 3.0e-36f && most < __int_as_float(0x7f800000) ? Peak<Out>::value / most : 0.0f;
 }
 
 template <class T> struct Same {};
@@ -188,7 +189,7 @@ __device__ __forceinline__ void normRow(const NormParams &p) {
       const int c = i * Threads + tid;
       const float most = p.group ? segmentMax(top[i], lanes) : rowTop;
       const float scale = most / Peak<Out>::value;
-      const float inv = inverse(scale);
+      const float inv = inverse<Out>(most);
       if (c < packets) {
         uint2 q;
         q.x = quantise4<Out>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
@@ -249,8 +250,9 @@ __device__ __forceinline__ void normRowGeneric(const NormParams &p, int cached) 
     float top = 0.0f;
     for (long long c = tid; c < p.cols; c += blockDim.x)
       top = hc::maxNan(top, fabsf(value(c) * rms * float(gain[c])));
-    const float scale = blockReduce<true>(top, scratch[1]) / Peak<Out>::value;
-    const float inv = inverse(scale);
+    const float most = blockReduce<true>(top, scratch[1]);
+    const float scale = most / Peak<Out>::value;
+    const float inv = inverse<Out>(most);
     if (tid == 0)
       p.scale[row * p.scalePitch] = scale;
     for (long long c = tid; c < p.cols; c += blockDim.x)
@@ -263,8 +265,9 @@ __device__ __forceinline__ void normRowGeneric(const NormParams &p, int cached) 
       float top = 0.0f;
       for (long long c = g * p.group + lane; c < end; c += 32)
         top = hc::maxNan(top, fabsf(value(c) * rms * float(gain[c])));
-      const float scale = segmentMax(top, 32) / Peak<Out>::value;
-      const float inv = inverse(scale);
+      const float most = segmentMax(top, 32);
+      const float scale = most / Peak<Out>::value;
+      const float inv = inverse<Out>(most);
       if (lane == 0)
         p.scale[row * p.scalePitch + g] = scale;
       for (long long c = g * p.group + lane; c < end; c += 32)

@@ -2,7 +2,11 @@
 // arguments, the choice of a kernel variant, the launch.
 #include "context.hpp"
 
+#include "../kernels/kv_params.h"
+
 #include <algorithm>
+#include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -42,10 +46,89 @@ struct W4Params {
   int vecA;
 };
 
+struct AppendParams {
+  HcKvCacheDev cache;
+  HcKvPlaceDev place;
+  const void *k, *v;
+  long long tokenStride, headStride;
+  long long tokenStrideV, headStrideV;
+  int touched;
+  int vec;
+};
+
+struct AttentionParams {
+  HcKvCacheDev cache;
+  HcKvPlaceDev place;
+  const void *q;
+  void *out;
+  float *lse;
+  long long qTokenStride, qHeadStride, outTokenStride, outHeadStride, lseStride;
+  float scaleLog2;
+  int share;
+  int window;
+  int rowTiles;
+  unsigned *counters;
+  float *partial;
+};
+
+static_assert(sizeof(HcKvCache) == sizeof(HcKvCacheDev) &&
+                  offsetof(HcKvCache, dtype) == offsetof(HcKvCacheDev, dtype),
+              "HcKvCache and its device form differ");
+static_assert(sizeof(HcKvPlace) == sizeof(HcKvPlaceDev) &&
+                  offsetof(HcKvPlace, maxNew) == offsetof(HcKvPlaceDev, maxNew),
+              "HcKvPlace and its device form differ");
+
 long long roundUp(long long a, long long b) { return ceilDiv(a, b) * b; }
 
 // Rows that the weight-streaming kernel of hcGemmW4 takes.
 constexpr long long kW4FewRows = 64;
+
+// Query rows (x head dimension) of a partial result in the attention's workspace, and
+// the CTAs per SM that can hold two of them each.
+constexpr size_t kSlotFloats = 8 * 256 + 2 * 16;
+constexpr long long kAttentionCtasPerSm = 2;
+
+// Checks of the cache and of the rows' place that every entry point makes; copies them.
+int checkKv(HcContext c, const char *who, const HcKvCache *cache, const HcKvPlace *place,
+            HcKvCacheDev &outCache, HcKvPlaceDev &outPlace) {
+  if (!cache || !place)
+    return c->fail("%s: null cache or place", who);
+  if (cache->dtype != HC_I8 && cache->dtype != HC_E4M3)
+    return c->fail("%s: unsupported cache dtype %d", who, cache->dtype);
+  if (cache->block < 16 || cache->block > 256 || cache->block % 16)
+    return c->fail("%s: block of %d tokens (a multiple of 16 up to 256 expected)", who,
+                   cache->block);
+  if (cache->dim < 16 || cache->dim > 256 || cache->dim % 16)
+    return c->fail("%s: head dimension %d (a multiple of 16 up to 256 expected)", who, cache->dim);
+  if (cache->pages < 0 || cache->heads < 1 || cache->heads > 65535)
+    return c->fail("%s: %d pages of %d heads", who, cache->pages, cache->heads);
+  if (cache->tokenStride < cache->dim || cache->headStride < 0 || cache->pageStride < 0 ||
+      cache->tokenStride % 16 || cache->headStride % 16 || cache->pageStride % 16 ||
+      !aligned(cache->k, 16) || !aligned(cache->v, 16))
+    return c->fail("%s: the cache's rows must be 16-byte aligned", who);
+  if (cache->scalePitch < cache->heads)
+    return c->fail("%s: scale pitch %lld is below the %d heads", who, cache->scalePitch,
+                   cache->heads);
+  if (place->seqs < 0 || place->width < 0 || place->tokens < 0 || place->maxNew < 0 ||
+      place->tablePitch < place->width ||
+      (long long)place->width * cache->block > 0x7fffffffLL - 512)
+    return c->fail("%s: invalid place (%d sequences, %d blocks, %d tokens, at most %d new)", who,
+                   place->seqs, place->width, place->tokens, place->maxNew);
+  if (!place->starts && place->tokens < place->seqs)
+    return c->fail("%s: %d rows for %d sequences of one new token", who, place->tokens,
+                   place->seqs);
+  if (place->seqs > 0 && place->tokens > 0 &&
+      (!place->lengths || (place->width > 0 && !place->table)))
+    return c->fail("%s: null lengths or table", who);
+  if (cache->pages > 0 && (!cache->k || !cache->v || !cache->kScale || !cache->vScale))
+    return c->fail("%s: null cache buffer", who);
+  std::memcpy(&outCache, cache, sizeof outCache);
+  std::memcpy(&outPlace, place, sizeof outPlace);
+  if (!place->starts)
+    outPlace.maxNew = std::min(outPlace.maxNew, 1);
+  outPlace.maxNew = std::min(outPlace.maxNew, outPlace.tokens);
+  return 0;
+}
 
 // Which image defines which family of kernels (names start with `prefix`).
 const struct {
@@ -59,6 +142,8 @@ const struct {
     {"hc_gemm_w4_", "gemm_w4"},
     {"hc_dequant_w4_", "gemm_w4"},
     {"hc_dequant_a8_", "gemm_w4"},
+    {"hc_kv_append_", "kv_append"},       // _{i8,e4m3}
+    {"hc_kv_attention_", "kv_attention"}, // _{i8,e4m3}_d{64,128,256}_r{1,2}
 };
 
 } // namespace
@@ -255,6 +340,97 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
     return hcGemmBf16(c, rows, weights, out, M, N, K, outPitch, pitch, ldc);
   }
   return hcGemmBf16(c, a, weights, out, M, N, K, lda, pitch, ldc);
+}
+
+int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place, const void *k,
+               const void *v, long long kTokenStride, long long kHeadStride,
+               long long vTokenStride, long long vHeadStride) {
+  if (!c)
+    return 1;
+  AppendParams p{};
+  if (checkKv(c, "hcKvAppend", cache, place, p.cache, p.place))
+    return 1;
+  if (kTokenStride < 0 || kHeadStride < 0 || vTokenStride < 0 || vHeadStride < 0)
+    return c->fail("hcKvAppend: negative strides");
+  if (p.place.seqs == 0 || p.place.tokens == 0 || p.place.maxNew == 0 || p.place.width == 0 ||
+      p.cache.pages == 0)
+    return 0;
+  if (!k || !v)
+    return c->fail("hcKvAppend: null buffer");
+  p.k = k, p.v = v;
+  p.tokenStride = kTokenStride, p.headStride = kHeadStride;
+  p.tokenStrideV = vTokenStride, p.headStrideV = vHeadStride;
+  p.touched = hcKvTouchedBlocks(p.place.maxNew, p.cache.block);
+  p.vec = kTokenStride % 8 == 0 && kHeadStride % 8 == 0 && vTokenStride % 8 == 0 &&
+          vHeadStride % 8 == 0 && aligned(k, 16) && aligned(v, 16);
+  const long long blocks = (long long)p.place.seqs * p.touched;
+  if (blocks > 0x7fffffffLL)
+    return c->fail("hcKvAppend: %d sequences of up to %d new tokens are too many", p.place.seqs,
+                   p.place.maxNew);
+  void *args[] = {&p};
+  return c->launch(p.cache.dtype == HC_I8 ? "hc_kv_append_i8" : "hc_kv_append_e4m3",
+                   size_t(blocks), size_t(p.cache.heads), 2, 128, args, 1, 0);
+}
+
+size_t hcKvAttentionWorkspaceBytes(HcContext c) {
+  if (!c)
+    return 0;
+  const size_t ctas = size_t(c->smCount * kAttentionCtasPerSm);
+  return size_t(roundUp((long long)ctas * 4, 256)) + ctas * 2 * kSlotFloats * 4;
+}
+
+int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, const void *q,
+                  void *out, float *lse, int share, float scale, int window,
+                  long long qTokenStride, long long qHeadStride, long long outTokenStride,
+                  long long outHeadStride, long long lseStride, void *workspace,
+                  size_t workspaceBytes) {
+  if (!c)
+    return 1;
+  AttentionParams p{};
+  if (checkKv(c, "hcKvAttention", cache, place, p.cache, p.place))
+    return 1;
+  if (share < 1 || share > 65535 || window < 0 || !std::isfinite(scale))
+    return c->fail("hcKvAttention: %d query heads per key/value head, window %d, scale %g", share,
+                   window, double(scale));
+  if (qTokenStride < 0 || qHeadStride < 0 || outTokenStride < 0 || outHeadStride < 0 ||
+      (lse && lseStride < (long long)p.cache.heads * share))
+    return c->fail("hcKvAttention: invalid strides");
+  if (p.place.seqs == 0 || p.place.tokens == 0)
+    return 0;
+  if (!q || !out)
+    return c->fail("hcKvAttention: null buffer");
+  if (!aligned(out, 8) || outTokenStride % 4 || outHeadStride % 4)
+    return c->fail("hcKvAttention: the rows of out must be 8-byte aligned");
+  if (!workspace || workspaceBytes < hcKvAttentionWorkspaceBytes(c) || !aligned(workspace, 256))
+    return c->fail("hcKvAttention: a 256-byte aligned workspace of %zu bytes is needed, got %zu",
+                   hcKvAttentionWorkspaceBytes(c), workspaceBytes);
+  p.q = q, p.out = out, p.lse = lse;
+  p.qTokenStride = qTokenStride, p.qHeadStride = qHeadStride;
+  p.outTokenStride = outTokenStride, p.outHeadStride = outHeadStride;
+  p.lseStride = lseStride;
+  p.scaleLog2 = scale * 1.44269504088896341f;
+  p.share = share, p.window = window;
+  const long long maxRows = (long long)std::max(p.place.maxNew, 1) * share;
+  const int cap = p.cache.dim <= 64 ? 64 : p.cache.dim <= 128 ? 128 : 256;
+  // Eight query rows per MMA; sixteen share one reading of the cache where there are as
+  // many and the registers allow it.
+  const int nt = maxRows > 8 && cap <= 128 ? 2 : 1;
+  const long long rowTiles = ceilDiv(maxRows, 8 * nt);
+  if (rowTiles * p.cache.heads > 0x7fffffffLL)
+    return c->fail("hcKvAttention: too many query rows per sequence (%lld)", maxRows);
+  p.rowTiles = int(rowTiles);
+  const int perSm = cap == 64 || (cap == 128 && nt == 1) ? 2 : 1;
+  const long long tiles = (long long)p.place.seqs * p.cache.heads * rowTiles *
+                          (ceilDiv((long long)p.place.width * p.cache.block, 128) + 1);
+  const long long ctas = std::max<long long>(1, std::min(tiles, c->smCount * perSm));
+  p.counters = static_cast<unsigned *>(workspace);
+  p.partial = reinterpret_cast<float *>(
+      static_cast<char *>(workspace) + roundUp(c->smCount * kAttentionCtasPerSm * 4, 256));
+  char name[64];
+  std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d",
+                p.cache.dtype == HC_I8 ? "i8" : "e4m3", cap, nt);
+  void *args[] = {&p};
+  return c->launch(name, size_t(ctas), 1, 1, 256, args, 1, size_t(8) * 8 * nt * cap * 4);
 }
 
 } // extern "C"

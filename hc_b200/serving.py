@@ -91,3 +91,87 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
         workspace = torch.empty(need, dtype=torch.uint8, device=a.device)
     native.gemm_w4(ctx, a, w, scale, zero, out, group, a_scale, a_group, workspace, stream)
     return out
+
+
+class KvCache:
+    """A paged 8-bit key/value cache with one scale per block of tokens and head.
+
+    ``k`` and ``v`` [pages, heads, block, dim], int8 or float8_e4m3fn, in any
+    layout with contiguous 16-byte aligned rows; ``k_scale`` and ``v_scale``
+    float32 [pages, heads].  ``block`` is a multiple of 16 up to 256, ``dim``
+    a multiple of 16 up to 256.  Which page holds which block of which
+    sequence is the caller's table, given with every call.
+    """
+
+    def __init__(self, k, v, k_scale, v_scale):
+        native, ctx, _ = _launcher(k)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._native = native.KvCache(ctx, k, v, k_scale, v_scale)
+        self._root = k.shape[3] ** -0.5
+
+    @classmethod
+    def empty(cls, pages, heads, block, dim, dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache with nothing in it (blocks are written before they are read)."""
+        k, v = (torch.zeros((pages, heads, block, dim), dtype=torch.int8,
+                            device=device).view(dtype) for _ in range(2))
+        scales = (torch.zeros((pages, heads), dtype=torch.float32, device=device)
+                  for _ in range(2))
+        return cls(k, v, *scales)
+
+
+def kv_append(cache, k, v, table, lengths, starts=None, *, max_new=None):
+    """Writes new keys and values into the cache.
+
+    ``k``, ``v`` bfloat16 [tokens, heads, dim]; ``table`` int32 [seqs, width]
+    the page of each block of each sequence; ``lengths`` int32 [seqs] the
+    tokens of each sequence, the new ones included; ``starts`` int32
+    [seqs + 1] where each sequence's rows begin (None: one row per sequence),
+    with ``max_new`` at least the most new tokens of a sequence.  A block's
+    scale grows to what its new tokens need (earlier tokens are rounded
+    again); pages that several sequences share must not be written.
+    """
+    native, ctx, stream = _launcher(k)
+    native.kv_append(ctx, cache._native, k, v, table, lengths, starts,
+                     -1 if max_new is None else max_new, stream)
+
+
+_scratch = {}
+
+
+def _attention_workspace(native, ctx, device, stream):
+    """Zeroed scratch of the attention: one per stream, and one of its own for every
+    call that is being captured, so that graphs may run beside each other."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(native.kv_attention_workspace_bytes(ctx), dtype=torch.uint8,
+                           device=device)
+    key = (device.index, stream)
+    buf = _scratch.get(key)
+    if buf is None:
+        buf = _scratch[key] = torch.zeros(native.kv_attention_workspace_bytes(ctx),
+                                          dtype=torch.uint8, device=device)
+    return buf
+
+
+def kv_attention(cache, q, table, lengths, starts=None, *, max_new=None, scale=None, window=0,
+                 out=None, return_lse=False):
+    """Attention of the new tokens over the cache they were appended to.
+
+    ``q`` bfloat16 [tokens, heads, dim] with a multiple of the cache's heads;
+    ``table``, ``lengths``, ``starts``, ``max_new`` as for :func:`kv_append`.
+    A token sees its own position and those before it, with ``window`` > 0 at
+    most that many; ``scale`` defaults to ``dim ** -0.5``.  Returns ``out`` in
+    ``q``'s shape, and with ``return_lse`` also the natural logarithm of each
+    row's sum of exponentials, float32 [tokens, heads].  A row that sees
+    nothing gives zeros and -inf; rows of no sequence are not written.
+    """
+    native, ctx, stream = _launcher(q)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = None
+    if return_lse:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    native.kv_attention(ctx, cache._native, q, out, lse, table, lengths, starts,
+                        -1 if max_new is None else max_new,
+                        cache._root if scale is None else scale, window,
+                        _attention_workspace(native, ctx, q.device, stream), stream)
+    return (out, lse) if return_lse else out

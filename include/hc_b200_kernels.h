@@ -537,6 +537,64 @@ HC_B200_API int hcGemmW4(HcContext c, const void *a, const float *aScale, const 
                          long long ldw, long long lds, long long ldz, long long ldc, int aDtype,
                          int scaleDtype);
 
+/* Paged key/value cache of 8-bit elements with one scale per block of tokens and head.
+ * A page holds `block` consecutive tokens of one sequence for all key/value heads:
+ * element [page, head, token, d] of k (and of v) lies at page * pageStride + head *
+ * headStride + token * tokenStride + d, and stands for that number times
+ * kScale[page * scalePitch + head].  dtype HC_I8 or HC_E4M3; block a multiple of 16 up
+ * to 256; dim a multiple of 16 up to 256; strides multiples of 16, 16-byte aligned. */
+typedef struct HcKvCache {
+  void *k, *v;
+  float *kScale, *vScale;
+  long long pageStride, headStride, tokenStride;
+  long long scalePitch;
+  int pages, block, heads, dim, dtype;
+} HcKvCache;
+
+/* Which rows of a call's arrays belong where: all of it is device memory and read by
+ * the kernels alone.  Sequence s holds lengths[s] tokens, the new ones of the call
+ * included, in the pages table[s * tablePitch + 0 .. width); its new tokens are rows
+ * starts[s] .. starts[s+1] of the call's arrays (starts null: row s), the newest
+ * positions of the sequence.  maxNew is at least the most new tokens of a sequence; it
+ * sizes the launch.  A page index that names no page of the cache stands for a block
+ * that is not there: nothing is written to it and its tokens are not visible.  Rows
+ * without a position (a length below the number of new tokens, blocks behind `width`,
+ * tokens behind maxNew) are not stored and see nothing. */
+typedef struct HcKvPlace {
+  const int *table, *lengths, *starts;
+  long long tablePitch;
+  int seqs, width, tokens, maxNew;
+} HcKvPlace;
+
+/* Writes new keys and values, bf16 [tokens, heads, dim] (dim contiguous), into the
+ * cache.  Per block and head: need = max |x| over the block's new tokens * fl(1 / peak)
+ * (peak 127 or 448, fl: as float), for e4m3 rounded up to a power of two; the block's scale becomes the larger of
+ * need and, where the block held earlier tokens of the sequence, its scale before; new
+ * elements are round(x / scale), earlier ones are rounded again where the scale grew.
+ * Infinities saturate, NaN is stored as NaN (e4m3) or 0 (int8).  Blocks that several
+ * sequences share must not be written: sequences' new tokens lie in pages of their own. */
+HC_B200_API int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place,
+                           const void *k, const void *v, long long kTokenStride,
+                           long long kHeadStride, long long vTokenStride,
+                           long long vHeadStride);
+
+/* Attention of the new tokens over the cache (after hcKvAppend): for query row i of a
+ * sequence at position pos and head h, with key/value head h / share,
+ *   out = sum_j p_j v_j,   p = softmax over visible j of  scale * q . k_j
+ * j is visible when j <= pos and, with window > 0, pos - j < window.  A row that sees
+ * nothing gives zeros and lse -inf.  q and out are bf16 [tokens, heads * share, dim]
+ * (dim contiguous), lse float [tokens, heads * share] or null: the natural logarithm
+ * of the sum of exp(scale * q . k_j).  Rows of no sequence stay as they were.
+ * workspace: hcKvAttentionWorkspaceBytes(c) bytes of device memory, 256-byte aligned,
+ * zeroed before its first use; every call leaves it ready for the next one.  Calls that
+ * may run at the same time (other streams, captured graphs) need one each. */
+HC_B200_API size_t hcKvAttentionWorkspaceBytes(HcContext c);
+HC_B200_API int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place,
+                              const void *q, void *out, float *lse, int share, float scale,
+                              int window, long long qTokenStride, long long qHeadStride,
+                              long long outTokenStride, long long outHeadStride,
+                              long long lseStride, void *workspace, size_t workspaceBytes);
+
 /* ---- host buffers ------------------------------------------------------------
  * The row-wise workloads and the bf16 GEMM on matrices that live in HOST
  * memory: every pointer below is a host pointer.  The matrix is cut into row

@@ -1,0 +1,380 @@
+"""Host side of the serving operators, without a GPU.
+
+* hc_b200/csrc/kernels/kv_params.h compiled for the host: whatever lengths,
+  starts and tables hold, positions and rows lie inside the buffers, and the
+  equal shares of the attention cover every tile once;
+* the C-ABI on a driver stand-in that records launches
+  (oracle/recording_cuda.c): refusals, kernel choice, grids, streams;
+* the oracle's 8-bit float against torch's.
+"""
+
+import ctypes as C
+import os
+import random
+import subprocess
+import sys
+import textwrap
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import serving as oracle
+
+REPO = Path(__file__).resolve().parent.parent
+
+
+def test_e4m3_rounding_is_torchs():
+    x = np.concatenate([np.random.default_rng(0).normal(size=4096) * 10.0 ** e
+                        for e in range(-4, 3)])
+    x = np.clip(x, -448, 448)
+    want = torch.from_numpy(x).float().to(torch.float8_e4m3fn)
+    assert np.array_equal(oracle.to_e4m3(x.astype(np.float32)), want.view(torch.uint8).numpy())
+    assert np.array_equal(oracle.e4m3_values()[oracle.to_e4m3(x.astype(np.float32))],
+                          want.double().numpy())
+
+
+def test_oracle_unpacks_the_low_half_first():
+    w = np.array([[0x21, 0x43]], np.uint8)
+    assert oracle.unpack_w4(w, np.ones((1, 1)), np.zeros((1, 1)), 3, 32).tolist() == [[1, 2, 3]]
+
+
+@pytest.fixture(scope="module")
+def params(tmp_path_factory):
+    out = tmp_path_factory.mktemp("kv") / "kv.so"
+    src = out.with_suffix(".cpp")
+    src.write_text(textwrap.dedent("""
+        #include "kv_params.h"
+        extern "C" void span(int seqs, int width, int tokens, int maxNew, int block, int length,
+                             int begin, int end, int *r) {
+          HcKvPlaceDev p{};
+          p.seqs = seqs, p.width = width, p.tokens = tokens, p.maxNew = maxNew;
+          HcKvSpan s = hcKvSpanOf(p, block, length, begin, end);
+          r[0] = s.row, r[1] = s.count, r[2] = s.first, r[3] = s.allRow, r[4] = s.allCount;
+        }
+        extern "C" int page(int e, int pages) { return hcKvPageOf(e, pages); }
+        extern "C" int touched(int n, int block) { return hcKvTouchedBlocks(n, block); }
+        extern "C" long long begin(long long c, long long t, long long n) {
+          return hcKvShareBegin(c, t, n); }
+        extern "C" int share(long long x, long long t, long long n) {
+          return hcKvShareOf(x, t, n); }
+        """))
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-static-libubsan", "-I",
+                    str(REPO / "hc_b200" / "csrc" / "kernels"), "-o", str(out), str(src)],
+                   check=True)
+    lib = C.CDLL(str(out))
+    lib.begin.restype = C.c_longlong
+    lib.begin.argtypes = lib.share.argtypes = [C.c_longlong] * 3
+    return lib
+
+
+def _span(lib, *args):
+    r = (C.c_int * 5)()
+    lib.span(*args, r)
+    return list(r)
+
+
+def test_spans_stay_inside_whatever_the_arrays_hold(params):
+    rng = random.Random(0)
+    wild = [-2 ** 31, -7, -1, 0, 1, 2, 15, 16, 17, 100, 2 ** 30, 2 ** 31 - 1]
+    for _ in range(20000):
+        block = rng.choice([16, 32, 256])
+        width, tokens = rng.choice([0, 1, 3, 1000]), rng.choice([0, 1, 5, 40, 2 ** 31 - 1])
+        max_new = rng.choice([0, 1, 4, 40])
+        length, begin, end = (rng.choice(wild) for _ in range(3))
+        row, count, first, all_row, all_count = _span(params, 4, width, tokens, max_new, block,
+                                                      length, begin, end)
+        assert 0 <= all_row and 0 <= all_count and all_row + all_count <= tokens
+        assert 0 <= count <= max(max_new, 0) and all_row <= row
+        assert row + count <= all_row + all_count
+        assert 0 <= first and first + count <= width * block
+        if count and length >= 0:  # the position belongs to the row
+            assert first - row == length - (all_row + all_count)
+
+
+def test_spans_are_the_oracles(params):
+    rng = random.Random(1)
+    for _ in range(3000):
+        block, width, max_new = 16, rng.randint(1, 4), rng.randint(1, 20)
+        n = rng.randint(0, 25)
+        length = rng.randint(0, 90)
+        want = oracle.place([length], [3, 3 + n], 40, width, block, max_new)[0]
+        row, count, first, _, _ = _span(params, 1, width, 40, max_new, block, length, 3, 3 + n)
+        assert count == want[2]
+        if count:
+            assert (row, first) == want[:2]
+
+
+def test_pages_and_touched_blocks(params):
+    assert [params.page(e, 5) for e in (-2 ** 31, -1, 0, 4, 5, 2 ** 31 - 1)] == [-1, -1, 0, 4, -1,
+                                                                                -1]
+    for block in (16, 64):
+        for n in range(0, 200):
+            most = max([0] + [(first + n - 1) // block - first // block + 1
+                              for first in range(block)] if n else [0])
+            assert params.touched(n, block) == most
+
+
+def test_shares_cover_every_tile_once(params):
+    for total in (1, 2, 7, 295, 296, 297, 1000, 99991, 10 ** 12 + 7):
+        for shares in (1, 2, 3, 148, 296):
+            n = min(shares, total)
+            bounds = [params.begin(c, total, n) for c in range(n + 1)]
+            assert bounds[0] == 0 and bounds[-1] == total
+            assert all(a < b for a, b in zip(bounds, bounds[1:]))
+            for c in range(0, n, max(1, n // 7)):
+                for x in (bounds[c], bounds[c + 1] - 1):
+                    assert params.share(x, total, n) == c
+
+
+# ---- the C-ABI on a recording driver --------------------------------------------------------
+SCRIPT = """
+import ctypes as C
+import sys
+sys.path.insert(0, {repo!r})
+from hc_b200 import capi
+fake = C.CDLL("libcuda.so.1")
+class Launch(C.Structure):
+    _fields_ = [("name", C.c_char * 96), ("grid", C.c_uint * 3), ("block", C.c_uint),
+                ("smem", C.c_uint), ("stream", C.c_ulonglong)]
+fake.recorded_launch.restype = C.POINTER(Launch)
+def launches():
+    got = [fake.recorded_launch(i).contents for i in range(fake.recorded_launches())]
+    got = [(l.name.decode(), tuple(l.grid), l.block, l.smem, l.stream) for l in got]
+    fake.recorded_clear()
+    return got
+def refused(match, call, *args, **kw):
+    try:
+        call(*args, **kw)
+    except capi.HcError as e:
+        assert match in str(e), (match, str(e))
+        assert not launches()
+        return
+    raise AssertionError("not refused: " + match)
+hc = capi.Context("cuda:0")
+P = 0x700000000  # an address that nothing dereferences
+launches()
+"""
+
+
+@pytest.fixture(scope="module")
+def recording(tmp_path_factory):
+    out = tmp_path_factory.mktemp("fake")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-w", "-Wl,-soname,libcuda.so.1", "-o",
+                    str(out / "libcuda.so.1"), str(REPO / "oracle" / "recording_cuda.c")],
+                   check=True)
+
+    def run(body):
+        env = dict(os.environ, LD_LIBRARY_PATH=str(out))
+        script = SCRIPT.format(repo=str(REPO)) + textwrap.dedent(body)
+        done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True,
+                              env=env, timeout=300)
+        assert done.returncode == 0, done.stdout + done.stderr
+
+    return run
+
+
+def test_norm_refusals_and_choice(recording):
+    recording("""
+    def norm(rows=4, cols=64, x=P, residual=P, summed=P, gain=P, out=P, scale=P, xp=None, rp=None,
+             sp=None, op=None, cp=8, group=0, eps=1e-5, dtype=capi.HC_BF16, out_dtype=capi.HC_I8):
+        hc.add_rms_norm(x, residual, summed, gain, out, scale, rows, cols, *(
+            cols if v is None else v for v in (xp, rp, sp, op)), cp, group, eps, dtype, out_dtype)
+    refused("unsupported dtype", norm, dtype=capi.HC_F64)
+    refused("unsupported output", norm, out_dtype=capi.HC_F32)
+    refused("invalid shape", norm, rows=-1)
+    refused("invalid shape", norm, xp=63)
+    refused("invalid shape", norm, rp=63)
+    refused("invalid group", norm, group=-2)
+    refused("invalid group", norm, group=32, out_dtype=capi.HC_BF16)
+    refused("scale pitch", norm, cols=1024, group=64)
+    refused("eps", norm, eps=float("nan"))
+    refused("null buffer", norm, scale=None)
+    refused("null buffer", norm, gain=None)
+    refused("no residual", norm, residual=None)
+    norm(rows=0); norm(cols=0)
+    assert not launches()
+    for cols, rows, kernel in ((64, 4, "bf16_i8_t64_v1"), (4096, 1, "bf16_i8_t512_v1"),
+                               (4096, 4000, "bf16_i8_t256_v2"), (8192, 4000, "bf16_i8_t256_v4"),
+                               (16384, 1, "bf16_i8_t512_v4"), (16392, 1, "bf16_i8_generic"),
+                               (100, 1, "bf16_i8_generic")):
+        norm(rows=rows, cols=cols)
+        (name, grid, block, smem, _), = launches()
+        assert name == "hc_add_rms_norm_" + kernel and grid == (rows, 1, 1), name
+    norm(cols=1024, x=P + 2); norm(cols=1024, op=1028); norm(cols=1024, group=96, cp=11)
+    assert all(l[0].endswith("generic") for l in launches())
+    norm(cols=60000)
+    assert launches()[0][3] == 0  # longer than shared memory: the row is computed again
+    """)
+
+
+def test_w4_refusals_and_choice(recording):
+    recording("""
+    def w4(m=1, n=4096, k=4096, group=128, a_group=0, a=P, a_scale=None, w=P, scale=P, zero=None,
+           out=P, ws=P, ws_bytes=1 << 40, lda=None, ldas=64, ldw=None, lds=1024, ldz=1024,
+           ldc=None, a_dtype=capi.HC_BF16, scale_dtype=capi.HC_BF16):
+        pick = lambda v, d: d if v is None else v
+        hc.gemm_w4(a, a_scale, w, scale, zero, out, ws, ws_bytes, m, n, k, group, a_group,
+                   pick(lda, k), ldas, pick(ldw, k // 2), lds, ldz, pick(ldc, n), a_dtype,
+                   scale_dtype)
+    refused("activation dtype", w4, a_dtype=capi.HC_F32)
+    refused("scale dtype", w4, scale_dtype=capi.HC_I8)
+    refused("invalid shape", w4, m=-1)
+    refused("invalid shape", w4, ldw=2047)
+    refused("invalid shape", w4, ldc=4095)
+    refused("multiple of 32", w4, group=33)
+    refused("multiple of 32", w4, group=0)
+    refused("pitch", w4, lds=31)
+    refused("pitch", w4, zero=P, ldz=31)
+    refused("activations' group", w4, a_dtype=capi.HC_I8, a_scale=P, a_group=100)
+    refused("null buffer", w4, a_dtype=capi.HC_I8)
+    refused("null buffer", w4, out=None)
+    refused("null buffer", w4, scale=None)
+    refused("workspace", w4, m=65, ws=None)
+    refused("workspace", w4, m=65, ws_bytes=4096 * 4096 * 2 - 1)
+    refused("workspace", w4, m=65, ws=P + 8)
+    w4(m=0); w4(n=0)
+    assert not launches()
+    lib = hc.lib
+    assert lib.hcGemmW4FewRows() == 64
+    assert lib.hcGemmW4WorkspaceBytes(64, 4096, 4096, capi.HC_BF16) == 0
+    assert lib.hcGemmW4WorkspaceBytes(65, 4090, 4097, capi.HC_BF16) == 4096 * 4097 * 2
+    assert lib.hcGemmW4WorkspaceBytes(65, 4090, 4097, capi.HC_I8) == 4096 * 4097 * 2 + 65 * 4104 * 2
+    for kw, kernel in ((dict(), "bf16_coarse_m1"), (dict(m=9), "bf16_coarse_m2"),
+                       (dict(m=33, group=64), "bf16_fine_m8"),
+                       (dict(m=17, group=1 << 20), "bf16_coarse_m4"),
+                       (dict(a_dtype=capi.HC_I8, a_scale=P), "i8_coarse_m1"),
+                       (dict(w=P + 1), "bf16_coarse_m1_any"),
+                       (dict(k=4098, ldw=2064), "bf16_coarse_m1_any")):
+        w4(**kw)
+        (name, grid, block, smem, _), = launches()
+        assert name == "hc_gemm_w4_" + kernel, name
+        assert grid[0] == 32 and grid[1] in (1, 2, 4, 8) and block == 256 and smem <= 227 << 10
+    # Whatever the sizes: shared memory within a CTA's limit.
+    import random
+    rng = random.Random(0)
+    for _ in range(500):
+        k = rng.choice([1, 31, 128, 4096, 30000, 1 << 20])
+        group = 32 * rng.choice([1, 2, 3, 4, 8, 1000])
+        w4(m=rng.randint(1, 64), n=rng.choice([1, 500, 100000]), k=k, group=group,
+           ldw=(k + 1) // 2, lds=1 << 16, a_dtype=rng.choice([capi.HC_BF16, capi.HC_I8]),
+           a_scale=P)
+        (name, grid, block, smem, _), = launches()
+        assert smem <= 200 << 10, (name, smem, k, group)
+    w4(m=300)
+    assert [l[0] for l in launches()] == ["hc_dequant_w4_bf16", "hc_gemm_bf16_umma_pair"]
+    w4(m=300, a_dtype=capi.HC_I8, a_scale=P)
+    assert [l[0] for l in launches()] == ["hc_dequant_w4_bf16", "hc_dequant_a8_bf16",
+                                          "hc_gemm_bf16_umma_pair"]
+    """)
+
+
+def test_cache_refusals_and_choice(recording):
+    recording("""
+    def cache(**kw):
+        c = capi.HcKvCache(P, P, P, P, 4 * 16 * 128, 16 * 128, 128, 4, 100, 16, 4, 128, capi.HC_I8)
+        for name, v in kw.items():
+            setattr(c, name, v)
+        return c
+    def place(**kw):
+        p = capi.HcKvPlace(P, P, P, 320, 8, 320, 8, 1)
+        for name, v in kw.items():
+            setattr(p, name, v)
+        return p
+    WS = hc.kv_attention_workspace_bytes()
+    def append(c=None, p=None, k=P, v=P, strides=(512, 128, 512, 128)):
+        hc.kv_append(c or cache(), p or place(), k, v, *strides)
+    def attend(c=None, p=None, q=P, out=P, lse=P, share=4, scale=1.0, window=0,
+               strides=(2048, 128, 2048, 128, 16), ws=P, ws_bytes=WS):
+        hc.kv_attention(c or cache(), p or place(), q, out, lse, share, scale, window, *strides, ws,
+                        ws_bytes)
+    for call in (append, attend):
+        refused("cache dtype", call, cache(dtype=capi.HC_BF16))
+        for block in (0, 8, 24, 272):
+            refused("block of", call, cache(block=block))
+        for dim in (0, 8, 120, 272):
+            refused("head dimension", call, cache(dim=dim))
+        refused("pages of", call, cache(pages=-1))
+        refused("pages of", call, cache(heads=0))
+        refused("16-byte aligned", call, cache(tokenStride=136))
+        refused("16-byte aligned", call, cache(tokenStride=112))
+        refused("16-byte aligned", call, cache(pageStride=8))
+        refused("16-byte aligned", call, cache(v=P + 8))
+        refused("scale pitch", call, cache(scalePitch=3))
+        refused("null cache buffer", call, cache(kScale=None))
+        refused("invalid place", call, p=place(seqs=-1))
+        refused("invalid place", call, p=place(maxNew=-1))
+        refused("invalid place", call, p=place(tablePitch=31))
+        refused("invalid place", call, p=place(width=1 << 30, tablePitch=1 << 30))
+        refused("rows for", call, p=place(starts=None, tokens=7))
+        refused("null lengths", call, p=place(lengths=None))
+        refused("null lengths", call, p=place(table=None))
+        call(p=place(seqs=0)); call(p=place(tokens=0))
+        assert not launches()
+    refused("negative strides", append, strides=(-1, 128, 512, 128))
+    refused("null buffer", append, k=None)
+    append(p=place(maxNew=0)); append(cache(pages=0))
+    assert not launches()
+    append()
+    assert launches()[0][:3] == ("hc_kv_append_i8", (8, 4, 2), 128)
+    append(cache(dtype=capi.HC_E4M3), place(maxNew=40, tokens=300))
+    assert launches()[0][:3] == ("hc_kv_append_e4m3", (8 * 4, 4, 2), 128)
+    append(p=place(maxNew=40, tokens=300, starts=None))  # one row per sequence
+    assert launches()[0][1] == (8, 4, 2)
+    refused("too many", append, p=place(seqs=1 << 30, maxNew=100, tokens=1 << 30))
+
+    refused("query heads", attend, share=0)
+    refused("query heads", attend, window=-1)
+    refused("query heads", attend, scale=float("inf"))
+    refused("invalid strides", attend, strides=(-1, 1, 1, 1, 16))
+    refused("invalid strides", attend, strides=(2048, 128, 2048, 128, 15))
+    refused("null buffer", attend, q=None)
+    refused("8-byte aligned", attend, out=P + 2)
+    refused("8-byte aligned", attend, strides=(2048, 128, 2050, 128, 16))
+    refused("workspace", attend, ws=None)
+    refused("workspace", attend, ws=P + 64)
+    refused("workspace", attend, ws_bytes=WS - 1)
+    for kw, kernel, ctas in (
+            (dict(), "i8_d128_r1", 296), (dict(share=9, lse=None), "i8_d128_r2", 148),
+            (dict(c=cache(dim=64, dtype=capi.HC_E4M3)), "e4m3_d64_r1", 296),
+            (dict(c=cache(dim=256, tokenStride=256), share=16, lse=None), "i8_d256_r1", 148),
+            (dict(p=place(seqs=1, width=1, tokens=1)), "i8_d128_r1", 8)):
+        attend(**kw)
+        (name, grid, block, smem, _), = launches()
+        assert name == "hc_kv_attention_" + kernel and grid == (ctas, 1, 1), (name, grid)
+        assert smem <= 64 << 10
+    """)
+
+
+def test_launches_go_to_the_stream_in_use(recording):
+    recording("""
+    def go():
+        hc.softmax_rows(P, P + (1 << 20), 4, 64, 64, 64)
+        return launches()[0][4]
+    own = go()
+    assert own == hc.stream
+    hc.use_stream(0x1234000)
+    assert go() == 0x1234000 and hc.stream == own
+    hc.use_stream(0)
+    assert go() == 0
+    hc.use_own_stream()
+    assert go() == own
+    hc.close()
+    """)
+
+
+def test_every_serving_kernel_is_found_by_its_name():
+    """The families that the launch code names lie in the images it says."""
+    from hc_b200 import capi
+    from tests.test_abi_cpu import _elf_symbols
+
+    lib = capi.load_kernels()
+    for image, count in (("add_rms_norm", 60), ("gemm_w4", 34), ("kv_append", 2),
+                         ("kv_attention", 10)):
+        blob = (REPO / "hc_b200" / "_native" / f"{image}.cubin").read_bytes()
+        names = [s for s in _elf_symbols(blob) if s.startswith("hc_")]
+        assert len(names) == count, (image, len(names))
+        for name in names:
+            assert lib.hcImageName(lib.hcImageOfKernel(name.encode())).decode() == image
