@@ -1000,7 +1000,6 @@ PYBIND11_MODULE(_dispatcher, m) {
   m.def("gemm_w4", &gemmW4, py::arg("ctx"), py::arg("a"), py::arg("w"), py::arg("scale"),
         py::arg("zero"), py::arg("out"), py::arg("group"), py::arg("a_scale") = py::none(),
         py::arg("a_group") = 0, py::arg("workspace") = py::none(), py::arg("stream") = py::none());
-  m.def("w4_few_rows", [] { return hcGemmW4FewRows(); });
   m.def("w4_workspace_bytes",
         [](long long rows, long long n, long long k, bool int8) {
           return hcGemmW4WorkspaceBytes(rows, n, k, int8 ? HC_I8 : HC_BF16);

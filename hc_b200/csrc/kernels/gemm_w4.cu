@@ -7,35 +7,40 @@
 // weights one after another ([N, K/2]); z is 8 where there are no zero points; sa is 1
 // for bf16 activations.
 //
-// With few rows the weights are the traffic (half a byte each, read once), so the
-// kernel streams them from HBM straight into registers, in the layout they are stored
-// in: no shared memory, no barrier in the stream.  The weights are the A operand of
-// mma.sync m16n8k16 (16 weight rows x 16 of K) and the activations the B operand: a
-// lane holds two rows' 32 consecutive weights of 128 (one 16-byte load each), and since
-// a sum does not care about the order of its terms, K is permuted so that these are the
-// very elements the lane feeds to 8 MMAs.  Legacy mma.sync rather than tcgen05: at
-// M <= 64 the stream of weights is the bound, operand registers need no detour through
-// shared memory, and one row costs what eight do.
-//   * unpacking: (w >> 4i) & 0x000f000f | 0x43004300 is the bf16 pair 128 + u of
-//     nibbles i and i + 4, one packed subtraction of 128 + z makes it exact (u - z);
-//     with int8 activations the MMA takes the unsigned nibbles themselves
-//     (m16n8k32, u8 x s8, exact int32 sums) and z * sum(a) is subtracted per group.
-//   * the sum of a group is formed in the MMA's fp32 (int32) accumulators and then
-//     multiplied by the group's scale into the fp32 total: no rounding of weights.
-//   * groups that are not multiples of 128 (32, 64, 96 ...): the four lanes of a row
-//     exchange words (a 4 x 4 transpose by shuffles) so that an MMA stays inside 32
-//     consecutive k.
-//   * a CTA is 8 warps on 128 (MT = 2: 256) weight rows and a slice of K; the
-//     activations of its slice lie in shared memory in fragment order.  A cluster of
-//     CTAs along K adds its partial sums through distributed shared memory, in a fixed
-//     order, so the result does not depend on timing.
+// With few rows the weights are the traffic (half a byte each, read once): every warp
+// streams its own rows through a private ring in shared memory (cp.async, no barrier
+// between warps in the stream), in the layout they are stored in.  The weights are the A operand of
+// mma.sync (16 weight rows) and the activations the B operand (8 columns): a lane holds
+// two rows' 32 consecutive weights of 128 (one 16-byte load each), and since a sum does
+// not care about the order of its terms, K is permuted so that these are the very
+// elements the lane feeds to the MMAs.  Legacy mma.sync rather than tcgen05: one row
+// costs what eight do, the operand registers need no detour, and at up to 16 rows the
+// stream of weights is the bound (mma.sync measured 549 TFLOP/s in bf16 and 1127 TOP/s
+// in int8 on this GPU, against 13 and 26 needed per row at full bandwidth).
+//   * bf16: the bits of a nibble ARE the f16 number u * 2^-24 (a subnormal, which the
+//     MMA takes as it is), and 16 u * 2^-24 one place further left: one AND per two
+//     weights and one shift per eight unpack them, exactly.  (The logic pipe has half
+//     the issue rate; shifting, masking, biasing and subtracting per pair held the
+//     stream at 1.4 TB/s.)  The activations become f16 by a power of two per row and
+//     segment of 128 (Fine: 32) k, those that meet 16 u a sixteenth of it: exact down
+//     to 2^-24 of the segment's largest.
+//     int8: the nibbles as unsigned bytes (m16n8k32, u8 x s8, exact int32 sums).
+//   * a segment's sum is formed in the MMA's accumulators; z * sum(a) comes off and the
+//     scale multiplies it into the fp32 total: no rounding of weights.
+//   * Fine: groups that are not multiples of 128 (32, 64, 96 ...): a lane reads its four
+//     words 16 bytes apart, so that an MMA stays inside 32 consecutive k.
+//   * a CTA of 16 warps per SM walks over tiles of 16 weight rows; its warps divide K
+//     among themselves (all 16 where K is long enough, else groups of warps take
+//     different tiles), so a warp meets the same activations in every tile and they are
+//     put into shared memory once.  A warp's loads run kSlots - 1 spans ahead, across
+//     tiles.
+//     The partial sums of a tile's warps meet in shared memory and are added in the
+//     order of K.
 #include "serving_math.cuh"
 
-#include <cooperative_groups.h>
 #include <type_traits>
 
 using namespace hcs;
-namespace cg = cooperative_groups;
 
 namespace {
 
@@ -49,17 +54,17 @@ struct W4Params {
   long long lda, ldas, ldw, lds, ldz, ldc;
   int M, N, K, group, aGroup;
   int scaleF32;
-  int sliceK; // K per CTA, a multiple of 128
-  int stepK;  // K staged in shared memory at a time, a multiple of 128
-  int vec;    // w: 16-byte aligned rows
-  int vecA;   // a: 16-byte aligned rows
+  int warpsK;   // warps that divide K: 1, 2, 4, 8 or 16
+  int perWarp;  // scales a warp keeps per weight row: groups of K it can meet
+  int vec;      // w: 16-byte aligned rows
+  int vecA;     // a: 16-byte (int8: 8-byte) aligned rows
 };
 
 constexpr int kSpan = 128; // K of one pair of 16-byte loads
 
-__device__ __forceinline__ void mmaBf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+__device__ __forceinline__ void mmaF16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
                "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -73,393 +78,422 @@ __device__ __forceinline__ void mmaU8S8(int (&d)[4], const uint32_t (&a)[4], uin
 }
 
 // The 16 bytes (32 weights) at byte `at` of a weight row that is `bytes` long; what
-// lies beyond the row reads as zero (its activations are zero).  Whole: rows are
-// 16-byte aligned and a multiple of 16 bytes long.
-template <bool Whole>
+// lies beyond the row reads as zero.
 __device__ __forceinline__ uint4 loadWeights(const uint8_t *row, long long at, int bytes,
                                              int vec) {
-  if constexpr (Whole) {
-    return at < bytes ? loadStream16(row + at) : make_uint4(0, 0, 0, 0);
-  } else {
-    if (vec && at + 16 <= bytes)
-      return loadStream16(row + at);
-    uint32_t v[4] = {0, 0, 0, 0};
+  if (vec && at + 16 <= bytes)
+    return loadStream16(row + at);
+  uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (at + i < bytes)
-        v[i >> 2] |= uint32_t(row[at + i]) << (8 * (i & 3));
-    return make_uint4(v[0], v[1], v[2], v[3]);
-  }
+  for (int i = 0; i < 16; ++i)
+    if (at + i < bytes)
+      v[i >> 2] |= uint32_t(row[at + i]) << (8 * (i & 3));
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// words[j] of lane t of a quad <-> words[t] of lane j: afterwards word c of lane t is
-// word t of what lane c had, i.e. the quad's words c are 32 consecutive k.
-__device__ __forceinline__ void transposeQuad(uint32_t (&v)[4], int t) {
-  const bool odd = t & 1, high = t & 2;
-  uint32_t s0 = odd ? v[0] : v[1], s1 = odd ? v[2] : v[3];
-  s0 = __shfl_xor_sync(0xffffffffu, s0, 1);
-  s1 = __shfl_xor_sync(0xffffffffu, s1, 1);
-  if (odd) {
-    v[0] = s0;
-    v[2] = s1;
-  } else {
-    v[1] = s0;
-    v[3] = s1;
-  }
-  uint32_t r0 = high ? v[0] : v[2], r1 = high ? v[1] : v[3];
-  r0 = __shfl_xor_sync(0xffffffffu, r0, 2);
-  r1 = __shfl_xor_sync(0xffffffffu, r1, 2);
-  if (high) {
-    v[0] = r0;
-    v[1] = r1;
-  } else {
-    v[2] = r0;
-    v[3] = r1;
-  }
-}
+constexpr int kWarps = 16;
+// A warp's ring: spans of 16 rows x 64 bytes, the 16-byte chunks of row r exchanged by
+// an XOR with (r / 2) % 4 (free of bank conflicts for 16-byte and Fine's 4-byte reads).
+constexpr int kSlots = 4;
+constexpr int kSlotBytes = 16 * 64;
 
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
-                                   *reinterpret_cast<const __nv_bfloat162 *>(&b));
-  return *reinterpret_cast<const uint32_t *>(&d);
-}
-
-// Eight weights -> four bf16 pairs (k0,k4) (k1,k5) (k2,k6) (k3,k7) of u - z; `bias` is
-// the pair 128 + z.
-__device__ __forceinline__ void unpackBf16(uint32_t w, uint32_t bias, uint32_t (&p)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = sub2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, bias);
-}
-
-// Shared memory: the activations of the current step in fragment order, then the
-// scales and zero points of the step's groups, [group][row].
-//   bf16: per span, n-tile and word j one 16-byte piece per lane: the 8 activations
-//         that meet word j of that lane, as pairs (0,4) (1,5) (2,6) (3,7);
-//   int8: 8 bytes per lane: bytes (0,2,4,6) and (1,3,5,7).
-template <int NT, int MT, bool A8, bool Fine> struct Layout {
-  static constexpr int rows = 8 * 16 * MT; // weight rows of a CTA
+// Shared memory: the activation rows, per span of 128 k and row the pieces of 8
+// activations in the order the lanes read them (piece (lane t, word j) at (4 j + t)
+// pieces), as f16 pairs (0,4) (1,5)/16 (2,6) (3,7)/16 or as bytes (0,2,4,6) (1,3,5,7);
+// then per segment of K (a span; Fine: 32) and column {sum of its activations in the
+// accumulator's unit, that unit times the activations' scale}; then per warp {scale,
+// zero} of its 16 weight rows and its groups; then the partial sums of two tiles per
+// warp; then 256 bytes of zeros that lanes without an activation row read.
+template <bool A8, bool Fine> struct Layout {
   static constexpr int pieceBytes = A8 ? 8 : 16;
-  static constexpr int spanBytes = NT * 4 * 32 * pieceBytes;
+  static constexpr int spanBytes = 16 * pieceBytes;
+  static constexpr int unit = Fine ? 32 : 128; // K of a segment
+  static constexpr int segments = kSpan / unit;
 };
 
-template <int NT, int MT, bool A8, bool Fine, bool Whole>
+// Whole: weight rows are 16-byte aligned and a multiple of 32 weights long.
+template <bool A8, bool Fine, bool Whole>
 __device__ __forceinline__ void w4Body(const W4Params &p) {
-  using L = Layout<NT, MT, A8, Fine>;
+  using L = Layout<A8, Fine>;
   using Acc = typename std::conditional<A8, int, float>::type;
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int row0 = int(blockIdx.x) * L::rows;
-  const int kBegin = int(blockIdx.y) * p.sliceK;
-  const int kEnd = min(p.K, kBegin + p.sliceK);
   const int rowBytes = (p.K + 1) >> 1;
+  const int spans = (p.K + kSpan - 1) / kSpan;
 
-  unsigned char *frag = smem;
-  const int maxGroups = (p.stepK + p.group - 1) / p.group + 1; // (as the host computes it)
-  float *sScale = reinterpret_cast<float *>(smem + size_t(p.stepK / kSpan) * L::spanBytes);
-  uint32_t *sBias = reinterpret_cast<uint32_t *>(sScale + maxGroups * L::rows);
-  int *sASum = reinterpret_cast<int *>(sBias + maxGroups * L::rows);       // int8: [group][8 NT]
-  float *sAScale = reinterpret_cast<float *>(sASum + maxGroups * 8 * NT); // int8: [group][8 NT]
+  // This warp's share of K and its tiles of 16 weight rows.
+  const int wk = warp & (p.warpsK - 1), team = warp / p.warpsK;
+  const int teams = kWarps / p.warpsK;
+  const int sLo = wk * spans / p.warpsK, sHi = (wk + 1) * spans / p.warpsK;
+  const int tiles = (p.N + 15) >> 4;
+  const int tile0 = int(blockIdx.x) * teams + team, tileStep = int(gridDim.x) * teams;
 
-  const uint8_t *wRow[2 * MT];
-  bool rowIn[2 * MT];
-#pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) {
-    const int r = row0 + warp * 16 * MT + (i >> 1) * 16 + (i & 1) * 8 + g;
-    rowIn[i] = r < p.N;
-    wRow[i] = p.w + (rowIn[i] ? (long long)r * p.ldw : 0);
-  }
-  float total[MT][NT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        total[m][n][i] = 0.0f;
+  // Rows of activations are 64 bytes (int8: 32) apart modulo the banks.
+  const int aPitch = spans * L::spanBytes + 4 * L::pieceBytes;
+  float2 *sAct = reinterpret_cast<float2 *>(smem + p.M * aPitch);
+  float2 *sScale = sAct + spans * L::segments * 8 + warp * p.perWarp * 16;
+  float *sPart = reinterpret_cast<float *>(sAct + spans * L::segments * 8 +
+                                           kWarps * p.perWarp * 16); // [2][warp][16 x 8]
+  unsigned char *sNone = reinterpret_cast<unsigned char *>(sPart + 2 * kWarps * 128);
 
-  constexpr int kAhead = MT == 1 ? 4 : 2; // spans in flight per warp
-  for (int k0 = kBegin; k0 < kEnd; k0 += p.stepK) {
-    const int spans = (min(kEnd, k0 + p.stepK) - k0 + kSpan - 1) / kSpan;
-    uint4 ring[kAhead][2 * MT];
-    auto fetch = [&](uint4 (&dst)[2 * MT], int s) {
-      const long long at = ((long long)k0 + s * kSpan + t * 32) >> 1;
+  // ---- the stream of weights: (tile, span) of this warp, kSlots - 1 spans ahead -------------
+  unsigned char *ring = sNone + 256 + warp * kSlots * kSlotBytes;
+  const int mix = (g >> 1) & 3; // (rows g and g + 8 alike)
+  const uint32_t ringAt = hc::smemAddr(ring) + g * 64 + (t ^ mix) * 16;
+  const int mine = tile0 < tiles && sLo < sHi ? (tiles - 1 - tile0) / tileStep + 1 : 0;
+  int fTile = tile0, fLeft = sHi - sLo, fCount = mine * (sHi - sLo);
+  uint32_t fSlot = 0; // bytes
+  const uint8_t *fRow[2];
+  auto rowsOf = [&](int tile) {
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i)
-        dst[i] = rowIn[i] && s < spans ? loadWeights<Whole>(wRow[i], at, rowBytes, p.vec)
-                                       : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 2; ++i) // rows past N read row N - 1 again and are not stored
+      fRow[i] = p.w + (long long)min(tile * 16 + i * 8 + g, p.N - 1) * p.ldw + sLo * 64 + t * 16;
+  };
+  rowsOf(fTile);
+  // In the last span of a row that is not a multiple of 128 weights, some lanes' bytes
+  // lie behind the row.
+  const bool ragged = sHi == spans && (spans - 1) * 64 + t * 16 >= rowBytes;
+  auto fetch = [&]() {
+    if (fCount > 0) {
+      --fCount;
+      if constexpr (Whole) { // (zeros for what is behind the row; the address is not read)
+        const int in = ragged && fLeft == 1 ? 0 : 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           ringAt + fSlot + i * 512),
+                       "l"(fRow[i]), "r"(in)
+                       : "memory");
+      } else {
+        const int at = (sHi - fLeft) * 64 + t * 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<uint4 *>(ring + fSlot + i * 512 + g * 64 + (t ^ mix) * 16) =
+              loadWeights(fRow[i] - at, at, rowBytes, p.vec);
+      }
+      fRow[0] += 64;
+      fRow[1] += 64;
+      fSlot = (fSlot + kSlotBytes) & (kSlots * kSlotBytes - 1);
+      if (--fLeft == 0) {
+        fLeft = sHi - sLo;
+        fTile += tileStep;
+        rowsOf(fTile);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int u = 0; u < kSlots - 1; ++u)
+    fetch();
+
+  // ---- its scales, a tile ahead in registers -------------------------------------------------
+  const int gLo = sLo * kSpan / p.group;
+  const int groups = sLo < sHi ? (min(p.K, sHi * kSpan) - 1) / p.group - gLo + 1 : 0;
+  constexpr int kHeld = Fine ? 8 : 2; // per lane; more are loaded when their tile begins
+  float heldScale[kHeld];
+  int heldZero[kHeld];
+  auto scaleAt = [&](long long at, long long atZero, float &s, int &z) {
+    s = p.scaleF32 ? static_cast<const float *>(p.scale)[at]
+                   : __bfloat162float(static_cast<const __nv_bfloat16 *>(p.scale)[at]);
+    z = p.zero ? p.zero[atZero] : 8;
+  };
+  auto loadScales = [&](int tile) {
+    const long long n = min(tile * 16 + (lane & 15), p.N - 1);
+    const long long at = n * p.lds + gLo + (lane >> 4), atZero = n * p.ldz + gLo + (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (tile < tiles && 2 * i + (lane >> 4) < groups)
+        scaleAt(at + 2 * i, atZero + 2 * i, heldScale[i], heldZero[i]);
+  };
+  auto putScales = [&](int tile) {
+    auto put = [&](int gi, float s, int z) {
+      sScale[gi * 16 + (lane & 15)] = make_float2(s, float(z));
     };
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s)
-      fetch(ring[s], s);
-
-    // Stage the step's activations and scales while the first weights travel.
-    if (k0 != kBegin)
-      __syncthreads(); // the previous step's have been read
-    const int firstGroup = k0 / p.group;
-    const int lastK = min(kEnd, k0 + spans * kSpan) - 1;
-    const int groups = lastK / p.group - firstGroup + 1;
-    if constexpr (A8) {
-      for (int i = tid; i < groups * 8 * NT; i += 256)
-        sASum[i] = 0;
-      __syncthreads();
+    for (int i = 0; i < kHeld; ++i) {
+      const int gi = 2 * i + (lane >> 4);
+      if (gi < groups)
+        put(gi, heldScale[i], heldZero[i]);
     }
-    const int pieces = spans * 16 * NT * 8; // 8 activations each
-    for (int i = tid; i < pieces; i += 256) {
-      const int m = i / (spans * 16), q = i - m * (spans * 16);
+    const long long n = min(tile * 16 + (lane & 15), p.N - 1);
+    for (int gi = 2 * kHeld + (lane >> 4); gi < groups; gi += 2) {
+      float s;
+      int z;
+      scaleAt(n * p.lds + gLo + gi, n * p.ldz + gLo + gi, s, z);
+      put(gi, s, z);
+    }
+  };
+  loadScales(tile0);
+
+  // ---- the activations, once -----------------------------------------------------------------
+  for (int i = tid; i < spans * L::segments * 8; i += 32 * kWarps)
+    if ((i & 7) >= p.M)
+      sAct[i] = make_float2(0.0f, 0.0f);
+  if (tid < 64)
+    reinterpret_cast<uint32_t *>(sNone)[tid] = 0;
+  constexpr int kLanes = Fine ? 4 : 16; // that hold a segment: 8 activations each
+  constexpr int kBatch = 4;             // pieces per thread whose loads travel together
+  const int perRow = spans * 16, pieces = p.M * perRow; // pieces of 8
+  for (int q0 = tid; q0 - tid < pieces; q0 += kBatch * 32 * kWarps) {
+    uint32_t v[kBatch][4];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = q0 + u * 32 * kWarps;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        v[u][c] = 0;
+      if (i >= pieces)
+        continue;
+      const int m = i / perRow, k = (i - m * perRow) * 8;
+      const char *src = static_cast<const char *>(p.a) +
+                        ((long long)m * p.lda + k) * (A8 ? 1 : 2);
+      if (p.vecA && k + 8 <= p.K) {
+        if constexpr (A8) {
+          const uint2 x = *reinterpret_cast<const uint2 *>(src);
+          v[u][0] = x.x;
+          v[u][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4 *>(src);
+          v[u][0] = x.x;
+          v[u][1] = x.y;
+          v[u][2] = x.z;
+          v[u][3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+          if (k + b < p.K) {
+            if constexpr (A8)
+              v[u][b >> 2] |= uint32_t(uint8_t(src[b])) << (8 * (b & 3));
+            else
+              v[u][b >> 1] |= uint32_t(reinterpret_cast<const uint16_t *>(src)[b])
+                              << (16 * (b & 1));
+          }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      // (Pieces come in sixteens: a whole or half warp is at work, segments are whole.)
+      const int i = q0 + u * 32 * kWarps;
+      if (i >= pieces)
+        continue;
+      const uint32_t mask = i - lane + 32 <= pieces ? 0xffffffffu : 0x0000ffffu;
+      const int m = i / perRow, q = i - m * perRow;
       const int span = q >> 4, hi = (q >> 2) & 3, lo = q & 3; // k = span*128 + hi*32 + lo*8
-      const int k = k0 + span * kSpan + hi * 32 + lo * 8;
       // Coarse: lane t holds 32 consecutive k, word j its j-th eight.  Fine: word c is
       // the c-th 32 of the span, lane t its t-th eight.
       const int ft = Fine ? lo : hi, fj = Fine ? hi : lo;
-      const int flane = (m & 7) * 4 + ft, nt = m >> 3;
-      unsigned char *dst =
-          frag + size_t(span) * L::spanBytes + ((nt * 4 + fj) * 32 + flane) * L::pieceBytes;
+      unsigned char *dst = smem + m * aPitch + span * L::spanBytes + (4 * fj + ft) * L::pieceBytes;
+      float2 note;
       if constexpr (A8) {
-        const int8_t *src = static_cast<const int8_t *>(p.a) + (long long)m * p.lda + k;
-        uint32_t x = 0, y = 0;
-        if (m < p.M && k < kEnd) {
-          if (p.vecA && k + 8 <= kEnd) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(src);
-            x = v.x;
-            y = v.y;
-          } else {
-            for (int b = 0; b < 8; ++b)
-              if (k + b < kEnd)
-                (b < 4 ? x : y) |= uint32_t(uint8_t(src[b])) << (8 * (b & 3));
-          }
-        }
+        const uint32_t x = v[u][0], y = v[u][1];
         *reinterpret_cast<uint2 *>(dst) =
             make_uint2(__byte_perm(x, y, 0x6420), __byte_perm(x, y, 0x7531));
-        // The sum of the group's activations (integers: the order does not matter).
-        if (m < p.M && k < kEnd) {
-          const int sum = __dp4a(int(x), 0x01010101, __dp4a(int(y), 0x01010101, 0));
-          atomicAdd(&sASum[(k / p.group - firstGroup) * 8 * NT + m], sum);
-        }
+        int sum = __dp4a(int(x), 0x01010101, __dp4a(int(y), 0x01010101, 0));
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1)
+          sum += __shfl_xor_sync(mask, sum, d);
+        note.x = float(sum);
+        note.y = 8 * q < p.K && p.aGroup < p.K
+                     ? p.aScale[(long long)m * p.ldas + 8 * q / p.aGroup]
+                     : 1.0f;
       } else {
-        const __nv_bfloat16 *src =
-            static_cast<const __nv_bfloat16 *>(p.a) + (long long)m * p.lda + k;
-        uint32_t v[4] = {0, 0, 0, 0};
-        if (m < p.M && k < kEnd) {
-          if (p.vecA && k + 8 <= kEnd) {
-            const uint4 q4 = *reinterpret_cast<const uint4 *>(src);
-            v[0] = q4.x;
-            v[1] = q4.y;
-            v[2] = q4.z;
-            v[3] = q4.w;
-          } else {
-            for (int b = 0; b < 8; ++b)
-              if (k + b < kEnd)
-                v[b >> 1] |= uint32_t(__bfloat16_as_ushort(src[b])) << (16 * (b & 1));
-          }
+        float e[8], sum = 0.0f, top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          e[2 * b] = __uint_as_float(v[u][b] << 16);
+          e[2 * b + 1] = __uint_as_float(v[u][b] & 0xffff0000u);
         }
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          sum += e[b];
+          top = fmaxf(top, fabsf(e[b]));
+        }
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) {
+          sum += __shfl_xor_sync(mask, sum, d);
+          top = fmaxf(top, __shfl_xor_sync(mask, top, d));
+        }
+        // up = 2^(14 - floor(log2 top)), within what float holds; down = 1 / up.
+        const int expo = int(__float_as_uint(top) >> 23);
+        const int shift = expo == 0 || expo == 255 ? 0 : max(-126, min(126, 14 - (expo - 127)));
+        const float up = __uint_as_float(uint32_t(127 + shift) << 23);
+        const float down = __uint_as_float(uint32_t(127 - shift) << 23);
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+          e[b] *= b & 1 ? up * 0.0625f : up;
+        auto pair = [](float a, float b) {
+          const __half2 h = __floats2half2_rn(a, b);
+          return *reinterpret_cast<const uint32_t *>(&h);
+        };
         *reinterpret_cast<uint4 *>(dst) =
-            make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632),
-                       __byte_perm(v[1], v[3], 0x5410), __byte_perm(v[1], v[3], 0x7632));
+            make_uint4(pair(e[0], e[4]), pair(e[1], e[5]), pair(e[2], e[6]), pair(e[3], e[7]));
+        // The accumulator counts in units of 2^-24 / up.
+        note.x = sum * up * 5.9604644775390625e-08f;
+        note.y = down * 16777216.0f;
       }
+      if ((q & (kLanes - 1)) == 0)
+        sAct[(span * L::segments + (Fine ? hi : 0)) * 8 + m] = note;
     }
-    for (int i = tid; i < groups * L::rows; i += 256) {
-      const int r = i / groups, gi = i - r * groups;
-      const int n = row0 + r;
-      float s = 0.0f;
-      int z = 8;
-      if (n < p.N) {
-        const long long at = (long long)n * p.lds + firstGroup + gi;
-        s = p.scaleF32 ? static_cast<const float *>(p.scale)[at]
-                       : __bfloat162float(static_cast<const __nv_bfloat16 *>(p.scale)[at]);
-        if (p.zero)
-          z = p.zero[(long long)n * p.ldz + firstGroup + gi];
-      }
-      sScale[gi * L::rows + r] = s;
-      const uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rn(128.0f + float(z)));
-      sBias[gi * L::rows + r] = A8 ? uint32_t(z) : (b << 16 | b);
-    }
-    if constexpr (A8) {
-      for (int i = tid; i < groups * 8 * NT; i += 256) {
-        const int gi = i / (8 * NT), m = i - gi * 8 * NT;
-        const int b = max(k0, (firstGroup + gi) * p.group);
-        sAScale[i] = m < p.M ? p.aScale[(long long)m * p.ldas + b / p.aGroup] : 0.0f;
-      }
-    }
-    __syncthreads();
+  }
+  __syncthreads();
 
-    Acc acc[MT][NT][4];
+  // ---- tiles ----------------------------------------------------------------------------------
+  float total[4];
+  const bool live = g < p.M;
+  const unsigned char *aRow = live ? smem + g * aPitch + t * L::pieceBytes : sNone;
+  const int aStep = live ? L::spanBytes : 0;
+  const int perGroup = p.group / L::unit;
+  int left = 0, gi = 0, parity = 0;
+  float2 c0, c1; // {scale, zero} of the current group, rows g and g + 8
+  auto scalesOf = [&]() {
+    c0 = sScale[gi * 16 + g];
+    c1 = sScale[gi * 16 + g + 8];
+  };
+  // One span; the tile's sums are in `total` after the last one.
+  uint32_t slot = 0;
+  auto step = [&](int s) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+    __syncwarp(); // (every lane's copies have arrived, and the slot before is read)
+    uint32_t words[2][4];
+    const unsigned char *from = ring + slot + g * 64;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (Fine) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int j = 0; j < 4; ++j)
+          words[i][j] = *reinterpret_cast<const uint32_t *>(from + i * 512 + 16 * (j ^ mix) + 4 * t);
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4 *>(from + i * 512 + 16 * (t ^ mix));
+        words[i][0] = v.x;
+        words[i][1] = v.y;
+        words[i][2] = v.z;
+        words[i][3] = v.w;
+      }
+    }
+    slot = (slot + kSlotBytes) & (kSlots * kSlotBytes - 1);
+    fetch(); // into the slot that the step before has read
+    const unsigned char *piece = aRow + s * aStep;
+    Acc acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (Fine || j == 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          acc[m][n][i] = 0;
-    // Adds the group sums, times their scales, to the totals.
-    auto flush = [&](int gi) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int r = warp * 16 * MT + m * 16 + g;
-        const float s0 = sScale[gi * L::rows + r], s1 = sScale[gi * L::rows + r + 8];
-        int z0 = 0, z1 = 0;
-        if constexpr (A8) {
-          z0 = int(sBias[gi * L::rows + r]);
-          z1 = int(sBias[gi * L::rows + r + 8]);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (A8) {
-              const int at = gi * 8 * NT + n * 8 + 2 * t + (i & 1);
-              const int exact = acc[m][n][i] - (i < 2 ? z0 : z1) * sASum[at];
-              total[m][n][i] =
-                  fmaf((i < 2 ? s0 : s1) * sAScale[at], float(exact), total[m][n][i]);
-            } else {
-              total[m][n][i] = fmaf(i < 2 ? s0 : s1, acc[m][n][i], total[m][n][i]);
-            }
-            acc[m][n][i] = 0;
-          }
-        }
+          acc[i] = 0;
       }
-    };
-
-    int current = 0; // group (within the step) that acc belongs to
-    for (int s0 = 0; s0 < spans; s0 += kAhead) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int s = s0 + u;
-        if (s >= spans)
-          break;
-        uint32_t words[2 * MT][4];
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-          words[i][0] = ring[u][i].x;
-          words[i][1] = ring[u][i].y;
-          words[i][2] = ring[u][i].z;
-          words[i][3] = ring[u][i].w;
-          if constexpr (Fine)
-            transposeQuad(words[i], t);
+      const uint32_t w0 = words[0][j], w1 = words[1][j];
+      if constexpr (A8) {
+        const uint32_t a[4] = {w0 & 0x0f0f0f0fu, w1 & 0x0f0f0f0fu, (w0 >> 4) & 0x0f0f0f0fu,
+                               (w1 >> 4) & 0x0f0f0f0fu};
+        const uint2 b = *reinterpret_cast<const uint2 *>(piece + 4 * j * L::pieceBytes);
+        mmaU8S8(acc, a, b.x, b.y);
+      } else {
+        const uint32_t h0 = w0 >> 8, h1 = w1 >> 8;
+        const uint32_t a0[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u,
+                                w1 & 0x00f000f0u};
+        const uint32_t a1[4] = {h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u,
+                                h1 & 0x00f000f0u};
+        const uint4 b = *reinterpret_cast<const uint4 *>(piece + 4 * j * L::pieceBytes);
+        mmaF16(acc, a0, b.x, b.y);
+        mmaF16(acc, a1, b.z, b.w);
+      }
+      if (Fine || j == 3) {
+        if (left == 0) { // (behind the last group there is nothing: its index stays)
+          gi = min(gi + 1, groups - 1);
+          left = perGroup;
+          scalesOf();
         }
-        fetch(ring[u], s + kAhead);
-        const unsigned char *piece = frag + size_t(s) * L::spanBytes + lane * L::pieceBytes;
+        --left;
+        const float4 v = *reinterpret_cast<const float4 *>(
+            sAct + (s * L::segments + (Fine ? j : 0)) * 8 + 2 * t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (Fine || j == 0) {
-            const int gi = (k0 + s * kSpan + (Fine ? j * 32 : 0)) / p.group - firstGroup;
-            // (behind the last element there is no such group, and nothing to add)
-            if (gi != current && gi < groups) {
-              flush(current);
-              current = gi;
-            }
-          }
-          uint32_t a[MT][2][4];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const uint32_t w0 = words[2 * m][j], w1 = words[2 * m + 1][j];
-            if constexpr (A8) {
-              a[m][0][0] = w0 & 0x0f0f0f0fu;
-              a[m][0][1] = w1 & 0x0f0f0f0fu;
-              a[m][0][2] = (w0 >> 4) & 0x0f0f0f0fu;
-              a[m][0][3] = (w1 >> 4) & 0x0f0f0f0fu;
-            } else {
-              const int r = warp * 16 * MT + m * 16 + g;
-              const uint32_t b0 = p.zero ? sBias[current * L::rows + r] : 0x43084308u;
-              const uint32_t b1 = p.zero ? sBias[current * L::rows + r + 8] : 0x43084308u;
-              uint32_t p0[4], p1[4];
-              unpackBf16(w0, b0, p0);
-              unpackBf16(w1, b1, p1);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                a[m][h][0] = p0[2 * h];
-                a[m][h][1] = p1[2 * h];
-                a[m][h][2] = p0[2 * h + 1];
-                a[m][h][3] = p1[2 * h + 1];
-              }
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const unsigned char *src = piece + (n * 4 + j) * 32 * L::pieceBytes;
-            if constexpr (A8) {
-              const uint2 b = *reinterpret_cast<const uint2 *>(src);
-#pragma unroll
-              for (int m = 0; m < MT; ++m)
-                mmaU8S8(acc[m][n], a[m][0], b.x, b.y);
-            } else {
-              const uint4 b = *reinterpret_cast<const uint4 *>(src);
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                mmaBf16(acc[m][n], a[m][0], b.x, b.y);
-                mmaBf16(acc[m][n], a[m][1], b.z, b.w);
-              }
-            }
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float2 &c = i < 2 ? c0 : c1;
+          const float sum = i & 1 ? v.z : v.x, unit = i & 1 ? v.w : v.y;
+          total[i] = fmaf(c.x * unit, fmaf(-c.y, sum, float(acc[i])), total[i]);
         }
       }
     }
-    flush(current);
-  }
+  };
+  const int firstLeft = (p.group - sLo * kSpan % p.group) / L::unit;
+  auto beginTile = [&](int tile) {
+    __syncwarp(); // the previous tile's scales have been read
+    putScales(tile);
+    loadScales(tile + tileStep);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      total[i] = 0.0f;
+    gi = 0;
+    left = firstLeft;
+    scalesOf();
+  };
+  auto endTile = [&](int tile, int turn) {
+    float *mine = sPart + (parity * kWarps + warp) * 128;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) // [column][row]
+      mine[(2 * t + (i & 1)) * 16 + (i >> 1) * 8 + g] = total[i];
+    if (p.warpsK == 1)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * p.warpsK) : "memory");
+    // One of the team's warps adds them, in turn; the others go on (the two halves of
+    // the buffer alternate, and that warp meets the others again before its half is
+    // written).
+    if (turn == wk) {
+      const float *from = sPart + (parity * kWarps + team * p.warpsK) * 128;
+      for (int i = lane; i < 16 * p.M; i += 32) {
+        float sum = 0.0f;
+        for (int w = 0; w < p.warpsK; ++w)
+          sum += from[w * 128 + i];
+        const int m = i >> 4, n = tile * 16 + (i & 15);
+        if (A8 && p.aGroup >= p.K && p.K > 0) // one scale per activation row
+          sum *= p.aScale[(long long)m * p.ldas];
+        if (n < p.N)
+          p.out[(long long)m * p.ldc + n] = __float2bfloat16_rn(sum);
+      }
+    }
+    parity ^= 1;
+  };
 
-  // Partial sums of the cluster's CTAs, [weight row][activation row], added in rank
-  // order: rank r finishes its share of the rows.
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = int(gridDim.y);
-  constexpr int pitch = 8 * NT + 1;
-  if (ranks == 1) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = n * 8 + 2 * t + (i & 1);
-          const int r = row0 + warp * 16 * MT + m * 16 + (i >> 1) * 8 + g;
-          if (r < p.N && col < p.M)
-            p.out[(long long)col * p.ldc + r] = __float2bfloat16_rn(total[m][n][i]);
-        }
-    return;
-  }
-  float *part = reinterpret_cast<float *>(smem);
-  __syncthreads(); // the staged operands have been read
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+  int turn = 0;
+  if (sLo < sHi) {
+    int tile = tile0;
+    for (int i = 0; i < mine; ++i) {
+      beginTile(tile);
+#pragma unroll 1
+      for (int s = sLo; s < sHi; ++s)
+        step(s);
+      endTile(tile, turn);
+      turn = turn + 1 == p.warpsK ? 0 : turn + 1;
+      tile += tileStep;
+    }
+  } else { // (K = 0)
+    for (int tile = tile0; tile < tiles; tile += tileStep) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        part[(warp * 16 * MT + m * 16 + (i >> 1) * 8 + g) * pitch + n * 8 + 2 * t + (i & 1)] =
-            total[m][n][i];
-  cluster.sync();
-  const int share = L::rows / ranks, mine = int(cluster.block_rank()) * share;
-  for (int i = tid; i < share * p.M; i += 256) {
-    const int col = i / share, r = mine + i - col * share;
-    float sum = 0.0f;
-    for (int c = 0; c < ranks; ++c)
-      sum += cluster.map_shared_rank(part, c)[r * pitch + col];
-    if (row0 + r < p.N)
-      p.out[(long long)col * p.ldc + row0 + r] = __float2bfloat16_rn(sum);
+        total[i] = 0.0f;
+      endTile(tile, turn);
+    }
   }
-  cluster.sync(); // no CTA leaves while its memory is read
 }
 
 } // namespace
 
-#define HC_W4(nt, mt, aname, A8, fname, Fine)                                              \
-  extern "C" __global__ void __launch_bounds__(256, 2)                                      \
-      hc_gemm_w4_##aname##_##fname##_m##nt(const __grid_constant__ W4Params p) {            \
-    w4Body<nt, mt, A8, Fine, true>(p);                                                      \
+#define HC_W4(aname, A8, fname, Fine)                                                       \
+  extern "C" __global__ void __launch_bounds__(512, 1)                                      \
+      hc_gemm_w4_##aname##_##fname(const __grid_constant__ W4Params p) {                    \
+    w4Body<A8, Fine, true>(p);                                                              \
   }                                                                                         \
-  extern "C" __global__ void __launch_bounds__(256)                                         \
-      hc_gemm_w4_##aname##_##fname##_m##nt##_any(const __grid_constant__ W4Params p) {      \
-    w4Body<nt, mt, A8, Fine, false>(p);                                                     \
+  extern "C" __global__ void __launch_bounds__(512, 1)                                      \
+      hc_gemm_w4_##aname##_##fname##_any(const __grid_constant__ W4Params p) {              \
+    w4Body<A8, Fine, false>(p);                                                             \
   }
-#define HC_W4_ROWS(aname, A8, fname, Fine)                                                  \
-  HC_W4(1, 1, aname, A8, fname, Fine)                                                       \
-  HC_W4(2, 1, aname, A8, fname, Fine)                                                       \
-  HC_W4(4, 1, aname, A8, fname, Fine)                                                       \
-  HC_W4(8, 1, aname, A8, fname, Fine)
-HC_W4_ROWS(bf16, false, coarse, false)
-HC_W4_ROWS(bf16, false, fine, true)
-HC_W4_ROWS(i8, true, coarse, false)
-HC_W4_ROWS(i8, true, fine, true)
+HC_W4(bf16, false, coarse, false)
+HC_W4(bf16, false, fine, true)
+HC_W4(i8, true, coarse, false)
+HC_W4(i8, true, fine, true)
 
 // ---- conversions for larger row counts ----------------------------------------------------
 // out[k, n] = bf16((u - z) * s): the weights transposed into the [K, N] layout of the
@@ -477,7 +511,7 @@ extern "C" __global__ void __launch_bounds__(256)
     // Thread: weight row tid / 4, 32 k at (tid % 4) * 32.
     const int r = tid >> 2, kk = (tid & 3) * 32;
     const long long n = n0 + r;
-    const uint4 q = n < p.N ? loadWeights<false>(p.w + n * p.ldw, (k0 + kk) >> 1, rowBytes, p.vec)
+    const uint4 q = n < p.N ? loadWeights(p.w + n * p.ldw, (k0 + kk) >> 1, rowBytes, p.vec)
                             : make_uint4(0, 0, 0, 0);
     const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll

@@ -14,7 +14,8 @@
 //
 // HBM bound (2 bytes read and 1 written per element), for one new token per sequence
 // latency bound.  A CTA owns one (sequence, block, head) of keys or of values: it reads
-// the new rows twice, the second time from L1, and nobody else writes its bytes.
+// the new rows once into registers (longer ones again from L1), and nobody else writes
+// its bytes.
 #include "kv_params.h"
 #include "serving_math.cuh"
 
@@ -32,26 +33,26 @@ struct AppendParams {
   int vec;     // 16-byte aligned rows of k and v
 };
 
-struct Eight {
-  float v[8];
+// Eight bf16 elements as they lie in memory.
+struct Raw {
+  uint32_t w[4] = {0, 0, 0, 0};
 };
 
-__device__ __forceinline__ Eight loadEight(const __nv_bfloat16 *p, int vec) {
-  Eight e;
+__device__ __forceinline__ Raw loadRaw(const __nv_bfloat16 *p, int vec) {
+  Raw x;
   if (vec) {
-    const uint4 r = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      e.v[2 * i] = __uint_as_float(w[i] << 16);
-      e.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    x.w[0] = v.x;
+    x.w[1] = v.y;
+    x.w[2] = v.z;
+    x.w[3] = v.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      e.v[i] = __bfloat162float(p[i]);
+    for (int i = 0; i < 4; ++i)
+      x.w[i] = uint32_t(__bfloat16_as_ushort(p[2 * i])) |
+               uint32_t(__bfloat16_as_ushort(p[2 * i + 1])) << 16;
   }
-  return e;
+  return x;
 }
 
 // Smallest power of two that is not below x (x >= 0, finite), as a float; 0 for 0.
@@ -91,17 +92,47 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   const bool held = lo > base;
   float old = held ? *scaleAt : 0.0f;
   old = old > 0.0f ? old : 0.0f;
+  // Pieces of 8 elements, thread by thread along the rows; (row, column) of a thread's
+  // next piece by addition.
   const int perRow = c.dim >> 3;
-  const int pieces = (hi - lo) * perRow;
-  float top = 0.0f;
-  for (int i = tid; i < pieces; i += threads) {
-    const int r = i / perRow, q = i - r * perRow;
-    const Eight e = loadEight(src + r * rowStride + q * 8, p.vec);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float a = fabsf(e.v[k]);
-      top = a < __int_as_float(0x7f800000) ? fmaxf(top, a) : top;
+  const int rows = hi - lo;
+  const int stepRow = threads / perRow, stepCol = threads - stepRow * perRow;
+  const int row0 = tid / perRow, col0 = tid - row0 * perRow;
+  auto advance = [&](int &r, int &q) {
+    r += stepRow;
+    q += stepCol;
+    if (q >= perRow) {
+      q -= perRow;
+      ++r;
     }
+  };
+  // The first pieces stay in registers between the passes (all of them for up to 32
+  // tokens of 128), the others are read again from L1.
+  constexpr int kHeld = 4;
+  Raw raw[kHeld];
+  float top = 0.0f;
+  auto magnitude = [&](const Raw &x) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // Finite bf16 magnitudes order like their bits; infinities and NaN count as 0.
+      const uint32_t w = x.w[k] & 0x7fff7fffu;
+      const uint32_t l = w << 16, h = w & 0xffff0000u;
+      top = fmaxf(top, l < 0x7f800000u ? __uint_as_float(l) : 0.0f);
+      top = fmaxf(top, h < 0x7f800000u ? __uint_as_float(h) : 0.0f);
+    }
+  };
+  int r = row0, q = col0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    raw[i] = r < rows ? loadRaw(src + r * rowStride + q * 8, p.vec) : Raw{};
+    advance(r, q);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    magnitude(raw[i]);
+  while (r < rows) {
+    magnitude(loadRaw(src + r * rowStride + q * 8, p.vec));
+    advance(r, q);
   }
   top = blockReduce<true>(top, scratch); // (a barrier: every thread has read the old scale)
   float need = __fmul_rn(top, 1.0f / Peak<Q>::value);
@@ -116,26 +147,50 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
     const int words = (lo - base) * (c.dim >> 2);
     const int wordsPerRow = c.dim >> 2;
     for (int i = tid; i < words; i += threads) {
-      const int r = i / wordsPerRow, w = i - r * wordsPerRow;
-      uint32_t *at = reinterpret_cast<uint32_t *>(dst + r * c.tokenStride) + w;
-      const uint32_t q = *at;
-      *at = quantise4<Q>(dequantise<Q>(q) * ratio, dequantise<Q>(q >> 8) * ratio,
-                         dequantise<Q>(q >> 16) * ratio, dequantise<Q>(q >> 24) * ratio);
+      const int row = i / wordsPerRow, w = i - row * wordsPerRow;
+      uint32_t *at = reinterpret_cast<uint32_t *>(dst + row * c.tokenStride) + w;
+      const uint32_t x = *at;
+      *at = quantise4<Q>(dequantise<Q>(x) * ratio, dequantise<Q>(x >> 8) * ratio,
+                         dequantise<Q>(x >> 16) * ratio, dequantise<Q>(x >> 24) * ratio);
     }
   }
-  // A power of two (every e4m3 scale this kernel makes) divides exactly by its inverse.
+  // A power of two (every e4m3 scale this kernel makes) divides exactly by its inverse;
+  // a scale of 0 leaves zeros (and NaN of what is not finite).
   const uint32_t bits = __float_as_uint(scale);
   const bool exact = (bits & 0x007fffffu) == 0 && bits >= 0x01000000u && bits < 0x7e000000u;
   const float inv = exact ? 1.0f / scale : 0.0f;
-  for (int i = tid; i < pieces; i += threads) {
-    const int r = i / perRow, q = i - r * perRow;
-    Eight e = loadEight(src + r * rowStride + q * 8, p.vec);
+  const bool product = exact || !(scale > 0.0f);
+  uint8_t *out = dst + (long long)(lo - base) * c.tokenStride;
+  auto store = [&](const Raw &x, int row, int col) {
+    float e[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      e.v[k] = exact || !(scale > 0.0f) ? e.v[k] * inv : __fdiv_rn(e.v[k], scale);
-    *reinterpret_cast<uint2 *>(dst + (long long)(lo - base + r) * c.tokenStride + q * 8) =
-        make_uint2(quantise4<Q>(e.v[0], e.v[1], e.v[2], e.v[3]),
-                   quantise4<Q>(e.v[4], e.v[5], e.v[6], e.v[7]));
+    for (int k = 0; k < 4; ++k) {
+      e[2 * k] = __uint_as_float(x.w[k] << 16);
+      e[2 * k + 1] = __uint_as_float(x.w[k] & 0xffff0000u);
+    }
+    if (product) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        e[k] *= inv;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        e[k] = __fdiv_rn(e[k], scale);
+    }
+    *reinterpret_cast<uint2 *>(out + row * c.tokenStride + col * 8) =
+        make_uint2(quantise4<Q>(e[0], e[1], e[2], e[3]), quantise4<Q>(e[4], e[5], e[6], e[7]));
+  };
+  r = row0;
+  q = col0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    if (r < rows)
+      store(raw[i], r, q);
+    advance(r, q);
+  }
+  while (r < rows) {
+    store(loadRaw(src + r * rowStride + q * 8, p.vec), r, q);
+    advance(r, q);
   }
 }
 

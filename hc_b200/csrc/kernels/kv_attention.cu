@@ -20,10 +20,11 @@
 //     conversion); q is brought into f16 range by a power of two per row, exact down to
 //     2^-14 of the row's largest element; the block's key scale multiplies the fp32
 //     scores; its value scale goes into the probabilities before they are rounded to
-//     f16: w = 2^15 * exp2(x - m) * vScale, where the running maximum m is that of
-//     x + log2(vScale), so w <= 2^15 whatever the scales are.  The sum of exp2(x - m),
-//     the maxima and the output are fp32; rounding w costs 2^-12 of a term (terms below
-//     2^-29 of the largest lose more, by at most 2^-40 of it).
+//     f16: w = 2^11 * exp2(x - m) * vScale, where m follows the running maximum of
+//     x + log2(vScale) and is at most 4 behind it, so w <= 2^15 whatever the scales are
+//     and the outputs are rescaled a few times per sequence only.  The sum of
+//     exp2(x - m), the maxima and the output are fp32; rounding w costs 2^-12 of a term
+//     (terms below 2^-25 of the largest lose more, by at most 2^-36 of it).
 //   * The tiles (128 tokens: 16 per warp of a CTA) of all (sequence, head, row tile)
 //     units stand in one line that is cut into equal shares, one per resident CTA, so a
 //     ragged batch is balanced and a single long sequence uses the whole GPU.  A unit
@@ -48,6 +49,8 @@ struct AttentionParams {
   int share;       // query heads per key/value head
   int window;      // 0: none
   int rowTiles;    // row tiles that maxNew * share rows can take
+  int sixteenths;  // block / 16, and ceil(2^32 / that) for more than one
+  uint32_t blockInverse;
   unsigned *counters; // [CTAs], zero between calls
   float *partial;     // [CTAs][2] slots
 };
@@ -55,6 +58,11 @@ struct AttentionParams {
 constexpr int kWarps = 8;
 constexpr int kTile = 16 * kWarps;
 constexpr float kNegInf = -INFINITY;
+// The reference that the exponentials are taken against follows the running maximum
+// only when that has grown by more than 2^kSlack: probabilities reach 2^kSlack, times
+// kWeight they fit f16.
+constexpr float kSlack = 4.0f;
+constexpr float kWeight = 2048.0f; // 2^(15 - kSlack)
 
 __device__ __forceinline__ void mmaF16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                        uint32_t b1) {
@@ -126,7 +134,9 @@ template <int DimCap, int NT> struct Shape {
   // at the end of a segment the warps' partial outputs [warps][rows][DimCap].)
 };
 
-template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(const AttentionParams &p) {
+// Whole: the head dimension is DimCap.
+template <class Q, int DimCap, int NT, bool Whole>
+__device__ __forceinline__ void attend(const AttentionParams &p) {
   using S = Shape<DimCap, NT>;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ long long sPrefix[kWarps * 32];
@@ -141,6 +151,9 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
   const HcKvCacheDev &c = p.cache;
   const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  // This lane's bytes within 16 tokens (a page spans less than 2^31 bytes).
+  const uint32_t kOffset = uint32_t(g) * uint32_t(c.tokenStride) + 16 * t;
+  const uint32_t vOffset = uint32_t(2 * t) * uint32_t(c.tokenStride) + S::valueBytes * g;
 
   // Tiles of one unit of a sequence, and its row tiles.
   auto tilesOf = [&](int seq, HcKvSpan &s, int &begin, int &rowTiles) -> int {
@@ -268,7 +281,6 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
     const int tile1 = int(min((long long)unitTiles, shareEnd - unitBegin));
     const int row0 = rowTile * S::rows;
     const int rowsHere = min(S::rows, span.count * p.share - row0);
-    const int kvEnd = span.first + span.count;
     const int *table = p.place.table + (long long)seq * p.place.tablePitch;
 
     // ---- query rows into shared memory as f16, a power of two per row ----------------
@@ -326,6 +338,10 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
     const int allLo = p.window > 0 ? max(0, lastPos - p.window + 1) : 0;
     const int anyLo = p.window > 0 ? max(0, firstPos - p.window + 1) : 0;
 
+    const uint8_t *kHead = static_cast<const uint8_t *>(c.k) + (long long)head * c.headStride;
+    const uint8_t *vHead = static_cast<const uint8_t *>(c.v) + (long long)head * c.headStride;
+    const float *kScales = c.kScale + head, *vScales = c.vScale + head;
+
     float o[S::mTiles][NT][4];
 #pragma unroll
     for (int i = 0; i < S::mTiles; ++i)
@@ -336,46 +352,54 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
           o[i][n][k] = 0.0f;
 
     // ---- the warp's 16 tokens of each tile -----------------------------------------------
+    auto posOf = [&](int tile) { return kvBegin + tile * kTile + warp * 16; };
+    // Blocks are multiples of 16 tokens: the quotient of two small numbers by a product.
+    auto blockOf = [&](int pos) {
+      return p.sixteenths == 1 ? pos >> 4
+                               : int(__umulhi(uint32_t(pos) >> 4, p.blockInverse));
+    };
     auto pageAt = [&](int tile) -> int {
-      const int pos = kvBegin + tile * kTile + warp * 16;
+      const int pos = posOf(tile);
       // Tokens that no row of this unit sees are passed over like missing pages.
       if (tile >= tile1 || pos > lastPos || pos + 15 < anyLo)
         return -1;
-      return hcKvPageOf(table[pos / c.block], c.pages);
+      return hcKvPageOf(__ldg(table + blockOf(pos)), c.pages);
     };
+    // All 16 rows lie inside the page, written or not: what is not visible is masked.
     uint4 kReg[2][S::keyPieces];
     uint32_t vReg[4][S::valuePieces][S::valueWords];
     float kScale = 0.0f, vScale = 0.0f;
     auto loadKeys = [&](int tile, int page) {
-      const int pos = kvBegin + tile * kTile + warp * 16;
-      const long long base = (long long)page * c.pageStride + (long long)head * c.headStride +
-                             (long long)(pos % c.block) * c.tokenStride;
-      const uint8_t *k = static_cast<const uint8_t *>(c.k) + base;
+      if (page < 0)
+        return;
+      const int pos = posOf(tile);
+      const uint8_t *k = kHead + (long long)page * c.pageStride +
+                         uint32_t(pos - blockOf(pos) * c.block) * uint32_t(c.tokenStride);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < S::keyPieces; ++j) {
-          const int tok = g + 8 * h, d = 64 * j + 16 * t;
-          kReg[h][j] = page >= 0 && pos + tok < kvEnd && d < c.dim
-                           ? loadStream16(k + tok * c.tokenStride + d)
+        for (int j = 0; j < S::keyPieces; ++j)
+          kReg[h][j] = Whole || 64 * j + 16 * t < c.dim
+                           ? loadStream16(k + (h ? kOffset + 8 * uint32_t(c.tokenStride) : kOffset) +
+                                          64 * j)
                            : make_uint4(0, 0, 0, 0);
-        }
-      if (page >= 0)
-        kScale = c.kScale[(long long)page * c.scalePitch + head];
+      kScale = __ldg(kScales + (long long)page * c.scalePitch);
     };
     auto loadValues = [&](int tile, int page) {
-      const int pos = kvBegin + tile * kTile + warp * 16;
-      const long long base = (long long)page * c.pageStride + (long long)head * c.headStride +
-                             (long long)(pos % c.block) * c.tokenStride;
-      const uint8_t *v = static_cast<const uint8_t *>(c.v) + base;
+      if (page < 0)
+        return;
+      const int pos = posOf(tile);
+      const uint8_t *v = vHead + (long long)page * c.pageStride +
+                         uint32_t(pos - blockOf(pos) * c.block) * uint32_t(c.tokenStride);
 #pragma unroll
       for (int h = 0; h < 4; ++h)
 #pragma unroll
         for (int j = 0; j < S::valuePieces; ++j) {
-          const int tok = 2 * t + (h & 1) + 8 * (h >> 1), d = 128 * j + S::valueBytes * g;
-          const bool in = page >= 0 && pos + tok < kvEnd && d < c.dim;
+          const uint8_t *at =
+              v + (vOffset + ((h & 1) + 8 * (h >> 1)) * uint32_t(c.tokenStride)) + 128 * j;
+          const bool in = Whole || 128 * j + S::valueBytes * g < c.dim;
           if constexpr (S::valueBytes == 16) {
-            const uint4 w = in ? loadStream16(v + tok * c.tokenStride + d) : make_uint4(0, 0, 0, 0);
+            const uint4 w = in ? loadStream16(at) : make_uint4(0, 0, 0, 0);
             vReg[h][j][0] = w.x;
             vReg[h][j][1] = w.y;
             vReg[h][j][2] = w.z;
@@ -385,20 +409,19 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
             if (in)
               asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
                            : "=r"(w.x), "=r"(w.y)
-                           : "l"(v + tok * c.tokenStride + d));
+                           : "l"(at));
             vReg[h][j][0] = w.x;
             vReg[h][j][1] = w.y;
           }
         }
-      if (page >= 0)
-        vScale = c.vScale[(long long)page * c.scalePitch + head];
+      vScale = __ldg(vScales + (long long)page * c.scalePitch);
     };
 
     int page = pageAt(tile0), nextPage = pageAt(tile0 + 1);
     loadKeys(tile0, page);
     loadValues(tile0, page);
     for (int tile = tile0; tile < tile1; ++tile) {
-      const int pos = kvBegin + tile * kTile + warp * 16;
+      const int pos = posOf(tile);
       const int afterPage = pageAt(tile + 2);
       const float sk = kScale, sv = vScale;
       float s[NT][4];
@@ -461,7 +484,7 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
             top[n][h] = v;
-            grows = grows || v > m[n][h];
+            grows = grows || v > m[n][h] + kSlack;
           }
         }
         if (__any_sync(0xffffffffu, grows)) {
@@ -491,7 +514,7 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
             const float ref = m[n][k & 1] == kNegInf ? 0.0f : m[n][k & 1];
             const float e = exp2Approx(s[n][k] - ref);
             l[n][k & 1] += e;
-            w[k] = whole || s[n][k] != kNegInf ? e * (sv * 32768.0f) : 0.0f;
+            w[k] = whole || s[n][k] != kNegInf ? e * (sv * kWeight) : 0.0f;
           }
           pb[n][0] = transpose8x8(halfPair(w[0], w[1]));
           pb[n][1] = transpose8x8(halfPair(w[2], w[3]));
@@ -634,12 +657,12 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
     const bool split = tile0 > 0 || tile1 < unitTiles;
     constexpr int kQuads = S::rows * DimCap / 4;
     auto finish = [&](int col, int d, float4 v, float top, float sum) {
-      // v: sum of 2^15 w V; sum: of exp2(x - top).
+      // v: sum of kWeight w V; sum: of exp2(x - top).
       const int r = row0 + col;
       const int qi = r / p.share, gh = r - qi * p.share;
       const long long token = span.row + qi;
       const int qHead = head * p.share + gh;
-      const float f = sum == 0.0f ? 0.0f : 1.0f / (32768.0f * sum);
+      const float f = sum == 0.0f ? 0.0f : 1.0f / (kWeight * sum);
       __nv_bfloat162 a = __floats2bfloat162_rn(v.x * f, v.y * f);
       __nv_bfloat162 b = __floats2bfloat162_rn(v.z * f, v.w * f);
       uint2 packed;
@@ -729,7 +752,12 @@ template <class Q, int DimCap, int NT> __device__ __forceinline__ void attend(co
 #define HC_ATTENTION(qname, Q, dim, nt, ctas)                                              \
   extern "C" __global__ void __launch_bounds__(256, ctas)                                   \
       hc_kv_attention_##qname##_d##dim##_r##nt(const __grid_constant__ AttentionParams p) { \
-    attend<Q, dim, nt>(p);                                                                  \
+    attend<Q, dim, nt, true>(p);                                                            \
+  }                                                                                         \
+  extern "C" __global__ void __launch_bounds__(256, ctas)                                   \
+      hc_kv_attention_##qname##_d##dim##_r##nt##_any(                                       \
+          const __grid_constant__ AttentionParams p) {                                      \
+    attend<Q, dim, nt, false>(p);                                                           \
   }
 #define HC_ATTENTION_DIMS(qname, Q)                                                        \
   HC_ATTENTION(qname, Q, 64, 1, 2)                                                          \

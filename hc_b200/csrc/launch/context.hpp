@@ -41,7 +41,6 @@ struct HcContextImpl {
   int pairSlotsF32 = 0; // the same for the float32 tensor-core kernel
   int pairSlotsBanded = 0; // the same for the dequant GEMM that converts band by band
   int pairSlotsW8 = 0;  // the same for the dequant GEMM that converts in its pipeline
-  long long w4Splits = 0;  // CTAs along K of the 4-bit products for few rows (0: chosen)
   long long w8Variant = 0; // 1: convert the weights in a pass of its own, 2: never
   // Programs without a precompiled body: 0 interpret them, 1 compile them at their
   // first launch and interpret where that is not possible, 2 fail where it is not.

@@ -479,11 +479,6 @@ int hcSetOption(HcContext c, const char *name, long long value) {
     c->w8Variant = value;
     return 0;
   }
-  if (std::strcmp(name, "w4_splits") == 0 &&
-      (value == 0 || value == 1 || value == 2 || value == 4 || value == 8)) {
-    c->w4Splits = value; // hcGemmW4, few rows: CTAs that share a tile's K (0: chosen)
-    return 0;
-  }
   if (std::strcmp(name, "conv_stacked") == 0 && value >= 0 && value <= 1) {
     c->convStacked = value; // 1: hcConvF32Tensor never stacks b_hi and b_lo into one MMA
     return 0;

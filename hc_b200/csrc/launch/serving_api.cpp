@@ -40,8 +40,8 @@ struct W4Params {
   long long lda, ldas, ldw, lds, ldz, ldc;
   int M, N, K, group, aGroup;
   int scaleF32;
-  int sliceK;
-  int stepK;
+  int warpsK;
+  int perWarp;
   int vec;
   int vecA;
 };
@@ -67,6 +67,8 @@ struct AttentionParams {
   int share;
   int window;
   int rowTiles;
+  int sixteenths;
+  uint32_t blockInverse;
   unsigned *counters;
   float *partial;
 };
@@ -80,8 +82,29 @@ static_assert(sizeof(HcKvPlace) == sizeof(HcKvPlaceDev) &&
 
 long long roundUp(long long a, long long b) { return ceilDiv(a, b) * b; }
 
-// Rows that the weight-streaming kernel of hcGemmW4 takes.
-constexpr long long kW4FewRows = 64;
+// The weight-streaming kernel of hcGemmW4 takes up to 8 activation rows that fit in
+// shared memory beside the scales of its 16 warps.
+constexpr long long kW4FewRows = 8;
+
+struct W4Few {
+  int warpsK, perWarp;
+  size_t smem;
+};
+W4Few w4Few(long long M, long long K, bool narrow, bool fine, long long group) {
+  const long long spans = ceilDiv(K, 128);
+  W4Few f{1, 0, 0};
+  while (f.warpsK < 16 && f.warpsK * 2 <= spans)
+    f.warpsK *= 2;
+  f.perWarp = int(ceilDiv(ceilDiv(spans, f.warpsK) * 128, group) + 1);
+  const long long piece = narrow ? 8 : 16;
+  f.smem = size_t(M * (spans * 16 * piece + 4 * piece) + spans * (fine ? 4 : 1) * 64 +
+                  16ll * f.perWarp * 128 + 2 * 16 * 512 + 256 + 16 * 4 * 1024 /* rings */);
+  return f;
+}
+bool w4TakesFew(long long M, long long K, bool narrow, bool fine, long long group) {
+  return M <= kW4FewRows && K <= (1 << 20) &&
+         w4Few(M, K, narrow, fine, group).smem <= 227 * 1024;
+}
 
 // Query rows (x head dimension) of a partial result in the attention's workspace, and
 // the CTAs per SM that can hold two of them each.
@@ -106,6 +129,9 @@ int checkKv(HcContext c, const char *who, const HcKvCache *cache, const HcKvPlac
       cache->tokenStride % 16 || cache->headStride % 16 || cache->pageStride % 16 ||
       !aligned(cache->k, 16) || !aligned(cache->v, 16))
     return c->fail("%s: the cache's rows must be 16-byte aligned", who);
+  if (cache->tokenStride > 0x7fffffffLL / cache->block)
+    return c->fail("%s: a page of %d tokens, %lld apart, spans 2^31 bytes or more", who,
+                   cache->block, cache->tokenStride);
   if (cache->scalePitch < cache->heads)
     return c->fail("%s: scale pitch %lld is below the %d heads", who, cache->scalePitch,
                    cache->heads);
@@ -136,14 +162,14 @@ const struct {
 } kFamilies[] = {
     // hc_add_rms_norm_{bf16,f32}_{same,i8,e4m3}_{t<threads>_v<packets>,generic}
     {"hc_add_rms_norm_", "add_rms_norm"},
-    // hc_gemm_w4_{bf16,i8}_{coarse,fine}_m{1,2,4,8}[_any]: activation type, groups that
-    // are multiples of 128 or not, eights of activation rows, weight rows that 16-byte
-    // loads do not tile; and the conversions
+    // hc_gemm_w4_{bf16,i8}_{coarse,fine}[_any]: activation type, groups that are
+    // multiples of 128 or not, weight rows that 16-byte loads do not tile; and the
+    // conversions
     {"hc_gemm_w4_", "gemm_w4"},
     {"hc_dequant_w4_", "gemm_w4"},
     {"hc_dequant_a8_", "gemm_w4"},
     {"hc_kv_append_", "kv_append"},       // _{i8,e4m3}
-    {"hc_kv_attention_", "kv_attention"}, // _{i8,e4m3}_d{64,128,256}_r{1,2}
+    {"hc_kv_attention_", "kv_attention"}, // _{i8,e4m3}_d{64,128,256}_r{1,2}[_any]
 };
 
 } // namespace
@@ -235,10 +261,8 @@ int hcAddRmsNorm(HcContext c, const void *x, const void *residual, void *summed,
   return c->launch(name, size_t(rows), 1, 1, size_t(threads), args, 1, 0);
 }
 
-long long hcGemmW4FewRows(void) { return kW4FewRows; }
-
 size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, int aDtype) {
-  if (M <= kW4FewRows || N <= 0 || K <= 0)
+  if (M <= 0 || N <= 0 || K <= 0 || w4TakesFew(M, K, aDtype == HC_I8, true, 32))
     return 0;
   const long long weights = roundUp(N, 16) * K * 2;
   return size_t(weights + (aDtype == HC_I8 ? M * roundUp(K, 8) * 2 : 0));
@@ -289,31 +313,17 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
   const bool narrow = aDtype == HC_I8;
   p.vecA = narrow ? lda % 8 == 0 && aligned(a, 8) : lda % 8 == 0 && aligned(a, 16);
   char name[64];
-  if (M <= kW4FewRows) {
-    const int nt = M <= 8 ? 1 : M <= 16 ? 2 : M <= 32 ? 4 : 8;
-    const long long tiles = ceilDiv(N, 128);
-    long long splits = c->w4Splits;
-    if (splits == 0) {
-      splits = 1;
-      while (splits < 8 && tiles * splits * 2 <= 4 * c->smCount && K > splits * 2 * 128)
-        splits *= 2;
-    }
-    p.sliceK = int(std::max<long long>(roundUp(ceilDiv(K, splits), 128), 128));
-    // A step of K in shared memory: 64 KiB of activations in fragment order at most.
-    const int spanBytes = nt * 4 * 32 * (narrow ? 8 : 16);
-    p.stepK = int(std::min<long long>(p.sliceK, 128ll * (64 * 1024 / spanBytes)));
-    // Groups of 32 bring 4 scales and zero points per 128 weights of each row.
-    p.stepK = int(std::min<long long>(p.stepK, std::max<long long>(128, 32 * group / 128 * 128)));
-    const size_t maxGroups = size_t(ceilDiv(p.stepK, group) + 1);
-    const size_t staged = size_t(p.stepK / 128) * spanBytes + maxGroups * 128 * 8 +
-                          maxGroups * 8 * nt * 8;
-    const size_t partial = splits > 1 ? size_t(128) * (8 * nt + 1) * 4 : 0;
-    std::snprintf(name, sizeof name, "hc_gemm_w4_%s_%s_m%d%s", narrow ? "i8" : "bf16",
-                  group % 128 == 0 || group >= K ? "coarse" : "fine", nt,
-                  p.vec && K % 32 == 0 ? "" : "_any");
+  const bool coarse = group % 128 == 0 || group >= K;
+  if (w4TakesFew(M, K, narrow, !coarse, group)) {
+    const W4Few f = w4Few(M, K, narrow, !coarse, group);
+    p.warpsK = f.warpsK;
+    p.perWarp = f.perWarp;
+    const long long teams = 16 / f.warpsK;
+    const long long ctas = std::min<long long>(c->smCount, ceilDiv(ceilDiv(N, 16), teams));
+    std::snprintf(name, sizeof name, "hc_gemm_w4_%s_%s%s", narrow ? "i8" : "bf16",
+                  coarse ? "coarse" : "fine", p.vec && K % 32 == 0 ? "" : "_any");
     void *args[] = {&p};
-    return c->launchCluster(name, size_t(tiles), size_t(splits), size_t(splits), 256, args,
-                            std::max(staged, partial));
+    return c->launch(name, size_t(ctas), 1, 1, 512, args, 1, f.smem);
   }
   const size_t need = hcGemmW4WorkspaceBytes(M, N, K, aDtype);
   if (K > 0 && (!workspace || workspaceBytes < need || !aligned(workspace, 16)))
@@ -419,6 +429,8 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   if (rowTiles * p.cache.heads > 0x7fffffffLL)
     return c->fail("hcKvAttention: too many query rows per sequence (%lld)", maxRows);
   p.rowTiles = int(rowTiles);
+  p.sixteenths = p.cache.block / 16;
+  p.blockInverse = p.sixteenths == 1 ? 0 : uint32_t((1ull << 32) / p.sixteenths + 1);
   const int perSm = cap == 64 || (cap == 128 && nt == 1) ? 2 : 1;
   const long long tiles = (long long)p.place.seqs * p.cache.heads * rowTiles *
                           (ceilDiv((long long)p.place.width * p.cache.block, 128) + 1);
@@ -427,8 +439,8 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   p.partial = reinterpret_cast<float *>(
       static_cast<char *>(workspace) + roundUp(c->smCount * kAttentionCtasPerSm * 4, 256));
   char name[64];
-  std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d",
-                p.cache.dtype == HC_I8 ? "i8" : "e4m3", cap, nt);
+  std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d%s",
+                p.cache.dtype == HC_I8 ? "i8" : "e4m3", cap, nt, p.cache.dim == cap ? "" : "_any");
   void *args[] = {&p};
   return c->launch(name, size_t(ctas), 1, 1, 256, args, 1, size_t(8) * 8 * nt * cap * 4);
 }

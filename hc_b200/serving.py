@@ -51,7 +51,7 @@ def add_rms_norm(x, gain, residual=None, *, eps=1e-5, out_dtype=None, group=0, o
     """
     native, ctx, stream = _launcher(x)
     if out is None:
-        out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        out = torch.empty_like(x, dtype=out_dtype)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"add_rms_norm: out is {out.dtype}, not {out_dtype}")
     if out.dtype == x.dtype:
@@ -59,9 +59,9 @@ def add_rms_norm(x, gain, residual=None, *, eps=1e-5, out_dtype=None, group=0, o
     elif scale is None:
         cols = x.shape[-1]
         groups = -(-cols // group) if 0 < group < cols else 1
-        scale = torch.empty((x.shape[0], groups), dtype=torch.float32, device=x.device)
+        scale = x.new_empty((x.shape[0], groups), dtype=torch.float32)
     if summed is None and residual is not None:
-        summed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        summed = torch.empty_like(x)
     native.add_rms_norm(ctx, x, gain, residual, summed, out, scale, group, eps, stream)
     return out, scale, summed
 
@@ -76,7 +76,7 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     :func:`add_rms_norm` returns them (``a_group``: its ``group``).  Returns
     ``out`` bfloat16 [M, N].
 
-    Up to 64 rows stream the weights as they are.  More rows convert them to
+    Up to 8 rows stream the weights as they are.  More rows convert them to
     bfloat16 first, into scratch memory taken from torch's allocator for the
     length of the call, and run the bf16 GEMM.
     """
@@ -84,11 +84,11 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     m, k = a.shape
     n = w.shape[0]
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+        out = a.new_empty((m, n), dtype=torch.bfloat16)
     workspace = None
-    if m > 64:
-        need = native.w4_workspace_bytes(m, n, k, a.dtype == torch.int8)
-        workspace = torch.empty(need, dtype=torch.uint8, device=a.device)
+    need = native.w4_workspace_bytes(m, n, k, a.dtype == torch.int8)
+    if need:
+        workspace = a.new_empty(need, dtype=torch.uint8)
     native.gemm_w4(ctx, a, w, scale, zero, out, group, a_scale, a_group, workspace, stream)
     return out
 
@@ -166,10 +166,10 @@ def kv_attention(cache, q, table, lengths, starts=None, *, max_new=None, scale=N
     """
     native, ctx, stream = _launcher(q)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q)
     lse = None
     if return_lse:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     native.kv_attention(ctx, cache._native, q, out, lse, table, lengths, starts,
                         -1 if max_new is None else max_new,
                         cache._root if scale is None else scale, window,

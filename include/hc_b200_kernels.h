@@ -125,8 +125,7 @@ HC_B200_API int hcSelfTestWaitTimeout(HcContext c, unsigned long long limitNs,
  * the workspace, 2 = inside the GEMM's pipeline (no workspace), 3 = inside the
  * GEMM kernel band by band into a ring of three bands (hcGemmW8A16BandedBytes of
  * workspace); 2 and 3 fail where the layout does not allow them, and all give
- * the same result bit for bit.  "w4_splits" (hcGemmW4 with few rows): 0 = the
- * library's choice, 1, 2, 4 or 8 CTAs share the K of a tile. */
+ * the same result bit for bit. */
 HC_B200_API int hcSetOption(HcContext c, const char *name, long long value);
 
 /* Run-time specialisation.  The reference compiles every kernel body at its
@@ -524,11 +523,12 @@ HC_B200_API int hcAddRmsNorm(HcContext c, const void *x, const void *residual, v
  * (z = 8 throughout).  `group` is a multiple of 32.  a is HC_BF16 (aScale null, as = 1)
  * or HC_I8 with float aScale [M, ceil(K/aGroup)], pitch ldas - what hcAddRmsNorm
  * writes; aGroup is 0 (one scale per row) or a multiple of `group`.  out is bf16.
- * Up to hcGemmW4FewRows() rows run on the kernel that streams the weights as they are
- * and need no workspace; more rows convert the weights to bf16 first (each rounded
- * once) and run hcGemmBf16: workspace of hcGemmW4WorkspaceBytes(M, N, K, aDtype)
- * bytes, 16-byte aligned, written by every call. */
-HC_B200_API long long hcGemmW4FewRows(void);
+ * Up to 8 rows that fit in shared memory (8 rows of K = 8192 in bf16 do) run on the
+ * kernel that streams the weights as they are and need no workspace; more rows convert
+ * the weights to bf16 first (each rounded once) and run hcGemmBf16.  workspace:
+ * hcGemmW4WorkspaceBytes(M, N, K, aDtype) bytes, 16-byte aligned, written by every call
+ * (null where that is 0).  With few rows a non-finite activation makes its row of the
+ * output NaN or infinite. */
 HC_B200_API size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, int aDtype);
 HC_B200_API int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w,
                          const void *scale, const void *zero, void *out, void *workspace,

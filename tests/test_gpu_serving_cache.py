@@ -10,8 +10,10 @@ probabilities round to f16 (2^-11 with the exponential's own 2^-21), and the
 output once to bf16 (2^-8):
     |out - o| <= 2^-8 |o| + (2^-11 + 2 * dE) * sum_j p_j |v_j|,
     dE = (dim / 16 + 4) * 2^-22 * scale * sum |q||k| at its largest + 2^-20.
-A probability below 2^-29 of the largest contribution may lose up to 2^-40 of
-it: (number of tokens) * 2^-40 * max |v| on top."""
+Probabilities are held as 2^11 p / (at most 2^4 times the largest so far) in
+f16, whose smallest step is 2^-24: one below 2^-25 of the largest contribution
+may lose up to half of that, 2^-36 of it: (number of tokens) * 2^-36 * max |v|
+on top."""
 
 import numpy as np
 import pytest
@@ -112,7 +114,7 @@ class Setup:
             most, _ = oracle.kv_attention((values[0], np.abs(values[1])), scales, *args)
         top = max(np.abs(values[0] * scales[0][:, :, None, None]).max(initial=0), 0)
         d_e = (self.dim / 16 + 4) * 2.0 ** -22 * scale * np.abs(q).max(initial=0) * top * self.dim
-        tail = max(self.lengths + [1]) * 2.0 ** -40 * np.abs(
+        tail = max(self.lengths + [1]) * 2.0 ** -36 * np.abs(
             values[1] * scales[1][:, :, None, None]).max(initial=0)
         got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
         room = 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2 * (d_e + 2.0 ** -20)) * most + tail
