@@ -48,7 +48,7 @@ KERNEL_SOURCES = [
     "gemm_w8a16_umma",
     "dequant_w8",
     "add_rms_norm",
-    "gemm_w4",
+    "gemm_w4", "gemm_w4_umma",
     "kv_append",
     "kv_attention",
     "selftest",

@@ -546,13 +546,22 @@ extern "C" __global__ void __launch_bounds__(256)
   }
 }
 
-// out[m, k] = bf16(a[m, k] * aScale[m, k / aGroup]), int8 activations.
+// Activations as bf16 rows that TMA can read: int8 ones, times their scales or (scaled
+// 0) as the integers they are; bf16 ones whose rows are not 16-byte aligned.
 extern "C" __global__ void __launch_bounds__(256)
-    hc_dequant_a8_bf16(const __grid_constant__ W4Params p, __nv_bfloat16 *out,
-                       long long outPitch) {
+    hc_repack_a8_bf16(const __grid_constant__ W4Params p, __nv_bfloat16 *out,
+                      long long outPitch, int scaled) {
   const long long m = blockIdx.x;
   const int8_t *a = static_cast<const int8_t *>(p.a) + m * p.lda;
   for (int k = int(blockIdx.y) * 256 + int(threadIdx.x); k < p.K; k += 256 * int(gridDim.y))
-    out[m * outPitch + k] =
-        __float2bfloat16_rn(float(a[k]) * p.aScale[m * p.ldas + k / p.aGroup]);
+    out[m * outPitch + k] = __float2bfloat16_rn(
+        scaled ? float(a[k]) * p.aScale[m * p.ldas + k / p.aGroup] : float(a[k]));
+}
+extern "C" __global__ void __launch_bounds__(256)
+    hc_repack_a16_bf16(const __grid_constant__ W4Params p, __nv_bfloat16 *out,
+                       long long outPitch, int) {
+  const long long m = blockIdx.x;
+  const __nv_bfloat16 *a = static_cast<const __nv_bfloat16 *>(p.a) + m * p.lda;
+  for (int k = int(blockIdx.y) * 256 + int(threadIdx.x); k < p.K; k += 256 * int(gridDim.y))
+    out[m * outPitch + k] = a[k];
 }

@@ -4,6 +4,8 @@
 
 #include "../kernels/kv_params.h"
 
+#include <cuda.h> // CUtensorMap (type only; no driver call is made here)
+
 #include <algorithm>
 #include <cmath>
 #include <cstddef>
@@ -46,6 +48,24 @@ struct W4Params {
   int vecA;
 };
 
+struct W4UmmaParams {
+  const void *scale;
+  const uint8_t *zero;
+  const float *rowScale;
+  void *out;
+  long long lds, ldz, rowScaleStride, ldc;
+  int M, N, K;
+  int group32;
+  uint32_t inverse;
+  int groups;
+  int cols;
+  int tilesM;
+  int stagesA, stagesB, stagesW;
+  int tmemCols;
+  int packed;
+  int *status;
+};
+
 struct AppendParams {
   HcKvCacheDev cache;
   HcKvPlaceDev place;
@@ -85,6 +105,21 @@ long long roundUp(long long a, long long b) { return ceilDiv(a, b) * b; }
 // The weight-streaming kernel of hcGemmW4 takes up to 8 activation rows that fit in
 // shared memory beside the scales of its 16 warps.
 constexpr long long kW4FewRows = 8;
+// Up to this many the weights are converted inside the tcgen05 kernel, for more by a pass
+// of their own in front of hcGemmBf16.
+constexpr long long kW4FusedRows = 1024;
+
+// The parts of hcGemmW4's workspace: the activations in bf16 (int8 ones, and bf16 ones
+// that TMA cannot describe), then the weights: converted, or packed ones that TMA cannot
+// describe copied to rows of 16 bytes.
+size_t w4RowBytes(long long M, long long K) {
+  return size_t(roundUp(M * roundUp(K, 8) * 2, 256));
+}
+size_t w4WeightBytes(long long M, long long N, long long K, bool tma) {
+  if (M > kW4FusedRows)
+    return size_t(roundUp(N, 16) * K * 2);
+  return tma ? 0 : size_t(N * roundUp(ceilDiv(K, 2), 16));
+}
 
 struct W4Few {
   int warpsK, perWarp;
@@ -165,9 +200,12 @@ const struct {
     // hc_gemm_w4_{bf16,i8}_{coarse,fine}[_any]: activation type, groups that are
     // multiples of 128 or not, weight rows that 16-byte loads do not tile; and the
     // conversions
+    // hc_gemm_w4_umma_{narrow,wide}_{coarse,fine}_{bf16,f32}: up to 64 activation rows per
+    // tile or up to 256, groups alike, type of the scales
+    {"hc_gemm_w4_umma_", "gemm_w4_umma"},
     {"hc_gemm_w4_", "gemm_w4"},
     {"hc_dequant_w4_", "gemm_w4"},
-    {"hc_dequant_a8_", "gemm_w4"},
+    {"hc_repack_", "gemm_w4"},
     {"hc_kv_append_", "kv_append"},       // _{i8,e4m3}
     {"hc_kv_attention_", "kv_attention"}, // _{i8,e4m3}_d{64,128,256}_r{1,2}[_any]
 };
@@ -261,11 +299,10 @@ int hcAddRmsNorm(HcContext c, const void *x, const void *residual, void *summed,
   return c->launch(name, size_t(rows), 1, 1, size_t(threads), args, 1, 0);
 }
 
-size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, int aDtype) {
+size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, long long ldw, int aDtype) {
   if (M <= 0 || N <= 0 || K <= 0 || w4TakesFew(M, K, aDtype == HC_I8, true, 32))
     return 0;
-  const long long weights = roundUp(N, 16) * K * 2;
-  return size_t(weights + (aDtype == HC_I8 ? M * roundUp(K, 8) * 2 : 0));
+  return w4RowBytes(M, K) + w4WeightBytes(M, N, K, ldw % 16 == 0);
 }
 
 int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, const void *scale,
@@ -325,31 +362,87 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
     void *args[] = {&p};
     return c->launch(name, size_t(ctas), 1, 1, 512, args, 1, f.smem);
   }
-  const size_t need = hcGemmW4WorkspaceBytes(M, N, K, aDtype);
-  if (K > 0 && (!workspace || workspaceBytes < need || !aligned(workspace, 16)))
-    return c->fail("hcGemmW4: %lld rows need a 16-byte aligned workspace of %zu bytes, got %zu",
+  if (c->ccMajor != 10)
+    return c->fail("hcGemmW4: more than a few rows need a device with tcgen05");
+  if (K == 0) // zeros
+    return hcGemmBf16(c, a, w, out, M, N, 0, lda, N, ldc);
+  const size_t rowBytes = w4RowBytes(M, K), need = rowBytes + w4WeightBytes(M, N, K, p.vec);
+  if (!workspace || workspaceBytes < need || !aligned(workspace, 256))
+    return c->fail("hcGemmW4: %lld rows need a 256-byte aligned workspace of %zu bytes, got %zu",
                    M, need, workspaceBytes);
+  // The activations as bf16 rows that TMA can read.  A single scale per int8 row stays
+  // out of them (the integers are exact in bf16) where the epilogue can apply it.
+  const bool fused = M <= kW4FusedRows;
+  const bool rowScaled = narrow && aGroup >= K && fused;
+  long long pitchA = lda;
+  if (narrow || lda % 8 || !aligned(a, 16)) {
+    void *rows = workspace;
+    pitchA = roundUp(K, 8);
+    int scaled = narrow && !rowScaled;
+    void *args[] = {&p, &rows, &pitchA, &scaled};
+    if (c->launch(narrow ? "hc_repack_a8_bf16" : "hc_repack_a16_bf16", size_t(M),
+                  size_t(std::min<long long>(ceilDiv(K, 256), 16)), 1, 256, args, 4, 0))
+      return 1;
+    a = rows;
+  }
+  void *const weights = static_cast<char *>(workspace) + rowBytes;
+  if (fused) {
+    if (!p.vec) {
+      const long long bytes = ceilDiv(K, 2);
+      if (hcCopy2D(c, w, weights, N, bytes, ldw, roundUp(bytes, 16), 1))
+        return 1;
+      w = weights;
+      ldw = roundUp(bytes, 16);
+    }
+    W4UmmaParams u{};
+    u.scale = scale, u.zero = p.zero, u.out = out;
+    u.rowScale = rowScaled ? aScale : nullptr;
+    u.rowScaleStride = ldas;
+    u.lds = lds, u.ldz = ldz, u.ldc = ldc;
+    u.M = p.M, u.N = p.N, u.K = p.K;
+    u.group32 = int(group / 32);
+    u.inverse = u.group32 == 1 ? 0 : uint32_t((1ull << 32) / unsigned(u.group32) + 1);
+    u.groups = int(groups);
+    u.packed = group == 32 && lds % 4 == 0 && aligned(scale, 8) &&
+               (!zero || (ldz % 4 == 0 && aligned(zero, 4)));
+    u.tilesM = int(ceilDiv(M, 256));
+    u.cols = int(roundUp(ceilDiv(M, u.tilesM), 16));
+    u.status = c->statusWord;
+    // Up to 64 columns: two CTAs per SM, half of the tensor memory each.
+    const bool two = u.cols <= 64;
+    u.tmemCols = two ? 256 : 512;
+    const long long stageBytes = (long long)u.cols * 256, wBytes = 16 * 1024;
+    u.stagesA = int(std::min(6ll, (u.tmemCols - roundUp(u.cols, 32)) / 64));
+    const long long room = (two ? 108ll : 224ll) * 1024;
+    u.stagesB = int(std::min(6ll, (room - 3 * wBytes) / stageBytes));
+    u.stagesW = int(std::min(6ll, (room - u.stagesB * stageBytes) / wBytes));
+    const long long tiles = ceilDiv(N, 128) * u.tilesM, pairs = ceilDiv(K, 256);
+    // CTAs that share a tile's K: as many as fit the GPU at once, 512 k each at least.
+    const long long slots = c->smCount * (two ? 2 : 1);
+    const long long splits = std::max<long long>(1, std::min({8ll, slots / tiles, pairs / 2}));
+    alignas(64) CUtensorMap mapB, mapW;
+    if (olxEncodeTensorMap2D(c->device, &mapB, /*bf16*/ 0, a, size_t(M), size_t(K),
+                             size_t(pitchA) * 2, unsigned(u.cols), 64, 128) ||
+        olxEncodeTensorMap2D(c->device, &mapW, /*bytes*/ 2, w, size_t(N), size_t(ceilDiv(K, 2)),
+                             size_t(ldw), 128, 128, 128))
+      return c->fail("tensor map encoding failed: %s", c->lastError.c_str());
+    std::snprintf(name, sizeof name, "hc_gemm_w4_umma_%s_%s_%s", two ? "narrow" : "wide",
+                  coarse ? "coarse" : "fine", p.scaleF32 ? "f32" : "bf16");
+    void *args[] = {&mapB, &mapW, &u};
+    return c->launchCluster(name, size_t(tiles), size_t(splits), size_t(splits), two ? 384 : 640,
+                            args,
+                            size_t(u.stagesB * stageBytes + u.stagesW * wBytes + 1024));
+  }
   const long long pitch = roundUp(N, 16);
-  void *weights = workspace;
-  if (K > 0) {
-    long long outPitch = pitch;
-    void *args[] = {&p, &weights, &outPitch};
-    if (ceilDiv(K, 128) > 65535)
-      return c->fail("hcGemmW4: K=%lld is too large for a conversion", K);
-    if (c->launch("hc_dequant_w4_bf16", size_t(ceilDiv(N, 64)), size_t(ceilDiv(K, 128)), 1, 256,
-                  args, 3, 0))
-      return 1;
-  }
-  if (narrow && K > 0) {
-    void *rows = static_cast<char *>(workspace) + pitch * K * 2;
-    long long outPitch = roundUp(K, 8);
-    void *args[] = {&p, &rows, &outPitch};
-    if (c->launch("hc_dequant_a8_bf16", size_t(M), size_t(std::min<long long>(ceilDiv(K, 256), 16)),
-                  1, 256, args, 3, 0))
-      return 1;
-    return hcGemmBf16(c, rows, weights, out, M, N, K, outPitch, pitch, ldc);
-  }
-  return hcGemmBf16(c, a, weights, out, M, N, K, lda, pitch, ldc);
+  long long outPitch = pitch;
+  void *converted = weights;
+  void *args[] = {&p, &converted, &outPitch};
+  if (ceilDiv(K, 128) > 65535)
+    return c->fail("hcGemmW4: K=%lld is too large for a conversion", K);
+  if (c->launch("hc_dequant_w4_bf16", size_t(ceilDiv(N, 64)), size_t(ceilDiv(K, 128)), 1, 256,
+                args, 3, 0))
+    return 1;
+  return hcGemmBf16(c, a, weights, out, M, N, K, pitchA, pitch, ldc);
 }
 
 int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place, const void *k,

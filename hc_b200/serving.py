@@ -76,9 +76,9 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     :func:`add_rms_norm` returns them (``a_group``: its ``group``).  Returns
     ``out`` bfloat16 [M, N].
 
-    Up to 8 rows stream the weights as they are.  More rows convert them to
-    bfloat16 first, into scratch memory taken from torch's allocator for the
-    length of the call, and run the bf16 GEMM.
+    Up to 8 rows stream the weights as they are; more rows run on the tensor
+    cores with the weights rounded to bfloat16.  Scratch memory is taken from
+    torch's allocator for the length of the call.
     """
     native, ctx, stream = _launcher(a)
     m, k = a.shape
@@ -86,7 +86,8 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     if out is None:
         out = a.new_empty((m, n), dtype=torch.bfloat16)
     workspace = None
-    need = native.w4_workspace_bytes(m, n, k, a.dtype == torch.int8)
+    need = native.w4_workspace_bytes(m, n, k, 1 if w.data_ptr() % 16 else w.stride(0),
+                                     a.dtype == torch.int8)
     if need:
         workspace = a.new_empty(need, dtype=torch.uint8)
     native.gemm_w4(ctx, a, w, scale, zero, out, group, a_scale, a_group, workspace, stream)

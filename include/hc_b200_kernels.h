@@ -524,12 +524,14 @@ HC_B200_API int hcAddRmsNorm(HcContext c, const void *x, const void *residual, v
  * or HC_I8 with float aScale [M, ceil(K/aGroup)], pitch ldas - what hcAddRmsNorm
  * writes; aGroup is 0 (one scale per row) or a multiple of `group`.  out is bf16.
  * Up to 8 rows that fit in shared memory (8 rows of K = 8192 in bf16 do) run on the
- * kernel that streams the weights as they are and need no workspace; more rows convert
- * the weights to bf16 first (each rounded once) and run hcGemmBf16.  workspace:
- * hcGemmW4WorkspaceBytes(M, N, K, aDtype) bytes, 16-byte aligned, written by every call
- * (null where that is 0).  With few rows a non-finite activation makes its row of the
+ * kernel that streams the weights as they are and need no workspace.  More rows run on
+ * the tensor cores (tcgen05) with the weights rounded to bf16, once each: converted
+ * inside that kernel up to 1024 rows, by a pass of their own for more.  workspace:
+ * hcGemmW4WorkspaceBytes(M, N, K, ldw, aDtype) bytes, 256-byte aligned, written by the
+ * call (null where that is 0); w that is not 16-byte aligned counts as an odd ldw.  With few rows a non-finite activation makes its row of the
  * output NaN or infinite. */
-HC_B200_API size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, int aDtype);
+HC_B200_API size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, long long ldw,
+                                          int aDtype);
 HC_B200_API int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w,
                          const void *scale, const void *zero, void *out, void *workspace,
                          size_t workspaceBytes, long long M, long long N, long long K,

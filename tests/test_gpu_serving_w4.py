@@ -73,7 +73,8 @@ def _check(c, out, a_group=0):
 
 SHAPES = [(1, 16, 128), (1, 128, 128), (1, 4096, 4096), (2, 130, 256), (5, 1000, 8160),
           (8, 64, 1024), (9, 333, 640), (16, 256, 4096), (17, 500, 1152), (32, 1024, 2048),
-          (33, 200, 512), (64, 384, 8192), (65, 384, 1024), (130, 300, 1088), (300, 520, 256)]
+          (33, 200, 512), (64, 384, 8192), (65, 384, 1024), (130, 300, 1088), (300, 520, 256), (256, 384, 2048),
+          (250, 130, 4224), (48, 1030, 4096), (1100, 200, 512)]
 
 
 @pytest.mark.parametrize("a8", [False, True])
