@@ -13,7 +13,8 @@
 //     operand.  u becomes 128 + u in bf16 by a shift, a mask and a bias; subtracting
 //     128 + z is exact, multiplying by the scale rounds once (bf16, half a step of 2^-8:
 //     accumulating in tensor memory leaves no place for a scale per group), and a byte
-//     permute puts neighbours in K side by side: 19 instructions for 8 weights.
+//     permute puts neighbours in K side by side: 19 instructions for 8 weights, which is
+//     what bounds few columns.
 //   * The activations (bf16, K-major) come by TMA into 128-byte-swizzled stages.
 //   * Warps 0 and 2 issue the copies, warp 1 the MMAs, the others convert stages
 //     in turn and drain the accumulator.  Few columns: two CTAs per SM of 256 tensor memory
@@ -76,21 +77,6 @@ __device__ __forceinline__ void ummaBf16TmemA(uint32_t dTmem, uint32_t aTmem, ui
                : "memory");
 }
 
-// 32 lanes x 32 columns: thread i writes columns [col, col + 32) of lane laneBase + i.
-__device__ __forceinline__ void tmemStore32x32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
-          taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-      "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-
 // 32 lanes x 16 columns.
 __device__ __forceinline__ void tmemLoad32x16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -109,14 +95,35 @@ __device__ __forceinline__ uint32_t asWord(__nv_bfloat162 v) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Eight weights -> four bf16 pairs in the order of K.
+// A stage of a ring and the parity of its barriers' phase, counted along: dividing the
+// use's number by the ring's length took half of a converter's instructions.
+struct RingAt {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void step(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// (v & mask) | bias in one instruction: an immediate may stand in one place only, so the
+// bias comes as a value that the compiler does not see through.
+__device__ __forceinline__ uint32_t maskBias(uint32_t v, uint32_t bias) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(r) : "r"(v), "r"(bias));
+  return r;
+}
+
+// Eight weights -> four bf16 pairs in the order of K.  one28: the pair 128, 128.
 template <bool ScaleF32>
-__device__ __forceinline__ void convert(uint32_t w, uint32_t bias, uint32_t scale,
+__device__ __forceinline__ void convert(uint32_t w, uint32_t one28, uint32_t bias, uint32_t scale,
                                         uint32_t *out) {
   uint32_t d[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t t = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const uint32_t t = maskBias(w >> (4 * i), one28);
     const __nv_bfloat162 x = __hsub2(asPair(t), asPair(bias));
     if constexpr (ScaleF32) {
       const float s = __uint_as_float(scale);
@@ -181,9 +188,12 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
   const int kb0 = 2 * int((long long)split * pairs / splits);
   const int blocks = 2 * int((long long)(split + 1) * pairs / splits) - kb0;
 
-  // Waits for use i of a ring's stage to be free.
-  auto freeOf = [&](uint64_t *bar, int i, int stages, int code) {
-    return mbarWait(smemAddr(&bar[i % stages]), ((i / stages) & 1) ^ 1, abortFlag, status, code);
+  // Waits for a ring's stage to be free, or filled.
+  auto freeOf = [&](uint64_t *bar, const RingAt &at, int code) {
+    return mbarWait(smemAddr(&bar[at.stage]), at.parity ^ 1, abortFlag, status, code);
+  };
+  auto filled = [&](uint64_t *bar, const RingAt &at, int code) {
+    return mbarWait(smemAddr(&bar[at.stage]), at.parity, abortFlag, status, code);
   };
   auto settle = [&]() { // after a wait gave up: copies may still be landing
     if (*abortFlag) {
@@ -196,10 +206,11 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
   if (warp == 0) {
     // --------------------------- activations by TMA ---------------------------
     if (lane == 0) {
-      for (int i = 0; i < blocks; ++i) {
-        if (!freeOf(bars.emptyB, i, p.stagesB, kStatusProducerWait))
+      RingAt ring;
+      for (int i = 0; i < blocks; ++i, ring.step(p.stagesB)) {
+        if (!freeOf(bars.emptyB, ring, kStatusProducerWait))
           break;
-        const int s = i % p.stagesB;
+        const int s = ring.stage;
         const uint32_t full = smemAddr(&bars.fullB[s]), at = smemBase + s * stageBytes;
         mbarExpectTx(full, stageBytes);
         tmaLoad2D(at, mapB, full, (kb0 + i) * kBK, m0);
@@ -210,10 +221,11 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
   } else if (warp == 2) {
     // ----------------------------- weights by TMA ------------------------------
     if (lane == 0) {
-      for (int i = 0; i < blocks / 2; ++i) {
-        if (!freeOf(bars.emptyW, i, p.stagesW, kStatusProducerWait))
+      RingAt ring;
+      for (int i = 0; i < blocks / 2; ++i, ring.step(p.stagesW)) {
+        if (!freeOf(bars.emptyW, ring, kStatusProducerWait))
           break;
-        const int s = i % p.stagesW;
+        const int s = ring.stage;
         const uint32_t full = smemAddr(&bars.fullW[s]);
         mbarExpectTx(full, kWBytes);
         tmaLoad2D(smemBase + wBase + s * kWBytes, mapW, full, (kb0 / 2 + i) * 128, n0);
@@ -225,12 +237,11 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
     if (lane == 0) {
       const uint32_t iDesc = makeInstrDescBf16(128, p.cols, false, false);
       bool ok = true;
-      for (int i = 0; i < blocks && ok; ++i) {
-        const int sa = i % p.stagesA, sb = i % p.stagesB;
-        ok = mbarWait(smemAddr(&bars.fullB[sb]), (i / p.stagesB) & 1, abortFlag, status,
-                      kStatusMmaWaitData) &&
-             mbarWait(smemAddr(&bars.fullA[sa]), (i / p.stagesA) & 1, abortFlag, status,
-                      kStatusMmaWaitData);
+      RingAt ringA, ringB;
+      for (int i = 0; i < blocks; ++i, ringA.step(p.stagesA), ringB.step(p.stagesB)) {
+        const int sa = ringA.stage, sb = ringB.stage;
+        ok = filled(bars.fullB, ringB, kStatusMmaWaitData) &&
+             filled(bars.fullA, ringA, kStatusMmaWaitData);
         if (!ok)
           break;
         tcgen05FenceAfter();
@@ -294,11 +305,16 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
     bool ok = true;
     if (grp < blocks)
       loadScales(grp);
-    for (int i = grp; i < blocks; i += 2) {
-      const int sw = (i >> 1) % p.stagesW, sa = i % p.stagesA;
+    uint32_t one28;
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(one28));
+    RingAt ringW, ringA;
+    if (grp)
+      ringA.step(p.stagesA);
+    for (int i = grp; i < blocks;
+         i += 2, ringW.step(p.stagesW), ringA.step(p.stagesA), ringA.step(p.stagesA)) {
+      const int sw = ringW.stage, sa = ringA.stage;
       if (lane == 0)
-        ok = mbarWait(smemAddr(&bars.fullW[sw]), ((i >> 1) / p.stagesW) & 1, abortFlag, status,
-                      kStatusConvertWait);
+        ok = filled(bars.fullW, ringW, kStatusConvertWait);
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok)
         break;
@@ -330,20 +346,20 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
       if (i + 2 < blocks)
         loadScales(i + 2);
       if (lane == 0)
-        ok = freeOf(bars.emptyA, i, p.stagesA, kStatusConvertWait);
+        ok = freeOf(bars.emptyA, ringA, kStatusConvertWait);
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok)
         break;
       tcgen05FenceAfter(); // the MMAs that read this stage are complete
 #pragma unroll
-      for (int h = 0; h < 2 / Halves; ++h) {
-        uint32_t v[32];
+      for (int c = 0; c < 16 / Halves; c += 2) {
+        uint32_t v[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int j = Fine ? (Halves == 1 ? h * 2 : 0) + (c >> 2) : 0;
-          convert<ScaleF32>(w[h * 8 + c], bias[j], factor[j], v + 4 * c);
+        for (int d = 0; d < 2; ++d) {
+          const int j = Fine ? (c + d) >> 2 : 0;
+          convert<ScaleF32>(w[c + d], one28, bias[j], factor[j], v + 4 * d);
         }
-        tmemStore32x32(aBase + laneBase + uint32_t(sa * 64 + (firstHalf + h) * 32), v);
+        tmemStore32x8(aBase + laneBase + uint32_t(sa * 64 + firstHalf * 32 + c * 4), v);
       }
       tmemStoreWait();
       tcgen05FenceBefore();

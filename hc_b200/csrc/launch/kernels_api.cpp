@@ -479,6 +479,12 @@ int hcSetOption(HcContext c, const char *name, long long value) {
     c->w8Variant = value;
     return 0;
   }
+  if (std::strcmp(name, "w4_variant") == 0 && value >= 0 && value <= 2) {
+    // hcGemmW4: 1 = the kernel that streams the weights for up to 8 rows (fails for
+    // more), 2 = the tcgen05 kernels whatever the rows, 0 = by size.
+    c->w4Variant = value;
+    return 0;
+  }
   if (std::strcmp(name, "conv_stacked") == 0 && value >= 0 && value <= 1) {
     c->convStacked = value; // 1: hcConvF32Tensor never stacks b_hi and b_lo into one MMA
     return 0;

@@ -112,8 +112,8 @@ constexpr long long kW4FusedRows = 1024;
 // The parts of hcGemmW4's workspace: the activations in bf16 (int8 ones, and bf16 ones
 // that TMA cannot describe), then the weights: converted, or packed ones that TMA cannot
 // describe copied to rows of 16 bytes.
-size_t w4RowBytes(long long M, long long K) {
-  return size_t(roundUp(M * roundUp(K, 8) * 2, 256));
+size_t w4RowBytes(long long M, long long K, bool tma) {
+  return tma ? 0 : size_t(roundUp(M * roundUp(K, 8) * 2, 256));
 }
 size_t w4WeightBytes(long long M, long long N, long long K, bool tma) {
   if (M > kW4FusedRows)
@@ -136,10 +136,11 @@ W4Few w4Few(long long M, long long K, bool narrow, bool fine, long long group) {
                   16ll * f.perWarp * 128 + 2 * 16 * 512 + 256 + 16 * 4 * 1024 /* rings */);
   return f;
 }
-bool w4TakesFew(long long M, long long K, bool narrow, bool fine, long long group) {
+bool w4FitsFew(long long M, long long K, bool narrow, bool fine, long long group) {
   return M <= kW4FewRows && K <= (1 << 20) &&
          w4Few(M, K, narrow, fine, group).smem <= 227 * 1024;
 }
+
 
 // Query rows (x head dimension) of a partial result in the attention's workspace, and
 // the CTAs per SM that can hold two of them each.
@@ -299,10 +300,11 @@ int hcAddRmsNorm(HcContext c, const void *x, const void *residual, void *summed,
   return c->launch(name, size_t(rows), 1, 1, size_t(threads), args, 1, 0);
 }
 
-size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, long long ldw, int aDtype) {
-  if (M <= 0 || N <= 0 || K <= 0 || w4TakesFew(M, K, aDtype == HC_I8, true, 32))
+size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, long long lda,
+                              long long ldw, int aDtype) {
+  if (M <= 0 || N <= 0 || K <= 0)
     return 0;
-  return w4RowBytes(M, K) + w4WeightBytes(M, N, K, ldw % 16 == 0);
+  return w4RowBytes(M, K, aDtype != HC_I8 && lda % 8 == 0) + w4WeightBytes(M, N, K, ldw % 16 == 0);
 }
 
 int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, const void *scale,
@@ -351,7 +353,12 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
   p.vecA = narrow ? lda % 8 == 0 && aligned(a, 8) : lda % 8 == 0 && aligned(a, 16);
   char name[64];
   const bool coarse = group % 128 == 0 || group >= K;
-  if (w4TakesFew(M, K, narrow, !coarse, group)) {
+  const bool few = c->w4Variant != 2 && w4FitsFew(M, K, narrow, !coarse, group);
+  if (c->w4Variant == 1 && !few)
+    return c->fail("hcGemmW4: %lld rows of %lld do not fit the kernel for few rows", M, K);
+  if (K == 0) // zeros
+    return hcGemmBf16(c, a, w, out, M, N, 0, lda, N, ldc);
+  if (few) {
     const W4Few f = w4Few(M, K, narrow, !coarse, group);
     p.warpsK = f.warpsK;
     p.perWarp = f.perWarp;
@@ -363,11 +370,11 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
     return c->launch(name, size_t(ctas), 1, 1, 512, args, 1, f.smem);
   }
   if (c->ccMajor != 10)
-    return c->fail("hcGemmW4: more than a few rows need a device with tcgen05");
-  if (K == 0) // zeros
-    return hcGemmBf16(c, a, w, out, M, N, 0, lda, N, ldc);
-  const size_t rowBytes = w4RowBytes(M, K), need = rowBytes + w4WeightBytes(M, N, K, p.vec);
-  if (!workspace || workspaceBytes < need || !aligned(workspace, 256))
+    return c->fail("hcGemmW4: this form needs a device with tcgen05");
+  const bool tmaRows = !narrow && lda % 8 == 0 && aligned(a, 16);
+  const size_t rowBytes = w4RowBytes(M, K, tmaRows);
+  const size_t need = rowBytes + w4WeightBytes(M, N, K, p.vec);
+  if (need && (!workspace || workspaceBytes < need || !aligned(workspace, 256)))
     return c->fail("hcGemmW4: %lld rows need a 256-byte aligned workspace of %zu bytes, got %zu",
                    M, need, workspaceBytes);
   // The activations as bf16 rows that TMA can read.  A single scale per int8 row stays
@@ -375,7 +382,7 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
   const bool fused = M <= kW4FusedRows;
   const bool rowScaled = narrow && aGroup >= K && fused;
   long long pitchA = lda;
-  if (narrow || lda % 8 || !aligned(a, 16)) {
+  if (!tmaRows) {
     void *rows = workspace;
     pitchA = roundUp(K, 8);
     int scaled = narrow && !rowScaled;

@@ -86,7 +86,8 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     if out is None:
         out = a.new_empty((m, n), dtype=torch.bfloat16)
     workspace = None
-    need = native.w4_workspace_bytes(m, n, k, 1 if w.data_ptr() % 16 else w.stride(0),
+    need = native.w4_workspace_bytes(m, n, k, 1 if a.data_ptr() % 16 else a.stride(0),
+                                     1 if w.data_ptr() % 16 else w.stride(0),
                                      a.dtype == torch.int8)
     if need:
         workspace = a.new_empty(need, dtype=torch.uint8)
