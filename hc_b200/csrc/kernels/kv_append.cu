@@ -13,9 +13,10 @@
 // bytes are determined by the inputs alone.
 //
 // HBM bound (2 bytes read and 1 written per element), for one new token per sequence
-// latency bound.  A CTA owns one (sequence, block, head) of keys or of values: it reads
-// the new rows once into registers (longer ones again from L1), and nobody else writes
-// its bytes.
+// latency bound.  A warp owns one (sequence, block, head) of keys or of values: it reads
+// the new rows once into registers (what does not fit there again from L1), reduces by
+// shuffles alone, and nobody else writes its bytes.  (A CTA per unit spent two thirds of
+// its instructions on setting up: 41 us instead of 26 for 16 prompts of 2048 tokens.)
 #include "kv_params.h"
 #include "serving_math.cuh"
 
@@ -65,12 +66,17 @@ __device__ __forceinline__ float powerAbove(float x) {
   return __uint_as_float((bits + 0x007fffffu) & 0x7f800000u);
 }
 
+constexpr int kWarps = 4;
+constexpr int kHeld = 16; // pieces of 8 elements per lane in registers
+
 template <class Q> __device__ __forceinline__ void appendBlock(const AppendParams &p) {
-  __shared__ float scratch[4];
   const HcKvCacheDev &c = p.cache;
-  const int seq = int(blockIdx.x) / p.touched, nth = int(blockIdx.x) % p.touched;
-  const int head = int(blockIdx.y), values = int(blockIdx.z);
-  const int tid = int(threadIdx.x), threads = int(blockDim.x);
+  const int seq = int(blockIdx.x) / p.touched, nth = int(blockIdx.x) - seq * p.touched;
+  const int lane = int(threadIdx.x) & 31;
+  const int unit = int(blockIdx.y) * kWarps + (int(threadIdx.x) >> 5);
+  if (unit >= 2 * c.heads)
+    return;
+  const int head = unit >> 1, values = unit & 1;
 
   const HcKvSpan s = hcKvLoadSpan(p.place, c.block, seq);
   const int b = s.first / c.block + nth;
@@ -83,8 +89,7 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
     return;
   uint8_t *dst = static_cast<uint8_t *>(values ? c.v : c.k) + (long long)page * c.pageStride +
                  (long long)head * c.headStride;
-  float *scaleAt =
-      (values ? c.vScale : c.kScale) + (long long)page * c.scalePitch + head;
+  float *scaleAt = (values ? c.vScale : c.kScale) + (long long)page * c.scalePitch + head;
   const long long rowStride = values ? p.tokenStrideV : p.tokenStride;
   const __nv_bfloat16 *src = (values ? p.v : p.k) + (long long)(s.row + lo - s.first) * rowStride +
                              (long long)head * (values ? p.headStrideV : p.headStride);
@@ -92,66 +97,80 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   const bool held = lo > base;
   float old = held ? *scaleAt : 0.0f;
   old = old > 0.0f ? old : 0.0f;
-  // Pieces of 8 elements, thread by thread along the rows; (row, column) of a thread's
-  // next piece by addition.
-  const int perRow = c.dim >> 3;
-  const int rows = hi - lo;
-  const int stepRow = threads / perRow, stepCol = threads - stepRow * perRow;
-  const int row0 = tid / perRow, col0 = tid - row0 * perRow;
-  auto advance = [&](int &r, int &q) {
-    r += stepRow;
-    q += stepCol;
-    if (q >= perRow) {
-      q -= perRow;
-      ++r;
+  // Pieces of 8 elements, lane by lane along the rows; a lane's next piece by addition.
+  const int perRow = c.dim >> 3, rows = hi - lo;
+  const int stepRow = 32 / perRow, stepCol = 32 - stepRow * perRow;
+  struct At {
+    int row, col;
+  };
+  const At first{lane / perRow, lane - lane / perRow * perRow};
+  auto advance = [&](At &at) {
+    at.row += stepRow;
+    at.col += stepCol;
+    if (at.col >= perRow) {
+      at.col -= perRow;
+      ++at.row;
     }
   };
-  // The first pieces stay in registers between the passes (all of them for up to 32
-  // tokens of 128), the others are read again from L1.
-  constexpr int kHeld = 4;
+  auto fetch = [&](const At &at) { return loadRaw(src + at.row * rowStride + at.col * 8, p.vec); };
+
   Raw raw[kHeld];
-  float top = 0.0f;
+  uint32_t top2 = 0; // magnitudes, as bits: they order like unsigned numbers
   auto magnitude = [&](const Raw &x) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      // Finite bf16 magnitudes order like their bits; infinities and NaN count as 0.
-      const uint32_t w = x.w[k] & 0x7fff7fffu;
-      const uint32_t l = w << 16, h = w & 0xffff0000u;
-      top = fmaxf(top, l < 0x7f800000u ? __uint_as_float(l) : 0.0f);
-      top = fmaxf(top, h < 0x7f800000u ? __uint_as_float(h) : 0.0f);
-    }
+    for (int k = 0; k < 4; ++k)
+      top2 = __vmaxu2(top2, x.w[k] & 0x7fff7fffu);
   };
-  int r = row0, q = col0;
+  // (One token is one turn: leaving early keeps the code that runs short, and at one
+  // token per sequence fetching instructions is what takes the time.)
+  const int turns = (rows * perRow + 31) >> 5;
+  At at = first;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
-    raw[i] = r < rows ? loadRaw(src + r * rowStride + q * 8, p.vec) : Raw{};
-    advance(r, q);
+    if (i >= turns)
+      break;
+    raw[i] = at.row < rows ? fetch(at) : Raw{};
+    advance(at);
   }
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i)
+  for (int i = 0; i < kHeld; ++i) {
+    if (i >= turns)
+      break;
     magnitude(raw[i]);
-  while (r < rows) {
-    magnitude(loadRaw(src + r * rowStride + q * 8, p.vec));
-    advance(r, q);
   }
-  top = blockReduce<true>(top, scratch); // (a barrier: every thread has read the old scale)
-  float need = __fmul_rn(top, 1.0f / Peak<Q>::value);
+  for (; at.row < rows; advance(at))
+    magnitude(fetch(at));
+  uint32_t top16 = max(top2 & 0xffffu, top2 >> 16);
+  top16 = __reduce_max_sync(0xffffffffu, top16);
+  if (top16 >= 0x7f80u) { // something is not finite: the largest of the others
+    uint32_t best = 0;
+    for (at = first; at.row < rows; advance(at)) {
+      const Raw x = fetch(at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t m = (x.w[k >> 1] >> (16 * (k & 1))) & 0x7fffu;
+        best = m < 0x7f80u ? max(best, m) : best;
+      }
+    }
+    top16 = __reduce_max_sync(0xffffffffu, best);
+  }
+  float need = __fmul_rn(__uint_as_float(top16 << 16), 1.0f / Peak<Q>::value);
   if constexpr (__is_same(Q, E4M3))
     need = powerAbove(need);
   const float scale = fmaxf(old, need);
-  if (tid == 0)
+  __syncwarp(); // every lane has read the old scale
+  if (lane == 0)
     *scaleAt = scale;
 
   if (held && scale > old) {
     const float ratio = __fdiv_rn(old, scale);
-    const int words = (lo - base) * (c.dim >> 2);
-    const int wordsPerRow = c.dim >> 2;
-    for (int i = tid; i < words; i += threads) {
+    const int wordsPerRow = c.dim >> 2, words = (lo - base) * wordsPerRow;
+    for (int i = lane; i < words; i += 32) {
       const int row = i / wordsPerRow, w = i - row * wordsPerRow;
-      uint32_t *at = reinterpret_cast<uint32_t *>(dst + row * c.tokenStride) + w;
-      const uint32_t x = *at;
-      *at = quantise4<Q>(dequantise<Q>(x) * ratio, dequantise<Q>(x >> 8) * ratio,
-                         dequantise<Q>(x >> 16) * ratio, dequantise<Q>(x >> 24) * ratio);
+      uint32_t *word = reinterpret_cast<uint32_t *>(dst + row * c.tokenStride) + w;
+      const uint32_t x = *word;
+      *word = quantise4<Q>(dequantise<Q>(x) * ratio, dequantise<Q>(x >> 8) * ratio,
+                           dequantise<Q>(x >> 16) * ratio, dequantise<Q>(x >> 24) * ratio);
     }
   }
   // A power of two (every e4m3 scale this kernel makes) divides exactly by its inverse;
@@ -161,7 +180,7 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   const float inv = exact ? 1.0f / scale : 0.0f;
   const bool product = exact || !(scale > 0.0f);
   uint8_t *out = dst + (long long)(lo - base) * c.tokenStride;
-  auto store = [&](const Raw &x, int row, int col) {
+  auto store = [&](const Raw &x, const At &to) {
     float e[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -177,21 +196,20 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
       for (int k = 0; k < 8; ++k)
         e[k] = __fdiv_rn(e[k], scale);
     }
-    *reinterpret_cast<uint2 *>(out + row * c.tokenStride + col * 8) =
+    *reinterpret_cast<uint2 *>(out + to.row * c.tokenStride + to.col * 8) =
         make_uint2(quantise4<Q>(e[0], e[1], e[2], e[3]), quantise4<Q>(e[4], e[5], e[6], e[7]));
   };
-  r = row0;
-  q = col0;
+  at = first;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
-    if (r < rows)
-      store(raw[i], r, q);
-    advance(r, q);
+    if (i >= turns)
+      break;
+    if (at.row < rows)
+      store(raw[i], at);
+    advance(at);
   }
-  while (r < rows) {
-    store(loadRaw(src + r * rowStride + q * 8, p.vec), r, q);
-    advance(r, q);
-  }
+  for (; at.row < rows; advance(at))
+    store(fetch(at), at);
 }
 
 } // namespace

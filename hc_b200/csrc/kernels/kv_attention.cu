@@ -25,12 +25,15 @@
 //     and the outputs are rescaled a few times per sequence only.  The sum of
 //     exp2(x - m), the maxima and the output are fp32; rounding w costs 2^-12 of a term
 //     (terms below 2^-25 of the largest lose more, by at most 2^-36 of it).
-//   * The tiles (128 tokens: 16 per warp of a CTA) of all (sequence, head, row tile)
-//     units stand in one line that is cut into equal shares, one per resident CTA, so a
-//     ragged batch is balanced and a single long sequence uses the whole GPU.  A unit
-//     that is cut is joined by the last of its CTAs to finish, from partial results in
-//     global memory, added in the order of the shares: the result does not depend on
-//     which one that is.
+//   * The tiles (16 tokens) of all (sequence, head, row tile) units stand in one line
+//     that is cut into equal shares, one per resident CTA, and a share into eight, one
+//     per warp: a ragged batch is balanced to a tile, and a single long sequence uses the
+//     whole GPU.  A warp walks through its part alone, whatever units it crosses (when
+//     the warps of a CTA went through units together, meeting at each one's end, the
+//     meetings took a third of the time); at the end the CTA joins the pieces of units
+//     that its warps share, and a unit that several CTAs share is joined by the last of
+//     them to finish, from partial results in global memory - all in the order of the
+//     line, so the result does not depend on timing.
 #include "kv_params.h"
 #include "serving_math.cuh"
 
@@ -49,14 +52,18 @@ struct AttentionParams {
   int share;       // query heads per key/value head
   int window;      // 0: none
   int rowTiles;    // row tiles that maxNew * share rows can take
-  int sixteenths;  // block / 16, and ceil(2^32 / that) for more than one
-  uint32_t blockInverse;
+  int stepBlocks, stepRows; // of a tile: whole blocks, and rows beyond them
+  // Quotients by products (ceil(2^32 / n), 0 for n = 1): of a position's sixteens by a
+  // block's, of a query row by `share`.
+  uint32_t blockInverse, shareInverse;
+  int vecQ; // rows of q that 16-byte loads can take
   unsigned *counters; // [CTAs], zero between calls
   float *partial;     // [CTAs][2] slots
 };
 
 constexpr int kWarps = 8;
-constexpr int kTile = 16 * kWarps;
+constexpr int kChunks = 64; // of 256 sequences whose places in the line are kept
+constexpr int kTile = 16;
 constexpr float kNegInf = -INFINITY;
 // The reference that the exponentials are taken against follows the running maximum
 // only when that has grown by more than 2^kSlack: probabilities reach 2^kSlack, times
@@ -130,8 +137,16 @@ template <int DimCap, int NT> struct Shape {
   static constexpr int mTiles = DimCap / 16;
   static constexpr int qPitch = DimCap + 8; // halves: rows 4 banks apart
   static constexpr int slotFloats = rows * DimCap + 2 * rows;
-  // (Shared memory, launched with kWarps * rows * DimCap * 4 bytes: the query rows, and
-  // at the end of a segment the warps' partial outputs [warps][rows][DimCap].)
+  // (Shared memory: every warp's query rows, its two pieces [rows][DimCap] of floats, and
+  // a factor per row of the pieces, or of the shares, that are joined:
+  // kWarps * rows * (2 * qPitch + 8 * DimCap) + 4 * rows * max(2 * kWarps, CTAs) bytes.)
+};
+
+// What a warp leaves of a unit that it does not have all of.
+struct Piece {
+  int unitBegin; // names the unit; -1: none
+  int tile0, tile1, unitTiles;
+  int head, row0, rowsHere, spanRow;
 };
 
 // Whole: the head dimension is DimCap.
@@ -139,21 +154,26 @@ template <class Q, int DimCap, int NT, bool Whole>
 __device__ __forceinline__ void attend(const AttentionParams &p) {
   using S = Shape<DimCap, NT>;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ long long sPrefix[kWarps * 32];
-  __shared__ float sRowFactor[S::rows];
-  __shared__ float sMax[kWarps][S::rows], sSum[kWarps][S::rows];
-  __shared__ float sFactor[kWarps][S::rows], sTop[S::rows], sTotal[S::rows];
-  __shared__ long long sWarpTotal[kWarps];
+  __shared__ int sChunk[kChunks + 1]; // where every 256 sequences begin in the line
+  __shared__ int sWarpTotal[kWarps], sWarpUnits[kWarps];
+  __shared__ float sTop[S::rows], sTotal[S::rows];
+  __shared__ float sRowFactor[kWarps][S::rows];
+  __shared__ float sMax[kWarps][2][S::rows], sSum[kWarps][2][S::rows];
+  __shared__ Piece sPiece[kWarps][2];
   __shared__ int sLast;
-  __half *sQ = reinterpret_cast<__half *>(smem);
-  float *sOut = reinterpret_cast<float *>(smem);
-
   const HcKvCacheDev &c = p.cache;
   const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  __half *sQ = reinterpret_cast<__half *>(smem) + warp * S::rows * S::qPitch;
+  float *const sPieces = reinterpret_cast<float *>(smem + kWarps * S::rows * S::qPitch * 2);
+  float *const sWeight = sPieces + 2 * kWarps * S::rows * DimCap; // [part][rows], when joining
   // This lane's bytes within 16 tokens (a page spans less than 2^31 bytes).
   const uint32_t kOffset = uint32_t(g) * uint32_t(c.tokenStride) + 16 * t;
   const uint32_t vOffset = uint32_t(2 * t) * uint32_t(c.tokenStride) + S::valueBytes * g;
+
+  auto queryOf = [&](int r) { // of a unit's sequence: row r of the `share` rows per query
+    return p.share == 1 ? r : int(__umulhi(uint32_t(r), p.shareInverse));
+  };
 
   // Tiles of one unit of a sequence, and its row tiles.
   auto tilesOf = [&](int seq, HcKvSpan &s, int &begin, int &rowTiles) -> int {
@@ -167,37 +187,38 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
   };
 
   // The line's length, and the sequence in which this CTA's share begins.
-  long long total = 0;
+  int total = 0, units = 0; // (the host has checked that they fit)
   bool placeless = false; // rows without a place in the cache
   for (int base = 0; base < p.place.seqs; base += 256) {
-    long long mine = 0;
+    int mine = 0, mineUnits = 0;
     if (base + tid < p.place.seqs) {
       HcKvSpan s;
       int begin, rt;
       const int n = tilesOf(base + tid, s, begin, rt);
-      mine = (long long)n * rt * c.heads;
+      mineUnits = n > 0 ? rt * c.heads : 0;
+      mine = n * mineUnits;
       placeless = placeless || s.count != s.allCount;
     }
-    // Inclusive scan over the CTA.
-    long long scan = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, scan, d);
-      if (lane >= d)
-        scan += other;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    mineUnits = __reduce_add_sync(0xffffffffu, mineUnits);
+    if (lane == 0) {
+      sWarpTotal[warp] = mine;
+      sWarpUnits[warp] = mineUnits;
     }
-    if (lane == 31)
-      sWarpTotal[warp] = scan;
     __syncthreads();
-    long long before = total;
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp)
-        before += sWarpTotal[w];
       total += sWarpTotal[w];
+      units += sWarpUnits[w];
     }
-    sPrefix[tid] = before + scan; // inclusive, from the start of the line
+    if (tid == 0 && base / 256 < kChunks)
+      sChunk[base / 256 + 1] = total;
     __syncthreads();
   }
+  if (tid == 0)
+    sChunk[0] = 0;
+  if (tid < 2 * kWarps)
+    sPiece[tid >> 1][tid & 1].unitBegin = -1;
+  __syncthreads();
   if (blockIdx.x == 0 && __syncthreads_or(placeless)) {
     // They see nothing: zeros.
     const int heads = c.heads * p.share;
@@ -215,107 +236,155 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
       }
     }
   }
-  const long long shares = min((long long)gridDim.x, total);
-  if ((long long)blockIdx.x >= shares)
+  // A share is a tile per warp at least.  A unit of n tiles is cut into about sqrt(n)
+  // shares at most: joining s of them costs as much as s tiles of a warp.
+  const unsigned shares =
+      min(gridDim.x, min(unsigned(total + kWarps - 1) / kWarps,
+                         unsigned(ceilf(sqrtf(float(total)) * sqrtf(float(units))))));
+  if (blockIdx.x >= shares)
     return;
-  long long at = hcKvShareBegin(blockIdx.x, total, shares);
-  const long long shareEnd = hcKvShareBegin((long long)blockIdx.x + 1, total, shares);
-  int seq = 0;
-  long long seqBegin = 0; // where that sequence begins in the line
-  if (p.place.seqs <= 256) {
-    // sPrefix holds the whole line: count the sequences that end at or before `at`.
-    const int done = tid < p.place.seqs && sPrefix[tid] <= at;
-    seq = __syncthreads_count(done);
-    seqBegin = seq > 0 ? sPrefix[seq - 1] : 0;
-  } else {
-    for (int base = 0;; base += 256) {
+  const HcKvShares line = hcKvSharesOf(unsigned(total), shares);
+  const int shareBegin = int(hcKvShareBegin(line, blockIdx.x));
+  const int shareTiles = int(line.each + (blockIdx.x < line.longer));
+  int at = shareBegin + int((unsigned)shareTiles * unsigned(warp) / kWarps);
+  const int myEnd = shareBegin + int((unsigned)shareTiles * unsigned(warp + 1) / kWarps);
+
+  // The sequence in which this warp's part begins, and where that begins in the line.
+  int seq = 0, seqBegin = 0;
+  if (at < myEnd) {
+    const int chunks = min((p.place.seqs + 255) / 256, kChunks);
+    while (seq / 256 + 1 < chunks && sChunk[seq / 256 + 1] <= at)
+      seq += 256;
+    seqBegin = sChunk[seq / 256];
+    for (;; seq += 32) { // (ends: `at` lies before the line's end)
       HcKvSpan s;
       int begin, rt;
-      long long mine = 0;
-      if (base + tid < p.place.seqs)
-        mine = (long long)tilesOf(base + tid, s, begin, rt) * rt * c.heads;
-      long long scan = mine;
+      int mine = 0;
+      if (seq + lane < p.place.seqs) {
+        const int n = tilesOf(seq + lane, s, begin, rt);
+        mine = n * rt * c.heads;
+      }
+      int scan = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, scan, d);
+        const int other = __shfl_up_sync(0xffffffffu, scan, d);
         if (lane >= d)
           scan += other;
       }
-      __syncthreads();
-      if (lane == 31)
-        sWarpTotal[warp] = scan;
-      __syncthreads();
-      long long before = seqBegin, all = seqBegin;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp)
-          before += sWarpTotal[w];
-        all += sWarpTotal[w];
-      }
-      sPrefix[tid] = before + scan;
-      __syncthreads();
-      if (all > at || base + 256 >= p.place.seqs) {
-        const int done = base + tid < p.place.seqs && sPrefix[tid] <= at;
-        const int n = __syncthreads_count(done);
-        seq = base + n;
-        seqBegin = n > 0 ? sPrefix[n - 1] : seqBegin;
+      const unsigned beyond = __ballot_sync(0xffffffffu, seqBegin + scan > at);
+      if (beyond) {
+        const int first = __ffs(beyond) - 1;
+        seqBegin += __shfl_sync(0xffffffffu, scan - mine, first);
+        seq += first;
         break;
       }
-      seqBegin = all;
+      seqBegin += __shfl_sync(0xffffffffu, scan, 31);
+      if (seq + 32 >= p.place.seqs)
+        break;
     }
   }
 
-  while (at < shareEnd) {
+  // sum: of exp2(x - top); v: four outputs, times kWeight * sum.
+  auto finish = [&](const Piece &u, int col, int d, float4 v, float top, float sum) {
+    const int r = u.row0 + col;
+    const int qi = queryOf(r), gh = r - qi * p.share;
+    const long long token = u.spanRow + qi;
+    const int qHead = u.head * p.share + gh;
+    const float f = sum == 0.0f ? 0.0f : 1.0f / (kWeight * sum);
+    __nv_bfloat162 a = __floats2bfloat162_rn(v.x * f, v.y * f);
+    __nv_bfloat162 b = __floats2bfloat162_rn(v.z * f, v.w * f);
+    uint2 packed;
+    packed.x = *reinterpret_cast<uint32_t *>(&a);
+    packed.y = *reinterpret_cast<uint32_t *>(&b);
+    if (d < c.dim)
+      *reinterpret_cast<uint2 *>(p.out + token * p.outTokenStride + qHead * p.outHeadStride + d) =
+          packed;
+    if (d == 0 && p.lse)
+      p.lse[token * p.lseStride + qHead] =
+          sum == 0.0f ? kNegInf : (top + __log2f(sum)) * 0.693147180559945309f;
+  };
+
+  int slot = 0; // of the warp's next piece
+  while (at < myEnd) {
     HcKvSpan span;
     int kvBegin, rowTiles;
-    int unitTiles = tilesOf(seq, span, kvBegin, rowTiles);
-    const long long inSeq = (long long)unitTiles * rowTiles * c.heads;
+    const int unitTiles = tilesOf(seq, span, kvBegin, rowTiles);
+    const int inSeq = unitTiles * rowTiles * c.heads;
     if (at - seqBegin >= inSeq) { // next sequence (those without tiles are passed over)
       seqBegin += inSeq;
       ++seq;
       continue;
     }
-    const int unit = int((at - seqBegin) / unitTiles);
-    const int head = unit / rowTiles, rowTile = unit - head * rowTiles;
-    const long long unitBegin = seqBegin + (long long)unit * unitTiles;
-    const int tile0 = int(at - unitBegin);
-    const int tile1 = int(min((long long)unitTiles, shareEnd - unitBegin));
+    const int unit = (at - seqBegin) / unitTiles;
+    const int head = rowTiles == 1 ? unit : unit / rowTiles;
+    const int rowTile = unit - head * rowTiles;
+    const int unitBegin = seqBegin + unit * unitTiles;
+    const int tile0 = at - unitBegin;
+    const int tile1 = min(unitTiles, myEnd - unitBegin);
     const int row0 = rowTile * S::rows;
     const int rowsHere = min(S::rows, span.count * p.share - row0);
     const int *table = p.place.table + (long long)seq * p.place.tablePitch;
 
     // ---- query rows into shared memory as f16, a power of two per row ----------------
-    __syncthreads(); // the previous segment's shared memory has been read
-    for (int r = warp; r < S::rows; r += kWarps) {
-      float v[DimCap / 32];
-      float top = 0.0f;
-      if (r < rowsHere) {
-        const int qi = (row0 + r) / p.share, gh = (row0 + r) - qi * p.share;
-        const __nv_bfloat16 *src = p.q + (long long)(span.row + qi) * p.qTokenStride +
-                                   (long long)(head * p.share + gh) * p.qHeadStride;
+    __syncwarp(); // the previous unit's have been read
+    constexpr int kPer = DimCap / 32; // consecutive elements of a lane
+#pragma unroll 1
+    for (int r0 = 0; r0 < S::rows; r0 += 4) {
+      uint32_t v[4][kPer / 2];
 #pragma unroll
-        for (int i = 0; i < DimCap / 32; ++i) {
-          const int d = i * 32 + lane;
-          v[i] = d < c.dim ? __bfloat162float(src[d]) : 0.0f;
-          top = fmaxf(top, fabsf(v[i]));
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          v[i][j] = 0;
+        if (r0 + i < rowsHere && lane * kPer < c.dim) {
+          const int qi = queryOf(row0 + r0 + i), gh = row0 + r0 + i - qi * p.share;
+          const __nv_bfloat16 *src = p.q + (long long)(span.row + qi) * p.qTokenStride +
+                                     (long long)(head * p.share + gh) * p.qHeadStride +
+                                     lane * kPer;
+          if (p.vecQ) {
+            if constexpr (kPer == 2) {
+              v[i][0] = *reinterpret_cast<const uint32_t *>(src);
+            } else if constexpr (kPer == 4) {
+              const uint2 x = *reinterpret_cast<const uint2 *>(src);
+              v[i][0] = x.x;
+              v[i][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4 *>(src);
+              v[i][0] = x.x;
+              v[i][1] = x.y;
+              v[i][2] = x.z;
+              v[i][3] = x.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              v[i][j >> 1] |= uint32_t(__bfloat16_as_ushort(src[j])) << (16 * (j & 1));
+          }
         }
-        top = segmentMax(top, 32);
-      } else {
-#pragma unroll
-        for (int i = 0; i < DimCap / 32; ++i)
-          v[i] = 0.0f;
       }
-      // 2^e <= top < 2^(e+1); zero, subnormal and infinite rows keep their values.
-      const int e = int(__float_as_uint(top) >> 23);
-      const bool plain = e == 0 || e == 255;
-      const float down = plain ? 1.0f : __uint_as_float(uint32_t(max(254 - e, 1)) << 23);
-      const float up = plain ? 1.0f : 1.0f / down;
-      if (lane == 0)
-        sRowFactor[r] = p.scaleLog2 * up;
 #pragma unroll
-      for (int i = 0; i < DimCap / 32; ++i)
-        sQ[r * S::qPitch + i * 32 + lane] = __float2half_rn(v[i] * down);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t top2 = 0; // magnitudes order like their bits
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          top2 = __vmaxu2(top2, v[i][j] & 0x7fff7fffu);
+        const uint32_t top =
+            __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16)) << 16;
+        // 2^e <= top < 2^(e+1); zero, subnormal and infinite rows keep their values.
+        const int e = int(top >> 23);
+        const bool plain = e == 0 || e == 255;
+        const float down = plain ? 1.0f : __uint_as_float(uint32_t(max(254 - e, 1)) << 23);
+        const float up = plain ? 1.0f : __uint_as_float(uint32_t(min(e, 253)) << 23);
+        if (lane == 0)
+          sRowFactor[warp][r0 + i] = p.scaleLog2 * up;
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          *reinterpret_cast<uint32_t *>(sQ + (r0 + i) * S::qPitch + lane * kPer + 2 * j) =
+              halfPair(__uint_as_float(v[i][j] << 16) * down,
+                       __uint_as_float(v[i][j] & 0xffff0000u) * down);
+      }
     }
-    __syncthreads();
+    __syncwarp();
 
     // ---- this lane's columns: query rows 2t and 2t + 1 of each n-tile ------------------
     float colFactor[NT][2], m[NT][2], l[NT][2];
@@ -325,21 +394,25 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = n * 8 + 2 * t + h;
-        colFactor[n][h] = sRowFactor[r];
+        colFactor[n][h] = sRowFactor[warp][r];
         m[n][h] = kNegInf;
         l[n][h] = 0.0f;
-        const int qi = min(row0 + r, row0 + rowsHere - 1) / p.share;
+        const int qi = queryOf(row0 + min(r, rowsHere - 1));
         seenHi[n][h] = span.first + qi;
         seenLo[n][h] = p.window > 0 ? max(0, span.first + qi - p.window + 1) : 0;
       }
-    const int firstPos = span.first + row0 / p.share;
-    const int lastPos = span.first + (row0 + rowsHere - 1) / p.share;
+    const int firstPos = span.first + queryOf(row0);
+    const int lastPos = span.first + queryOf(row0 + rowsHere - 1);
     // Positions that every row sees: [allLo, firstPos].
     const int allLo = p.window > 0 ? max(0, lastPos - p.window + 1) : 0;
     const int anyLo = p.window > 0 ? max(0, firstPos - p.window + 1) : 0;
 
-    const uint8_t *kHead = static_cast<const uint8_t *>(c.k) + (long long)head * c.headStride;
-    const uint8_t *vHead = static_cast<const uint8_t *>(c.v) + (long long)head * c.headStride;
+    const uint8_t *kLane =
+        static_cast<const uint8_t *>(c.k) + (long long)head * c.headStride + kOffset;
+    const uint8_t *vLane =
+        static_cast<const uint8_t *>(c.v) + (long long)head * c.headStride + vOffset;
+    // Tokens of this segment's tiles that some row sees: [anyLo, lookEnd).
+    const int lookEnd = min(lastPos + 1, kvBegin + tile1 * kTile);
     const float *kScales = c.kScale + head, *vScales = c.vScale + head;
 
     float o[S::mTiles][NT][4];
@@ -352,51 +425,60 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
           o[i][n][k] = 0.0f;
 
     // ---- the warp's 16 tokens of each tile -----------------------------------------------
-    auto posOf = [&](int tile) { return kvBegin + tile * kTile + warp * 16; };
-    // Blocks are multiples of 16 tokens: the quotient of two small numbers by a product.
-    auto blockOf = [&](int pos) {
-      return p.sixteenths == 1 ? pos >> 4
-                               : int(__umulhi(uint32_t(pos) >> 4, p.blockInverse));
+    // The tile that is looked up next (two ahead of the one at work): its first position,
+    // the block it lies in and its place there, stepped along without divisions.
+    int lookPos = kvBegin + tile0 * kTile;
+    int lookBlock = lookPos >> 4;
+    if (c.block > 16)
+      lookBlock = int(__umulhi(uint32_t(lookBlock), p.blockInverse));
+    int lookRow = lookPos - lookBlock * c.block;
+    // Where a tile's rows lie in the cache; page < 0: not there, or seen by no row.
+    struct Spot {
+      int page;
+      uint64_t at;
     };
-    auto pageAt = [&](int tile) -> int {
-      const int pos = posOf(tile);
-      // Tokens that no row of this unit sees are passed over like missing pages.
-      if (tile >= tile1 || pos > lastPos || pos + 15 < anyLo)
-        return -1;
-      return hcKvPageOf(__ldg(table + blockOf(pos)), c.pages);
+    auto look = [&]() -> Spot {
+      Spot s{-1, 0};
+      if (lookPos < lookEnd && lookPos + 15 >= anyLo)
+        s.page = hcKvPageOf(__ldg(table + lookBlock), c.pages);
+      s.at = uint32_t(lookRow) * uint32_t(c.tokenStride);
+      lookPos += kTile;
+      lookBlock += p.stepBlocks;
+      lookRow += p.stepRows;
+      if (lookRow >= c.block) {
+        lookRow -= c.block;
+        ++lookBlock;
+      }
+      return s;
     };
     // All 16 rows lie inside the page, written or not: what is not visible is masked.
     uint4 kReg[2][S::keyPieces];
     uint32_t vReg[4][S::valuePieces][S::valueWords];
     float kScale = 0.0f, vScale = 0.0f;
-    auto loadKeys = [&](int tile, int page) {
-      if (page < 0)
+    auto loadKeys = [&](Spot &s) {
+      if (s.page < 0)
         return;
-      const int pos = posOf(tile);
-      const uint8_t *k = kHead + (long long)page * c.pageStride +
-                         uint32_t(pos - blockOf(pos) * c.block) * uint32_t(c.tokenStride);
+      s.at += uint64_t(uint32_t(s.page)) * uint32_t(c.pageStride);
+      const uint8_t *k = kLane + s.at;
+      const uint8_t *k8 = k + 8 * uint32_t(c.tokenStride);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < S::keyPieces; ++j)
-          kReg[h][j] = Whole || 64 * j + 16 * t < c.dim
-                           ? loadStream16(k + (h ? kOffset + 8 * uint32_t(c.tokenStride) : kOffset) +
-                                          64 * j)
-                           : make_uint4(0, 0, 0, 0);
-      kScale = __ldg(kScales + (long long)page * c.scalePitch);
+      for (int j = 0; j < S::keyPieces; ++j) {
+        const bool in = Whole || 64 * j + 16 * t < c.dim;
+        kReg[0][j] = in ? loadStream16(k + 64 * j) : make_uint4(0, 0, 0, 0);
+        kReg[1][j] = in ? loadStream16(k8 + 64 * j) : make_uint4(0, 0, 0, 0);
+      }
+      kScale = __ldg(kScales + uint64_t(uint32_t(s.page)) * uint32_t(c.scalePitch));
     };
-    auto loadValues = [&](int tile, int page) {
-      if (page < 0)
+    auto loadValues = [&](const Spot &s) {
+      if (s.page < 0)
         return;
-      const int pos = posOf(tile);
-      const uint8_t *v = vHead + (long long)page * c.pageStride +
-                         uint32_t(pos - blockOf(pos) * c.block) * uint32_t(c.tokenStride);
+      const uint8_t *v = vLane + s.at;
 #pragma unroll
       for (int h = 0; h < 4; ++h)
 #pragma unroll
         for (int j = 0; j < S::valuePieces; ++j) {
           const uint8_t *at =
-              v + (vOffset + ((h & 1) + 8 * (h >> 1)) * uint32_t(c.tokenStride)) + 128 * j;
+              v + uint64_t(((h & 1) + 8 * (h >> 1)) * uint32_t(c.tokenStride)) + 128 * j;
           const bool in = Whole || 128 * j + S::valueBytes * g < c.dim;
           if constexpr (S::valueBytes == 16) {
             const uint4 w = in ? loadStream16(at) : make_uint4(0, 0, 0, 0);
@@ -414,15 +496,16 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
             vReg[h][j][1] = w.y;
           }
         }
-      vScale = __ldg(vScales + (long long)page * c.scalePitch);
+      vScale = __ldg(vScales + uint64_t(uint32_t(s.page)) * uint32_t(c.scalePitch));
     };
 
-    int page = pageAt(tile0), nextPage = pageAt(tile0 + 1);
-    loadKeys(tile0, page);
-    loadValues(tile0, page);
-    for (int tile = tile0; tile < tile1; ++tile) {
-      const int pos = posOf(tile);
-      const int afterPage = pageAt(tile + 2);
+    Spot now = look(), next = look();
+    loadKeys(now);
+    loadValues(now);
+    int pos = kvBegin + tile0 * kTile;
+#pragma unroll 1
+    for (int tile = tile0; tile < tile1; ++tile, pos += kTile) {
+      const Spot after = look();
       const float sk = kScale, sv = vScale;
       float s[NT][4];
 #pragma unroll
@@ -430,7 +513,7 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           s[n][k] = 0.0f;
-      if (page >= 0) {
+      if (now.page >= 0) {
 #pragma unroll
         for (int j = 0; j < S::keyPieces; ++j) {
           const uint32_t w0[4] = {kReg[0][j].x, kReg[0][j].y, kReg[0][j].z, kReg[0][j].w};
@@ -454,11 +537,11 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
           }
         }
       }
-      const int nowPage = page;
-      page = nextPage;
-      nextPage = afterPage;
-      loadKeys(tile + 1, page);
-      if (nowPage >= 0) {
+      const bool there = now.page >= 0;
+      now = next;
+      next = after;
+      loadKeys(now);
+      if (there) {
         // Scores in units of log2, masked; the largest one with its value scale.
         float lsv = 0.0f;
         if (sv > 0.0f && sv < INFINITY)
@@ -564,7 +647,7 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
           addValues(vReg, pb);
         } else {
           for (int col = 0; col < S::rows; ++col) {
-            const int qi = min(row0 + col, row0 + rowsHere - 1) / p.share;
+            const int qi = queryOf(row0 + min(col, rowsHere - 1));
             const int hiPos = span.first + qi;
             const int loPos = p.window > 0 ? max(0, hiPos - p.window + 1) : 0;
             uint32_t vr[4][S::valuePieces][S::valueWords];
@@ -605,111 +688,128 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
           }
         }
       }
-      loadValues(tile + 1, page);
+      loadValues(now);
     }
 
-    // ---- join the warps -------------------------------------------------------------------
+    // ---- a whole unit is finished, a piece is kept -----------------------------------------
+    const Piece piece{unitBegin, tile0, tile1, unitTiles, head, row0, rowsHere, span.row};
+    float *const held = sPieces + (warp * 2 + slot) * S::rows * DimCap;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v = l[n][h];
-        v += __shfl_xor_sync(0xffffffffu, v, 4);
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (g == 0) {
-          sMax[warp][n * 8 + 2 * t + h] = m[n][h];
-          sSum[warp][n * 8 + 2 * t + h] = v;
-        }
-      }
-    __syncthreads(); // also: the query rows in sOut's place have been read
-    if (tid < S::rows) {
-      float top = kNegInf, sum = 0.0f;
-      for (int w = 0; w < kWarps; ++w)
-        top = fmaxf(top, sMax[w][tid]);
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = sMax[w][tid] == kNegInf ? 0.0f : exp2Approx(sMax[w][tid] - top);
-        sFactor[w][tid] = f;
-        // (a warp whose scores are NaN has a sum but no maximum)
-        sum += sMax[w][tid] == kNegInf ? sSum[w][tid] : sSum[w][tid] * f;
-      }
-      sTop[tid] = top;
-      sTotal[tid] = sum;
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        float sum = l[n][h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int col = n * 8 + 2 * t + h;
-        float *dst = sOut + (warp * S::rows + col) * DimCap;
+        if (g == 0) {
+          sMax[warp][slot][col] = m[n][h];
+          sSum[warp][slot][col] = sum;
+        }
+        float *dst = held + col * DimCap + S::valueBytes * g;
 #pragma unroll
         for (int j = 0; j < S::valuePieces; ++j)
 #pragma unroll
           for (int w = 0; w < S::valueWords; ++w) {
             const int i = (j * S::valueWords + w) * 2;
-            // dims 4w .. 4w + 3 of the lane's run
-            *reinterpret_cast<float4 *>(dst + 128 * j + S::valueBytes * g + 4 * w) =
+            *reinterpret_cast<float4 *>(dst + 128 * j + 4 * w) =
                 make_float4(o[i][n][h], o[i][n][h + 2], o[i + 1][n][h], o[i + 1][n][h + 2]);
           }
       }
-    __syncthreads();
-
-    const bool split = tile0 > 0 || tile1 < unitTiles;
-    constexpr int kQuads = S::rows * DimCap / 4;
-    auto finish = [&](int col, int d, float4 v, float top, float sum) {
-      // v: sum of kWeight w V; sum: of exp2(x - top).
-      const int r = row0 + col;
-      const int qi = r / p.share, gh = r - qi * p.share;
-      const long long token = span.row + qi;
-      const int qHead = head * p.share + gh;
-      const float f = sum == 0.0f ? 0.0f : 1.0f / (kWeight * sum);
-      __nv_bfloat162 a = __floats2bfloat162_rn(v.x * f, v.y * f);
-      __nv_bfloat162 b = __floats2bfloat162_rn(v.z * f, v.w * f);
-      uint2 packed;
-      packed.x = *reinterpret_cast<uint32_t *>(&a);
-      packed.y = *reinterpret_cast<uint32_t *>(&b);
-      if (d < c.dim)
-        *reinterpret_cast<uint2 *>(p.out + token * p.outTokenStride + qHead * p.outHeadStride + d) =
-            packed;
-      if (d == 0 && p.lse)
-        p.lse[token * p.lseStride + qHead] =
-            sum == 0.0f ? kNegInf : (top + __log2f(sum)) * 0.693147180559945309f;
-    };
-    auto joined = [&](int col, int d) {
-      float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float4 x = *reinterpret_cast<const float4 *>(sOut + (w * S::rows + col) * DimCap + d);
-        const float f = sFactor[w][col];
-        v.x = fmaf(x.x, f, v.x);
-        v.y = fmaf(x.y, f, v.y);
-        v.z = fmaf(x.z, f, v.z);
-        v.w = fmaf(x.w, f, v.w);
-      }
-      return v;
-    };
-    if (!split) {
-      for (int i = tid; i < kQuads; i += 256) {
+    if (tile0 == 0 && tile1 == unitTiles) {
+      __syncwarp();
+#pragma unroll 1
+      for (int i = lane; i < rowsHere * (DimCap / 4); i += 32) {
         const int col = i / (DimCap / 4), d = (i - col * (DimCap / 4)) * 4;
-        if (col < rowsHere)
-          finish(col, d, joined(col, d), sTop[col], sTotal[col]);
+        finish(piece, col, d, *reinterpret_cast<const float4 *>(held + col * DimCap + d),
+               sMax[warp][slot][col], sSum[warp][slot][col]);
       }
+      __syncwarp();
     } else {
-      const int firstShare = hcKvShareOf(unitBegin, total, shares);
-      const int lastShare = hcKvShareOf(unitBegin + unitTiles - 1, total, shares);
-      auto slotOf = [&](int share) {
-        return p.partial + ((long long)share * 2 + (share == firstShare)) * S::slotFloats;
-      };
-      float *slot = slotOf(int(blockIdx.x));
-      for (int i = tid; i < kQuads; i += 256) {
-        const int col = i / (DimCap / 4), d = (i - col * (DimCap / 4)) * 4;
-        if (col < rowsHere)
-          __stcg(reinterpret_cast<float4 *>(slot + col * DimCap + d), joined(col, d));
+      if (lane == 0)
+        sPiece[warp][slot] = piece;
+      ++slot; // (a part has two ends: at most two pieces)
+    }
+    at = unitBegin + tile1;
+  }
+
+  // ---- join the warps' pieces, unit by unit -----------------------------------------------------
+  __syncthreads();
+  constexpr int kQuads = S::rows * DimCap / 4;
+  for (int e0 = 0; e0 < 2 * kWarps;) {
+    const Piece u = sPiece[e0 >> 1][e0 & 1];
+    if (u.unitBegin < 0) {
+      ++e0;
+      continue;
+    }
+    int e1 = e0 + 1, lastTile = u.tile1; // pieces [e0, e1) are the unit's (or empty)
+    for (; e1 < 2 * kWarps; ++e1) {
+      const Piece &x = sPiece[e1 >> 1][e1 & 1];
+      if (x.unitBegin >= 0) {
+        if (x.unitBegin != u.unitBegin)
+          break;
+        lastTile = x.tile1;
       }
-      if (tid < rowsHere) {
-        __stcg(slot + S::rows * DimCap + tid, sTop[tid]);
-        __stcg(slot + S::rows * DimCap + S::rows + tid, sTotal[tid]);
+    }
+    // Factors of the pieces: thread (row, piece), sixteen neighbours hold a row's.
+    static_assert(2 * kWarps == 16, "a row's pieces are reduced over sixteen lanes");
+    for (int i = tid; i < 16 * S::rows; i += 256) {
+      const int col = i >> 4, e = i & 15;
+      const bool in = e >= e0 && e < e1 && sPiece[e >> 1][e & 1].unitBegin >= 0;
+      const float part = in ? sMax[e >> 1][e & 1][col] : kNegInf;
+      float top = part;
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float f = part == kNegInf ? 0.0f : exp2Approx(part - top);
+      // (a piece whose scores are NaN has a sum but no maximum)
+      float sum = in ? sSum[e >> 1][e & 1][col] * (part == kNegInf ? 1.0f : f) : 0.0f;
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      sWeight[e * S::rows + col] = f;
+      if (e == 0) {
+        sTop[col] = top;
+        sTotal[col] = sum;
       }
+    }
+    __syncthreads();
+    const bool split = u.tile0 > 0 || lastTile < u.unitTiles;
+    const int firstShare = split ? int(hcKvShareOf(line, u.unitBegin)) : 0;
+    const int lastShare = split ? int(hcKvShareOf(line, u.unitBegin + u.unitTiles - 1)) : 0;
+    auto slotOf = [&](int share) {
+      return p.partial + ((long long)share * 2 + (share == firstShare)) * S::slotFloats;
+    };
+    auto add = [](float4 &v, const float4 &x, float f) {
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
+      v.z = fmaf(x.z, f, v.z);
+      v.w = fmaf(x.w, f, v.w);
+    };
+    float *mine = slotOf(int(blockIdx.x));
+    for (int i = tid; i < kQuads; i += 256) {
+      const int col = i / (DimCap / 4), d = (i - col * (DimCap / 4)) * 4;
+      if (col >= u.rowsHere)
+        continue;
+      float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+      for (int e = e0; e < e1; ++e) {
+        const float f = sWeight[e * S::rows + col];
+        if (f != 0.0f) // (0 also for slots that hold nothing)
+          add(v, *reinterpret_cast<const float4 *>(sPieces + (e * S::rows + col) * DimCap + d), f);
+      }
+      if (!split) {
+        finish(u, col, d, v, sTop[col], sTotal[col]);
+      } else {
+        __stcg(reinterpret_cast<float4 *>(mine + col * DimCap + d), v);
+        if (d == 0) {
+          __stcg(mine + S::rows * DimCap + col, sTop[col]);
+          __stcg(mine + S::rows * DimCap + S::rows + col, sTotal[col]);
+        }
+      }
+    }
+    if (split) {
       __threadfence();
       __syncthreads();
       if (tid == 0) // wraps to 0 with the last arrival
@@ -718,32 +818,56 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
       __syncthreads();
       if (sLast) {
         __threadfence();
+        // A warp per row: the shares' maxima and sums, 32 at a time.
+        const int parts = lastShare - firstShare + 1;
+        for (int col = warp; col < u.rowsHere; col += kWarps) {
+          float top = kNegInf;
+          for (int x = lane; x < parts; x += 32)
+            top = fmaxf(top, __ldcg(slotOf(firstShare + x) + S::rows * DimCap + col));
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          float sum = 0.0f;
+          for (int x = lane; x < parts; x += 32) {
+            const float *from = slotOf(firstShare + x) + S::rows * DimCap;
+            const float part = __ldcg(from + col), more = __ldcg(from + S::rows + col);
+            const float f = part == kNegInf ? 0.0f : exp2Approx(part - top);
+            sum += part == kNegInf ? more : more * f;
+            sWeight[x * S::rows + col] = f;
+          }
+          sum = warpSum(sum);
+          if (lane == 0) {
+            sTop[col] = top;
+            sTotal[col] = sum;
+          }
+        }
+        __syncthreads();
         for (int i = tid; i < kQuads; i += 256) {
           const int col = i / (DimCap / 4), d = (i - col * (DimCap / 4)) * 4;
-          if (col >= rowsHere)
+          if (col >= u.rowsHere)
             continue;
-          float top = kNegInf;
-          for (int x = firstShare; x <= lastShare; ++x)
-            top = fmaxf(top, __ldcg(slotOf(x) + S::rows * DimCap + col));
-          float sum = 0.0f;
           float4 v = make_float4(0, 0, 0, 0);
-          for (int x = firstShare; x <= lastShare; ++x) {
-            const float *from = slotOf(x);
-            const float part = __ldcg(from + S::rows * DimCap + col);
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(from + col * DimCap + d));
-            const float add = __ldcg(from + S::rows * DimCap + S::rows + col);
-            const float f = part == kNegInf ? 0.0f : exp2Approx(part - top);
-            sum += part == kNegInf ? add : add * f;
-            v.x = fmaf(y.x, f, v.x);
-            v.y = fmaf(y.y, f, v.y);
-            v.z = fmaf(y.z, f, v.z);
-            v.w = fmaf(y.w, f, v.w);
+          int x = 0;
+          for (; x + 8 <= parts; x += 8) { // (eight loads travel together)
+            float4 y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              y[k] = __ldcg(reinterpret_cast<const float4 *>(slotOf(firstShare + x + k) +
+                                                             col * DimCap + d));
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              add(v, y[k], sWeight[(x + k) * S::rows + col]);
           }
-          finish(col, d, v, top, sum);
+          for (; x < parts; ++x)
+            add(v,
+                __ldcg(reinterpret_cast<const float4 *>(slotOf(firstShare + x) + col * DimCap + d)),
+                sWeight[x * S::rows + col]);
+          finish(u, col, d, v, sTop[col], sTotal[col]);
         }
       }
     }
-    at = unitBegin + tile1;
+    __syncthreads(); // the factors and sLast have been read
+    e0 = e1;
   }
 }
 

@@ -82,12 +82,23 @@ HC_KV_FN int hcKvTouchedBlocks(int maxNew, int block) {
 }
 
 // ---- equal shares of a ragged batch ---------------------------------------------------
-// The tiles of all units (sequence, head, rows) stand in one line of `total`; share c of
-// `shares` (at most total) is [begin(c), begin(c + 1)).  No share is empty.
-HC_KV_FN long long hcKvShareBegin(long long c, long long total, long long shares) {
-  return c * total / shares;
+// The tiles of all units (sequence, head, rows) stand in one line of `total` tiles, cut
+// into `shares` (at most total) of total / shares, the first ones one tile longer.  No
+// share is empty.
+struct HcKvShares {
+  unsigned each, longer; // tiles of a share; how many have one more
+};
+HC_KV_FN HcKvShares hcKvSharesOf(unsigned total, unsigned shares) {
+  HcKvShares s;
+  s.each = total / shares;
+  s.longer = total - s.each * shares;
+  return s;
+}
+HC_KV_FN unsigned hcKvShareBegin(const HcKvShares &s, unsigned c) {
+  return c * s.each + (c < s.longer ? c : s.longer);
 }
 // The share that holds tile x.
-HC_KV_FN int hcKvShareOf(long long x, long long total, long long shares) {
-  return int(((x + 1) * shares - 1) / total);
+HC_KV_FN unsigned hcKvShareOf(const HcKvShares &s, unsigned x) {
+  const unsigned head = s.longer * (s.each + 1);
+  return x < head ? x / (s.each + 1) : s.longer + (x - head) / s.each;
 }

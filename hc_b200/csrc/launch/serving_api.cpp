@@ -87,8 +87,9 @@ struct AttentionParams {
   int share;
   int window;
   int rowTiles;
-  int sixteenths;
-  uint32_t blockInverse;
+  int stepBlocks, stepRows;
+  uint32_t blockInverse, shareInverse;
+  int vecQ;
   unsigned *counters;
   float *partial;
 };
@@ -168,6 +169,9 @@ int checkKv(HcContext c, const char *who, const HcKvCache *cache, const HcKvPlac
   if (cache->tokenStride > 0x7fffffffLL / cache->block)
     return c->fail("%s: a page of %d tokens, %lld apart, spans 2^31 bytes or more", who,
                    cache->block, cache->tokenStride);
+  if (cache->pageStride > 0x7fffffffLL || cache->scalePitch > 0x7fffffffLL)
+    return c->fail("%s: pages %lld bytes (scales %lld) apart: below 2^31 expected", who,
+                   cache->pageStride, cache->scalePitch);
   if (cache->scalePitch < cache->heads)
     return c->fail("%s: scale pitch %lld is below the %d heads", who, cache->scalePitch,
                    cache->heads);
@@ -479,7 +483,7 @@ int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place, cons
                    p.place.maxNew);
   void *args[] = {&p};
   return c->launch(p.cache.dtype == HC_I8 ? "hc_kv_append_i8" : "hc_kv_append_e4m3",
-                   size_t(blocks), size_t(p.cache.heads), 2, 128, args, 1, 0);
+                   size_t(blocks), size_t(ceilDiv(2 * p.cache.heads, 4)), 1, 128, args, 1, 0);
 }
 
 size_t hcKvAttentionWorkspaceBytes(HcContext c) {
@@ -526,15 +530,23 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   // many and the registers allow it.
   const int nt = maxRows > 8 && cap <= 128 ? 2 : 1;
   const long long rowTiles = ceilDiv(maxRows, 8 * nt);
-  if (rowTiles * p.cache.heads > 0x7fffffffLL)
-    return c->fail("hcKvAttention: too many query rows per sequence (%lld)", maxRows);
-  p.rowTiles = int(rowTiles);
-  p.sixteenths = p.cache.block / 16;
-  p.blockInverse = p.sixteenths == 1 ? 0 : uint32_t((1ull << 32) / p.sixteenths + 1);
-  const int perSm = cap == 64 || (cap == 128 && nt == 1) ? 2 : 1;
   const long long tiles = (long long)p.place.seqs * p.cache.heads * rowTiles *
-                          (ceilDiv((long long)p.place.width * p.cache.block, 128) + 1);
-  const long long ctas = std::max<long long>(1, std::min(tiles, c->smCount * perSm));
+                          (ceilDiv((long long)p.place.width * p.cache.block, 16) + 1);
+  // (The kernel counts tiles in 31 bits and divides row numbers by products.)
+  if (tiles > 0x7fffffffLL || maxRows * share > 0x7fffffffLL)
+    return c->fail("hcKvAttention: %d sequences of up to %lld query rows against %lld tokens are "
+                   "too many for one call",
+                   p.place.seqs, maxRows, (long long)p.place.width * p.cache.block);
+  p.rowTiles = int(rowTiles);
+  p.stepBlocks = 16 / p.cache.block;
+  p.stepRows = 16 % p.cache.block;
+  auto inverse = [](unsigned n) { return n == 1 ? 0u : uint32_t((1ull << 32) / n + 1); };
+  p.blockInverse = inverse(unsigned(p.cache.block) / 16);
+  p.shareInverse = inverse(unsigned(share));
+  p.vecQ = aligned(q, 16) && qTokenStride % 8 == 0 && qHeadStride % 8 == 0;
+  const int perSm = cap == 64 || (cap == 128 && nt == 1) ? 2 : 1;
+  const long long ctas =
+      std::max<long long>(1, std::min(ceilDiv(tiles, 8), c->smCount * perSm));
   p.counters = static_cast<unsigned *>(workspace);
   p.partial = reinterpret_cast<float *>(
       static_cast<char *>(workspace) + roundUp(c->smCount * kAttentionCtasPerSm * 4, 256));
@@ -542,7 +554,9 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d%s",
                 p.cache.dtype == HC_I8 ? "i8" : "e4m3", cap, nt, p.cache.dim == cap ? "" : "_any");
   void *args[] = {&p};
-  return c->launch(name, size_t(ctas), 1, 1, 256, args, 1, size_t(8) * 8 * nt * cap * 4);
+  return c->launch(name, size_t(ctas), 1, 1, 256, args, 1,
+                   size_t(8) * 8 * nt * (2 * (cap + 8) + 8 * cap) +
+                       size_t(4) * 8 * nt * std::max<long long>(16, ctas));
 }
 
 } // extern "C"
