@@ -13,10 +13,12 @@
 // bytes are determined by the inputs alone.
 //
 // HBM bound (2 bytes read and 1 written per element), for one new token per sequence
-// latency bound.  A warp owns one (sequence, block, head) of keys or of values: it reads
-// the new rows once into registers (what does not fit there again from L1), reduces by
-// shuffles alone, and nobody else writes its bytes.  (A CTA per unit spent two thirds of
-// its instructions on setting up: 41 us instead of 26 for 16 prompts of 2048 tokens.)
+// latency bound.  A warp owns one unit, a (sequence, block, head) of keys or of values: it
+// reads the new rows once into registers (what does not fit there again from L1), reduces
+// by shuffles alone, and nobody else writes its bytes.  Where that gives the GPU too few
+// warps a CTA takes a unit.  (For 16 prompts of 2048 tokens a CTA per unit spends most of
+// its instructions on setting up: 38 us against 31; for one chunk of 512 tokens warps
+// alone took 19 us.)
 #include "kv_params.h"
 #include "serving_math.cuh"
 
@@ -69,14 +71,31 @@ __device__ __forceinline__ float powerAbove(float x) {
 constexpr int kWarps = 4;
 constexpr int kHeld = 16; // pieces of 8 elements per lane in registers
 
-template <class Q> __device__ __forceinline__ void appendBlock(const AppendParams &p) {
+// Threads: 32, a warp per unit and four units per CTA; 256, a CTA per unit.
+template <class Q, int Threads> __device__ __forceinline__ void appendBlock(const AppendParams &p) {
+  __shared__ uint32_t sTop[8];
   const HcKvCacheDev &c = p.cache;
   const int seq = int(blockIdx.x) / p.touched, nth = int(blockIdx.x) - seq * p.touched;
-  const int lane = int(threadIdx.x) & 31;
-  const int unit = int(blockIdx.y) * kWarps + (int(threadIdx.x) >> 5);
+  const int lane = int(threadIdx.x) & (Threads - 1);
+  const int unit =
+      Threads == 32 ? int(blockIdx.y) * kWarps + (int(threadIdx.x) >> 5) : int(blockIdx.y);
   if (unit >= 2 * c.heads)
     return;
   const int head = unit >> 1, values = unit & 1;
+  // The largest over the unit's threads.
+  auto largest = [&](uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if constexpr (Threads > 32) {
+      __syncthreads(); // (an earlier result has been read)
+      if ((threadIdx.x & 31) == 0)
+        sTop[threadIdx.x >> 5] = v;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < Threads / 32; ++w)
+        v = max(v, sTop[w]);
+    }
+    return v;
+  };
 
   const HcKvSpan s = hcKvLoadSpan(p.place, c.block, seq);
   const int b = s.first / c.block + nth;
@@ -99,20 +118,32 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   old = old > 0.0f ? old : 0.0f;
   // Pieces of 8 elements, lane by lane along the rows; a lane's next piece by addition.
   const int perRow = c.dim >> 3, rows = hi - lo;
-  const int stepRow = 32 / perRow, stepCol = 32 - stepRow * perRow;
+  const int stepRow = Threads / perRow, stepCol = Threads - stepRow * perRow;
   struct At {
     int row, col;
+    const __nv_bfloat16 *from;
+    uint8_t *to;
   };
-  const At first{lane / perRow, lane - lane / perRow * perRow};
+  At first{lane / perRow, lane - lane / perRow * perRow, nullptr, nullptr};
+  first.from = src + first.row * rowStride + first.col * 8;
+  first.to = dst + (long long)(lo - base + first.row) * c.tokenStride + first.col * 8;
+  const long long stepFrom = stepRow * rowStride + stepCol * 8, wrapFrom = rowStride - 8 * perRow;
+  const long long stepTo = stepRow * c.tokenStride + stepCol * 8, wrapTo = c.tokenStride - 8 * perRow;
   auto advance = [&](At &at) {
     at.row += stepRow;
-    at.col += stepCol;
-    if (at.col >= perRow) {
-      at.col -= perRow;
-      ++at.row;
+    at.from += stepFrom;
+    at.to += stepTo;
+    if (stepCol) {
+      at.col += stepCol;
+      if (at.col >= perRow) {
+        at.col -= perRow;
+        ++at.row;
+        at.from += wrapFrom;
+        at.to += wrapTo;
+      }
     }
   };
-  auto fetch = [&](const At &at) { return loadRaw(src + at.row * rowStride + at.col * 8, p.vec); };
+  auto fetch = [&](const At &at) { return loadRaw(at.from, p.vec); };
 
   Raw raw[kHeld];
   uint32_t top2 = 0; // magnitudes, as bits: they order like unsigned numbers
@@ -123,7 +154,7 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   };
   // (One token is one turn: leaving early keeps the code that runs short, and at one
   // token per sequence fetching instructions is what takes the time.)
-  const int turns = (rows * perRow + 31) >> 5;
+  const int turns = (rows * perRow + Threads - 1) / Threads;
   At at = first;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
@@ -141,7 +172,7 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   for (; at.row < rows; advance(at))
     magnitude(fetch(at));
   uint32_t top16 = max(top2 & 0xffffu, top2 >> 16);
-  top16 = __reduce_max_sync(0xffffffffu, top16);
+  top16 = largest(top16);
   if (top16 >= 0x7f80u) { // something is not finite: the largest of the others
     uint32_t best = 0;
     for (at = first; at.row < rows; advance(at)) {
@@ -152,20 +183,21 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
         best = m < 0x7f80u ? max(best, m) : best;
       }
     }
-    top16 = __reduce_max_sync(0xffffffffu, best);
+    top16 = largest(best);
   }
   float need = __fmul_rn(__uint_as_float(top16 << 16), 1.0f / Peak<Q>::value);
   if constexpr (__is_same(Q, E4M3))
     need = powerAbove(need);
   const float scale = fmaxf(old, need);
-  __syncwarp(); // every lane has read the old scale
+  if constexpr (Threads == 32)
+    __syncwarp(); // every lane has read the old scale (in a CTA: before `largest`)
   if (lane == 0)
     *scaleAt = scale;
 
   if (held && scale > old) {
     const float ratio = __fdiv_rn(old, scale);
     const int wordsPerRow = c.dim >> 2, words = (lo - base) * wordsPerRow;
-    for (int i = lane; i < words; i += 32) {
+    for (int i = lane; i < words; i += Threads) {
       const int row = i / wordsPerRow, w = i - row * wordsPerRow;
       uint32_t *word = reinterpret_cast<uint32_t *>(dst + row * c.tokenStride) + w;
       const uint32_t x = *word;
@@ -179,7 +211,6 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
   const bool exact = (bits & 0x007fffffu) == 0 && bits >= 0x01000000u && bits < 0x7e000000u;
   const float inv = exact ? 1.0f / scale : 0.0f;
   const bool product = exact || !(scale > 0.0f);
-  uint8_t *out = dst + (long long)(lo - base) * c.tokenStride;
   auto store = [&](const Raw &x, const At &to) {
     float e[8];
 #pragma unroll
@@ -196,7 +227,7 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
       for (int k = 0; k < 8; ++k)
         e[k] = __fdiv_rn(e[k], scale);
     }
-    *reinterpret_cast<uint2 *>(out + to.row * c.tokenStride + to.col * 8) =
+    *reinterpret_cast<uint2 *>(to.to) =
         make_uint2(quantise4<Q>(e[0], e[1], e[2], e[3]), quantise4<Q>(e[4], e[5], e[6], e[7]));
   };
   at = first;
@@ -214,11 +245,14 @@ template <class Q> __device__ __forceinline__ void appendBlock(const AppendParam
 
 } // namespace
 
-extern "C" __global__ void __launch_bounds__(128)
-    hc_kv_append_i8(const __grid_constant__ AppendParams p) {
-  appendBlock<I8>(p);
-}
-extern "C" __global__ void __launch_bounds__(128)
-    hc_kv_append_e4m3(const __grid_constant__ AppendParams p) {
-  appendBlock<E4M3>(p);
-}
+#define HC_APPEND(name, Q)                                                                 \
+  extern "C" __global__ void __launch_bounds__(128)                                         \
+      hc_kv_append_##name##_warp(const __grid_constant__ AppendParams p) {                  \
+    appendBlock<Q, 32>(p);                                                                  \
+  }                                                                                         \
+  extern "C" __global__ void __launch_bounds__(256)                                         \
+      hc_kv_append_##name##_cta(const __grid_constant__ AppendParams p) {                   \
+    appendBlock<Q, 256>(p);                                                                 \
+  }
+HC_APPEND(i8, I8)
+HC_APPEND(e4m3, E4M3)

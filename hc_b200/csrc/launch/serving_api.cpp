@@ -160,7 +160,7 @@ int checkKv(HcContext c, const char *who, const HcKvCache *cache, const HcKvPlac
                    cache->block);
   if (cache->dim < 16 || cache->dim > 256 || cache->dim % 16)
     return c->fail("%s: head dimension %d (a multiple of 16 up to 256 expected)", who, cache->dim);
-  if (cache->pages < 0 || cache->heads < 1 || cache->heads > 65535)
+  if (cache->pages < 0 || cache->heads < 1 || cache->heads > 32767)
     return c->fail("%s: %d pages of %d heads", who, cache->pages, cache->heads);
   if (cache->tokenStride < cache->dim || cache->headStride < 0 || cache->pageStride < 0 ||
       cache->tokenStride % 16 || cache->headStride % 16 || cache->pageStride % 16 ||
@@ -211,7 +211,7 @@ const struct {
     {"hc_gemm_w4_", "gemm_w4"},
     {"hc_dequant_w4_", "gemm_w4"},
     {"hc_repack_", "gemm_w4"},
-    {"hc_kv_append_", "kv_append"},       // _{i8,e4m3}
+    {"hc_kv_append_", "kv_append"},       // _{i8,e4m3}_{warp,cta}
     {"hc_kv_attention_", "kv_attention"}, // _{i8,e4m3}_d{64,128,256}_r{1,2}[_any]
 };
 
@@ -481,9 +481,18 @@ int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place, cons
   if (blocks > 0x7fffffffLL)
     return c->fail("hcKvAppend: %d sequences of up to %d new tokens are too many", p.place.seqs,
                    p.place.maxNew);
+  // A warp per unit (a block's keys or values of one head) where they are many, or small
+  // (four turns of eight elements per lane); else a CTA.
+  const long long units = blocks * 2 * p.cache.heads;
+  const bool warps = units >= 16 * c->smCount ||
+                     (long long)std::min(p.place.maxNew, p.cache.block) * p.cache.dim <= 1024;
+  char name[64];
+  std::snprintf(name, sizeof name, "hc_kv_append_%s_%s", p.cache.dtype == HC_I8 ? "i8" : "e4m3",
+                warps ? "warp" : "cta");
   void *args[] = {&p};
-  return c->launch(p.cache.dtype == HC_I8 ? "hc_kv_append_i8" : "hc_kv_append_e4m3",
-                   size_t(blocks), size_t(ceilDiv(2 * p.cache.heads, 4)), 1, 128, args, 1, 0);
+  return c->launch(name, size_t(blocks),
+                   size_t(warps ? ceilDiv(2 * p.cache.heads, 4) : 2 * p.cache.heads), 1,
+                   warps ? 128 : 256, args, 1, 0);
 }
 
 size_t hcKvAttentionWorkspaceBytes(HcContext c) {

@@ -232,42 +232,76 @@ def test_w4_refusals_and_choice(recording):
     refused("null buffer", w4, a_dtype=capi.HC_I8)
     refused("null buffer", w4, out=None)
     refused("null buffer", w4, scale=None)
-    refused("workspace", w4, m=65, ws=None)
-    refused("workspace", w4, m=65, ws_bytes=4096 * 4096 * 2 - 1)
-    refused("workspace", w4, m=65, ws=P + 8)
+    refused("workspace", w4, m=1025, ws=None)
+    refused("workspace", w4, m=1025, ws_bytes=4096 * 4096 * 2 - 1)
+    refused("workspace", w4, m=9, a_dtype=capi.HC_I8, a_scale=P, ws=None)
+    refused("workspace", w4, m=9, lda=4097, ws_bytes=9 * 8192 - 1)
+    refused("workspace", w4, m=9, w=P + 8, ws_bytes=4096 * 2048 - 1)
+    refused("workspace", w4, m=1025, ws=P + 8)
     w4(m=0); w4(n=0)
     assert not launches()
-    lib = hc.lib
-    assert lib.hcGemmW4FewRows() == 64
-    assert lib.hcGemmW4WorkspaceBytes(64, 4096, 4096, capi.HC_BF16) == 0
-    assert lib.hcGemmW4WorkspaceBytes(65, 4090, 4097, capi.HC_BF16) == 4096 * 4097 * 2
-    assert lib.hcGemmW4WorkspaceBytes(65, 4090, 4097, capi.HC_I8) == 4096 * 4097 * 2 + 65 * 4104 * 2
-    for kw, kernel in ((dict(), "bf16_coarse_m1"), (dict(m=9), "bf16_coarse_m2"),
-                       (dict(m=33, group=64), "bf16_fine_m8"),
-                       (dict(m=17, group=1 << 20), "bf16_coarse_m4"),
-                       (dict(a_dtype=capi.HC_I8, a_scale=P), "i8_coarse_m1"),
-                       (dict(w=P + 1), "bf16_coarse_m1_any"),
-                       (dict(k=4098, ldw=2064), "bf16_coarse_m1_any")):
+    need = lambda m, n, k, lda, ldw, t=capi.HC_BF16: hc.lib.hcGemmW4WorkspaceBytes(m, n, k, lda, ldw, t)
+    up = lambda x, to: -(-x // to) * to
+    assert need(1024, 4096, 4096, 4096, 2048) == 0
+    assert need(64, 4090, 4097, 4097, 2064) == up(64 * 4104 * 2, 256)
+    assert need(64, 4090, 4097, 4104, 2049) == 4090 * 2064
+    assert need(64, 4096, 4096, 4096, 2048, capi.HC_I8) == 64 * 4096 * 2
+    assert need(1025, 4090, 4096, 4096, 2048) == 4096 * 4096 * 2
+    assert need(1025, 4096, 4096, 4096, 2048, capi.HC_I8) == (1025 + 4096) * 4096 * 2
+    # Few rows: one launch.
+    for kw, kernel in ((dict(), "bf16_coarse"), (dict(m=8), "bf16_coarse"),
+                       (dict(m=3, group=64), "bf16_fine"),
+                       (dict(m=5, group=1 << 20), "bf16_coarse"),
+                       (dict(a_dtype=capi.HC_I8, a_scale=P), "i8_coarse"),
+                       (dict(w=P + 1), "bf16_coarse_any"),
+                       (dict(k=4098, ldw=2064), "bf16_coarse_any")):
         w4(**kw)
         (name, grid, block, smem, _), = launches()
         assert name == "hc_gemm_w4_" + kernel, name
-        assert grid[0] == 32 and grid[1] in (1, 2, 4, 8) and block == 256 and smem <= 227 << 10
-    # Whatever the sizes: shared memory within a CTA's limit.
+        assert grid == (148, 1, 1) and block == 512 and smem <= 227 << 10
+    # More rows: the tcgen05 kernel, the K axis divided where there are few tiles.
+    for kw, names, grid in (
+            (dict(m=9), ["narrow_coarse_bf16"], (32, 8, 1)),
+            (dict(m=64, group=32, lds=128, scale_dtype=capi.HC_F32), ["narrow_fine_f32"], (32, 8, 1)),
+            (dict(m=65), ["wide_coarse_bf16"], (32, 4, 1)),
+            (dict(m=1024), ["wide_coarse_bf16"], (128, 1, 1)),
+            (dict(m=16, n=130, k=100, lda=104, ldw=64), ["narrow_coarse_bf16"], (2, 1, 1)),
+            (dict(m=16, w=P + 4), ["copy", "narrow_coarse_bf16"], (32, 8, 1)),
+            (dict(m=16, lda=4097), ["hc_repack_a16_bf16", "narrow_coarse_bf16"], (32, 8, 1)),
+            (dict(m=16, a_dtype=capi.HC_I8, a_scale=P), ["hc_repack_a8_bf16", "narrow_coarse_bf16"],
+             (32, 8, 1))):
+        w4(**kw)
+        got = launches()
+        assert len(got) == len(names), got
+        for (name, *_), want in zip(got, names):
+            assert want in name, (name, want)
+        name, shape, block, smem, _ = got[-1]
+        assert shape == grid, (kw, shape)
+        assert block == (384 if "narrow" in name else 640)
+        assert smem <= (113 if "narrow" in name else 227) << 10
+    # Whatever the sizes: shared memory within a CTA's limit, a cluster of at most eight.
     import random
     rng = random.Random(0)
     for _ in range(500):
         k = rng.choice([1, 31, 128, 4096, 30000, 1 << 20])
         group = 32 * rng.choice([1, 2, 3, 4, 8, 1000])
-        w4(m=rng.randint(1, 64), n=rng.choice([1, 500, 100000]), k=k, group=group,
-           ldw=(k + 1) // 2, lds=1 << 16, a_dtype=rng.choice([capi.HC_BF16, capi.HC_I8]),
-           a_scale=P)
-        (name, grid, block, smem, _), = launches()
-        assert smem <= 200 << 10, (name, smem, k, group)
-    w4(m=300)
+        w4(m=rng.randint(1, 1024), n=rng.choice([1, 500, 100000]), k=k, group=group,
+           lda=k + 7 & ~7, ldw=((k + 1) // 2) + 15 & ~15, lds=1 << 16, ldz=1 << 16,
+           zero=rng.choice([None, P]), a_dtype=rng.choice([capi.HC_BF16, capi.HC_I8]), a_scale=P)
+        name, grid, block, smem, _ = launches()[-1]
+        assert smem <= 227 << 10, (name, smem, k, group)
+        assert "umma" not in name or grid[1] <= 8
+    w4(m=1025)
     assert [l[0] for l in launches()] == ["hc_dequant_w4_bf16", "hc_gemm_bf16_umma_pair"]
-    w4(m=300, a_dtype=capi.HC_I8, a_scale=P)
-    assert [l[0] for l in launches()] == ["hc_dequant_w4_bf16", "hc_dequant_a8_bf16",
+    w4(m=1025, a_dtype=capi.HC_I8, a_scale=P)
+    assert [l[0] for l in launches()] == ["hc_repack_a8_bf16", "hc_dequant_w4_bf16",
                                           "hc_gemm_bf16_umma_pair"]
+    # The choice can be made by hand.
+    hc.set_option("w4_variant", 2)
+    w4()
+    assert launches()[0][0] == "hc_gemm_w4_umma_narrow_coarse_bf16"
+    hc.set_option("w4_variant", 1)
+    refused("few rows", w4, m=9)
     """)
 
 
@@ -303,6 +337,10 @@ def test_cache_refusals_and_choice(recording):
         refused("16-byte aligned", call, cache(pageStride=8))
         refused("16-byte aligned", call, cache(v=P + 8))
         refused("scale pitch", call, cache(scalePitch=3))
+        refused("spans 2^31", call, cache(tokenStride=1 << 27))
+        refused("below 2^31", call, cache(pageStride=1 << 31))
+        refused("below 2^31", call, cache(scalePitch=1 << 31))
+        refused("pages of", call, cache(heads=1 << 15, scalePitch=1 << 15))
         refused("null cache buffer", call, cache(kScale=None))
         refused("invalid place", call, p=place(seqs=-1))
         refused("invalid place", call, p=place(maxNew=-1))
@@ -318,9 +356,9 @@ def test_cache_refusals_and_choice(recording):
     append(p=place(maxNew=0)); append(cache(pages=0))
     assert not launches()
     append()
-    assert launches()[0][:3] == ("hc_kv_append_i8", (8, 2, 1), 128)
+    assert launches()[0][:3] == ("hc_kv_append_i8_warp", (8, 2, 1), 128)
     append(cache(dtype=capi.HC_E4M3), place(maxNew=40, tokens=300))
-    assert launches()[0][:3] == ("hc_kv_append_e4m3", (8 * 4, 2, 1), 128)
+    assert launches()[0][:3] == ("hc_kv_append_e4m3_cta", (8 * 4, 8, 1), 256)
     append(p=place(maxNew=40, tokens=300, starts=None))  # one row per sequence
     assert launches()[0][1] == (8, 2, 1)
     refused("too many", append, p=place(seqs=1 << 30, maxNew=100, tokens=1 << 30))
@@ -371,8 +409,8 @@ def test_every_serving_kernel_is_found_by_its_name():
     from tests.test_abi_cpu import _elf_symbols
 
     lib = capi.load_kernels()
-    for image, count in (("add_rms_norm", 60), ("gemm_w4", 34), ("kv_append", 2),
-                         ("kv_attention", 10)):
+    for image, count in (("add_rms_norm", 60), ("gemm_w4", 11), ("gemm_w4_umma", 8),
+                         ("kv_append", 4), ("kv_attention", 20)):
         blob = (REPO / "hc_b200" / "_native" / f"{image}.cubin").read_bytes()
         names = [s for s in _elf_symbols(blob) if s.startswith("hc_")]
         assert len(names) == count, (image, len(names))
