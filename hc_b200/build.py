@@ -50,7 +50,7 @@ KERNEL_SOURCES = [
     "add_rms_norm",
     "gemm_w4", "gemm_w4_umma",
     "kv_append",
-    "kv_attention",
+    "kv_attention", "kv_attention_umma",
     "selftest",
 ]
 

@@ -1,0 +1,845 @@
+// Attention over the paged 8-bit key/value cache for many query rows per key/value head
+// (chunks of a prompt, and drafts whose query heads share a head); the formula, the
+// scales, the masks and the roundings are those of kv_attention.cu.
+//
+// 128 query rows against T tokens (128, or 64 for heads of 256) at a time on tcgen05:
+//   S[128, T] = Q K^T       Q and K in shared memory, f16
+//   O[128, D] += P V        P in tensor memory (f16), V in shared memory as it lies in
+//                           the cache, tokens by dims: an MN-major operand
+// Roles of a CTA, which keeps to one unit (sequence, head, 128 rows), or a part of its
+// tokens where there are few units:
+//   * 8 warps bring the keys and values of a tile from the cache into registers a tile
+//     ahead, widen them to f16 (exact) and store them in the swizzled layout;
+//   * one thread issues the MMAs: the scores of tile j + 1 before the outputs of tile j;
+//   * two groups of 4 warps take the score tiles in turn, a thread per row: maximum,
+//     exponentials, sum, and P back to tensor memory.  Only the reference that the
+//     exponentials are taken against is handed from tile to tile; it is kept until the
+//     maximum has grown by 2^4 over it, so O is rescaled in place a few times per unit.
+// Per tile of 128 x 128 x 128 the MMAs take 1024 cycles, the exponentials 1024 (16 per
+// cycle), and the instructions of widening and softmax about as many issue slots: the
+// three run beside each other.  Reading the cache is small beside that (32 KiB a tile,
+// mostly from L2).
+#include "kv_params.h"
+#include "serving_math.cuh"
+
+using namespace hc;
+using namespace hcs;
+
+namespace {
+
+struct KvRowsParams {
+  HcKvCacheDev cache;
+  HcKvPlaceDev place;
+  const __nv_bfloat16 *q; // [tokens, heads * share, dim]
+  __nv_bfloat16 *out;
+  float *lse; // [tokens, heads * share] or null
+  long long qTokenStride, qHeadStride, outTokenStride, outHeadStride, lseStride;
+  float scaleLog2; // scale * log2(e)
+  int share;       // query heads per key/value head
+  int window;      // 0: none
+  int rowTiles;    // tiles of 128 rows that maxNew * share rows can take
+  int splits;      // parts that a unit's tokens may be divided into
+  // Quotients by products (ceil(2^32 / n), 0 for n = 1): of a position's sixteens by a
+  // block's, of a query row by `share`.
+  uint32_t blockInverse, shareInverse;
+  int vecQ;           // rows of q that 16-byte loads can take
+  unsigned *counters; // [units], zero between calls
+  float *partial;     // [units][splits] slots
+  int *status;
+};
+
+constexpr int kThreads = 17 * 32;
+constexpr int kConvertWarps = 8, kMmaWarp = 16; // warps 8..15 convert
+constexpr float kNegInf = -INFINITY;
+constexpr float kSlack = 4.0f;
+constexpr float kWeight = 2048.0f; // 2^(15 - kSlack): probabilities fit f16
+constexpr int kStatusRowsConvert = 9, kStatusRowsSoftmax = 10;
+
+__device__ __forceinline__ float exp2Approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t halfPair(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Two floats at a time.
+__device__ __forceinline__ uint64_t pairOf(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Four stored elements -> two f16 pairs, exactly.  int8: 0x6400 | u is 1024 + u in f16,
+// with the sign bit flipped u = x + 128, and 1152 comes off again.
+template <class Q> __device__ __forceinline__ uint2 widen(uint32_t w) {
+  uint2 r;
+  if constexpr (__is_same(Q, I8)) {
+    const uint32_t bias = 0x64806480u, x = w ^ 0x80808080u;
+    const __half2 b = *reinterpret_cast<const __half2 *>(&bias);
+    const uint32_t lo = __byte_perm(x, 0x64646464u, 0x4140);
+    const uint32_t hi = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 l = __hsub2(*reinterpret_cast<const __half2 *>(&lo), b);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&hi), b);
+    r.x = *reinterpret_cast<const uint32_t *>(&l);
+    r.y = *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r.x) : "h"(uint16_t(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r.y) : "h"(uint16_t(w >> 16)));
+  }
+  return r;
+}
+
+// Instruction descriptor of kind::f16 with f16 inputs and f32 accumulation.
+__host__ __device__ constexpr uint32_t instrDescF16(int m, int n, bool bMnMajor) {
+  return (1u << 4) | (uint32_t(bMnMajor) << 16) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] * B[smem], f16.
+__device__ __forceinline__ void ummaTmemA(uint32_t dTmem, uint32_t aTmem, uint64_t bDesc,
+                                          uint32_t iDesc, uint32_t accumulate) {
+  asm volatile("{\n"
+               ".reg .pred p;\n"
+               "setp.ne.b32 p, %4, 0;\n"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+               "}\n" ::"r"(dTmem),
+               "r"(aTmem), "l"(bDesc), "r"(iDesc), "r"(accumulate)
+               : "memory");
+}
+
+// Waits for the loads in flight; what depends on `v` stays behind it.
+__device__ __forceinline__ void tmemLoadWaitFor(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
+                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),
+                 "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
+                 "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]),
+                 "+r"(v[27]), "+r"(v[28])
+               :
+               : "memory");
+  asm volatile("" : "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+
+struct alignas(8) RowsBarriers {
+  uint64_t keysFull[2], valuesFull[2]; // the converting warps
+  uint64_t scored[2];                  // S written, the keys read (MMA commit)
+  uint64_t weighted[2];                // P written (the warps of a group)
+  uint64_t decided[2];                 // the reference of a tile stands
+  uint64_t added[2];                   // P and the values read, O complete (MMA commit)
+  uint32_t tmemBase;
+  int abortFlag;
+};
+
+// The scales of 16 tokens; there = 0: the table names no page for them.
+struct alignas(16) Group {
+  float key, value, logValue, there; // value: times kWeight
+};
+
+template <int DimCap> struct RowsShape {
+  static constexpr int tokens = DimCap == 256 ? 64 : 128;
+  static constexpr int groups = tokens / 16;
+  static constexpr uint32_t chunkBytes = tokens * 128; // 64 dims of a tile's tokens
+  static constexpr uint32_t tileBytes = chunkBytes * (DimCap / 64);
+  static constexpr uint32_t qBytes = 128 * 128 * (DimCap / 64);
+  // (Shared memory: qBytes + 4 * tileBytes + 1024 to align.)
+  // Tensor memory columns: two tiles of scores, the outputs, two of weights.
+  static constexpr uint32_t atO = 2 * tokens, atP = atO + DimCap;
+  static constexpr int lanesPerRow = DimCap / 16;
+  static constexpr int rowsPerTurn = 256 / lanesPerRow;
+  static constexpr int turns = tokens / rowsPerTurn;
+  static constexpr int slotFloats = 128 * (DimCap + 2);
+};
+
+template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const KvRowsParams &p) {
+  using S = RowsShape<DimCap>;
+  constexpr int T = S::tokens;
+  extern __shared__ __align__(16) unsigned char smemRaw[];
+  __shared__ RowsBarriers bars;
+  __shared__ Group sGroup[4][S::groups];
+  __shared__ float sFactor[128]; // of a query row: its power of two, scale * log2(e)
+  __shared__ float sRef[128], sSum[2][128], sSumRef[2][128];
+  __shared__ int sPoisoned, sLast;
+  const HcKvCacheDev &c = p.cache;
+  const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+
+  // ---- the unit ------------------------------------------------------------------------
+  // Later rows see more tokens: they go first.
+  const unsigned lower = unsigned(blockIdx.x) / unsigned(c.heads);
+  const int head = int(blockIdx.x - lower * unsigned(c.heads));
+  const unsigned higher = lower / unsigned(p.place.seqs);
+  const int seq = int(lower - higher * unsigned(p.place.seqs));
+  const int rowTile = p.rowTiles - 1 - int(higher);
+  const HcKvSpan span = hcKvLoadSpan(p.place, c.block, seq);
+  auto queryOf = [&](int r) {
+    return p.share == 1 ? r : int(__umulhi(uint32_t(r), p.shareInverse));
+  };
+  if (rowTile == 0 && blockIdx.y == 0 && span.count != span.allCount) {
+    // Rows without a place in the cache see nothing: zeros.
+    for (int row = span.allRow; row < span.allRow + span.allCount; ++row) {
+      if (row >= span.row && row < span.row + span.count)
+        continue;
+      for (int i = tid; i < p.share * c.dim; i += kThreads) {
+        const int h = i / c.dim, d = i - h * c.dim;
+        p.out[row * p.outTokenStride + (head * p.share + h) * p.outHeadStride + d] =
+            __float2bfloat16_rn(0.0f);
+        if (d == 0 && p.lse)
+          p.lse[row * p.lseStride + head * p.share + h] = kNegInf;
+      }
+    }
+  }
+  const int row0 = rowTile * 128;
+  const int rowsHere = min(128, span.count * p.share - row0);
+  if (rowsHere <= 0)
+    return;
+  const int firstPos = span.first + queryOf(row0);
+  const int lastPos = span.first + queryOf(row0 + rowsHere - 1);
+  // Some row sees positions [anyLo, lastPos], every row sees [allLo, firstPos].
+  const int anyLo = p.window > 0 ? max(0, firstPos - p.window + 1) : 0;
+  const int allLo = p.window > 0 ? max(0, lastPos - p.window + 1) : 0;
+  const int kvBegin = anyLo & ~15;
+  const int unitTiles = (lastPos - kvBegin) / T + 1;
+  // A part has four tiles at least.
+  const int parts = min(p.splits, max(1, unitTiles / 4));
+  if (int(blockIdx.y) >= parts)
+    return;
+  const int tile0 = int((long long)unitTiles * blockIdx.y / parts);
+  const int tiles = int((long long)unitTiles * (blockIdx.y + 1) / parts) - tile0;
+  const int pos0 = kvBegin + tile0 * T; // of the part's first tile
+
+  // ---- setting up -------------------------------------------------------------------------
+  const uint32_t smemBase = (smemAddr(smemRaw) + 1023u) & ~1023u;
+  unsigned char *smem = smemRaw + (smemBase - smemAddr(smemRaw));
+  volatile int *abortFlag = &bars.abortFlag;
+  int *status = p.status;
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbarInit(smemAddr(&bars.keysFull[s]), kConvertWarps);
+      mbarInit(smemAddr(&bars.valuesFull[s]), kConvertWarps);
+      mbarInit(smemAddr(&bars.scored[s]), 1);
+      mbarInit(smemAddr(&bars.weighted[s]), 4);
+      mbarInit(smemAddr(&bars.decided[s]), 4);
+      mbarInit(smemAddr(&bars.added[s]), 1);
+    }
+    bars.abortFlag = 0;
+    sPoisoned = 0;
+    fenceBarrierInit();
+  }
+  if (warp == kMmaWarp) {
+    tmemAlloc<1>(smemAddr(&bars.tmemBase), 512);
+    tmemRelinquish<1>();
+  } else {
+    // Query rows as f16, a power of two per row, K-major and swizzled: a warp takes 8.
+    constexpr int kPer = DimCap / 32; // consecutive elements of a lane
+#pragma unroll 1
+    for (int r0 = warp * 8; r0 < warp * 8 + 8; r0 += 4) {
+      uint32_t v[4][kPer / 2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          v[i][j] = 0;
+        if (r0 + i < rowsHere && lane * kPer < c.dim) {
+          const int qi = queryOf(row0 + r0 + i), gh = row0 + r0 + i - qi * p.share;
+          const __nv_bfloat16 *src = p.q + (long long)(span.row + qi) * p.qTokenStride +
+                                     (long long)(head * p.share + gh) * p.qHeadStride +
+                                     lane * kPer;
+          if (p.vecQ) {
+            if constexpr (kPer == 2) {
+              v[i][0] = *reinterpret_cast<const uint32_t *>(src);
+            } else if constexpr (kPer == 4) {
+              const uint2 x = *reinterpret_cast<const uint2 *>(src);
+              v[i][0] = x.x;
+              v[i][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4 *>(src);
+              v[i][0] = x.x;
+              v[i][1] = x.y;
+              v[i][2] = x.z;
+              v[i][3] = x.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              v[i][j >> 1] |= uint32_t(__bfloat16_as_ushort(src[j])) << (16 * (j & 1));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + i;
+        uint32_t top2 = 0; // magnitudes order like their bits
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          top2 = __vmaxu2(top2, v[i][j] & 0x7fff7fffu);
+        const uint32_t top =
+            __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16)) << 16;
+        // 2^e <= top < 2^(e+1); zero, subnormal and infinite rows keep their values.
+        const int e = int(top >> 23);
+        const bool plain = e == 0 || e == 255;
+        const float down = plain ? 1.0f : __uint_as_float(uint32_t(max(254 - e, 1)) << 23);
+        const float up = plain ? 1.0f : __uint_as_float(uint32_t(min(e, 253)) << 23);
+        if (lane == 0)
+          sFactor[r] = p.scaleLog2 * up;
+        const int byte = lane * kPer * 2, chunk = byte >> 7, in = byte & 127;
+        unsigned char *dst = smem + chunk * (128 * 128) + r * 128 +
+                             ((((in >> 4) ^ (r & 7)) << 4) | (in & 15));
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          *reinterpret_cast<uint32_t *>(dst + 4 * j) =
+              halfPair(__uint_as_float(v[i][j] << 16) * down,
+                       __uint_as_float(v[i][j] & 0xffff0000u) * down);
+      }
+    }
+    fenceProxyAsync();
+  }
+  tcgen05FenceBefore();
+  __syncthreads();
+  tcgen05FenceAfter();
+  const uint32_t tmemBase = bars.tmemBase;
+  const uint32_t kBase = smemBase + S::qBytes, vBase = kBase + 2 * S::tileBytes;
+
+  // Lane 0 waits for the warp.
+  auto await = [&](uint64_t &bar, int use, int code) {
+    bool ok = true;
+    if (lane == 0)
+      ok = mbarWait(smemAddr(&bar), uint32_t(use) & 1u, abortFlag, status, code);
+    return __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+  };
+
+  bool ok = true;
+  if (warp == kMmaWarp) {
+    // ------------------------------- MMA issuer ---------------------------------
+    if (lane == 0) {
+      constexpr uint32_t scoreDesc = instrDescF16(128, T, false);
+      constexpr uint32_t outDesc = instrDescF16(128, DimCap, true);
+      auto score = [&](int j) {
+        const int b = j & 1;
+        if (!mbarWait(smemAddr(&bars.keysFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                      kStatusMmaWaitData))
+          return false;
+        tcgen05FenceAfter();
+#pragma unroll
+        for (int kk = 0; kk < DimCap / 16; ++kk) {
+          const uint64_t a =
+              makeSmemDesc(smemBase + (kk >> 2) * (128 * 128), 16, 1024) + uint64_t((kk & 3) * 2);
+          const uint64_t k =
+              makeSmemDesc(kBase + b * S::tileBytes + (kk >> 2) * S::chunkBytes, 16, 1024) +
+              uint64_t((kk & 3) * 2);
+          umma<1>(tmemBase + uint32_t(b * T), a, k, scoreDesc, kk != 0);
+        }
+        ummaCommit(smemAddr(&bars.scored[b]));
+        return true;
+      };
+      ok = score(0);
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int b = j & 1;
+        // (The scores of tile j - 1 have been read: its weights were waited for.)
+        ok = (j + 1 >= tiles || score(j + 1)) &&
+             mbarWait(smemAddr(&bars.valuesFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                      kStatusMmaWaitData) &&
+             mbarWait(smemAddr(&bars.weighted[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                      kStatusMmaWaitTmem);
+        if (!ok)
+          break;
+        tcgen05FenceAfter();
+#pragma unroll
+        for (int kk = 0; kk < T / 16; ++kk)
+          ummaTmemA(tmemBase + S::atO, tmemBase + S::atP + uint32_t(b * (T / 2) + kk * 8),
+                    makeSmemDesc(vBase + b * S::tileBytes, S::chunkBytes, 1024) +
+                        uint64_t(kk * 128),
+                    outDesc, (j | kk) != 0);
+        ummaCommit(smemAddr(&bars.added[b]));
+      }
+      if (!ok) { // MMAs may still be reading
+        const unsigned long long t0 = globalTimerNs();
+        while (globalTimerNs() - t0 < 1000000ull) {
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------- converters ---------------------------------
+    const int ct = tid - 256;
+    const int piece = ct % S::lanesPerRow, rowOf = ct / S::lanesPerRow;
+    const bool inDim = piece * 16 < c.dim;
+    const int *table = p.place.table + (long long)seq * p.place.tablePitch;
+    const uint8_t *const keys =
+        static_cast<const uint8_t *>(c.k) + (long long)head * c.headStride + piece * 16;
+    const uint8_t *const values =
+        static_cast<const uint8_t *>(c.v) + (long long)head * c.headStride + piece * 16;
+    // Where the two 16-byte chunks go within a row (the second half of a row's lanes in
+    // the other order: no two lanes of a store phase share banks).
+    const int swap = (piece >> 2) & 1;
+    const uint32_t chunkAt = uint32_t(piece >> 2) * S::chunkBytes;
+    const int first16 = (piece & 3) * 2;
+
+    struct Spot {
+      int page; // < 0: not there, or seen by no row
+      uint32_t row;
+    };
+    Spot spot[S::turns];
+    uint4 kReg[S::turns], vReg[S::turns];
+    float kScale[S::turns], vScale[S::turns];
+    const bool scales = piece == 0 && (rowOf & 15) == 0;
+    auto look = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i) {
+        const int pos = pos0 + j * T + i * S::rowsPerTurn + rowOf;
+        int block = pos >> 4;
+        if (c.block > 16)
+          block = int(__umulhi(uint32_t(block), p.blockInverse));
+        spot[i].page = -1;
+        spot[i].row = uint32_t(pos - block * c.block) * uint32_t(c.tokenStride);
+        // (A group of 16 tokens that some row sees has its scales and page looked up.)
+        if (j < tiles && (pos | 15) >= anyLo && (pos & ~15) <= lastPos)
+          spot[i].page = hcKvPageOf(__ldg(table + block), c.pages);
+      }
+    };
+    auto seen = [&](int j, int i) { // by some row
+      const int pos = pos0 + j * T + i * S::rowsPerTurn + rowOf;
+      return spot[i].page >= 0 && inDim && pos >= anyLo && pos <= lastPos;
+    };
+    auto load = [&](int j, const uint8_t *from, uint4 (&reg)[S::turns]) {
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i)
+        reg[i] = seen(j, i) ? __ldg(reinterpret_cast<const uint4 *>(
+                                  from + uint64_t(uint32_t(spot[i].page)) * uint32_t(c.pageStride) +
+                                  spot[i].row))
+                            : make_uint4(0, 0, 0, 0);
+    };
+    auto loadScales = [&]() {
+      if (!scales)
+        return;
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i) {
+        kScale[i] = vScale[i] = 0.0f;
+        if (spot[i].page >= 0) {
+          const uint64_t at = uint64_t(uint32_t(spot[i].page)) * uint32_t(c.scalePitch) + head;
+          kScale[i] = __ldg(c.kScale + at);
+          vScale[i] = __ldg(c.vScale + at);
+        }
+      }
+    };
+    auto store = [&](uint32_t base, const uint4 (&reg)[S::turns]) {
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i) {
+        const int r = i * S::rowsPerTurn + rowOf;
+        const uint2 a = widen<Q>(reg[i].x), b = widen<Q>(reg[i].y);
+        const uint2 d = widen<Q>(reg[i].z), e = widen<Q>(reg[i].w);
+        const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(d.x, d.y, e.x, e.y);
+        unsigned char *row = smem + (base - smemBase) + chunkAt + r * 128;
+        *reinterpret_cast<uint4 *>(row + (((first16 + swap) ^ (r & 7)) << 4)) = swap ? hi : lo;
+        *reinterpret_cast<uint4 *>(row + (((first16 + 1 - swap) ^ (r & 7)) << 4)) =
+            swap ? lo : hi;
+      }
+      fenceProxyAsync();
+      __syncwarp();
+    };
+    // NaN among the values (e4m3 only) must not reach rows that do not see its token:
+    // 0 * NaN is NaN.  Where some rows see the token and others do not, zeros stand in
+    // for them and the rows that do are mended at the end.
+    auto clean = [&](int j) {
+      if constexpr (__is_same(Q, E4M3)) {
+        const int pos = pos0 + j * T;
+        if (pos >= allLo && pos + T - 1 <= firstPos)
+          return;
+#pragma unroll
+        for (int i = 0; i < S::turns; ++i) {
+          const int at = pos + i * S::rowsPerTurn + rowOf;
+          if (at >= allLo && at <= firstPos)
+            continue;
+          uint32_t *w = &vReg[i].x, bad = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t nan = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            w[k] &= ~nan;
+            bad |= nan;
+          }
+          if (bad)
+            sPoisoned = 1;
+        }
+      }
+    };
+
+    look(0);
+    load(0, keys, kReg);
+    load(0, values, vReg);
+    loadScales();
+    for (int j = 0; j < tiles; ++j) {
+      const int b = j & 1;
+      if (scales) { // (slot j - 4 has been read: the outputs of tile j - 3 were waited for)
+#pragma unroll
+        for (int i = 0; i < S::turns; ++i) {
+          Group g;
+          g.key = kScale[i];
+          g.value = vScale[i] * kWeight;
+          g.logValue = vScale[i] > 0.0f && vScale[i] < INFINITY ? fmaxf(__log2f(vScale[i]), -96.0f)
+                                                                 : 0.0f;
+          g.there = spot[i].page >= 0 ? 1.0f : 0.0f;
+          sGroup[j & 3][(i * S::rowsPerTurn + rowOf) >> 4] = g;
+        }
+      }
+      clean(j);
+      look(j + 1);
+      if (j >= 2 && !(ok = await(bars.scored[b], (j >> 1) - 1, kStatusRowsConvert)))
+        break;
+      store(kBase + b * S::tileBytes, kReg);
+      if (lane == 0)
+        mbarArrive(smemAddr(&bars.keysFull[b]));
+      load(j + 1, keys, kReg);
+      loadScales();
+      if (j >= 2 && !(ok = await(bars.added[b], (j >> 1) - 1, kStatusRowsConvert)))
+        break;
+      store(vBase + b * S::tileBytes, vReg);
+      if (lane == 0)
+        mbarArrive(smemAddr(&bars.valuesFull[b]));
+      load(j + 1, values, vReg);
+    }
+  } else {
+    // --------------------------------- softmax -----------------------------------
+    const int group = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t laneBase = uint32_t((warp & 3) * 32) << 16;
+    const float rowFactor = sFactor[r];
+    const int qi = queryOf(row0 + min(r, rowsHere - 1));
+    const int seenHi = span.first + qi;
+    const int seenLo = p.window > 0 ? max(0, seenHi - p.window + 1) : 0;
+    float ref = kNegInf; // what `sum` was taken against
+    float sum = 0.0f;
+    for (int j = group; j < tiles; j += 2) {
+      const int b = j & 1, pos = pos0 + j * T;
+      if (!(ok = await(bars.scored[b], j >> 1, kStatusRowsSoftmax)))
+        break;
+      tcgen05FenceAfter();
+      const Group *const groups = sGroup[j & 3];
+      const uint32_t sAt = tmemBase + laneBase + uint32_t(b * T);
+      const uint32_t pAt = tmemBase + laneBase + S::atP + uint32_t(b * (T / 2));
+      const bool whole = pos >= allLo && pos + T - 1 <= firstPos;
+      uint32_t s[2][32];
+
+      // The largest score with its value scale.
+      float top = kNegInf;
+      tmemLoad32x32(sAt, s[0]);
+#pragma unroll
+      for (int k = 0; k < T / 32; ++k) {
+        uint32_t(&v)[32] = s[k & 1];
+        tmemLoadWaitFor(v);
+        if (k + 1 < T / 32)
+          tmemLoad32x32(sAt + 32 * (k + 1), s[(k + 1) & 1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Group g = groups[2 * k + h];
+          const float f = g.key * rowFactor;
+          if (g.there == 0.0f)
+            continue;
+          float most = kNegInf;
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int at = pos + 32 * k + 16 * h + i;
+              if (at >= seenLo && at <= seenHi)
+                most = fmaxf(most, __uint_as_float(v[16 * h + i]) * f);
+            }
+          } else if (f >= 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              most = fmaxf(most, __uint_as_float(v[16 * h + i]));
+            most *= f;
+          } else {
+            most = INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              most = fminf(most, __uint_as_float(v[16 * h + i]));
+            most *= f;
+          }
+          top = fmaxf(top, most + g.logValue);
+        }
+      }
+
+      // The reference: handed on by the tile before.
+      float old = kNegInf;
+      if (j > 0) {
+        if (!(ok = await(bars.decided[b ^ 1], (j - 1) >> 1, kStatusRowsSoftmax)))
+          break;
+        old = sRef[r];
+      }
+      const float now = top > old + kSlack ? top : old;
+      if (now != old || j == 0)
+        sRef[r] = now;
+      __syncwarp();
+      if (lane == 0)
+        mbarArrive(smemAddr(&bars.decided[b]));
+      if (now != ref) {
+        sum *= exp2Approx(ref - now); // (0 against -inf: there was no sum)
+        ref = now;
+      }
+      if (__any_sync(0xffffffffu, now != old) && j > 0) {
+        if (!(ok = await(bars.added[b ^ 1], (j - 1) >> 1, kStatusRowsSoftmax)))
+          break;
+        tcgen05FenceAfter();
+        const float f = now == old ? 1.0f : exp2Approx(old - now);
+#pragma unroll 1
+        for (int d = 0; d < DimCap; d += 32) {
+          tmemLoad32x32(tmemBase + laneBase + S::atO + d, s[0]);
+          tmemLoadWaitFor(s[0]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              o[i] = __float_as_uint(__uint_as_float(s[0][8 * k + i]) * f);
+            tmemStore32x8(tmemBase + laneBase + S::atO + d + 8 * k, o);
+          }
+        }
+      }
+      // The weights of tile j - 2 have been read.
+      if (j >= 2 && !(ok = await(bars.added[b], (j >> 1) - 1, kStatusRowsSoftmax)))
+        break;
+
+      const float base = now == kNegInf ? 0.0f : now;
+      const uint64_t minusBase = pairOf(-base, -base);
+      uint64_t sum2 = pairOf(0.0f, 0.0f);
+      tmemLoad32x32(sAt, s[0]);
+#pragma unroll
+      for (int k = 0; k < T / 32; ++k) {
+        uint32_t(&v)[32] = s[k & 1];
+        tmemLoadWaitFor(v);
+        if (k + 1 < T / 32)
+          tmemLoad32x32(sAt + 32 * (k + 1), s[(k + 1) & 1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Group g = groups[2 * k + h];
+          const float f = g.key * rowFactor;
+          uint32_t w[8];
+          if (g.there == 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              w[i] = 0;
+          } else if (whole) {
+            const uint64_t f2 = pairOf(f, f), v2 = pairOf(g.value, g.value);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint64_t x = fma2(pairOf(__uint_as_float(v[16 * h + 2 * i]),
+                                       __uint_as_float(v[16 * h + 2 * i + 1])),
+                                f2, minusBase);
+              float lo, hi;
+              unpair(x, lo, hi);
+              x = pairOf(exp2Approx(lo), exp2Approx(hi));
+              sum2 = add2(sum2, x);
+              unpair(mul2(x, v2), lo, hi);
+              w[i] = halfPair(lo, hi);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float e[2];
+#pragma unroll
+              for (int k2 = 0; k2 < 2; ++k2) {
+                const int at = pos + 32 * k + 16 * h + 2 * i + k2;
+                const bool in = at >= seenLo && at <= seenHi;
+                const float x =
+                    exp2Approx(fmaf(__uint_as_float(v[16 * h + 2 * i + k2]), f, -base));
+                sum += in ? x : 0.0f;
+                e[k2] = in ? x * g.value : 0.0f;
+              }
+              w[i] = halfPair(e[0], e[1]);
+            }
+          }
+          tmemStore32x8(pAt + uint32_t(16 * k + 8 * h), w);
+        }
+      }
+      float lo, hi;
+      unpair(sum2, lo, hi);
+      sum += lo + hi;
+      tmemStoreWait();
+      tcgen05FenceBefore();
+      __syncwarp();
+      if (lane == 0)
+        mbarArrive(smemAddr(&bars.weighted[b]));
+    }
+    sSum[group][r] = sum;
+    sSumRef[group][r] = ref;
+  }
+  __syncwarp();
+  __syncthreads();
+
+  // ---- the outputs ---------------------------------------------------------------------------
+  const int unit = int(blockIdx.x);
+  auto slotOf = [&](int part) {
+    return p.partial + ((long long)unit * p.splits + part) * S::slotFloats;
+  };
+  auto finish = [&](int r, int d, float4 v, float f) {
+    const int qi = queryOf(row0 + r), gh = row0 + r - qi * p.share;
+    __nv_bfloat162 x = __floats2bfloat162_rn(v.x * f, v.y * f);
+    __nv_bfloat162 y = __floats2bfloat162_rn(v.z * f, v.w * f);
+    uint2 packed;
+    packed.x = *reinterpret_cast<uint32_t *>(&x);
+    packed.y = *reinterpret_cast<uint32_t *>(&y);
+    if (d < c.dim)
+      *reinterpret_cast<uint2 *>(p.out + (long long)(span.row + qi) * p.outTokenStride +
+                                 (long long)(head * p.share + gh) * p.outHeadStride + d) = packed;
+  };
+  auto finishSum = [&](int r, float top, float sum) {
+    const int qi = queryOf(row0 + r), gh = row0 + r - qi * p.share;
+    if (p.lse)
+      p.lse[(long long)(span.row + qi) * p.lseStride + head * p.share + gh] =
+          sum == 0.0f ? kNegInf : (top + __log2f(sum)) * 0.693147180559945309f;
+  };
+  const bool aborted = *abortFlag != 0;
+  if (warp < 8 && !aborted) {
+    if (await(bars.added[(tiles - 1) & 1], (tiles - 1) >> 1, kStatusEpilogueWait)) {
+      tcgen05FenceAfter();
+      const int group = warp >> 2, r = (warp & 3) * 32 + lane;
+      const float top = sRef[r];
+      float sum = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float part = sSum[g][r], against = sSumRef[g][r];
+        sum += against == top ? part : part * exp2Approx(against - top);
+      }
+      const float f = sum == 0.0f ? 0.0f : 1.0f / (kWeight * sum);
+      float *slot = slotOf(int(blockIdx.y));
+      const int qi = queryOf(row0 + min(r, rowsHere - 1));
+      const int seenHi = span.first + qi;
+      const int seenLo = p.window > 0 ? max(0, seenHi - p.window + 1) : 0;
+#pragma unroll 1
+      for (int d0 = group * (DimCap / 2); d0 < (group + 1) * (DimCap / 2); d0 += 32) {
+        uint32_t v[32];
+        tmemLoad32x32(tmemBase + (uint32_t((warp & 3) * 32) << 16) + S::atO + d0, v);
+        tmemLoadWaitFor(v);
+        if (r >= rowsHere)
+          continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float4 o = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                 __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+          if (__is_same(Q, E4M3) && sPoisoned && d0 + 4 * i < c.dim) {
+            // The row's tokens that not every row sees: [seenLo, allLo) and (firstPos, seenHi].
+            const int *table = p.place.table + (long long)seq * p.place.tablePitch;
+            const int end = min(seenHi, pos0 + tiles * T - 1);
+#pragma unroll 1
+            for (int at = max(seenLo, pos0); at <= end; ++at) {
+              if (at >= allLo && at <= firstPos) {
+                at = firstPos;
+                continue;
+              }
+              const int page = hcKvPageOf(table[at / c.block], c.pages);
+              if (page < 0)
+                continue;
+              const uint32_t w = *reinterpret_cast<const uint32_t *>(
+                  static_cast<const uint8_t *>(c.v) + (long long)page * c.pageStride +
+                  (long long)head * c.headStride + (long long)(at % c.block) * c.tokenStride +
+                  d0 + 4 * i);
+              const uint32_t nan = __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              const float bad = __uint_as_float(0x7fc00000u);
+              o.x = nan & 0xffu ? bad : o.x;
+              o.y = nan & 0xff00u ? bad : o.y;
+              o.z = nan & 0xff0000u ? bad : o.z;
+              o.w = nan & 0xff000000u ? bad : o.w;
+            }
+          }
+          if (parts == 1)
+            finish(r, d0 + 4 * i, o, f);
+          else // [dims / 4][rows]
+            __stcg(reinterpret_cast<float4 *>(slot) + (d0 / 4 + i) * 128 + r, o);
+        }
+      }
+      if (group == 0 && r < rowsHere) {
+        if (parts == 1) {
+          finishSum(r, top, sum);
+        } else {
+          __stcg(slot + 128 * DimCap + r, top);
+          __stcg(slot + 128 * DimCap + 128 + r, sum);
+        }
+      }
+      tcgen05FenceBefore();
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tcgen05FenceAfter();
+    tmemFree<1>(tmemBase, 512);
+  }
+  if (parts == 1)
+    return;
+
+  // ---- the last part to finish joins them, in their order ------------------------------------
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) // wraps to 0 with the last arrival
+    sLast = atomicInc(p.counters + unit, unsigned(parts - 1)) == unsigned(parts - 1);
+  __syncthreads();
+  if (!sLast)
+    return;
+  __threadfence();
+  float *const sWeight = reinterpret_cast<float *>(smem); // [part][rows]
+  if (tid < rowsHere) {
+    float top = kNegInf;
+    for (int x = 0; x < parts; ++x)
+      top = fmaxf(top, __ldcg(slotOf(x) + 128 * DimCap + tid));
+    float sum = 0.0f;
+    for (int x = 0; x < parts; ++x) {
+      const float part = __ldcg(slotOf(x) + 128 * DimCap + tid);
+      const float more = __ldcg(slotOf(x) + 128 * DimCap + 128 + tid);
+      // (a part whose scores are NaN has a sum but no maximum)
+      const float f = part == kNegInf ? 0.0f : exp2Approx(part - top);
+      sum += part == kNegInf ? more : more * f;
+      sWeight[x * 128 + tid] = f;
+    }
+    sSum[0][tid] = sum;
+    finishSum(tid, top, sum);
+  }
+  __syncthreads();
+  for (int i = tid; i < 128 * (DimCap / 4); i += kThreads) {
+    const int r = i & 127, d = (i >> 7) * 4;
+    if (r >= rowsHere)
+      continue;
+    float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int x = 0; x < parts; ++x) {
+      const float4 y = __ldcg(reinterpret_cast<const float4 *>(slotOf(x)) + i);
+      const float f = sWeight[x * 128 + r];
+      if (f != 0.0f) {
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+      }
+    }
+    finish(r, d, v, sSum[0][r] == 0.0f ? 0.0f : 1.0f / (kWeight * sSum[0][r]));
+  }
+}
+
+} // namespace
+
+#define HC_ATTENTION_ROWS(qname, Q, dim)                                                   \
+  extern "C" __global__ void __launch_bounds__(kThreads, 1)                                 \
+      hc_kv_attention_rows_##qname##_d##dim(const __grid_constant__ KvRowsParams p) {       \
+    attendRows<Q, dim>(p);                                                                  \
+  }
+HC_ATTENTION_ROWS(i8, I8, 64)
+HC_ATTENTION_ROWS(i8, I8, 128)
+HC_ATTENTION_ROWS(i8, I8, 256)
+HC_ATTENTION_ROWS(e4m3, E4M3, 64)
+HC_ATTENTION_ROWS(e4m3, E4M3, 128)
+HC_ATTENTION_ROWS(e4m3, E4M3, 256)

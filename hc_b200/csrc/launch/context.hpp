@@ -41,6 +41,7 @@ struct HcContextImpl {
   int pairSlotsF32 = 0; // the same for the float32 tensor-core kernel
   int pairSlotsBanded = 0; // the same for the dequant GEMM that converts band by band
   int pairSlotsW8 = 0;  // the same for the dequant GEMM that converts in its pipeline
+  long long attentionVariant = 0; // hcKvAttention: 1 sixteen rows at a time, 2 tcgen05
   long long w4Variant = 0; // hcGemmW4: 1 the kernel for few rows, 2 never that one
   long long w8Variant = 0; // 1: convert the weights in a pass of its own, 2: never
   // Programs without a precompiled body: 0 interpret them, 1 compile them at their

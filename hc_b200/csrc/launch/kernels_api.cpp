@@ -485,6 +485,12 @@ int hcSetOption(HcContext c, const char *name, long long value) {
     c->w4Variant = value;
     return 0;
   }
+  if (std::strcmp(name, "attention_variant") == 0 && value >= 0 && value <= 2) {
+    // hcKvAttention: 1 = 8 or 16 query rows at a time, a warp per part of the cache,
+    // 2 = 128 rows at a time on tcgen05, 0 = by the number of rows.
+    c->attentionVariant = value;
+    return 0;
+  }
   if (std::strcmp(name, "conv_stacked") == 0 && value >= 0 && value <= 1) {
     c->convStacked = value; // 1: hcConvF32Tensor never stacks b_hi and b_lo into one MMA
     return 0;

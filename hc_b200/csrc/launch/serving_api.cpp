@@ -94,6 +94,25 @@ struct AttentionParams {
   float *partial;
 };
 
+struct KvRowsParams {
+  HcKvCacheDev cache;
+  HcKvPlaceDev place;
+  const void *q;
+  void *out;
+  float *lse;
+  long long qTokenStride, qHeadStride, outTokenStride, outHeadStride, lseStride;
+  float scaleLog2;
+  int share;
+  int window;
+  int rowTiles;
+  int splits;
+  uint32_t blockInverse, shareInverse;
+  int vecQ;
+  unsigned *counters;
+  float *partial;
+  int *status;
+};
+
 static_assert(sizeof(HcKvCache) == sizeof(HcKvCacheDev) &&
                   offsetof(HcKvCache, dtype) == offsetof(HcKvCacheDev, dtype),
               "HcKvCache and its device form differ");
@@ -147,6 +166,37 @@ bool w4FitsFew(long long M, long long K, bool narrow, bool fine, long long group
 // the CTAs per SM that can hold two of them each.
 constexpr size_t kSlotFloats = 8 * 256 + 2 * 16;
 constexpr long long kAttentionCtasPerSm = 2;
+
+// A slot of the kernel for many query rows, in floats, one per CTA of a divided unit.
+constexpr size_t rowsSlotFloats(int cap) { return size_t(128) * (cap + 2); }
+// The workspace: counters, then the slots of either kernel.
+size_t attentionCounterBytes(HcContext c) {
+  return size_t(roundUp(c->smCount * kAttentionCtasPerSm * 4, 256));
+}
+size_t attentionSlotBytes(HcContext c) {
+  return size_t(c->smCount * kAttentionCtasPerSm) * 2 * kSlotFloats * 4;
+}
+size_t rowsSlotBytes(HcContext c) { return size_t(c->smCount) * rowsSlotFloats(256) * 4; }
+
+// Query rows of a sequence and key/value head from which the tcgen05 kernel takes over.
+constexpr long long kManyRows = 64;
+
+// Parts that a unit's tiles of tokens are divided into: those whose turns through the GPU
+// are shortest, a turn costing its tiles and about eight more (the rows' conversion, the
+// first tile's way through, joining).  `slots`, `units`: what the workspace holds.
+int rowSplits(long long units, long long tiles, long long sms, long long slots, long long most) {
+  long long best = 1, bestCost = 0;
+  for (long long s = 1; s <= 64; ++s) {
+    if (s > 1 && (s * 4 > tiles || s * units > slots || units > most))
+      break;
+    const long long cost = ceilDiv(units * s, sms) * (ceilDiv(tiles, s) + 8);
+    if (s == 1 || cost < bestCost) {
+      best = s;
+      bestCost = cost;
+    }
+  }
+  return int(best);
+}
 
 // Checks of the cache and of the rows' place that every entry point makes; copies them.
 int checkKv(HcContext c, const char *who, const HcKvCache *cache, const HcKvPlace *place,
@@ -212,6 +262,8 @@ const struct {
     {"hc_dequant_w4_", "gemm_w4"},
     {"hc_repack_", "gemm_w4"},
     {"hc_kv_append_", "kv_append"},       // _{i8,e4m3}_{warp,cta}
+    // hc_kv_attention_rows_{i8,e4m3}_d{64,128,256}: many query rows, on tcgen05
+    {"hc_kv_attention_rows_", "kv_attention_umma"},
     {"hc_kv_attention_", "kv_attention"}, // _{i8,e4m3}_d{64,128,256}_r{1,2}[_any]
 };
 
@@ -498,8 +550,7 @@ int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place, cons
 size_t hcKvAttentionWorkspaceBytes(HcContext c) {
   if (!c)
     return 0;
-  const size_t ctas = size_t(c->smCount * kAttentionCtasPerSm);
-  return size_t(roundUp((long long)ctas * 4, 256)) + ctas * 2 * kSlotFloats * 4;
+  return attentionCounterBytes(c) + std::max(attentionSlotBytes(c), rowsSlotBytes(c));
 }
 
 int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, const void *q,
@@ -535,33 +586,61 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   p.share = share, p.window = window;
   const long long maxRows = (long long)std::max(p.place.maxNew, 1) * share;
   const int cap = p.cache.dim <= 64 ? 64 : p.cache.dim <= 128 ? 128 : 256;
-  // Eight query rows per MMA; sixteen share one reading of the cache where there are as
-  // many and the registers allow it.
-  const int nt = maxRows > 8 && cap <= 128 ? 2 : 1;
-  const long long rowTiles = ceilDiv(maxRows, 8 * nt);
-  const long long tiles = (long long)p.place.seqs * p.cache.heads * rowTiles *
-                          (ceilDiv((long long)p.place.width * p.cache.block, 16) + 1);
-  // (The kernel counts tiles in 31 bits and divides row numbers by products.)
-  if (tiles > 0x7fffffffLL || maxRows * share > 0x7fffffffLL)
-    return c->fail("hcKvAttention: %d sequences of up to %lld query rows against %lld tokens are "
-                   "too many for one call",
-                   p.place.seqs, maxRows, (long long)p.place.width * p.cache.block);
-  p.rowTiles = int(rowTiles);
+  // (The kernels divide row numbers by products.)
+  if (maxRows * share > 0x7fffffffLL)
+    return c->fail("hcKvAttention: up to %lld query rows are too many for one call", maxRows);
   p.stepBlocks = 16 / p.cache.block;
   p.stepRows = 16 % p.cache.block;
   auto inverse = [](unsigned n) { return n == 1 ? 0u : uint32_t((1ull << 32) / n + 1); };
   p.blockInverse = inverse(unsigned(p.cache.block) / 16);
   p.shareInverse = inverse(unsigned(share));
   p.vecQ = aligned(q, 16) && qTokenStride % 8 == 0 && qHeadStride % 8 == 0;
+  p.counters = static_cast<unsigned *>(workspace);
+  p.partial =
+      reinterpret_cast<float *>(static_cast<char *>(workspace) + attentionCounterBytes(c));
+  char name[64];
+  const char *const type = p.cache.dtype == HC_I8 ? "i8" : "e4m3";
+  if (c->attentionVariant != 1 && c->ccMajor == 10 &&
+      (maxRows >= kManyRows || c->attentionVariant == 2)) {
+    KvRowsParams u{};
+    u.cache = p.cache, u.place = p.place;
+    u.q = p.q, u.out = p.out, u.lse = p.lse;
+    u.qTokenStride = qTokenStride, u.qHeadStride = qHeadStride;
+    u.outTokenStride = outTokenStride, u.outHeadStride = outHeadStride, u.lseStride = lseStride;
+    u.scaleLog2 = p.scaleLog2, u.share = share, u.window = window;
+    u.rowTiles = int(ceilDiv(maxRows, 128));
+    u.blockInverse = p.blockInverse, u.shareInverse = p.shareInverse, u.vecQ = p.vecQ;
+    u.counters = p.counters, u.partial = p.partial, u.status = c->statusWord;
+    const long long units = (long long)p.place.seqs * p.cache.heads * u.rowTiles;
+    if (units > 0x7fffffffLL)
+      return c->fail("hcKvAttention: %lld tiles of query rows are too many", units);
+    const int step = cap == 256 ? 64 : 128;
+    long long reach = (long long)p.place.width * p.cache.block; // tokens that a row can see
+    if (window > 0)
+      reach = std::min<long long>(reach, window + ceilDiv(128, share));
+    u.splits = rowSplits(units, ceilDiv(reach, step), c->smCount,
+                         (long long)(rowsSlotBytes(c) / (rowsSlotFloats(cap) * 4)),
+                         c->smCount * kAttentionCtasPerSm);
+    std::snprintf(name, sizeof name, "hc_kv_attention_rows_%s_d%d", type, cap);
+    void *args[] = {&u};
+    return c->launch(name, size_t(units), size_t(u.splits), 1, 544, args, 1,
+                     size_t(cap / 64) * 128 * (128 + 4 * step) + 1024);
+  }
+  // Eight query rows per MMA; sixteen share one reading of the cache where there are as
+  // many and the registers allow it.
+  const int nt = maxRows > 8 && cap <= 128 ? 2 : 1;
+  const long long rowTiles = ceilDiv(maxRows, 8 * nt);
+  const long long tiles = (long long)p.place.seqs * p.cache.heads * rowTiles *
+                          (ceilDiv((long long)p.place.width * p.cache.block, 16) + 1);
+  if (tiles > 0x7fffffffLL) // (the kernel counts them in 31 bits)
+    return c->fail("hcKvAttention: %d sequences of up to %lld query rows against %lld tokens are "
+                   "too many for one call",
+                   p.place.seqs, maxRows, (long long)p.place.width * p.cache.block);
+  p.rowTiles = int(rowTiles);
   const int perSm = cap == 64 || (cap == 128 && nt == 1) ? 2 : 1;
   const long long ctas =
       std::max<long long>(1, std::min(ceilDiv(tiles, 8), c->smCount * perSm));
-  p.counters = static_cast<unsigned *>(workspace);
-  p.partial = reinterpret_cast<float *>(
-      static_cast<char *>(workspace) + roundUp(c->smCount * kAttentionCtasPerSm * 4, 256));
-  char name[64];
-  std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d%s",
-                p.cache.dtype == HC_I8 ? "i8" : "e4m3", cap, nt, p.cache.dim == cap ? "" : "_any");
+  std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d%s", type, cap, nt, p.cache.dim == cap ? "" : "_any");
   void *args[] = {&p};
   return c->launch(name, size_t(ctas), 1, 1, 256, args, 1,
                    size_t(8) * 8 * nt * (2 * (cap + 8) + 8 * cap) +

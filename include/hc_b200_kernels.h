@@ -125,7 +125,10 @@ HC_B200_API int hcSelfTestWaitTimeout(HcContext c, unsigned long long limitNs,
  * the workspace, 2 = inside the GEMM's pipeline (no workspace), 3 = inside the
  * GEMM kernel band by band into a ring of three bands (hcGemmW8A16BandedBytes of
  * workspace); 2 and 3 fail where the layout does not allow them, and all give
- * the same result bit for bit. */
+ * the same result bit for bit.  "w4_variant" (hcGemmW4): 0 = by size, 1 = the kernel
+ * for few rows (fails where they do not fit), 2 = tcgen05 whatever the rows.
+ * "attention_variant" (hcKvAttention): 0 = by the number of query rows, 1 = 8 or 16
+ * rows at a time, 2 = 128 rows at a time on tcgen05. */
 HC_B200_API int hcSetOption(HcContext c, const char *name, long long value);
 
 /* Run-time specialisation.  The reference compiles every kernel body at its
@@ -545,7 +548,8 @@ HC_B200_API int hcGemmW4(HcContext c, const void *a, const float *aScale, const 
  * element [page, head, token, d] of k (and of v) lies at page * pageStride + head *
  * headStride + token * tokenStride + d, and stands for that number times
  * kScale[page * scalePitch + head].  dtype HC_I8 or HC_E4M3; block a multiple of 16 up
- * to 256; dim a multiple of 16 up to 256; strides multiples of 16, 16-byte aligned. */
+ * to 256; dim a multiple of 16 up to 256; at most 32767 heads; strides multiples of 16,
+ * 16-byte aligned; pageStride, scalePitch and block * tokenStride below 2^31. */
 typedef struct HcKvCache {
   void *k, *v;
   float *kScale, *vScale;

@@ -410,7 +410,8 @@ def test_every_serving_kernel_is_found_by_its_name():
 
     lib = capi.load_kernels()
     for image, count in (("add_rms_norm", 60), ("gemm_w4", 11), ("gemm_w4_umma", 8),
-                         ("kv_append", 4), ("kv_attention", 20)):
+                         ("kv_append", 4), ("kv_attention", 20),
+                         ("kv_attention_umma", 6)):
         blob = (REPO / "hc_b200" / "_native" / f"{image}.cubin").read_bytes()
         names = [s for s in _elf_symbols(blob) if s.startswith("hc_")]
         assert len(names) == count, (image, len(names))
