@@ -393,11 +393,9 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     const uint32_t chunkAt = uint32_t(piece >> 2) * S::chunkBytes;
     const int first16 = (piece & 3) * 2;
 
-    struct Spot {
-      int page; // < 0: not there, or seen by no row
-      uint32_t row;
-    };
-    Spot spot[S::turns];
+    // Of a token: its page (< 0: not there) and its bytes from `keys`, or ~0: seen by no row.
+    int page[S::turns];
+    uint64_t from[S::turns];
     uint4 kReg[S::turns], vReg[S::turns];
     float kScale[S::turns], vScale[S::turns];
     const bool scales = piece == 0 && (rowOf & 15) == 0;
@@ -408,24 +406,21 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         int block = pos >> 4;
         if (c.block > 16)
           block = int(__umulhi(uint32_t(block), p.blockInverse));
-        spot[i].page = -1;
-        spot[i].row = uint32_t(pos - block * c.block) * uint32_t(c.tokenStride);
         // (A group of 16 tokens that some row sees has its scales and page looked up.)
+        page[i] = -1;
         if (j < tiles && (pos | 15) >= anyLo && (pos & ~15) <= lastPos)
-          spot[i].page = hcKvPageOf(__ldg(table + block), c.pages);
+          page[i] = hcKvPageOf(__ldg(table + block), c.pages);
+        from[i] = ~0ull;
+        if (page[i] >= 0 && inDim && pos >= anyLo && pos <= lastPos)
+          from[i] = uint64_t(uint32_t(page[i])) * uint32_t(c.pageStride) +
+                    uint32_t(pos - block * c.block) * uint32_t(c.tokenStride);
       }
     };
-    auto seen = [&](int j, int i) { // by some row
-      const int pos = pos0 + j * T + i * S::rowsPerTurn + rowOf;
-      return spot[i].page >= 0 && inDim && pos >= anyLo && pos <= lastPos;
-    };
-    auto load = [&](int j, const uint8_t *from, uint4 (&reg)[S::turns]) {
+    auto load = [&](const uint8_t *base, uint4 (&reg)[S::turns]) {
 #pragma unroll
       for (int i = 0; i < S::turns; ++i)
-        reg[i] = seen(j, i) ? __ldg(reinterpret_cast<const uint4 *>(
-                                  from + uint64_t(uint32_t(spot[i].page)) * uint32_t(c.pageStride) +
-                                  spot[i].row))
-                            : make_uint4(0, 0, 0, 0);
+        reg[i] = from[i] != ~0ull ? __ldg(reinterpret_cast<const uint4 *>(base + from[i]))
+                                  : make_uint4(0, 0, 0, 0);
     };
     auto loadScales = [&]() {
       if (!scales)
@@ -433,8 +428,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
 #pragma unroll
       for (int i = 0; i < S::turns; ++i) {
         kScale[i] = vScale[i] = 0.0f;
-        if (spot[i].page >= 0) {
-          const uint64_t at = uint64_t(uint32_t(spot[i].page)) * uint32_t(c.scalePitch) + head;
+        if (page[i] >= 0) {
+          const uint64_t at = uint64_t(uint32_t(page[i])) * uint32_t(c.scalePitch) + head;
           kScale[i] = __ldg(c.kScale + at);
           vScale[i] = __ldg(c.vScale + at);
         }
@@ -482,8 +477,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     };
 
     look(0);
-    load(0, keys, kReg);
-    load(0, values, vReg);
+    load(keys, kReg);
+    load(values, vReg);
     loadScales();
     for (int j = 0; j < tiles; ++j) {
       const int b = j & 1;
@@ -495,7 +490,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
           g.value = vScale[i] * kWeight;
           g.logValue = vScale[i] > 0.0f && vScale[i] < INFINITY ? fmaxf(__log2f(vScale[i]), -96.0f)
                                                                  : 0.0f;
-          g.there = spot[i].page >= 0 ? 1.0f : 0.0f;
+          g.there = page[i] >= 0 ? 1.0f : 0.0f;
           sGroup[j & 3][(i * S::rowsPerTurn + rowOf) >> 4] = g;
         }
       }
@@ -506,14 +501,14 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       store(kBase + b * S::tileBytes, kReg);
       if (lane == 0)
         mbarArrive(smemAddr(&bars.keysFull[b]));
-      load(j + 1, keys, kReg);
+      load(keys, kReg);
       loadScales();
       if (j >= 2 && !(ok = await(bars.added[b], (j >> 1) - 1, kStatusRowsConvert)))
         break;
       store(vBase + b * S::tileBytes, vReg);
       if (lane == 0)
         mbarArrive(smemAddr(&bars.valuesFull[b]));
-      load(j + 1, values, vReg);
+      load(values, vReg);
     }
   } else {
     // --------------------------------- softmax -----------------------------------
@@ -534,17 +529,15 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       const uint32_t sAt = tmemBase + laneBase + uint32_t(b * T);
       const uint32_t pAt = tmemBase + laneBase + S::atP + uint32_t(b * (T / 2));
       const bool whole = pos >= allLo && pos + T - 1 <= firstPos;
-      uint32_t s[2][32];
+      uint32_t v[32];
 
       // The largest score with its value scale.
       float top = kNegInf;
-      tmemLoad32x32(sAt, s[0]);
-#pragma unroll
+      // (Loops over 32 columns, not unrolled: the instructions of all roles stay cached.)
+#pragma unroll 1
       for (int k = 0; k < T / 32; ++k) {
-        uint32_t(&v)[32] = s[k & 1];
+        tmemLoad32x32(sAt + uint32_t(32 * k), v);
         tmemLoadWaitFor(v);
-        if (k + 1 < T / 32)
-          tmemLoad32x32(sAt + 32 * (k + 1), s[(k + 1) & 1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const Group g = groups[2 * k + h];
@@ -599,14 +592,14 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         const float f = now == old ? 1.0f : exp2Approx(old - now);
 #pragma unroll 1
         for (int d = 0; d < DimCap; d += 32) {
-          tmemLoad32x32(tmemBase + laneBase + S::atO + d, s[0]);
-          tmemLoadWaitFor(s[0]);
+          tmemLoad32x32(tmemBase + laneBase + S::atO + d, v);
+          tmemLoadWaitFor(v);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              o[i] = __float_as_uint(__uint_as_float(s[0][8 * k + i]) * f);
+              o[i] = __float_as_uint(__uint_as_float(v[8 * k + i]) * f);
             tmemStore32x8(tmemBase + laneBase + S::atO + d + 8 * k, o);
           }
         }
@@ -618,13 +611,10 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
-      tmemLoad32x32(sAt, s[0]);
-#pragma unroll
+#pragma unroll 1
       for (int k = 0; k < T / 32; ++k) {
-        uint32_t(&v)[32] = s[k & 1];
+        tmemLoad32x32(sAt + uint32_t(32 * k), v);
         tmemLoadWaitFor(v);
-        if (k + 1 < T / 32)
-          tmemLoad32x32(sAt + 32 * (k + 1), s[(k + 1) & 1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const Group g = groups[2 * k + h];
