@@ -60,6 +60,11 @@ __device__ __forceinline__ float exp2Approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t halfPair(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
@@ -379,41 +384,52 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     }
   } else if (warp >= 8) {
     // ------------------------------- converters ---------------------------------
-    const int ct = tid - 256;
-    const int piece = ct % S::lanesPerRow, rowOf = ct / S::lanesPerRow;
+    // A lane takes 16 bytes of a token: four lanes 64 dims of one, neighbouring fours
+    // neighbouring tokens, so that no two lanes of a store phase share banks; a warp takes
+    // whole rows.
+    constexpr int kRowBits = S::lanesPerRow == 4 ? 3 : S::lanesPerRow == 8 ? 2 : 1;
+    const int chunk = lane >> (2 + kRowBits), first16 = (lane & 3) * 2;
+    const int piece = chunk * 4 + (lane & 3);
+    const int rowOf = ((warp - 8) << kRowBits) + ((lane >> 2) & ((1 << kRowBits) - 1));
     const bool inDim = piece * 16 < c.dim;
     const int *table = p.place.table + (long long)seq * p.place.tablePitch;
     const uint8_t *const keys =
         static_cast<const uint8_t *>(c.k) + (long long)head * c.headStride + piece * 16;
     const uint8_t *const values =
         static_cast<const uint8_t *>(c.v) + (long long)head * c.headStride + piece * 16;
-    // Where the two 16-byte chunks go within a row (the second half of a row's lanes in
-    // the other order: no two lanes of a store phase share banks).
-    const int swap = (piece >> 2) & 1;
-    const uint32_t chunkAt = uint32_t(piece >> 2) * S::chunkBytes;
-    const int first16 = (piece & 3) * 2;
+    const uint32_t inGroup = uint32_t(rowOf & 15) * uint32_t(c.tokenStride);
+    const uint32_t storeAt = uint32_t(chunk) * S::chunkBytes + uint32_t(rowOf) * 128;
+    const uint32_t store0 = storeAt + ((first16 ^ (rowOf & 7)) << 4);
+    const uint32_t store1 = storeAt + (((first16 + 1) ^ (rowOf & 7)) << 4);
 
-    // Of a token: its page (< 0: not there) and its bytes from `keys`, or ~0: seen by no row.
-    int page[S::turns];
-    uint64_t from[S::turns];
+    // Lane g of a warp looks up the place of the tile's sixteen tokens g.
+    int page = -1;
+    float kScale = 0.0f, vScale = 0.0f;
+    uint64_t from[S::turns]; // this lane's bytes of each turn, ~0: seen by no row
     uint4 kReg[S::turns], vReg[S::turns];
-    float kScale[S::turns], vScale[S::turns];
-    const bool scales = piece == 0 && (rowOf & 15) == 0;
     auto look = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < S::turns; ++i) {
-        const int pos = pos0 + j * T + i * S::rowsPerTurn + rowOf;
+      page = -1;
+      uint64_t base = ~0ull;
+      const int pos = pos0 + j * T + lane * 16;
+      if (lane < S::groups && j < tiles && pos + 15 >= anyLo && pos <= lastPos) {
         int block = pos >> 4;
         if (c.block > 16)
           block = int(__umulhi(uint32_t(block), p.blockInverse));
-        // (A group of 16 tokens that some row sees has its scales and page looked up.)
-        page[i] = -1;
-        if (j < tiles && (pos | 15) >= anyLo && (pos & ~15) <= lastPos)
-          page[i] = hcKvPageOf(__ldg(table + block), c.pages);
-        from[i] = ~0ull;
-        if (page[i] >= 0 && inDim && pos >= anyLo && pos <= lastPos)
-          from[i] = uint64_t(uint32_t(page[i])) * uint32_t(c.pageStride) +
-                    uint32_t(pos - block * c.block) * uint32_t(c.tokenStride);
+        page = hcKvPageOf(__ldg(table + block), c.pages);
+        if (page >= 0)
+          base = uint64_t(uint32_t(page)) * uint32_t(c.pageStride) +
+                 uint32_t(pos - block * c.block) * uint32_t(c.tokenStride);
+      }
+      const int row = pos0 + j * T + rowOf;
+      const bool inside = pos0 + j * T >= anyLo && pos0 + j * T + T - 1 <= lastPos;
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i) {
+        const uint64_t at =
+            __shfl_sync(0xffffffffu, base, (i * S::rowsPerTurn + rowOf) >> 4);
+        const int pos = row + i * S::rowsPerTurn;
+        from[i] = at == ~0ull || !inDim || (!inside && (pos < anyLo || pos > lastPos))
+                      ? ~0ull
+                      : at + inGroup;
       }
     };
     auto load = [&](const uint8_t *base, uint4 (&reg)[S::turns]) {
@@ -422,30 +438,24 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         reg[i] = from[i] != ~0ull ? __ldg(reinterpret_cast<const uint4 *>(base + from[i]))
                                   : make_uint4(0, 0, 0, 0);
     };
-    auto loadScales = [&]() {
-      if (!scales)
-        return;
-#pragma unroll
-      for (int i = 0; i < S::turns; ++i) {
-        kScale[i] = vScale[i] = 0.0f;
-        if (page[i] >= 0) {
-          const uint64_t at = uint64_t(uint32_t(page[i])) * uint32_t(c.scalePitch) + head;
-          kScale[i] = __ldg(c.kScale + at);
-          vScale[i] = __ldg(c.vScale + at);
-        }
+    auto loadScales = [&]() { // the first warp hands them on
+      kScale = vScale = 0.0f;
+      if (warp == 8 && page >= 0) {
+        const uint64_t at = uint64_t(uint32_t(page)) * uint32_t(c.scalePitch) + head;
+        kScale = __ldg(c.kScale + at);
+        vScale = __ldg(c.vScale + at);
       }
     };
     auto store = [&](uint32_t base, const uint4 (&reg)[S::turns]) {
+      unsigned char *const to = smem + (base - smemBase);
 #pragma unroll
       for (int i = 0; i < S::turns; ++i) {
-        const int r = i * S::rowsPerTurn + rowOf;
         const uint2 a = widen<Q>(reg[i].x), b = widen<Q>(reg[i].y);
         const uint2 d = widen<Q>(reg[i].z), e = widen<Q>(reg[i].w);
-        const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(d.x, d.y, e.x, e.y);
-        unsigned char *row = smem + (base - smemBase) + chunkAt + r * 128;
-        *reinterpret_cast<uint4 *>(row + (((first16 + swap) ^ (r & 7)) << 4)) = swap ? hi : lo;
-        *reinterpret_cast<uint4 *>(row + (((first16 + 1 - swap) ^ (r & 7)) << 4)) =
-            swap ? lo : hi;
+        *reinterpret_cast<uint4 *>(to + store0 + i * S::rowsPerTurn * 128) =
+            make_uint4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<uint4 *>(to + store1 + i * S::rowsPerTurn * 128) =
+            make_uint4(d.x, d.y, e.x, e.y);
       }
       fenceProxyAsync();
       __syncwarp();
@@ -482,17 +492,14 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     loadScales();
     for (int j = 0; j < tiles; ++j) {
       const int b = j & 1;
-      if (scales) { // (slot j - 4 has been read: the outputs of tile j - 3 were waited for)
-#pragma unroll
-        for (int i = 0; i < S::turns; ++i) {
-          Group g;
-          g.key = kScale[i];
-          g.value = vScale[i] * kWeight;
-          g.logValue = vScale[i] > 0.0f && vScale[i] < INFINITY ? fmaxf(__log2f(vScale[i]), -96.0f)
-                                                                 : 0.0f;
-          g.there = page[i] >= 0 ? 1.0f : 0.0f;
-          sGroup[j & 3][(i * S::rowsPerTurn + rowOf) >> 4] = g;
-        }
+      if (warp == 8 && lane < S::groups) {
+        // (Slot j - 4 has been read: the outputs of tile j - 3 were waited for.)
+        Group g;
+        g.key = kScale;
+        g.value = vScale * kWeight;
+        g.logValue = vScale > 0.0f && vScale < INFINITY ? fmaxf(__log2f(vScale), -96.0f) : 0.0f;
+        g.there = page >= 0 ? 1.0f : 0.0f;
+        sGroup[j & 3][lane] = g;
       }
       clean(j);
       look(j + 1);
@@ -554,8 +561,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
             }
           } else if (f >= 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              most = fmaxf(most, __uint_as_float(v[16 * h + i]));
+            for (int i = 0; i < 16; i += 2)
+              most = max3(most, __uint_as_float(v[16 * h + i]), __uint_as_float(v[16 * h + i + 1]));
             most *= f;
           } else {
             most = INFINITY;
