@@ -8,9 +8,9 @@
 //                           the cache, tokens by dims: an MN-major operand
 // Roles of a CTA, which keeps to one unit (sequence, head, 128 rows), or a part of its
 // tokens where there are few units:
-//   * 8 warps bring the keys and values of a tile from the cache into registers a tile
-//     ahead, widen them to f16 (exact) and store them in the swizzled layout;
-//   * one thread issues the MMAs: the scores of tile j + 1 before the outputs of tile j;
+//   * 4 warps bring the keys of a tile from the cache into registers a tile ahead, widen
+//     them to f16 (exact) and store them in the swizzled layout; 4 others the values;
+//   * one thread issues the MMAs: the scores of tile j + 2 before the outputs of tile j;
 //   * two groups of 4 warps take the score tiles in turn, a thread per row: maximum,
 //     exponentials, sum, and P back to tensor memory.  Only the reference that the
 //     exponentials are taken against is handed from tile to tile; it is kept until the
@@ -49,7 +49,7 @@ struct KvRowsParams {
 };
 
 constexpr int kThreads = 17 * 32;
-constexpr int kConvertWarps = 8, kMmaWarp = 16; // warps 8..15 convert
+constexpr int kMmaWarp = 16; // warps 8..11 convert keys, 12..15 values
 constexpr float kNegInf = -INFINITY;
 constexpr float kSlack = 4.0f;
 constexpr float kWeight = 2048.0f; // 2^(15 - kSlack): probabilities fit f16
@@ -171,7 +171,7 @@ template <int DimCap> struct RowsShape {
   // Tensor memory columns: two tiles of scores, the outputs, two of weights.
   static constexpr uint32_t atO = 2 * tokens, atP = atO + DimCap;
   static constexpr int lanesPerRow = DimCap / 16;
-  static constexpr int rowsPerTurn = 256 / lanesPerRow;
+  static constexpr int rowsPerTurn = 128 / lanesPerRow;
   static constexpr int turns = tokens / rowsPerTurn;
   static constexpr int slotFloats = 128 * (DimCap + 2);
 };
@@ -182,6 +182,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   extern __shared__ __align__(16) unsigned char smemRaw[];
   __shared__ RowsBarriers bars;
   __shared__ Group sGroup[4][S::groups];
+  __shared__ int sPlain[4]; // every group of the tile is there, with a key scale >= 0
   __shared__ float sFactor[128]; // of a query row: its power of two, scale * log2(e)
   __shared__ float sRef[128], sSum[2][128], sSumRef[2][128];
   __shared__ int sPoisoned, sLast;
@@ -239,8 +240,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   int *status = p.status;
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbarInit(smemAddr(&bars.keysFull[s]), kConvertWarps);
-      mbarInit(smemAddr(&bars.valuesFull[s]), kConvertWarps);
+      mbarInit(smemAddr(&bars.keysFull[s]), 4);
+      mbarInit(smemAddr(&bars.valuesFull[s]), 4);
       mbarInit(smemAddr(&bars.scored[s]), 1);
       mbarInit(smemAddr(&bars.weighted[s]), 4);
       mbarInit(smemAddr(&bars.decided[s]), 4);
@@ -356,15 +357,16 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         ummaCommit(smemAddr(&bars.scored[b]));
         return true;
       };
-      ok = score(0);
+      ok = score(0) && (tiles < 2 || score(1));
       for (int j = 0; ok && j < tiles; ++j) {
         const int b = j & 1;
-        // (The scores of tile j - 1 have been read: its weights were waited for.)
-        ok = (j + 1 >= tiles || score(j + 1)) &&
+        // The scores of tile j have been read when its weights stand: their place is
+        // taken first, so that its group of warps waits for one product only.
+        ok = mbarWait(smemAddr(&bars.weighted[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                      kStatusMmaWaitTmem) &&
+             (j + 2 >= tiles || score(j + 2)) &&
              mbarWait(smemAddr(&bars.valuesFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
-                      kStatusMmaWaitData) &&
-             mbarWait(smemAddr(&bars.weighted[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
-                      kStatusMmaWaitTmem);
+                      kStatusMmaWaitData);
         if (!ok)
           break;
         tcgen05FenceAfter();
@@ -390,13 +392,12 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     constexpr int kRowBits = S::lanesPerRow == 4 ? 3 : S::lanesPerRow == 8 ? 2 : 1;
     const int chunk = lane >> (2 + kRowBits), first16 = (lane & 3) * 2;
     const int piece = chunk * 4 + (lane & 3);
-    const int rowOf = ((warp - 8) << kRowBits) + ((lane >> 2) & ((1 << kRowBits) - 1));
+    const int rowOf = ((warp & 3) << kRowBits) + ((lane >> 2) & ((1 << kRowBits) - 1));
     const bool inDim = piece * 16 < c.dim;
     const int *table = p.place.table + (long long)seq * p.place.tablePitch;
-    const uint8_t *const keys =
-        static_cast<const uint8_t *>(c.k) + (long long)head * c.headStride + piece * 16;
-    const uint8_t *const values =
-        static_cast<const uint8_t *>(c.v) + (long long)head * c.headStride + piece * 16;
+    const bool ofKeys = warp < 12;
+    const uint8_t *const source = static_cast<const uint8_t *>(ofKeys ? c.k : c.v) +
+                                  (long long)head * c.headStride + piece * 16;
     const uint32_t inGroup = uint32_t(rowOf & 15) * uint32_t(c.tokenStride);
     const uint32_t storeAt = uint32_t(chunk) * S::chunkBytes + uint32_t(rowOf) * 128;
     const uint32_t store0 = storeAt + ((first16 ^ (rowOf & 7)) << 4);
@@ -406,7 +407,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     int page = -1;
     float kScale = 0.0f, vScale = 0.0f;
     uint64_t from[S::turns]; // this lane's bytes of each turn, ~0: seen by no row
-    uint4 kReg[S::turns], vReg[S::turns];
+    uint4 reg[S::turns];
     auto look = [&](int j) {
       page = -1;
       uint64_t base = ~0ull;
@@ -429,14 +430,12 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         const int pos = row + i * S::rowsPerTurn;
         from[i] = at == ~0ull || !inDim || (!inside && (pos < anyLo || pos > lastPos))
                       ? ~0ull
-                      : at + inGroup;
+                      : at + (inGroup + ((i * S::rowsPerTurn) & 15) * uint32_t(c.tokenStride));
       }
     };
-    auto load = [&](const uint8_t *base, uint4 (&reg)[S::turns]) {
-#pragma unroll
-      for (int i = 0; i < S::turns; ++i)
-        reg[i] = from[i] != ~0ull ? __ldg(reinterpret_cast<const uint4 *>(base + from[i]))
-                                  : make_uint4(0, 0, 0, 0);
+    auto load = [&](int i) {
+      reg[i] = from[i] != ~0ull ? __ldg(reinterpret_cast<const uint4 *>(source + from[i]))
+                                : make_uint4(0, 0, 0, 0);
     };
     auto loadScales = [&]() { // the first warp hands them on
       kScale = vScale = 0.0f;
@@ -446,34 +445,20 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         vScale = __ldg(c.vScale + at);
       }
     };
-    auto store = [&](uint32_t base, const uint4 (&reg)[S::turns]) {
-      unsigned char *const to = smem + (base - smemBase);
-#pragma unroll
-      for (int i = 0; i < S::turns; ++i) {
-        const uint2 a = widen<Q>(reg[i].x), b = widen<Q>(reg[i].y);
-        const uint2 d = widen<Q>(reg[i].z), e = widen<Q>(reg[i].w);
-        *reinterpret_cast<uint4 *>(to + store0 + i * S::rowsPerTurn * 128) =
-            make_uint4(a.x, a.y, b.x, b.y);
-        *reinterpret_cast<uint4 *>(to + store1 + i * S::rowsPerTurn * 128) =
-            make_uint4(d.x, d.y, e.x, e.y);
-      }
-      fenceProxyAsync();
-      __syncwarp();
-    };
     // NaN among the values (e4m3 only) must not reach rows that do not see its token:
     // 0 * NaN is NaN.  Where some rows see the token and others do not, zeros stand in
     // for them and the rows that do are mended at the end.
     auto clean = [&](int j) {
       if constexpr (__is_same(Q, E4M3)) {
         const int pos = pos0 + j * T;
-        if (pos >= allLo && pos + T - 1 <= firstPos)
+        if (ofKeys || (pos >= allLo && pos + T - 1 <= firstPos))
           return;
 #pragma unroll
         for (int i = 0; i < S::turns; ++i) {
           const int at = pos + i * S::rowsPerTurn + rowOf;
           if (at >= allLo && at <= firstPos)
             continue;
-          uint32_t *w = &vReg[i].x, bad = 0;
+          uint32_t *w = &reg[i].x, bad = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t nan = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -487,35 +472,46 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     };
 
     look(0);
-    load(keys, kReg);
-    load(values, vReg);
+#pragma unroll
+    for (int i = 0; i < S::turns; ++i)
+      load(i);
     loadScales();
+    uint64_t *const full = ofKeys ? bars.keysFull : bars.valuesFull;
+    uint64_t *const free = ofKeys ? bars.scored : bars.added;
+    unsigned char *const tile = smem + ((ofKeys ? kBase : vBase) - smemBase);
     for (int j = 0; j < tiles; ++j) {
       const int b = j & 1;
-      if (warp == 8 && lane < S::groups) {
-        // (Slot j - 4 has been read: the outputs of tile j - 3 were waited for.)
-        Group g;
-        g.key = kScale;
-        g.value = vScale * kWeight;
-        g.logValue = vScale > 0.0f && vScale < INFINITY ? fmaxf(__log2f(vScale), -96.0f) : 0.0f;
-        g.there = page >= 0 ? 1.0f : 0.0f;
-        sGroup[j & 3][lane] = g;
-      }
+      Group g;
+      g.key = kScale;
+      g.value = vScale * kWeight;
+      g.logValue = vScale > 0.0f && vScale < INFINITY ? fmaxf(__log2f(vScale), -96.0f) : 0.0f;
+      g.there = page >= 0 ? 1.0f : 0.0f;
       clean(j);
       look(j + 1);
-      if (j >= 2 && !(ok = await(bars.scored[b], (j >> 1) - 1, kStatusRowsConvert)))
+      if (j >= 2 && !(ok = await(free[b], (j >> 1) - 1, kStatusRowsConvert)))
         break;
-      store(kBase + b * S::tileBytes, kReg);
-      if (lane == 0)
-        mbarArrive(smemAddr(&bars.keysFull[b]));
-      load(keys, kReg);
+      if (warp == 8 && lane < S::groups) {
+        // (Slot j - 4 has been read: the scores of tile j - 2 came after it.)
+        sGroup[j & 3][lane] = g;
+        const bool plain =
+            __all_sync((1u << S::groups) - 1u, g.there != 0.0f && g.key >= 0.0f);
+        if (lane == 0)
+          sPlain[j & 3] = plain && p.scaleLog2 >= 0.0f;
+      }
       loadScales();
-      if (j >= 2 && !(ok = await(bars.added[b], (j >> 1) - 1, kStatusRowsConvert)))
-        break;
-      store(vBase + b * S::tileBytes, vReg);
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i) {
+        const uint2 w0 = widen<Q>(reg[i].x), w1 = widen<Q>(reg[i].y);
+        const uint2 w2 = widen<Q>(reg[i].z), w3 = widen<Q>(reg[i].w);
+        load(i); // of the next tile
+        unsigned char *to = tile + b * S::tileBytes + i * S::rowsPerTurn * 128;
+        *reinterpret_cast<uint4 *>(to + store0) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+        *reinterpret_cast<uint4 *>(to + store1) = make_uint4(w2.x, w2.y, w3.x, w3.y);
+      }
+      fenceProxyAsync();
+      __syncwarp();
       if (lane == 0)
-        mbarArrive(smemAddr(&bars.valuesFull[b]));
-      load(values, vReg);
+        mbarArrive(smemAddr(&full[b]));
     }
   } else {
     // --------------------------------- softmax -----------------------------------
@@ -536,11 +532,41 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       const uint32_t sAt = tmemBase + laneBase + uint32_t(b * T);
       const uint32_t pAt = tmemBase + laneBase + S::atP + uint32_t(b * (T / 2));
       const bool whole = pos >= allLo && pos + T - 1 <= firstPos;
-      uint32_t v[32];
+      const bool plain = whole && sPlain[j & 3];
+      uint32_t v[32], u[32];
 
-      // The largest score with its value scale.
+      // The largest score with its value scale.  (Loops that are not unrolled further: the
+      // instructions of all roles stay cached.  A tile whose tokens every row sees loads 32
+      // columns while it works on 32.)
       float top = kNegInf;
-      // (Loops over 32 columns, not unrolled: the instructions of all roles stay cached.)
+      auto most16 = [](const uint32_t (&x)[32], int at) {
+        float a = fmaxf(__uint_as_float(x[at]), __uint_as_float(x[at + 1]));
+        float b = fmaxf(__uint_as_float(x[at + 2]), __uint_as_float(x[at + 3]));
+#pragma unroll
+        for (int i = 4; i < 16; i += 4) {
+          a = max3(a, __uint_as_float(x[at + i]), __uint_as_float(x[at + i + 1]));
+          b = max3(b, __uint_as_float(x[at + i + 2]), __uint_as_float(x[at + i + 3]));
+        }
+        return fmaxf(a, b);
+      };
+      if (plain) {
+        tmemLoad32x32(sAt, v);
+#pragma unroll 1
+        for (int k = 0; k < T / 64; ++k) {
+          const Group g0 = groups[4 * k], g1 = groups[4 * k + 1];
+          const Group g2 = groups[4 * k + 2], g3 = groups[4 * k + 3];
+          tmemLoadWaitFor(v);
+          tmemLoad32x32(sAt + uint32_t(64 * k + 32), u);
+          top = max3(top, fmaf(most16(v, 0), g0.key * rowFactor, g0.logValue),
+                     fmaf(most16(v, 16), g1.key * rowFactor, g1.logValue));
+          tmemLoadWaitFor(u);
+          // (at the end the first columns again, for the weights)
+          tmemLoad32x32(sAt + uint32_t(64 * (k + 1) & (T - 1)), v);
+          top = max3(top, fmaf(most16(u, 0), g2.key * rowFactor, g2.logValue),
+                     fmaf(most16(u, 16), g3.key * rowFactor, g3.logValue));
+        }
+        tmemLoadWaitFor(v);
+      } else {
 #pragma unroll 1
       for (int k = 0; k < T / 32; ++k) {
         tmemLoad32x32(sAt + uint32_t(32 * k), v);
@@ -552,27 +578,15 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
           if (g.there == 0.0f)
             continue;
           float most = kNegInf;
-          if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int at = pos + 32 * k + 16 * h + i;
-              if (at >= seenLo && at <= seenHi)
-                most = fmaxf(most, __uint_as_float(v[16 * h + i]) * f);
-            }
-          } else if (f >= 0.0f) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 2)
-              most = max3(most, __uint_as_float(v[16 * h + i]), __uint_as_float(v[16 * h + i + 1]));
-            most *= f;
-          } else {
-            most = INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              most = fminf(most, __uint_as_float(v[16 * h + i]));
-            most *= f;
+          for (int i = 0; i < 16; ++i) {
+            const int at = pos + 32 * k + 16 * h + i;
+            if (at >= seenLo && at <= seenHi)
+              most = fmaxf(most, __uint_as_float(v[16 * h + i]) * f);
           }
           top = fmaxf(top, most + g.logValue);
         }
+      }
       }
 
       // The reference: handed on by the tile before.
@@ -599,14 +613,14 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         const float f = now == old ? 1.0f : exp2Approx(old - now);
 #pragma unroll 1
         for (int d = 0; d < DimCap; d += 32) {
-          tmemLoad32x32(tmemBase + laneBase + S::atO + d, v);
-          tmemLoadWaitFor(v);
+          tmemLoad32x32(tmemBase + laneBase + S::atO + d, u);
+          tmemLoadWaitFor(u);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              o[i] = __float_as_uint(__uint_as_float(v[8 * k + i]) * f);
+              o[i] = __float_as_uint(__uint_as_float(u[8 * k + i]) * f);
             tmemStore32x8(tmemBase + laneBase + S::atO + d + 8 * k, o);
           }
         }
@@ -618,6 +632,43 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
+      auto weigh32 = [&](const uint32_t (&x)[32], const Group &g0, const Group &g1, uint32_t at) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Group &g = h ? g1 : g0;
+          const float f = g.key * rowFactor;
+          const uint64_t f2 = pairOf(f, f), v2 = pairOf(g.value, g.value);
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint64_t y = fma2(pairOf(__uint_as_float(x[16 * h + 2 * i]),
+                                     __uint_as_float(x[16 * h + 2 * i + 1])),
+                              f2, minusBase);
+            float lo, hi;
+            unpair(y, lo, hi);
+            y = pairOf(exp2Approx(lo), exp2Approx(hi));
+            sum2 = add2(sum2, y);
+            unpair(mul2(y, v2), lo, hi);
+            w[i] = halfPair(lo, hi);
+          }
+          tmemStore32x8(pAt + at + uint32_t(8 * h), w);
+        }
+      };
+      if (plain) {
+#pragma unroll 1
+        for (int k = 0; k < T / 64; ++k) {
+          const Group g0 = groups[4 * k], g1 = groups[4 * k + 1];
+          const Group g2 = groups[4 * k + 2], g3 = groups[4 * k + 3];
+          if (k)
+            tmemLoadWaitFor(v);
+          tmemLoad32x32(sAt + uint32_t(64 * k + 32), u);
+          weigh32(v, g0, g1, uint32_t(32 * k));
+          tmemLoadWaitFor(u);
+          if (k + 1 < T / 64)
+            tmemLoad32x32(sAt + uint32_t(64 * (k + 1)), v);
+          weigh32(u, g2, g3, uint32_t(32 * k + 16));
+        }
+      } else {
 #pragma unroll 1
       for (int k = 0; k < T / 32; ++k) {
         tmemLoad32x32(sAt + uint32_t(32 * k), v);
@@ -631,20 +682,6 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               w[i] = 0;
-          } else if (whole) {
-            const uint64_t f2 = pairOf(f, f), v2 = pairOf(g.value, g.value);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint64_t x = fma2(pairOf(__uint_as_float(v[16 * h + 2 * i]),
-                                       __uint_as_float(v[16 * h + 2 * i + 1])),
-                                f2, minusBase);
-              float lo, hi;
-              unpair(x, lo, hi);
-              x = pairOf(exp2Approx(lo), exp2Approx(hi));
-              sum2 = add2(sum2, x);
-              unpair(mul2(x, v2), lo, hi);
-              w[i] = halfPair(lo, hi);
-            }
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -663,6 +700,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
           }
           tmemStore32x8(pAt + uint32_t(16 * k + 8 * h), w);
         }
+      }
       }
       float lo, hi;
       unpair(sum2, lo, hi);
