@@ -4,13 +4,13 @@
 //
 // 128 query rows against T tokens (128, or 64 for heads of 256) at a time on tcgen05:
 //   S[128, T] = Q K^T       Q and K in shared memory, f16
-//   O[128, D] += P V        P in tensor memory (f16), V in shared memory as it lies in
+//   O[128, D] += P V        P in tensor memory (f16, over its scores), V in shared memory as it lies in
 //                           the cache, tokens by dims: an MN-major operand
 // Roles of a CTA, which keeps to one unit (sequence, head, 128 rows), or a part of its
 // tokens where there are few units:
 //   * 4 warps bring the keys of a tile from the cache into registers a tile ahead, widen
 //     them to f16 (exact) and store them in the swizzled layout; 4 others the values;
-//   * one thread issues the MMAs: the scores of tile j + 2 before the outputs of tile j;
+//   * one thread issues the MMAs: the outputs of tile j, then the scores of tile j + 3;
 //   * two groups of 4 warps take the score tiles in turn, a thread per row: maximum,
 //     exponentials, sum, and P back to tensor memory.  Only the reference that the
 //     exponentials are taken against is handed from tile to tile; it is kept until the
@@ -46,6 +46,13 @@ struct KvRowsParams {
   unsigned *counters; // [units], zero between calls
   float *partial;     // [units][splits] slots
   int *status;
+};
+
+struct Yes {
+  static constexpr bool value = true;
+};
+struct No {
+  static constexpr bool value = false;
 };
 
 constexpr int kThreads = 17 * 32;
@@ -146,9 +153,31 @@ __device__ __forceinline__ void tmemLoadWaitFor(uint32_t (&v)[32]) {
   asm volatile("" : "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
 
+// mbarWait (hc_ptx.cuh) without its hint to sleep: what waits here waits for hundreds of
+// cycles, and waking up from a longer sleep took 8 % of the kernel's time.
+__device__ __forceinline__ bool waitFor(uint32_t bar, uint32_t parity, volatile int *abortFlag,
+                                        int *status, int code) {
+  if (mbarTryWait(bar, parity))
+    return true;
+  const unsigned long long start = globalTimerNs();
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbarTryWait(bar, parity))
+      return true;
+    if ((spin & 63u) == 0) {
+      if (*abortFlag)
+        return false;
+      if (globalTimerNs() - start > kWaitLimitNs) {
+        *abortFlag = 1;
+        atomicCAS(status, kStatusOk, code);
+        return false;
+      }
+    }
+  }
+}
+
 struct alignas(8) RowsBarriers {
   uint64_t keysFull[2], valuesFull[2]; // the converting warps
-  uint64_t scored[2];                  // S written, the keys read (MMA commit)
+  uint64_t scored[3];                  // S written, the keys read (MMA commit)
   uint64_t weighted[2];                // P written (the warps of a group)
   uint64_t decided[2];                 // the reference of a tile stands
   uint64_t added[2];                   // P and the values read, O complete (MMA commit)
@@ -168,8 +197,9 @@ template <int DimCap> struct RowsShape {
   static constexpr uint32_t tileBytes = chunkBytes * (DimCap / 64);
   static constexpr uint32_t qBytes = 128 * 128 * (DimCap / 64);
   // (Shared memory: qBytes + 4 * tileBytes + 1024 to align.)
-  // Tensor memory columns: two tiles of scores, the outputs, two of weights.
-  static constexpr uint32_t atO = 2 * tokens, atP = atO + DimCap;
+  // Tensor memory columns: three tiles of scores (a tile's weights overwrite them), the
+  // outputs.
+  static constexpr uint32_t atO = 3 * tokens;
   static constexpr int lanesPerRow = DimCap / 16;
   static constexpr int rowsPerTurn = 128 / lanesPerRow;
   static constexpr int turns = tokens / rowsPerTurn;
@@ -181,11 +211,12 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   constexpr int T = S::tokens;
   extern __shared__ __align__(16) unsigned char smemRaw[];
   __shared__ RowsBarriers bars;
-  __shared__ Group sGroup[4][S::groups];
-  __shared__ int sPlain[4]; // every group of the tile is there, with a key scale >= 0
+  __shared__ Group sGroup[8][S::groups];
+  __shared__ int sPlain[8]; // every group of the tile is there, with a key scale >= 0
   __shared__ float sFactor[128]; // of a query row: its power of two, scale * log2(e)
   __shared__ float sRef[128], sSum[2][128], sSumRef[2][128];
   __shared__ int sPoisoned, sLast;
+  __shared__ uint64_t sPlace[8][S::groups]; // of the converting warps
   const HcKvCacheDev &c = p.cache;
   const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
 
@@ -242,11 +273,12 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     for (int s = 0; s < 2; ++s) {
       mbarInit(smemAddr(&bars.keysFull[s]), 4);
       mbarInit(smemAddr(&bars.valuesFull[s]), 4);
-      mbarInit(smemAddr(&bars.scored[s]), 1);
       mbarInit(smemAddr(&bars.weighted[s]), 4);
       mbarInit(smemAddr(&bars.decided[s]), 4);
       mbarInit(smemAddr(&bars.added[s]), 1);
     }
+    for (int s = 0; s < 3; ++s)
+      mbarInit(smemAddr(&bars.scored[s]), 1);
     bars.abortFlag = 0;
     sPoisoned = 0;
     fenceBarrierInit();
@@ -329,7 +361,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   auto await = [&](uint64_t &bar, int use, int code) {
     bool ok = true;
     if (lane == 0)
-      ok = mbarWait(smemAddr(&bar), uint32_t(use) & 1u, abortFlag, status, code);
+      ok = waitFor(smemAddr(&bar), uint32_t(use) & 1u, abortFlag, status, code);
     return __shfl_sync(0xffffffffu, int(ok), 0) != 0;
   };
 
@@ -339,44 +371,50 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     if (lane == 0) {
       constexpr uint32_t scoreDesc = instrDescF16(128, T, false);
       constexpr uint32_t outDesc = instrDescF16(128, DimCap, true);
+      // K-major rows of 128 bytes (64 dims), 8-row groups 1024 bytes apart; the values are
+      // MN-major: chunks of 64 dims apart, 8-token groups 1024 bytes.
+      const uint64_t qDesc = makeSmemDesc(smemBase, 16, 1024);
+      const uint64_t kDesc = makeSmemDesc(kBase, 16, 1024);
+      const uint64_t vDesc = makeSmemDesc(vBase, S::chunkBytes, 1024);
+      int scoreAt = 0, weightAt = 0; // of three
       auto score = [&](int j) {
         const int b = j & 1;
-        if (!mbarWait(smemAddr(&bars.keysFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
-                      kStatusMmaWaitData))
+        if (!waitFor(smemAddr(&bars.keysFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                     kStatusMmaWaitData))
           return false;
         tcgen05FenceAfter();
+        const uint64_t k = kDesc + uint32_t(b) * (S::tileBytes >> 4);
+        const uint32_t to = tmemBase + uint32_t(scoreAt * T);
 #pragma unroll
-        for (int kk = 0; kk < DimCap / 16; ++kk) {
-          const uint64_t a =
-              makeSmemDesc(smemBase + (kk >> 2) * (128 * 128), 16, 1024) + uint64_t((kk & 3) * 2);
-          const uint64_t k =
-              makeSmemDesc(kBase + b * S::tileBytes + (kk >> 2) * S::chunkBytes, 16, 1024) +
-              uint64_t((kk & 3) * 2);
-          umma<1>(tmemBase + uint32_t(b * T), a, k, scoreDesc, kk != 0);
-        }
-        ummaCommit(smemAddr(&bars.scored[b]));
+        for (int kk = 0; kk < DimCap / 16; ++kk)
+          umma<1>(to, qDesc + uint64_t((kk >> 2) * (128 * 128 >> 4) + (kk & 3) * 2),
+                  k + uint64_t((kk >> 2) * (S::chunkBytes >> 4) + (kk & 3) * 2), scoreDesc,
+                  kk != 0);
+        ummaCommit(smemAddr(&bars.scored[scoreAt]));
+        scoreAt = scoreAt == 2 ? 0 : scoreAt + 1;
         return true;
       };
-      ok = score(0) && (tiles < 2 || score(1));
+      for (int j = 0; ok && j < min(3, tiles); ++j)
+        ok = score(j);
       for (int j = 0; ok && j < tiles; ++j) {
         const int b = j & 1;
-        // The scores of tile j have been read when its weights stand: their place is
-        // taken first, so that its group of warps waits for one product only.
-        ok = mbarWait(smemAddr(&bars.weighted[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
-                      kStatusMmaWaitTmem) &&
-             (j + 2 >= tiles || score(j + 2)) &&
-             mbarWait(smemAddr(&bars.valuesFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
-                      kStatusMmaWaitData);
+        ok = waitFor(smemAddr(&bars.valuesFull[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                     kStatusMmaWaitData) &&
+             waitFor(smemAddr(&bars.weighted[b]), uint32_t(j >> 1) & 1u, abortFlag, status,
+                     kStatusMmaWaitTmem);
         if (!ok)
           break;
         tcgen05FenceAfter();
+        const uint64_t v = vDesc + uint32_t(b) * (S::tileBytes >> 4);
+        const uint32_t from = tmemBase + uint32_t(weightAt * T);
+        weightAt = weightAt == 2 ? 0 : weightAt + 1;
 #pragma unroll
         for (int kk = 0; kk < T / 16; ++kk)
-          ummaTmemA(tmemBase + S::atO, tmemBase + S::atP + uint32_t(b * (T / 2) + kk * 8),
-                    makeSmemDesc(vBase + b * S::tileBytes, S::chunkBytes, 1024) +
-                        uint64_t(kk * 128),
-                    outDesc, (j | kk) != 0);
+          ummaTmemA(tmemBase + S::atO, from + uint32_t(kk * 8), v + uint64_t(kk * 128), outDesc,
+                    (j | kk) != 0);
         ummaCommit(smemAddr(&bars.added[b]));
+        // The place of tile j's scores and weights is free behind these MMAs.
+        ok = j + 3 >= tiles || score(j + 3);
       }
       if (!ok) { // MMAs may still be reading
         const unsigned long long t0 = globalTimerNs();
@@ -403,39 +441,56 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     const uint32_t store0 = storeAt + ((first16 ^ (rowOf & 7)) << 4);
     const uint32_t store1 = storeAt + (((first16 + 1) ^ (rowOf & 7)) << 4);
 
-    // Lane g of a warp looks up the place of the tile's sixteen tokens g.
-    int page = -1;
+    // Lane g of a warp looks up the place of the tile's sixteen tokens g; the table is read
+    // a tile ahead of that.
+    int page = -1, entry = -1, rowAt = 0;
     float kScale = 0.0f, vScale = 0.0f;
     uint64_t from[S::turns]; // this lane's bytes of each turn, ~0: seen by no row
+    bool clear = false;      // of the warp: none of them is
     uint4 reg[S::turns];
-    auto look = [&](int j) {
-      page = -1;
-      uint64_t base = ~0ull;
+    uint64_t *const place = sPlace[warp - 8];
+    auto find = [&](int j) {
       const int pos = pos0 + j * T + lane * 16;
+      entry = -1;
       if (lane < S::groups && j < tiles && pos + 15 >= anyLo && pos <= lastPos) {
         int block = pos >> 4;
         if (c.block > 16)
           block = int(__umulhi(uint32_t(block), p.blockInverse));
-        page = hcKvPageOf(__ldg(table + block), c.pages);
-        if (page >= 0)
-          base = uint64_t(uint32_t(page)) * uint32_t(c.pageStride) +
-                 uint32_t(pos - block * c.block) * uint32_t(c.tokenStride);
-      }
-      const int row = pos0 + j * T + rowOf;
-      const bool inside = pos0 + j * T >= anyLo && pos0 + j * T + T - 1 <= lastPos;
-#pragma unroll
-      for (int i = 0; i < S::turns; ++i) {
-        const uint64_t at =
-            __shfl_sync(0xffffffffu, base, (i * S::rowsPerTurn + rowOf) >> 4);
-        const int pos = row + i * S::rowsPerTurn;
-        from[i] = at == ~0ull || !inDim || (!inside && (pos < anyLo || pos > lastPos))
-                      ? ~0ull
-                      : at + (inGroup + ((i * S::rowsPerTurn) & 15) * uint32_t(c.tokenStride));
+        entry = __ldg(table + block);
+        rowAt = pos - block * c.block;
       }
     };
-    auto load = [&](int i) {
-      reg[i] = from[i] != ~0ull ? __ldg(reinterpret_cast<const uint4 *>(source + from[i]))
-                                : make_uint4(0, 0, 0, 0);
+    auto look = [&](int j) {
+      page = hcKvPageOf(entry, c.pages);
+      const uint64_t base = page < 0 ? ~0ull
+                                     : uint64_t(uint32_t(page)) * uint32_t(c.pageStride) +
+                                           uint32_t(rowAt) * uint32_t(c.tokenStride);
+      if (lane < S::groups)
+        place[lane] = base;
+      const int first = pos0 + j * T;
+      const bool inside = first >= anyLo && first + T - 1 <= lastPos && c.dim == DimCap;
+      clear = __all_sync(0xffffffffu, inside && (lane >= S::groups || page >= 0));
+      find(j + 1);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i)
+        from[i] = place[(i * S::rowsPerTurn + rowOf) >> 4] + inGroup +
+                  ((i * S::rowsPerTurn) & 15) * uint32_t(c.tokenStride);
+      if (!clear) {
+#pragma unroll
+        for (int i = 0; i < S::turns; ++i) {
+          const int pos = first + i * S::rowsPerTurn + rowOf;
+          if (!inDim || pos < anyLo || pos > lastPos ||
+              place[(i * S::rowsPerTurn + rowOf) >> 4] == ~0ull)
+            from[i] = ~0ull;
+        }
+      }
+      __syncwarp();
+    };
+    auto load = [&](auto all, int i) {
+      reg[i] = make_uint4(0, 0, 0, 0);
+      if (decltype(all)::value || from[i] != ~0ull)
+        reg[i] = __ldg(reinterpret_cast<const uint4 *>(source + from[i]));
     };
     auto loadScales = [&]() { // the first warp hands them on
       kScale = vScale = 0.0f;
@@ -471,43 +526,59 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       }
     };
 
+    find(0);
     look(0);
 #pragma unroll
     for (int i = 0; i < S::turns; ++i)
-      load(i);
+      load(No{}, i);
     loadScales();
     uint64_t *const full = ofKeys ? bars.keysFull : bars.valuesFull;
-    uint64_t *const free = ofKeys ? bars.scored : bars.added;
-    unsigned char *const tile = smem + ((ofKeys ? kBase : vBase) - smemBase);
+    unsigned char *const ring = smem + ((ofKeys ? kBase : vBase) - smemBase);
+    int scoredAt = 0, scoredUse = 0; // of tile j - 2, in a ring of three
     for (int j = 0; j < tiles; ++j) {
       const int b = j & 1;
-      Group g;
-      g.key = kScale;
-      g.value = vScale * kWeight;
-      g.logValue = vScale > 0.0f && vScale < INFINITY ? fmaxf(__log2f(vScale), -96.0f) : 0.0f;
-      g.there = page >= 0 ? 1.0f : 0.0f;
       clean(j);
-      look(j + 1);
-      if (j >= 2 && !(ok = await(free[b], (j >> 1) - 1, kStatusRowsConvert)))
-        break;
-      if (warp == 8 && lane < S::groups) {
-        // (Slot j - 4 has been read: the scores of tile j - 2 came after it.)
-        sGroup[j & 3][lane] = g;
-        const bool plain =
-            __all_sync((1u << S::groups) - 1u, g.there != 0.0f && g.key >= 0.0f);
+      if (j >= 2) {
+        ok = ofKeys ? await(bars.scored[scoredAt], scoredUse, kStatusRowsConvert)
+                    : await(bars.added[b], (j >> 1) - 1, kStatusRowsConvert);
+        if (!ok)
+          break;
+        if (++scoredAt == 3) {
+          scoredAt = 0;
+          ++scoredUse;
+        }
+      }
+      if (warp == 8) {
+        // (Slot j - 8 has been read: the scores of tile j - 2 came behind its weights.)
+        Group g;
+        g.key = kScale;
+        g.value = vScale * kWeight;
+        g.logValue = vScale > 0.0f && vScale < INFINITY ? fmaxf(__log2f(vScale), -96.0f) : 0.0f;
+        g.there = page >= 0 ? 1.0f : 0.0f;
+        const bool plain = __all_sync(
+            0xffffffffu, lane >= S::groups || (page >= 0 && kScale >= 0.0f && p.scaleLog2 >= 0.0f));
+        if (lane < S::groups)
+          sGroup[j & 7][lane] = g;
         if (lane == 0)
-          sPlain[j & 3] = plain && p.scaleLog2 >= 0.0f;
+          sPlain[j & 7] = plain;
       }
+      look(j + 1);
       loadScales();
+      auto convert = [&](auto all) {
 #pragma unroll
-      for (int i = 0; i < S::turns; ++i) {
-        const uint2 w0 = widen<Q>(reg[i].x), w1 = widen<Q>(reg[i].y);
-        const uint2 w2 = widen<Q>(reg[i].z), w3 = widen<Q>(reg[i].w);
-        load(i); // of the next tile
-        unsigned char *to = tile + b * S::tileBytes + i * S::rowsPerTurn * 128;
-        *reinterpret_cast<uint4 *>(to + store0) = make_uint4(w0.x, w0.y, w1.x, w1.y);
-        *reinterpret_cast<uint4 *>(to + store1) = make_uint4(w2.x, w2.y, w3.x, w3.y);
-      }
+        for (int i = 0; i < S::turns; ++i) {
+          const uint2 w0 = widen<Q>(reg[i].x), w1 = widen<Q>(reg[i].y);
+          const uint2 w2 = widen<Q>(reg[i].z), w3 = widen<Q>(reg[i].w);
+          load(all, i); // of the next tile
+          unsigned char *to = ring + b * S::tileBytes + i * S::rowsPerTurn * 128;
+          *reinterpret_cast<uint4 *>(to + store0) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+          *reinterpret_cast<uint4 *>(to + store1) = make_uint4(w2.x, w2.y, w3.x, w3.y);
+        }
+      };
+      if (clear)
+        convert(Yes{});
+      else
+        convert(No{});
       fenceProxyAsync();
       __syncwarp();
       if (lane == 0)
@@ -523,16 +594,22 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     const int seenLo = p.window > 0 ? max(0, seenHi - p.window + 1) : 0;
     float ref = kNegInf; // what `sum` was taken against
     float sum = 0.0f;
+    int at3 = group, use3 = 0; // of tile j in the ring of three
     for (int j = group; j < tiles; j += 2) {
       const int b = j & 1, pos = pos0 + j * T;
-      if (!(ok = await(bars.scored[b], j >> 1, kStatusRowsSoftmax)))
+      if (!(ok = await(bars.scored[at3], use3, kStatusRowsSoftmax)))
         break;
       tcgen05FenceAfter();
-      const Group *const groups = sGroup[j & 3];
-      const uint32_t sAt = tmemBase + laneBase + uint32_t(b * T);
-      const uint32_t pAt = tmemBase + laneBase + S::atP + uint32_t(b * (T / 2));
+      const Group *const groups = sGroup[j & 7];
+      // The weights overwrite the scores, 16 columns per 32: those have been loaded then.
+      const uint32_t sAt = tmemBase + laneBase + uint32_t(at3 * T), pAt = sAt;
+      at3 += 2;
+      if (at3 >= 3) {
+        at3 -= 3;
+        ++use3;
+      }
       const bool whole = pos >= allLo && pos + T - 1 <= firstPos;
-      const bool plain = whole && sPlain[j & 3];
+      const bool plain = whole && sPlain[j & 7];
       uint32_t v[32], u[32];
 
       // The largest score with its value scale.  (Loops that are not unrolled further: the
@@ -625,10 +702,6 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
           }
         }
       }
-      // The weights of tile j - 2 have been read.
-      if (j >= 2 && !(ok = await(bars.added[b], (j >> 1) - 1, kStatusRowsSoftmax)))
-        break;
-
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
