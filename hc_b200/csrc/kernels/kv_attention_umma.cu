@@ -48,13 +48,6 @@ struct KvRowsParams {
   int *status;
 };
 
-struct Yes {
-  static constexpr bool value = true;
-};
-struct No {
-  static constexpr bool value = false;
-};
-
 constexpr int kThreads = 17 * 32;
 constexpr int kMmaWarp = 16; // warps 8..11 convert keys, 12..15 values
 constexpr float kNegInf = -INFINITY;
@@ -139,18 +132,25 @@ __device__ __forceinline__ void ummaTmemA(uint32_t dTmem, uint32_t aTmem, uint64
                : "memory");
 }
 
+// 32 lanes x 16 columns.
+__device__ __forceinline__ void tmemLoad32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+                 "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                 "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(taddr)
+               : "memory");
+}
+
 // Waits for the loads in flight; what depends on `v` stays behind it.
-__device__ __forceinline__ void tmemLoadWaitFor(uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmemLoadWaitFor(uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
                  "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),
-                 "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
-                 "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]),
-                 "+r"(v[27]), "+r"(v[28])
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                :
                : "memory");
-  asm volatile("" : "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
 
 // mbarWait (hc_ptx.cuh) without its hint to sleep: what waits here waits for hundreds of
@@ -216,7 +216,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   __shared__ float sFactor[128]; // of a query row: its power of two, scale * log2(e)
   __shared__ float sRef[128], sSum[2][128], sSumRef[2][128];
   __shared__ int sPoisoned, sLast;
-  __shared__ uint64_t sPlace[8][S::groups]; // of the converting warps
+  __shared__ uint64_t sPlace[8][2][S::groups]; // of the converting warps
   const HcKvCacheDev &c = p.cache;
   const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
 
@@ -445,10 +445,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     // a tile ahead of that.
     int page = -1, entry = -1, rowAt = 0;
     float kScale = 0.0f, vScale = 0.0f;
-    uint64_t from[S::turns]; // this lane's bytes of each turn, ~0: seen by no row
-    bool clear = false;      // of the warp: none of them is
-    uint4 reg[S::turns];
-    uint64_t *const place = sPlace[warp - 8];
+    bool clear[2] = {false, false}; // of a tile (even, odd): every token is there and seen
+    uint4 reg[4];                   // four turns are in flight
     auto find = [&](int j) {
       const int pos = pos0 + j * T + lane * 16;
       entry = -1;
@@ -466,31 +464,29 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
                                      : uint64_t(uint32_t(page)) * uint32_t(c.pageStride) +
                                            uint32_t(rowAt) * uint32_t(c.tokenStride);
       if (lane < S::groups)
-        place[lane] = base;
+        sPlace[warp - 8][j & 1][lane] = base;
       const int first = pos0 + j * T;
       const bool inside = first >= anyLo && first + T - 1 <= lastPos && c.dim == DimCap;
-      clear = __all_sync(0xffffffffu, inside && (lane >= S::groups || page >= 0));
+      const bool whole = __all_sync(0xffffffffu, inside && (lane >= S::groups || page >= 0));
+      clear[0] = j & 1 ? clear[0] : whole;
+      clear[1] = j & 1 ? whole : clear[1];
       find(j + 1);
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < S::turns; ++i)
-        from[i] = place[(i * S::rowsPerTurn + rowOf) >> 4] + inGroup +
-                  ((i * S::rowsPerTurn) & 15) * uint32_t(c.tokenStride);
-      if (!clear) {
-#pragma unroll
-        for (int i = 0; i < S::turns; ++i) {
-          const int pos = first + i * S::rowsPerTurn + rowOf;
-          if (!inDim || pos < anyLo || pos > lastPos ||
-              place[(i * S::rowsPerTurn + rowOf) >> 4] == ~0ull)
-            from[i] = ~0ull;
-        }
-      }
-      __syncwarp();
     };
-    auto load = [&](auto all, int i) {
+    // Four turns of tile j, from `turn` on, into registers.
+    auto load = [&](int j, int turn, int i) {
+      const int row = (turn + i) * S::rowsPerTurn + rowOf;
+      const uint64_t at = sPlace[warp - 8][j & 1][row >> 4];
+      bool in = true;
+      if (!(j & 1 ? clear[1] : clear[0])) {
+        const int pos = pos0 + j * T + row;
+        in = at != ~0ull && inDim && pos >= anyLo && pos <= lastPos;
+      }
       reg[i] = make_uint4(0, 0, 0, 0);
-      if (decltype(all)::value || from[i] != ~0ull)
-        reg[i] = __ldg(reinterpret_cast<const uint4 *>(source + from[i]));
+      if (in)
+        reg[i] = __ldg(reinterpret_cast<const uint4 *>(
+            source + at +
+            (inGroup + ((i * S::rowsPerTurn) & 15) * uint32_t(c.tokenStride))));
     };
     auto loadScales = [&]() { // the first warp hands them on
       kScale = vScale = 0.0f;
@@ -503,41 +499,33 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     // NaN among the values (e4m3 only) must not reach rows that do not see its token:
     // 0 * NaN is NaN.  Where some rows see the token and others do not, zeros stand in
     // for them and the rows that do are mended at the end.
-    auto clean = [&](int j) {
+    auto clean = [&](int at, uint4 &v) {
       if constexpr (__is_same(Q, E4M3)) {
-        const int pos = pos0 + j * T;
-        if (ofKeys || (pos >= allLo && pos + T - 1 <= firstPos))
+        if (at >= allLo && at <= firstPos)
           return;
+        uint32_t *w = &v.x, bad = 0;
 #pragma unroll
-        for (int i = 0; i < S::turns; ++i) {
-          const int at = pos + i * S::rowsPerTurn + rowOf;
-          if (at >= allLo && at <= firstPos)
-            continue;
-          uint32_t *w = &reg[i].x, bad = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t nan = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            w[k] &= ~nan;
-            bad |= nan;
-          }
-          if (bad)
-            sPoisoned = 1;
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t nan = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+          w[k] &= ~nan;
+          bad |= nan;
         }
+        if (bad)
+          sPoisoned = 1;
       }
     };
 
     find(0);
     look(0);
 #pragma unroll
-    for (int i = 0; i < S::turns; ++i)
-      load(No{}, i);
+    for (int i = 0; i < 4; ++i)
+      load(0, 0, i);
     loadScales();
     uint64_t *const full = ofKeys ? bars.keysFull : bars.valuesFull;
     unsigned char *const ring = smem + ((ofKeys ? kBase : vBase) - smemBase);
     int scoredAt = 0, scoredUse = 0; // of tile j - 2, in a ring of three
     for (int j = 0; j < tiles; ++j) {
       const int b = j & 1;
-      clean(j);
       if (j >= 2) {
         ok = ofKeys ? await(bars.scored[scoredAt], scoredUse, kStatusRowsConvert)
                     : await(bars.added[b], (j >> 1) - 1, kStatusRowsConvert);
@@ -564,21 +552,27 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       }
       look(j + 1);
       loadScales();
-      auto convert = [&](auto all) {
+      const int first = pos0 + j * T + rowOf;
+      const bool edge = !ofKeys && (pos0 + j * T < allLo || pos0 + j * T + T - 1 > firstPos);
+      // (Four turns at a time: all of them unrolled do not stay in the instruction cache
+      // beside the other roles, which cost a third of the kernel's time.)
+#pragma unroll 1
+      for (int turn = 0; turn < S::turns; turn += 4) {
+        const bool ahead = turn + 4 >= S::turns; // the loads are the next tile's
+        unsigned char *to = ring + b * S::tileBytes + turn * S::rowsPerTurn * 128;
 #pragma unroll
-        for (int i = 0; i < S::turns; ++i) {
+        for (int i = 0; i < 4; ++i) {
+          if (edge)
+            clean(first + (turn + i) * S::rowsPerTurn, reg[i]);
           const uint2 w0 = widen<Q>(reg[i].x), w1 = widen<Q>(reg[i].y);
           const uint2 w2 = widen<Q>(reg[i].z), w3 = widen<Q>(reg[i].w);
-          load(all, i); // of the next tile
-          unsigned char *to = ring + b * S::tileBytes + i * S::rowsPerTurn * 128;
-          *reinterpret_cast<uint4 *>(to + store0) = make_uint4(w0.x, w0.y, w1.x, w1.y);
-          *reinterpret_cast<uint4 *>(to + store1) = make_uint4(w2.x, w2.y, w3.x, w3.y);
+          load(ahead ? j + 1 : j, ahead ? 0 : turn + 4, i);
+          *reinterpret_cast<uint4 *>(to + store0 + i * S::rowsPerTurn * 128) =
+              make_uint4(w0.x, w0.y, w1.x, w1.y);
+          *reinterpret_cast<uint4 *>(to + store1 + i * S::rowsPerTurn * 128) =
+              make_uint4(w2.x, w2.y, w3.x, w3.y);
         }
-      };
-      if (clear)
-        convert(Yes{});
-      else
-        convert(No{});
+      }
       fenceProxyAsync();
       __syncwarp();
       if (lane == 0)
@@ -610,60 +604,48 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       }
       const bool whole = pos >= allLo && pos + T - 1 <= firstPos;
       const bool plain = whole && sPlain[j & 7];
-      uint32_t v[32], u[32];
+      uint32_t v[16], u[16];
 
-      // The largest score with its value scale.  (Loops that are not unrolled further: the
-      // instructions of all roles stay cached.  A tile whose tokens every row sees loads 32
-      // columns while it works on 32.)
+      // The largest score with its value scale.  Sixteen columns are loaded while sixteen
+      // are worked on, in loops that are not unrolled further.
       float top = kNegInf;
-      auto most16 = [](const uint32_t (&x)[32], int at) {
-        float a = fmaxf(__uint_as_float(x[at]), __uint_as_float(x[at + 1]));
-        float b = fmaxf(__uint_as_float(x[at + 2]), __uint_as_float(x[at + 3]));
+      auto seen = [&](int at) { return at >= seenLo && at <= seenHi; };
+      auto most16 = [&](const uint32_t (&x)[16], const Group &g) {
+        float a = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        float c = fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]));
 #pragma unroll
         for (int i = 4; i < 16; i += 4) {
-          a = max3(a, __uint_as_float(x[at + i]), __uint_as_float(x[at + i + 1]));
-          b = max3(b, __uint_as_float(x[at + i + 2]), __uint_as_float(x[at + i + 3]));
+          a = max3(a, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          c = max3(c, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
         }
-        return fmaxf(a, b);
+        top = fmaxf(top, fmaf(fmaxf(a, c), g.key * rowFactor, g.logValue));
       };
       if (plain) {
-        tmemLoad32x32(sAt, v);
+        tmemLoad32x16(sAt, v);
 #pragma unroll 1
-        for (int k = 0; k < T / 64; ++k) {
-          const Group g0 = groups[4 * k], g1 = groups[4 * k + 1];
-          const Group g2 = groups[4 * k + 2], g3 = groups[4 * k + 3];
+        for (int k = 0; k < T / 32; ++k) {
+          const Group g0 = groups[2 * k], g1 = groups[2 * k + 1];
           tmemLoadWaitFor(v);
-          tmemLoad32x32(sAt + uint32_t(64 * k + 32), u);
-          top = max3(top, fmaf(most16(v, 0), g0.key * rowFactor, g0.logValue),
-                     fmaf(most16(v, 16), g1.key * rowFactor, g1.logValue));
+          tmemLoad32x16(sAt + uint32_t(32 * k + 16), u);
+          most16(v, g0);
           tmemLoadWaitFor(u);
           // (at the end the first columns again, for the weights)
-          tmemLoad32x32(sAt + uint32_t(64 * (k + 1) & (T - 1)), v);
-          top = max3(top, fmaf(most16(u, 0), g2.key * rowFactor, g2.logValue),
-                     fmaf(most16(u, 16), g3.key * rowFactor, g3.logValue));
+          tmemLoad32x16(sAt + (uint32_t(32 * (k + 1)) & (T - 1)), v);
+          most16(u, g1);
         }
-        tmemLoadWaitFor(v);
       } else {
 #pragma unroll 1
-      for (int k = 0; k < T / 32; ++k) {
-        tmemLoad32x32(sAt + uint32_t(32 * k), v);
-        tmemLoadWaitFor(v);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Group g = groups[2 * k + h];
-          const float f = g.key * rowFactor;
+        for (int k = 0; k < T / 16; ++k) {
+          const Group g = groups[k];
           if (g.there == 0.0f)
             continue;
-          float most = kNegInf;
+          tmemLoad32x16(sAt + uint32_t(16 * k), v);
+          tmemLoadWaitFor(v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = pos + 32 * k + 16 * h + i;
-            if (at >= seenLo && at <= seenHi)
-              most = fmaxf(most, __uint_as_float(v[16 * h + i]) * f);
-          }
-          top = fmaxf(top, most + g.logValue);
+          for (int i = 0; i < 16; ++i)
+            if (seen(pos + 16 * k + i))
+              top = fmaxf(top, fmaf(__uint_as_float(v[i]), g.key * rowFactor, g.logValue));
         }
-      }
       }
 
       // The reference: handed on by the tile before.
@@ -683,97 +665,83 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         sum *= exp2Approx(ref - now); // (0 against -inf: there was no sum)
         ref = now;
       }
+      if (plain)
+        tmemLoadWaitFor(v);
       if (__any_sync(0xffffffffu, now != old) && j > 0) {
         if (!(ok = await(bars.added[b ^ 1], (j - 1) >> 1, kStatusRowsSoftmax)))
           break;
         tcgen05FenceAfter();
         const float f = now == old ? 1.0f : exp2Approx(old - now);
 #pragma unroll 1
-        for (int d = 0; d < DimCap; d += 32) {
-          tmemLoad32x32(tmemBase + laneBase + S::atO + d, u);
+        for (int d = 0; d < DimCap; d += 16) {
+          tmemLoad32x16(tmemBase + laneBase + S::atO + uint32_t(d), u);
           tmemLoadWaitFor(u);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 2; ++k) {
             uint32_t o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               o[i] = __float_as_uint(__uint_as_float(u[8 * k + i]) * f);
-            tmemStore32x8(tmemBase + laneBase + S::atO + d + 8 * k, o);
+            tmemStore32x8(tmemBase + laneBase + S::atO + uint32_t(d + 8 * k), o);
           }
         }
       }
+
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
-      auto weigh32 = [&](const uint32_t (&x)[32], const Group &g0, const Group &g1, uint32_t at) {
+      auto weigh16 = [&](const uint32_t (&x)[16], const Group &g, uint32_t at) {
+        const float f = g.key * rowFactor;
+        const uint64_t f2 = pairOf(f, f), v2 = pairOf(g.value, g.value);
+        uint32_t w[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Group &g = h ? g1 : g0;
-          const float f = g.key * rowFactor;
-          const uint64_t f2 = pairOf(f, f), v2 = pairOf(g.value, g.value);
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint64_t y = fma2(pairOf(__uint_as_float(x[16 * h + 2 * i]),
-                                     __uint_as_float(x[16 * h + 2 * i + 1])),
-                              f2, minusBase);
-            float lo, hi;
-            unpair(y, lo, hi);
-            y = pairOf(exp2Approx(lo), exp2Approx(hi));
-            sum2 = add2(sum2, y);
-            unpair(mul2(y, v2), lo, hi);
-            w[i] = halfPair(lo, hi);
-          }
-          tmemStore32x8(pAt + at + uint32_t(8 * h), w);
+        for (int i = 0; i < 8; ++i) {
+          uint64_t y =
+              fma2(pairOf(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2, minusBase);
+          float lo, hi;
+          unpair(y, lo, hi);
+          y = pairOf(exp2Approx(lo), exp2Approx(hi));
+          sum2 = add2(sum2, y);
+          unpair(mul2(y, v2), lo, hi);
+          w[i] = halfPair(lo, hi);
         }
+        tmemStore32x8(pAt + at, w);
       };
       if (plain) {
 #pragma unroll 1
-        for (int k = 0; k < T / 64; ++k) {
-          const Group g0 = groups[4 * k], g1 = groups[4 * k + 1];
-          const Group g2 = groups[4 * k + 2], g3 = groups[4 * k + 3];
+        for (int k = 0; k < T / 32; ++k) {
+          const Group g0 = groups[2 * k], g1 = groups[2 * k + 1];
           if (k)
             tmemLoadWaitFor(v);
-          tmemLoad32x32(sAt + uint32_t(64 * k + 32), u);
-          weigh32(v, g0, g1, uint32_t(32 * k));
+          tmemLoad32x16(sAt + uint32_t(32 * k + 16), u);
+          weigh16(v, g0, uint32_t(16 * k));
           tmemLoadWaitFor(u);
-          if (k + 1 < T / 64)
-            tmemLoad32x32(sAt + uint32_t(64 * (k + 1)), v);
-          weigh32(u, g2, g3, uint32_t(32 * k + 16));
+          if (k + 1 < T / 32)
+            tmemLoad32x16(sAt + uint32_t(32 * (k + 1)), v);
+          weigh16(u, g1, uint32_t(16 * k + 8));
         }
       } else {
 #pragma unroll 1
-      for (int k = 0; k < T / 32; ++k) {
-        tmemLoad32x32(sAt + uint32_t(32 * k), v);
-        tmemLoadWaitFor(v);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Group g = groups[2 * k + h];
-          const float f = g.key * rowFactor;
+        for (int k = 0; k < T / 16; ++k) {
+          const Group g = groups[k];
           uint32_t w[8];
-          if (g.there == 0.0f) {
+          tmemLoad32x16(sAt + uint32_t(16 * k), v);
+          tmemLoadWaitFor(v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              w[i] = 0;
-          } else {
+          for (int i = 0; i < 16; i += 2) {
+            float e[2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float e[2];
-#pragma unroll
-              for (int k2 = 0; k2 < 2; ++k2) {
-                const int at = pos + 32 * k + 16 * h + 2 * i + k2;
-                const bool in = at >= seenLo && at <= seenHi;
-                const float x =
-                    exp2Approx(fmaf(__uint_as_float(v[16 * h + 2 * i + k2]), f, -base));
-                sum += in ? x : 0.0f;
-                e[k2] = in ? x * g.value : 0.0f;
-              }
-              w[i] = halfPair(e[0], e[1]);
+            for (int h = 0; h < 2; ++h) {
+              const bool in = g.there != 0.0f && seen(pos + 16 * k + i + h);
+              const float x =
+                  exp2Approx(fmaf(__uint_as_float(v[i + h]), g.key * rowFactor, -base));
+              sum += in ? x : 0.0f;
+              e[h] = in ? x * g.value : 0.0f;
             }
+            w[i >> 1] = halfPair(e[0], e[1]);
           }
-          tmemStore32x8(pAt + uint32_t(16 * k + 8 * h), w);
+          tmemStore32x8(pAt + uint32_t(8 * k), w);
         }
-      }
       }
       float lo, hi;
       unpair(sum2, lo, hi);
@@ -830,14 +798,14 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       const int seenHi = span.first + qi;
       const int seenLo = p.window > 0 ? max(0, seenHi - p.window + 1) : 0;
 #pragma unroll 1
-      for (int d0 = group * (DimCap / 2); d0 < (group + 1) * (DimCap / 2); d0 += 32) {
-        uint32_t v[32];
-        tmemLoad32x32(tmemBase + (uint32_t((warp & 3) * 32) << 16) + S::atO + d0, v);
+      for (int d0 = group * (DimCap / 2); d0 < (group + 1) * (DimCap / 2); d0 += 16) {
+        uint32_t v[16];
+        tmemLoad32x16(tmemBase + (uint32_t((warp & 3) * 32) << 16) + S::atO + d0, v);
         tmemLoadWaitFor(v);
         if (r >= rowsHere)
           continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           float4 o = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
                                  __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
           if (__is_same(Q, E4M3) && sPoisoned && d0 + 4 * i < c.dim) {
