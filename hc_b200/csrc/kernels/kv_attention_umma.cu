@@ -153,15 +153,15 @@ __device__ __forceinline__ void tmemLoadWaitFor(uint32_t (&v)[16]) {
                : "memory");
 }
 
-// mbarWait (hc_ptx.cuh) without its hint to sleep: what waits here waits for hundreds of
-// cycles, and waking up from a longer sleep took 8 % of the kernel's time.
+// mbarWait (hc_ptx.cuh) with a shorter sleep between its looks: what waits here waits for
+// hundreds of cycles (20 us as there took 8 % more of the kernel's time).
 __device__ __forceinline__ bool waitFor(uint32_t bar, uint32_t parity, volatile int *abortFlag,
                                         int *status, int code) {
   if (mbarTryWait(bar, parity))
     return true;
   const unsigned long long start = globalTimerNs();
   for (uint32_t spin = 1;; ++spin) {
-    if (mbarTryWait(bar, parity))
+    if (mbarTryWaitFor(bar, parity, 500u))
       return true;
     if ((spin & 63u) == 0) {
       if (*abortFlag)
@@ -446,7 +446,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     int page = -1, entry = -1, rowAt = 0;
     float kScale = 0.0f, vScale = 0.0f;
     bool clear[2] = {false, false}; // of a tile (even, odd): every token is there and seen
-    uint4 reg[4];                   // four turns are in flight
+    uint4 reg[S::turns];            // a tile is in flight
     auto find = [&](int j) {
       const int pos = pos0 + j * T + lane * 16;
       entry = -1;
@@ -473,9 +473,9 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       find(j + 1);
       __syncwarp();
     };
-    // Four turns of tile j, from `turn` on, into registers.
-    auto load = [&](int j, int turn, int i) {
-      const int row = (turn + i) * S::rowsPerTurn + rowOf;
+    // A turn of tile j.
+    auto load = [&](int j, int i) {
+      const int row = i * S::rowsPerTurn + rowOf;
       const uint64_t at = sPlace[warp - 8][j & 1][row >> 4];
       bool in = true;
       if (!(j & 1 ? clear[1] : clear[0])) {
@@ -518,8 +518,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     find(0);
     look(0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      load(0, 0, i);
+    for (int i = 0; i < S::turns; ++i)
+      load(0, i);
     loadScales();
     uint64_t *const full = ofKeys ? bars.keysFull : bars.valuesFull;
     unsigned char *const ring = smem + ((ofKeys ? kBase : vBase) - smemBase);
@@ -554,24 +554,21 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       loadScales();
       const int first = pos0 + j * T + rowOf;
       const bool edge = !ofKeys && (pos0 + j * T < allLo || pos0 + j * T + T - 1 > firstPos);
-      // (Four turns at a time: all of them unrolled do not stay in the instruction cache
-      // beside the other roles, which cost a third of the kernel's time.)
-#pragma unroll 1
-      for (int turn = 0; turn < S::turns; turn += 4) {
-        const bool ahead = turn + 4 >= S::turns; // the loads are the next tile's
-        unsigned char *to = ring + b * S::tileBytes + turn * S::rowsPerTurn * 128;
+      if (edge) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (edge)
-            clean(first + (turn + i) * S::rowsPerTurn, reg[i]);
-          const uint2 w0 = widen<Q>(reg[i].x), w1 = widen<Q>(reg[i].y);
-          const uint2 w2 = widen<Q>(reg[i].z), w3 = widen<Q>(reg[i].w);
-          load(ahead ? j + 1 : j, ahead ? 0 : turn + 4, i);
-          *reinterpret_cast<uint4 *>(to + store0 + i * S::rowsPerTurn * 128) =
-              make_uint4(w0.x, w0.y, w1.x, w1.y);
-          *reinterpret_cast<uint4 *>(to + store1 + i * S::rowsPerTurn * 128) =
-              make_uint4(w2.x, w2.y, w3.x, w3.y);
-        }
+        for (int i = 0; i < S::turns; ++i)
+          clean(first + i * S::rowsPerTurn, reg[i]);
+      }
+      unsigned char *const to = ring + b * S::tileBytes;
+#pragma unroll
+      for (int i = 0; i < S::turns; ++i) {
+        const uint2 w0 = widen<Q>(reg[i].x), w1 = widen<Q>(reg[i].y);
+        const uint2 w2 = widen<Q>(reg[i].z), w3 = widen<Q>(reg[i].w);
+        load(j + 1, i); // (four turns ahead only: 242 us instead of 210)
+        *reinterpret_cast<uint4 *>(to + store0 + i * S::rowsPerTurn * 128) =
+            make_uint4(w0.x, w0.y, w1.x, w1.y);
+        *reinterpret_cast<uint4 *>(to + store1 + i * S::rowsPerTurn * 128) =
+            make_uint4(w2.x, w2.y, w3.x, w3.y);
       }
       fenceProxyAsync();
       __syncwarp();

@@ -178,8 +178,12 @@ size_t attentionSlotBytes(HcContext c) {
 }
 size_t rowsSlotBytes(HcContext c) { return size_t(c->smCount) * rowsSlotFloats(256) * 4; }
 
-// Query rows of a sequence and key/value head from which the tcgen05 kernel takes over.
-constexpr long long kManyRows = 64;
+// Query rows of a sequence and key/value head from which the tcgen05 kernel takes over:
+// one more than the other kernel takes at a time.  (Measured, us, sixteen rows a time
+// against tcgen05, one sequence of 16384 tokens of int8 and 32 of 4096 of e4m3:
+//   16 rows  dim 64: 29, 48 / 29, 53   dim 128: 39, 66 / 35, 76   dim 256: 48, 126 / 54, 140
+//   24 rows  dim 64: 37, 66 / 31, 56   dim 128: 41, 101 / 36, 79  dim 256: 62, 160 / 55, 140)
+constexpr long long kManyRows = 17;
 
 // Parts that a unit's tiles of tokens are divided into: those whose turns through the GPU
 // are shortest, a turn costing its tiles and about eight more (the rows' conversion, the
