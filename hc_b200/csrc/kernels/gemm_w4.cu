@@ -497,52 +497,70 @@ HC_W4(i8, true, fine, true)
 
 // ---- conversions for larger row counts ----------------------------------------------------
 // out[k, n] = bf16((u - z) * s): the weights transposed into the [K, N] layout of the
-// bf16 GEMM, tiles of 64 weight rows x 128 k through shared memory.  The product is
+// bf16 GEMM, tiles of 128 weight rows x 128 k through shared memory.  The product is
 // rounded to bf16 here (half a step of 2^-8), which the few-row kernel above does not do.
+// A thread takes 32 k of two neighbouring rows, so that a pair of bf16 is a pair of the
+// output's neighbours: 128 + u by a mask and a bias, exact differences, one rounded
+// product.  Bound by its stores.
 extern "C" __global__ void __launch_bounds__(256)
     hc_dequant_w4_bf16(const __grid_constant__ W4Params p, __nv_bfloat16 *out,
                        long long outPitch) {
-  __shared__ __nv_bfloat16 tile[128][64 + 2];
+  __shared__ uint32_t tile[128][64 + 4]; // [k][pairs of rows]
   const int tid = int(threadIdx.x);
   const int rowBytes = (p.K + 1) >> 1;
-  const long long n0 = (long long)blockIdx.x * 64;
+  const long long n0 = (long long)blockIdx.x * 128;
   const int k0 = int(blockIdx.y) * 128;
   {
-    // Thread: weight row tid / 4, 32 k at (tid % 4) * 32.
-    const int r = tid >> 2, kk = (tid & 3) * 32;
-    const long long n = n0 + r;
-    const uint4 q = n < p.N ? loadWeights(p.w + n * p.ldw, (k0 + kk) >> 1, rowBytes, p.vec)
-                            : make_uint4(0, 0, 0, 0);
-    const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+    const int r = tid & 63, kk = (tid >> 6) * 32;
+    uint4 q[2];
+    float s[2] = {0.0f, 0.0f};
+    uint32_t z[2] = {8, 8};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // Groups are multiples of 32 columns: one scale for the thread's 32 weights.
-      float s = 0.0f, z = 8.0f;
-      const int k = k0 + kk + j * 8;
-      if (n < p.N && k < p.K) {
-        const long long at = k / p.group;
-        s = p.scaleF32 ? static_cast<const float *>(p.scale)[n * p.lds + at]
-                       : __bfloat162float(
-                             static_cast<const __nv_bfloat16 *>(p.scale)[n * p.lds + at]);
+    for (int i = 0; i < 2; ++i) {
+      const long long n = n0 + 2 * r + i;
+      q[i] = make_uint4(0, 0, 0, 0);
+      if (n < p.N && k0 + kk < p.K) {
+        q[i] = loadWeights(p.w + n * p.ldw, (k0 + kk) >> 1, rowBytes, p.vec);
+        // Groups are multiples of 32 columns: one scale for the thread's 32 weights.
+        const long long at = (k0 + kk) / p.group;
+        s[i] = p.scaleF32 ? static_cast<const float *>(p.scale)[n * p.lds + at]
+                          : __bfloat162float(
+                                static_cast<const __nv_bfloat16 *>(p.scale)[n * p.lds + at]);
         if (p.zero)
-          z = float(p.zero[n * p.ldz + at]);
+          z[i] = p.zero[n * p.ldz + at];
       }
+    }
+    uint32_t one28;
+    asm volatile("mov.b32 %0, 0x43004300;" : "=r"(one28));
+    // 128 + z in bf16 (exact up to z = 127).
+    const uint32_t biasBits = 0x43004300u + z[0] + (z[1] << 16);
+    const __nv_bfloat162 bias = *reinterpret_cast<const __nv_bfloat162 *>(&biasBits);
+    const __nv_bfloat162 scale = __floats2bfloat162_rn(s[0], s[1]);
+    const uint32_t wa[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+    const uint32_t wb[4] = {q[1].x, q[1].y, q[1].z, q[1].w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        tile[kk + j * 8 + i][r] =
-            __float2bfloat16_rn((float((words[j] >> (4 * i)) & 15u) - z) * s);
+    for (int j = 0; j < 16; ++j) { // byte j of both rows: k of 2j and 2j + 1
+      const uint32_t both = __byte_perm(wa[j >> 2], wb[j >> 2], 0x4400 + 0x1111 * (j & 3));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v;
+        asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(v) : "r"(both >> (4 * h)), "r"(one28));
+        const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), bias);
+        const __nv_bfloat162 y =
+            p.scaleF32 ? __floats2bfloat162_rn(__low2float(x) * s[0], __high2float(x) * s[1])
+                       : __hmul2(x, scale);
+        tile[kk + 2 * j + h][r] = *reinterpret_cast<const uint32_t *>(&y);
+      }
     }
   }
   __syncthreads();
-  // Rows of 64 n: 32 threads per row, one bf16 pair each.
-  for (int i = tid; i < 128 * 32; i += 256) {
-    const int kk = i >> 5, c = (i & 31) * 2;
-    const int k = k0 + kk;
-    const long long n = n0 + c;
-    if (k < p.K && n < outPitch) { // outPitch is even, columns past N hold zeros
-      const __nv_bfloat162 pair = __halves2bfloat162(tile[kk][c], tile[kk][c + 1]);
-      *reinterpret_cast<__nv_bfloat162 *>(out + (long long)k * outPitch + n) = pair;
-    }
+  // Rows of 128 n: 16 threads each, 16 bytes per thread.  outPitch is a multiple of 16;
+  // columns past N hold zeros.
+  for (int i = tid; i < 128 * 16; i += 256) {
+    const int kk = i >> 4, c = (i & 15) * 8;
+    if (k0 + kk < p.K && n0 + c < outPitch)
+      *reinterpret_cast<uint4 *>(out + (long long)(k0 + kk) * outPitch + n0 + c) =
+          *reinterpret_cast<const uint4 *>(&tile[kk][c / 2]);
   }
 }
 

@@ -506,7 +506,7 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
   void *args[] = {&p, &converted, &outPitch};
   if (ceilDiv(K, 128) > 65535)
     return c->fail("hcGemmW4: K=%lld is too large for a conversion", K);
-  if (c->launch("hc_dequant_w4_bf16", size_t(ceilDiv(N, 64)), size_t(ceilDiv(K, 128)), 1, 256,
+  if (c->launch("hc_dequant_w4_bf16", size_t(ceilDiv(N, 128)), size_t(ceilDiv(K, 128)), 1, 256,
                 args, 3, 0))
     return 1;
   return hcGemmBf16(c, a, weights, out, M, N, K, pitchA, pitch, ldc);
