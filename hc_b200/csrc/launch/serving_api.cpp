@@ -105,6 +105,7 @@ struct KvRowsParams {
   int share;
   int window;
   int rowTiles;
+  int compact;
   int splits;
   uint32_t blockInverse, shareInverse;
   int vecQ;
@@ -124,7 +125,7 @@ long long roundUp(long long a, long long b) { return ceilDiv(a, b) * b; }
 
 // The weight-streaming kernel of hcGemmW4 takes up to 8 activation rows that fit in
 // shared memory beside the scales of its 16 warps.
-constexpr long long kW4FewRows = 8;
+constexpr long long kW4FewRows = 8; // (both sides measured: gemm_w4.cu)
 // Up to this many the weights are converted inside the tcgen05 kernel, for more by a pass
 // of their own in front of hcGemmBf16.
 constexpr long long kW4FusedRows = 1024;
@@ -170,9 +171,7 @@ constexpr long long kAttentionCtasPerSm = 2;
 // A slot of the kernel for many query rows, in floats, one per CTA of a divided unit.
 constexpr size_t rowsSlotFloats(int cap) { return size_t(128) * (cap + 2); }
 // The workspace: counters, then the slots of either kernel.
-size_t attentionCounterBytes(HcContext c) {
-  return size_t(roundUp(c->smCount * kAttentionCtasPerSm * 4, 256));
-}
+constexpr long long kCounters = HC_KV_COUNTER_BYTES / 4;
 size_t attentionSlotBytes(HcContext c) {
   return size_t(c->smCount * kAttentionCtasPerSm) * 2 * kSlotFloats * 4;
 }
@@ -554,7 +553,7 @@ int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace *place, cons
 size_t hcKvAttentionWorkspaceBytes(HcContext c) {
   if (!c)
     return 0;
-  return attentionCounterBytes(c) + std::max(attentionSlotBytes(c), rowsSlotBytes(c));
+  return HC_KV_COUNTER_BYTES + std::max(attentionSlotBytes(c), rowsSlotBytes(c));
 }
 
 int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, const void *q,
@@ -601,7 +600,7 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   p.vecQ = aligned(q, 16) && qTokenStride % 8 == 0 && qHeadStride % 8 == 0;
   p.counters = static_cast<unsigned *>(workspace);
   p.partial =
-      reinterpret_cast<float *>(static_cast<char *>(workspace) + attentionCounterBytes(c));
+      reinterpret_cast<float *>(static_cast<char *>(workspace) + HC_KV_COUNTER_BYTES);
   char name[64];
   const char *const type = p.cache.dtype == HC_I8 ? "i8" : "e4m3";
   if (c->attentionVariant != 1 && c->ccMajor == 10 &&
@@ -613,9 +612,14 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
     u.outTokenStride = outTokenStride, u.outHeadStride = outHeadStride, u.lseStride = lseStride;
     u.scaleLog2 = p.scaleLog2, u.share = share, u.window = window;
     u.rowTiles = int(ceilDiv(maxRows, 128));
+    // Where few sequences have as many rows as the longest: the units that there are.
+    long long unitsOfHead = (long long)p.place.seqs * u.rowTiles;
+    const long long most = (long long)p.place.tokens * share / 128 + p.place.seqs;
+    u.compact = most < unitsOfHead;
+    unitsOfHead = std::min(unitsOfHead, most);
     u.blockInverse = p.blockInverse, u.shareInverse = p.shareInverse, u.vecQ = p.vecQ;
     u.counters = p.counters, u.partial = p.partial, u.status = c->statusWord;
-    const long long units = (long long)p.place.seqs * p.cache.heads * u.rowTiles;
+    const long long units = unitsOfHead * p.cache.heads;
     if (units > 0x7fffffffLL)
       return c->fail("hcKvAttention: %lld tiles of query rows are too many", units);
     const int step = cap == 256 ? 64 : 128;
@@ -624,7 +628,7 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
       reach = std::min<long long>(reach, window + ceilDiv(128, share));
     u.splits = rowSplits(units, ceilDiv(reach, step), c->smCount,
                          (long long)(rowsSlotBytes(c) / (rowsSlotFloats(cap) * 4)),
-                         c->smCount * kAttentionCtasPerSm);
+                         kCounters);
     std::snprintf(name, sizeof name, "hc_kv_attention_rows_%s_d%d", type, cap);
     void *args[] = {&u};
     return c->launch(name, size_t(units), size_t(u.splits), 1, 544, args, 1,
@@ -643,7 +647,7 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
   p.rowTiles = int(rowTiles);
   const int perSm = cap == 64 || (cap == 128 && nt == 1) ? 2 : 1;
   const long long ctas =
-      std::max<long long>(1, std::min(ceilDiv(tiles, 8), c->smCount * perSm));
+      std::max<long long>(1, std::min({ceilDiv(tiles, 8), c->smCount * perSm, kCounters}));
   std::snprintf(name, sizeof name, "hc_kv_attention_%s_d%d_r%d%s", type, cap, nt, p.cache.dim == cap ? "" : "_any");
   void *args[] = {&p};
   return c->launch(name, size_t(ctas), 1, 1, 256, args, 1,

@@ -86,9 +86,10 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     if out is None:
         out = a.new_empty((m, n), dtype=torch.bfloat16)
     workspace = None
-    need = native.w4_workspace_bytes(m, n, k, 1 if a.data_ptr() % 16 else a.stride(0),
-                                     1 if w.data_ptr() % 16 else w.stride(0),
-                                     a.dtype == torch.int8)
+    # (A single row may report any stride; an unaligned array counts as one of odd pitch.)
+    lda = 1 if a.data_ptr() % 16 else max(a.stride(0), k)
+    ldw = 1 if w.data_ptr() % 16 else max(w.stride(0), (k + 1) // 2)
+    need = native.w4_workspace_bytes(m, n, k, lda, ldw, a.dtype == torch.int8)
     if need:
         workspace = a.new_empty(need, dtype=torch.uint8)
     native.gemm_w4(ctx, a, w, scale, zero, out, group, a_scale, a_group, workspace, stream)
@@ -138,19 +139,21 @@ def kv_append(cache, k, v, table, lengths, starts=None, *, max_new=None):
 
 
 _scratch = {}
+_COUNTER_BYTES = 4096  # HC_KV_COUNTER_BYTES of the C-ABI
 
 
 def _attention_workspace(native, ctx, device, stream):
-    """Zeroed scratch of the attention: one per stream, and one of its own for every
-    call that is being captured, so that graphs may run beside each other."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(native.kv_attention_workspace_bytes(ctx), dtype=torch.uint8,
-                           device=device)
+    """Scratch of the attention, its counters zeroed: one per stream, and one of its own
+    for every call that is being captured, so that graphs may run beside each other."""
+    capturing = torch.cuda.is_current_stream_capturing()
     key = (device.index, stream)
-    buf = _scratch.get(key)
+    buf = None if capturing else _scratch.get(key)
     if buf is None:
-        buf = _scratch[key] = torch.zeros(native.kv_attention_workspace_bytes(ctx),
-                                          dtype=torch.uint8, device=device)
+        buf = torch.empty(native.kv_attention_workspace_bytes(ctx), dtype=torch.uint8,
+                          device=device)
+        buf[:_COUNTER_BYTES].zero_()
+        if not capturing:
+            _scratch[key] = buf
     return buf
 
 

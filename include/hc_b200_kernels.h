@@ -592,9 +592,13 @@ HC_B200_API int hcKvAppend(HcContext c, const HcKvCache *cache, const HcKvPlace 
  * nothing gives zeros and lse -inf.  q and out are bf16 [tokens, heads * share, dim]
  * (dim contiguous), lse float [tokens, heads * share] or null: the natural logarithm
  * of the sum of exp(scale * q . k_j).  Rows of no sequence stay as they were.
+ * Up to 16 rows of a sequence and key/value head (maxNew * share) stream the cache;
+ * more run on the tensor cores (tcgen05), 128 at a time.
  * workspace: hcKvAttentionWorkspaceBytes(c) bytes of device memory, 256-byte aligned,
- * zeroed before its first use; every call leaves it ready for the next one.  Calls that
- * may run at the same time (other streams, captured graphs) need one each. */
+ * its first HC_KV_COUNTER_BYTES zeroed before its first use; every call leaves it ready
+ * for the next one.  Calls that may run at the same time (other streams, captured
+ * graphs) need one each. */
+#define HC_KV_COUNTER_BYTES 4096
 HC_B200_API size_t hcKvAttentionWorkspaceBytes(HcContext c);
 HC_B200_API int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place,
                               const void *q, void *out, float *lse, int share, float scale,

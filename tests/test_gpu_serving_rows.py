@@ -83,6 +83,21 @@ def test_rows_divide_a_long_sequence(store, dim):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("seqs", [3, 40, 1100])
+def test_rows_one_prompt_among_single_tokens(store, seqs):
+    """A prompt beside sequences of one token, of none and without a place: the units
+    that there are, found over more than one pass of a CTA's threads."""
+    rng = np.random.default_rng(seqs)
+    lengths = rng.integers(0, 60, seqs)
+    fresh = np.minimum(rng.integers(0, 2, seqs), lengths)
+    lengths[seqs // 2], fresh[seqs // 2] = 400, 390
+    fresh[1] = lengths[1] + 2  # more new tokens than the sequence is long
+    s = Setup(store, lengths.tolist(), fresh.tolist(), block=16, share=3, dim=64, heads=2)
+    s.append()
+    s.check_attention(*s.attend())
+
+
 def test_rows_missing_pages():
     """Blocks that are not there among those that are, whole tiles of them too."""
     s = Setup("int8", [900, 300], [60, 300], block=16, share=4, dim=128)

@@ -210,3 +210,18 @@ def test_refusals():
     a8["a_scale"] = torch.ones(2, 3, device="cuda")
     with pytest.raises(RuntimeError, match="activations' group"):
         serving.gemm_w4(**a8, a_group=100)
+
+
+def test_single_rows_of_any_stride():
+    """A single row may report any stride, too deep for the kernel for few rows or not."""
+    for k in (4098, 120002):
+        c = _case(1, 48, k, 64, True, seed=k)
+        want = serving.gemm_w4(**c)
+        _check(c, want)
+        a = torch.zeros(k + 16, dtype=torch.bfloat16, device="cuda")
+        a[:k] = c["a"][0]
+        got = serving.gemm_w4(**{**c, "a": a.as_strided((1, k), (8, 1))})
+        assert torch.equal(got, want)
+        w = c["w"][:1].clone().as_strided((1, (k + 1) // 2), (16, 1))
+        one = {**c, "w": w, "scale": c["scale"][:1], "zero": c["zero"][:1]}
+        assert torch.equal(serving.gemm_w4(**one), want[:, :1])
