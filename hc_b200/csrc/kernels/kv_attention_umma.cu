@@ -49,7 +49,7 @@ struct KvRowsParams {
   // Quotients by products (ceil(2^32 / n), 0 for n = 1): of a position's sixteens by a
   // block's, of a query row by `share`.
   uint32_t blockInverse, shareInverse;
-  int vecQ;           // rows of q that 16-byte loads can take
+  int vecQ, vecOut;   // rows of q and of out that 16-byte accesses can take
   unsigned *counters; // [units], zero between calls
   float *partial;     // [units][splits] slots
   int *status;
@@ -183,6 +183,7 @@ __device__ __forceinline__ bool waitFor(uint32_t bar, uint32_t parity, volatile 
 }
 
 struct alignas(8) RowsBarriers {
+  uint64_t queriesFull;                // the softmax warps
   uint64_t keysFull[2], valuesFull[2]; // the converting warps
   uint64_t scored[3];                  // S written, the keys read (MMA commit)
   uint64_t weighted[2];                // P written (the warps of a group)
@@ -332,6 +333,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     }
     for (int s = 0; s < 3; ++s)
       mbarInit(smemAddr(&bars.scored[s]), 1);
+    mbarInit(smemAddr(&bars.queriesFull), 8);
     bars.abortFlag = 0;
     sPoisoned = 0;
     fenceBarrierInit();
@@ -339,70 +341,6 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   if (warp == kMmaWarp) {
     tmemAlloc<1>(smemAddr(&bars.tmemBase), 512);
     tmemRelinquish<1>();
-  } else {
-    // Query rows as f16, a power of two per row, K-major and swizzled: a warp takes 8.
-    constexpr int kPer = DimCap / 32; // consecutive elements of a lane
-#pragma unroll 1
-    for (int r0 = warp * 8; r0 < warp * 8 + 8; r0 += 4) {
-      uint32_t v[4][kPer / 2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < kPer / 2; ++j)
-          v[i][j] = 0;
-        if (r0 + i < rowsHere && lane * kPer < c.dim) {
-          const int qi = queryOf(row0 + r0 + i), gh = row0 + r0 + i - qi * p.share;
-          const __nv_bfloat16 *src = p.q + (long long)(span.row + qi) * p.qTokenStride +
-                                     (long long)(head * p.share + gh) * p.qHeadStride +
-                                     lane * kPer;
-          if (p.vecQ) {
-            if constexpr (kPer == 2) {
-              v[i][0] = *reinterpret_cast<const uint32_t *>(src);
-            } else if constexpr (kPer == 4) {
-              const uint2 x = *reinterpret_cast<const uint2 *>(src);
-              v[i][0] = x.x;
-              v[i][1] = x.y;
-            } else {
-              const uint4 x = *reinterpret_cast<const uint4 *>(src);
-              v[i][0] = x.x;
-              v[i][1] = x.y;
-              v[i][2] = x.z;
-              v[i][3] = x.w;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-              v[i][j >> 1] |= uint32_t(__bfloat16_as_ushort(src[j])) << (16 * (j & 1));
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + i;
-        uint32_t top2 = 0; // magnitudes order like their bits
-#pragma unroll
-        for (int j = 0; j < kPer / 2; ++j)
-          top2 = __vmaxu2(top2, v[i][j] & 0x7fff7fffu);
-        const uint32_t top =
-            __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16)) << 16;
-        // 2^e <= top < 2^(e+1); zero, subnormal and infinite rows keep their values.
-        const int e = int(top >> 23);
-        const bool plain = e == 0 || e == 255;
-        const float down = plain ? 1.0f : __uint_as_float(uint32_t(max(254 - e, 1)) << 23);
-        const float up = plain ? 1.0f : __uint_as_float(uint32_t(min(e, 253)) << 23);
-        if (lane == 0)
-          sFactor[r] = p.scaleLog2 * up;
-        const int byte = lane * kPer * 2, chunk = byte >> 7, in = byte & 127;
-        unsigned char *dst = smem + chunk * (128 * 128) + r * 128 +
-                             ((((in >> 4) ^ (r & 7)) << 4) | (in & 15));
-#pragma unroll
-        for (int j = 0; j < kPer / 2; ++j)
-          *reinterpret_cast<uint32_t *>(dst + 4 * j) =
-              halfPair(__uint_as_float(v[i][j] << 16) * down,
-                       __uint_as_float(v[i][j] & 0xffff0000u) * down);
-      }
-    }
-    fenceProxyAsync();
   }
   tcgen05FenceBefore();
   __syncthreads();
@@ -447,6 +385,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         scoreAt = scoreAt == 2 ? 0 : scoreAt + 1;
         return true;
       };
+      ok = waitFor(smemAddr(&bars.queriesFull), 0, abortFlag, status, kStatusMmaWaitData);
       for (int j = 0; ok && j < min(3, tiles); ++j)
         ok = score(j);
       for (int j = 0; ok && j < tiles; ++j) {
@@ -630,6 +569,73 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     }
   } else {
     // --------------------------------- softmax -----------------------------------
+    // Query rows as f16, a power of two per row, K-major and swizzled: a warp takes 16.
+    constexpr int kPer = DimCap / 32; // consecutive elements of a lane
+#pragma unroll 1
+    for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += 8) {
+      uint32_t v[8][kPer / 2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          v[i][j] = 0;
+        if (r0 + i < rowsHere && lane * kPer < c.dim) {
+          const int qi = queryOf(row0 + r0 + i), gh = row0 + r0 + i - qi * p.share;
+          const __nv_bfloat16 *src = p.q + (long long)(span.row + qi) * p.qTokenStride +
+                                     (long long)(head * p.share + gh) * p.qHeadStride +
+                                     lane * kPer;
+          if (p.vecQ) {
+            if constexpr (kPer == 2) {
+              v[i][0] = *reinterpret_cast<const uint32_t *>(src);
+            } else if constexpr (kPer == 4) {
+              const uint2 x = *reinterpret_cast<const uint2 *>(src);
+              v[i][0] = x.x;
+              v[i][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4 *>(src);
+              v[i][0] = x.x;
+              v[i][1] = x.y;
+              v[i][2] = x.z;
+              v[i][3] = x.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              v[i][j >> 1] |= uint32_t(__bfloat16_as_ushort(src[j])) << (16 * (j & 1));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + i;
+        uint32_t top2 = 0; // magnitudes order like their bits
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          top2 = __vmaxu2(top2, v[i][j] & 0x7fff7fffu);
+        const uint32_t top =
+            __reduce_max_sync(0xffffffffu, max(top2 & 0xffffu, top2 >> 16)) << 16;
+        // 2^e <= top < 2^(e+1); zero, subnormal and infinite rows keep their values.
+        const int e = int(top >> 23);
+        const bool plain = e == 0 || e == 255;
+        const float down = plain ? 1.0f : __uint_as_float(uint32_t(max(254 - e, 1)) << 23);
+        const float up = plain ? 1.0f : __uint_as_float(uint32_t(min(e, 253)) << 23);
+        if (lane == 0)
+          sFactor[r] = p.scaleLog2 * up;
+        const int byte = lane * kPer * 2, chunk = byte >> 7, in = byte & 127;
+        unsigned char *dst = smem + chunk * (128 * 128) + r * 128 +
+                             ((((in >> 4) ^ (r & 7)) << 4) | (in & 15));
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j)
+          *reinterpret_cast<uint32_t *>(dst + 4 * j) =
+              halfPair(__uint_as_float(v[i][j] << 16) * down,
+                       __uint_as_float(v[i][j] & 0xffff0000u) * down);
+      }
+    }
+    fenceProxyAsync();
+    __syncwarp();
+    if (lane == 0)
+      mbarArrive(smemAddr(&bars.queriesFull));
+    ok = await(bars.queriesFull, 0, kStatusRowsSoftmax); // (the rows' factors)
     const int group = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t laneBase = uint32_t((warp & 3) * 32) << 16;
     const float rowFactor = sFactor[r];
@@ -639,7 +645,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     float ref = kNegInf; // what `sum` was taken against
     float sum = 0.0f;
     int at3 = group, use3 = 0; // of tile j in the ring of three
-    for (int j = group; j < tiles; j += 2) {
+    for (int j = group; ok && j < tiles; j += 2) {
       const int b = j & 1, pos = pos0 + j * T;
       if (!(ok = await(bars.scored[at3], use3, kStatusRowsSoftmax)))
         break;
@@ -813,16 +819,35 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   auto slotOf = [&](int part) {
     return p.partial + ((long long)unit * p.splits + part) * S::slotFloats;
   };
-  auto finish = [&](int r, int d, float4 v, float f) {
-    const int qi = queryOf(row0 + r), gh = row0 + r - qi * p.share;
+  // Rows go out through shared memory (the queries' place), 16 bytes per thread and whole
+  // rows per warp: a thread per row storing its own took 4 us per unit.  The 16-byte
+  // chunks of a row are exchanged by an XOR with the row.
+  auto keep = [&](int r, int d, float4 v, float f) {
     __nv_bfloat162 x = __floats2bfloat162_rn(v.x * f, v.y * f);
     __nv_bfloat162 y = __floats2bfloat162_rn(v.z * f, v.w * f);
     uint2 packed;
     packed.x = *reinterpret_cast<uint32_t *>(&x);
     packed.y = *reinterpret_cast<uint32_t *>(&y);
-    if (d < c.dim)
-      *reinterpret_cast<uint2 *>(p.out + (long long)(span.row + qi) * p.outTokenStride +
-                                 (long long)(head * p.share + gh) * p.outHeadStride + d) = packed;
+    *reinterpret_cast<uint2 *>(smem + r * (2 * DimCap) + (((d >> 3) ^ (r & 7)) << 4) +
+                               (d & 4) * 2) = packed;
+  };
+  auto writeRows = [&]() {
+    for (int i = tid; i < rowsHere * (DimCap / 8); i += kThreads) {
+      const int r = i / (DimCap / 8), ch = i - r * (DimCap / 8);
+      if (ch * 8 >= c.dim)
+        continue;
+      const uint4 v =
+          *reinterpret_cast<const uint4 *>(smem + r * (2 * DimCap) + ((ch ^ (r & 7)) << 4));
+      const int qi = queryOf(row0 + r), gh = row0 + r - qi * p.share;
+      __nv_bfloat16 *to = p.out + (long long)(span.row + qi) * p.outTokenStride +
+                          (long long)(head * p.share + gh) * p.outHeadStride + ch * 8;
+      if (p.vecOut) {
+        *reinterpret_cast<uint4 *>(to) = v;
+      } else {
+        *reinterpret_cast<uint2 *>(to) = make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2 *>(to + 4) = make_uint2(v.z, v.w);
+      }
+    }
   };
   auto finishSum = [&](int r, float top, float sum) {
     const int qi = queryOf(row0 + r), gh = row0 + r - qi * p.share;
@@ -884,7 +909,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
             }
           }
           if (parts == 1)
-            finish(r, d0 + 4 * i, o, f);
+            keep(r, d0 + 4 * i, o, f);
           else // [dims / 4][rows]
             __stcg(reinterpret_cast<float4 *>(slot) + (d0 / 4 + i) * 128 + r, o);
         }
@@ -906,8 +931,11 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     tcgen05FenceAfter();
     tmemFree<1>(tmemBase, 512);
   }
-  if (parts == 1)
+  if (parts == 1) {
+    if (!aborted)
+      writeRows();
     return;
+  }
 
   // ---- the last part to finish joins them, in their order ------------------------------------
   __threadfence();
@@ -918,7 +946,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   if (!sLast)
     return;
   __threadfence();
-  float *const sWeight = reinterpret_cast<float *>(smem); // [part][rows]
+  float *const sWeight = reinterpret_cast<float *>(smem + S::qBytes); // [part][rows]
   if (tid < rowsHere) {
     float top = kNegInf;
     for (int x = 0; x < parts; ++x)
@@ -952,8 +980,10 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         v.w = fmaf(y.w, f, v.w);
       }
     }
-    finish(r, d, v, sSum[0][r] == 0.0f ? 0.0f : 1.0f / (kWeight * sSum[0][r]));
+    keep(r, d, v, sSum[0][r] == 0.0f ? 0.0f : 1.0f / (kWeight * sSum[0][r]));
   }
+  __syncthreads();
+  writeRows();
 }
 
 } // namespace

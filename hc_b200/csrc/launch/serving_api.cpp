@@ -108,7 +108,7 @@ struct KvRowsParams {
   int compact;
   int splits;
   uint32_t blockInverse, shareInverse;
-  int vecQ;
+  int vecQ, vecOut;
   unsigned *counters;
   float *partial;
   int *status;
@@ -618,6 +618,7 @@ int hcKvAttention(HcContext c, const HcKvCache *cache, const HcKvPlace *place, c
     u.compact = most < unitsOfHead;
     unitsOfHead = std::min(unitsOfHead, most);
     u.blockInverse = p.blockInverse, u.shareInverse = p.shareInverse, u.vecQ = p.vecQ;
+    u.vecOut = aligned(out, 16) && outTokenStride % 8 == 0 && outHeadStride % 8 == 0;
     u.counters = p.counters, u.partial = p.partial, u.status = c->statusWord;
     const long long units = unitsOfHead * p.cache.heads;
     if (units > 0x7fffffffLL)
