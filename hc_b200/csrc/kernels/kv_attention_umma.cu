@@ -723,26 +723,6 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       }
       if (plain)
         tmemLoadWaitFor(v);
-      if (__any_sync(0xffffffffu, now != old) && j > 0) {
-        if (!(ok = await(bars.added[b ^ 1], (j - 1) >> 1, kStatusRowsSoftmax)))
-          break;
-        tcgen05FenceAfter();
-        const float f = now == old ? 1.0f : exp2Approx(old - now);
-#pragma unroll 1
-        for (int d = 0; d < DimCap; d += 16) {
-          tmemLoad32x16(tmemBase + laneBase + S::atO + uint32_t(d), u);
-          tmemLoadWaitFor(u);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t o[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              o[i] = __float_as_uint(__uint_as_float(u[8 * k + i]) * f);
-            tmemStore32x8(tmemBase + laneBase + S::atO + uint32_t(d + 8 * k), o);
-          }
-        }
-      }
-
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
@@ -802,6 +782,26 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       float lo, hi;
       unpair(sum2, lo, hi);
       sum += lo + hi;
+      // O, where the reference has moved: the outputs of the tile before are in it by now.
+      if (__any_sync(0xffffffffu, now != old) && j > 0) {
+        if (!(ok = await(bars.added[b ^ 1], (j - 1) >> 1, kStatusRowsSoftmax)))
+          break;
+        tcgen05FenceAfter();
+        const float f = now == old ? 1.0f : exp2Approx(old - now);
+#pragma unroll 1
+        for (int d = 0; d < DimCap; d += 16) {
+          tmemLoad32x16(tmemBase + laneBase + S::atO + uint32_t(d), u);
+          tmemLoadWaitFor(u);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              o[i] = __float_as_uint(__uint_as_float(u[8 * k + i]) * f);
+            tmemStore32x8(tmemBase + laneBase + S::atO + uint32_t(d + 8 * k), o);
+          }
+        }
+      }
       tmemStoreWait();
       tcgen05FenceBefore();
       __syncwarp();
