@@ -87,18 +87,40 @@ HC_KV_FN int hcKvTouchedBlocks(int maxNew, int block) {
 // share is empty.
 struct HcKvShares {
   unsigned each, longer; // tiles of a share; how many have one more
+  // Or, where every unit is alike: its tiles, and the shares that it is cut into (0: as
+  // above).  No share then holds pieces of two units.
+  unsigned unitTiles, perUnit;
 };
 HC_KV_FN HcKvShares hcKvSharesOf(unsigned total, unsigned shares) {
   HcKvShares s;
   s.each = total / shares;
   s.longer = total - s.each * shares;
+  s.unitTiles = s.perUnit = 0;
+  return s;
+}
+// perUnit: at most unitTiles.
+HC_KV_FN HcKvShares hcKvSharesOfUnits(unsigned unitTiles, unsigned perUnit) {
+  HcKvShares s;
+  s.each = s.longer = 0;
+  s.unitTiles = unitTiles;
+  s.perUnit = perUnit;
   return s;
 }
 HC_KV_FN unsigned hcKvShareBegin(const HcKvShares &s, unsigned c) {
+  if (s.perUnit) {
+    const unsigned unit = c / s.perUnit, part = c - unit * s.perUnit;
+    return unit * s.unitTiles +
+           unsigned((unsigned long long)s.unitTiles * part / s.perUnit);
+  }
   return c * s.each + (c < s.longer ? c : s.longer);
 }
 // The share that holds tile x.
 HC_KV_FN unsigned hcKvShareOf(const HcKvShares &s, unsigned x) {
+  if (s.perUnit) { // the last part that begins at x or before it
+    const unsigned unit = x / s.unitTiles, r = x - unit * s.unitTiles;
+    return unit * s.perUnit +
+           unsigned(((unsigned long long)(r + 1) * s.perUnit - 1) / s.unitTiles);
+  }
   const unsigned head = s.longer * (s.each + 1);
   return x < head ? x / (s.each + 1) : s.longer + (x - head) / s.each;
 }

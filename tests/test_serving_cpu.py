@@ -59,14 +59,18 @@ def params(tmp_path_factory):
           return hcKvShareBegin(hcKvSharesOf(t, n), c); }
         extern "C" unsigned share(unsigned x, unsigned t, unsigned n) {
           return hcKvShareOf(hcKvSharesOf(t, n), x); }
+        extern "C" unsigned unit_begin(unsigned c, unsigned t, unsigned n) {
+          return hcKvShareBegin(hcKvSharesOfUnits(t, n), c); }
+        extern "C" unsigned unit_share(unsigned x, unsigned t, unsigned n) {
+          return hcKvShareOf(hcKvSharesOfUnits(t, n), x); }
         """))
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-fsanitize=undefined",
                     "-fno-sanitize-recover", "-static-libubsan", "-I",
                     str(REPO / "hc_b200" / "csrc" / "kernels"), "-o", str(out), str(src)],
                    check=True)
     lib = C.CDLL(str(out))
-    lib.begin.restype = lib.share.restype = C.c_uint
-    lib.begin.argtypes = lib.share.argtypes = [C.c_uint] * 3
+    for fn in (lib.begin, lib.share, lib.unit_begin, lib.unit_share):
+        fn.restype, fn.argtypes = C.c_uint, [C.c_uint] * 3
     return lib
 
 
@@ -127,6 +131,19 @@ def test_shares_cover_every_tile_once(params):
             for c in range(0, n, max(1, n // 7)):
                 for x in (bounds[c], bounds[c + 1] - 1):
                     assert params.share(x, total, n) == c
+
+
+def test_shares_of_like_units_end_with_them(params):
+    for tiles in (1, 2, 7, 94, 297, 99991, 2 ** 27 - 1):
+        for per in (1, 2, 3, 12, 37, 296):
+            n = min(per, tiles)
+            units = min(16, (2 ** 31 - 1) // tiles)
+            bounds = [params.unit_begin(c, tiles, n) for c in range(units * n + 1)]
+            assert bounds[::n] == [u * tiles for u in range(units + 1)]
+            assert all(a < b for a, b in zip(bounds, bounds[1:]))
+            for c in range(0, units * n, max(1, n // 7)):
+                for x in (bounds[c], bounds[c + 1] - 1):
+                    assert params.unit_share(x, tiles, n) == c
 
 
 # ---- the C-ABI on a recording driver --------------------------------------------------------
