@@ -16,12 +16,14 @@
 // latency bound.  A warp owns one unit, a (sequence, block, head) of keys or of values: it
 // reads the new rows once into registers (what does not fit there again from L1), reduces
 // by shuffles alone, and nobody else writes its bytes.  Where that gives the GPU too few
-// warps a CTA takes a unit.  Measured: 16 prompts of up to 2048 tokens, 8 heads of 128, in
-// 31 us by warps (3.6 TB/s of reads and writes; 38 by CTAs, which spend most instructions
-// on setting up); one chunk of 512 tokens in 5.0 us by CTAs (19 by warps); one token in
-// 2.8 us.
+// warps a CTA takes a unit.  Measured: 16 prompts of up to 2048 tokens, 8 heads of 128, to
+// e4m3 in 25 us by warps (4.4 TB/s of reads and writes; when both were tried, 31 by warps
+// and 38 by CTAs, which spend most instructions on setting up), to int8, which divides, in
+// 55; one chunk of 512 tokens in 4.5 us by CTAs (19 by warps); one token in 2.8 us.
 #include "kv_params.h"
 #include "serving_math.cuh"
+
+#include <type_traits>
 
 using namespace hcs;
 
@@ -155,13 +157,16 @@ template <class Q, int Threads> __device__ __forceinline__ void appendBlock(cons
   };
   // (One token is one turn: leaving early keeps the code that runs short, and at one
   // token per sequence fetching instructions is what takes the time.)
-  const int turns = (rows * perRow + Threads - 1) / Threads;
+  // Only rows of 16-byte loads are held, and only for the usual way of storing them is the
+  // code unrolled: with every combination of the two unrolled, fetching instructions took
+  // half of the time.
+  const int turns = p.vec ? (rows * perRow + Threads - 1) / Threads : 0;
   At at = first;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     if (i >= turns)
       break;
-    raw[i] = at.row < rows ? fetch(at) : Raw{};
+    raw[i] = at.row < rows ? loadRaw(at.from, 1) : Raw{};
     advance(at);
   }
 #pragma unroll
@@ -170,12 +175,14 @@ template <class Q, int Threads> __device__ __forceinline__ void appendBlock(cons
       break;
     magnitude(raw[i]);
   }
+#pragma unroll 1
   for (; at.row < rows; advance(at))
     magnitude(fetch(at));
   uint32_t top16 = max(top2 & 0xffffu, top2 >> 16);
   top16 = largest(top16);
   if (top16 >= 0x7f80u) { // something is not finite: the largest of the others
     uint32_t best = 0;
+#pragma unroll 1
     for (at = first; at.row < rows; advance(at)) {
       const Raw x = fetch(at);
 #pragma unroll
@@ -212,36 +219,37 @@ template <class Q, int Threads> __device__ __forceinline__ void appendBlock(cons
   const bool exact = (bits & 0x007fffffu) == 0 && bits >= 0x01000000u && bits < 0x7e000000u;
   const float inv = exact ? 1.0f / scale : 0.0f;
   const bool product = exact || !(scale > 0.0f);
-  auto store = [&](const Raw &x, const At &to) {
+  auto store = [&](auto multiply, const Raw &x, const At &to) {
     float e[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       e[2 * k] = __uint_as_float(x.w[k] << 16);
       e[2 * k + 1] = __uint_as_float(x.w[k] & 0xffff0000u);
     }
-    if (product) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        e[k] *= inv;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        e[k] = __fdiv_rn(e[k], scale);
-    }
+    for (int k = 0; k < 8; ++k)
+      e[k] = decltype(multiply)::value ? e[k] * inv : __fdiv_rn(e[k], scale);
     *reinterpret_cast<uint2 *>(to.to) =
         make_uint2(quantise4<Q>(e[0], e[1], e[2], e[3]), quantise4<Q>(e[4], e[5], e[6], e[7]));
   };
   at = first;
+  if (product) {
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    if (i >= turns)
-      break;
-    if (at.row < rows)
-      store(raw[i], at);
-    advance(at);
+    for (int i = 0; i < kHeld; ++i) {
+      if (i >= turns)
+        break;
+      if (at.row < rows)
+        store(std::true_type{}, raw[i], at);
+      advance(at);
+    }
+#pragma unroll 1
+    for (; at.row < rows; advance(at))
+      store(std::true_type{}, fetch(at), at);
+  } else {
+#pragma unroll 1
+    for (; at.row < rows; advance(at)) // (the rows come from L1 again)
+      store(std::false_type{}, fetch(at), at);
   }
-  for (; at.row < rows; advance(at))
-    store(fetch(at), at);
 }
 
 } // namespace
