@@ -4,8 +4,8 @@
 //
 // 128 query rows against T tokens (128, or 64 for heads of 256) at a time on tcgen05:
 //   S[128, T] = Q K^T       Q and K in shared memory, f16
-//   O[128, D] += P V        P in tensor memory (f16, over its scores), V in shared memory as it lies in
-//                           the cache, tokens by dims: an MN-major operand
+//   O[128, D] += P V        P in tensor memory (f16, over its scores), V in shared memory
+//                           as it lies in the cache, tokens by dims: an MN-major operand
 // Roles of a CTA, which keeps to one unit (sequence, head, 128 rows), or a part of its
 // tokens where there are few units:
 //   * 4 warps bring the keys of a tile from the cache into registers a tile ahead, widen
@@ -20,8 +20,8 @@
 // three run beside each other.  Reading the cache is small beside that (32 KiB a tile,
 // mostly from L2).
 // Measured: 512 new tokens of 32 heads (8 for keys and values, dim 128) at 16384 tokens in
-// 209 us with int8 and 196 with e4m3, 650 and 690 TFLOP/s, against 1143 and 1020 us with
-// kv_attention.cu; dim 64 172 us, dim 256 415.  Counters show half of the issue slots
+// 198 us with int8 and 188 with e4m3, 690 and 720 TFLOP/s, against 1143 and 1020 us with
+// kv_attention.cu; dim 64 166 us, dim 256 424.  Counters show half of the issue slots
 // taken (8600 instructions per tile, half of them conversion), the tensor pipe at a
 // quarter and no single pipe full: what is left are the latencies of the hand-overs
 // between the roles.
@@ -189,6 +189,7 @@ struct alignas(8) RowsBarriers {
   uint64_t weighted[2];                // P written (the warps of a group)
   uint64_t decided[2];                 // the reference of a tile stands
   uint64_t added[2];                   // P and the values read, O complete (MMA commit)
+  uint64_t done;                       // all of it
   uint32_t tmemBase;
   int abortFlag;
 };
@@ -334,6 +335,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     for (int s = 0; s < 3; ++s)
       mbarInit(smemAddr(&bars.scored[s]), 1);
     mbarInit(smemAddr(&bars.queriesFull), 8);
+    mbarInit(smemAddr(&bars.done), 1);
     bars.abortFlag = 0;
     sPoisoned = 0;
     fenceBarrierInit();
@@ -408,6 +410,8 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         // The place of tile j's scores and weights is free behind these MMAs.
         ok = j + 3 >= tiles || score(j + 3);
       }
+      if (ok)
+        ummaCommit(smemAddr(&bars.done));
       if (!ok) { // MMAs may still be reading
         const unsigned long long t0 = globalTimerNs();
         while (globalTimerNs() - t0 < 1000000ull) {
@@ -662,8 +666,9 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       const bool plain = whole && sPlain[j & 7];
       uint32_t v[16], u[16];
 
-      // The largest score with its value scale.  Sixteen columns are loaded while sixteen
-      // are worked on, in loops that are not unrolled further.
+      // The largest score with its value scale, in loops that are not unrolled further.
+      // (No load stays in flight across a branch or a loop's end, where the compiler might
+      // move a register that it has not reached yet.)
       float top = kNegInf;
       auto seen = [&](int at) { return at >= seenLo && at <= seenHi; };
       auto most16 = [&](const uint32_t (&x)[16], const Group &g) {
@@ -677,16 +682,14 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         top = fmaxf(top, fmaf(fmaxf(a, c), g.key * rowFactor, g.logValue));
       };
       if (plain) {
-        tmemLoad32x16(sAt, v);
 #pragma unroll 1
         for (int k = 0; k < T / 32; ++k) {
+          tmemLoad32x16(sAt + uint32_t(32 * k), v);
+          tmemLoad32x16(sAt + uint32_t(32 * k + 16), u);
           const Group g0 = groups[2 * k], g1 = groups[2 * k + 1];
           tmemLoadWaitFor(v);
-          tmemLoad32x16(sAt + uint32_t(32 * k + 16), u);
-          most16(v, g0);
           tmemLoadWaitFor(u);
-          // (at the end the first columns again, for the weights)
-          tmemLoad32x16(sAt + (uint32_t(32 * (k + 1)) & (T - 1)), v);
+          most16(v, g0);
           most16(u, g1);
         }
       } else {
@@ -721,8 +724,6 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         sum *= exp2Approx(ref - now); // (0 against -inf: there was no sum)
         ref = now;
       }
-      if (plain)
-        tmemLoadWaitFor(v);
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
@@ -746,14 +747,12 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       if (plain) {
 #pragma unroll 1
         for (int k = 0; k < T / 32; ++k) {
-          const Group g0 = groups[2 * k], g1 = groups[2 * k + 1];
-          if (k)
-            tmemLoadWaitFor(v);
+          tmemLoad32x16(sAt + uint32_t(32 * k), v);
           tmemLoad32x16(sAt + uint32_t(32 * k + 16), u);
-          weigh16(v, g0, uint32_t(16 * k));
+          const Group g0 = groups[2 * k], g1 = groups[2 * k + 1];
+          tmemLoadWaitFor(v);
           tmemLoadWaitFor(u);
-          if (k + 1 < T / 32)
-            tmemLoad32x16(sAt + uint32_t(32 * (k + 1)), v);
+          weigh16(v, g0, uint32_t(16 * k));
           weigh16(u, g1, uint32_t(16 * k + 8));
         }
       } else {
@@ -784,6 +783,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       sum += lo + hi;
       // O, where the reference has moved: the outputs of the tile before are in it by now.
       if (__any_sync(0xffffffffu, now != old) && j > 0) {
+        // (Use before last: complete, the scores of tile j came behind it.)
         if (!(ok = await(bars.added[b ^ 1], (j - 1) >> 1, kStatusRowsSoftmax)))
           break;
         tcgen05FenceAfter();
@@ -857,7 +857,9 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   };
   const bool aborted = *abortFlag != 0;
   if (warp < 8 && !aborted) {
-    if (await(bars.added[(tiles - 1) & 1], (tiles - 1) >> 1, kStatusEpilogueWait)) {
+    // (A barrier of its own: a wait for the last use of `added` would also pass while the
+    // use before the last but one is incomplete.)
+    if (await(bars.done, 0, kStatusEpilogueWait)) {
       tcgen05FenceAfter();
       const int group = warp >> 2, r = (warp & 3) * 32 + lane;
       const float top = sRef[r];

@@ -98,6 +98,42 @@ def test_rows_one_prompt_among_single_tokens(store, seqs):
     s.check_attention(*s.attend())
 
 
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_again_and_again(store, dim):
+    """Sequences of few tiles, many times over: nothing is read before it is complete, and
+    every row is written (the outputs are NaN before each call)."""
+    s = Setup(store, [310, 700, 1, 129, 260], [310, 150, 1, 1, 33], block=32, share=3, dim=dim)
+    s.append()
+    first, first_lse = s.attend()
+    s.check_attention(first, first_lse)
+    out = torch.empty_like(first)
+    for _ in range(300):
+        out.fill_(float("nan"))
+        _, lse = s.attend(out=out)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)
+
+
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("dim,share", [(64, 3), (128, 1), (256, 3)])
+def test_workspace_holds_nothing_but_counters(rows_kernel, store, dim, share, variant):
+    """Whatever the workspace holds behind its counters, it is written before it is read."""
+    rows_kernel.set_option("attention_variant", variant)
+    for lengths, fresh in (([310, 700, 1, 129, 260], [310, 150, 1, 1, 33]), ([9000], [5]),
+                           ([3000, 17, 900], [1, 1, 1])):
+        s = Setup(store, lengths, fresh, block=32, share=share, dim=dim)
+        s.append()
+        want, want_lse = s.attend()
+        s.check_attention(want, want_lse)
+        for _ in range(5):
+            for buf in serving._scratch.values():
+                buf[4096:].fill_(0xFF)
+            out = torch.full_like(s.q, float("nan"))
+            _, lse = s.attend(out=out)
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 def test_rows_missing_pages():
     """Blocks that are not there among those that are, whole tiles of them too."""
     s = Setup("int8", [900, 300], [60, 300], block=16, share=4, dim=128)
