@@ -668,7 +668,9 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
 
       // The largest score with its value scale, in loops that are not unrolled further.
       // (No load stays in flight across a branch or a loop's end, where the compiler might
-      // move a register that it has not reached yet.)
+      // move a register that it has not reached yet; and the warp is brought together in
+      // front of each load behind code whose path differs by lane: all 32 lanes have to
+      // reach it at once.)
       float top = kNegInf;
       auto seen = [&](int at) { return at >= seenLo && at <= seenHi; };
       auto most16 = [&](const uint32_t (&x)[16], const Group &g) {
@@ -698,6 +700,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
           const Group g = groups[k];
           if (g.there == 0.0f)
             continue;
+          __syncwarp();
           tmemLoad32x16(sAt + uint32_t(16 * k), v);
           tmemLoadWaitFor(v);
 #pragma unroll
@@ -724,6 +727,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         sum *= exp2Approx(ref - now); // (0 against -inf: there was no sum)
         ref = now;
       }
+      __syncwarp();
       const float base = now == kNegInf ? 0.0f : now;
       const uint64_t minusBase = pairOf(-base, -base);
       uint64_t sum2 = pairOf(0.0f, 0.0f);
@@ -760,6 +764,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         for (int k = 0; k < T / 16; ++k) {
           const Group g = groups[k];
           uint32_t w[8];
+          __syncwarp();
           tmemLoad32x16(sAt + uint32_t(16 * k), v);
           tmemLoadWaitFor(v);
 #pragma unroll
@@ -877,12 +882,11 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
 #pragma unroll 1
       for (int d0 = group * (DimCap / 2); d0 < (group + 1) * (DimCap / 2); d0 += 16) {
         uint32_t v[16];
+        __syncwarp(); // (the lanes' paths through the turn before differ)
         tmemLoad32x16(tmemBase + (uint32_t((warp & 3) * 32) << 16) + S::atO + d0, v);
         tmemLoadWaitFor(v);
-        if (r >= rowsHere)
-          continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4 && r < rowsHere; ++i) {
           float4 o = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
                                  __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
           if (__is_same(Q, E4M3) && sPoisoned && d0 + 4 * i < c.dim) {
@@ -924,6 +928,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
           __stcg(slot + 128 * DimCap + 128 + r, sum);
         }
       }
+      __syncwarp();
       tcgen05FenceBefore();
     }
   }

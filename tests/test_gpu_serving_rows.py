@@ -179,3 +179,23 @@ def test_rows_is_the_choice_for_many(rows_kernel):
         s.check_attention(out, lse)
         outs.append(out)
     assert torch.equal(outs[0], outs[2]) and not torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("fresh,share", [(45, 1), (61, 3), (130, 1), (7, 5)])
+def test_rows_nan_values_where_rows_end_inside_a_warp(dim, fresh, share):
+    """The last warp of a unit has rows in some of its lanes only, and each of them passes
+    over another number of the tokens that are mended: again and again the same."""
+    s = Setup("e4m3", [400], [fresh], block=16, share=share, dim=dim, heads=2)
+    s.append()
+    clean, clean_lse = s.attend()
+    want = torch.zeros(clean.shape, dtype=torch.bool)
+    view, first = s.cache.v.view(torch.uint8), 400 - fresh
+    for i, back in enumerate(range(0, fresh, 3)):
+        head, d = i % 2, (7 * i) % dim
+        view[s.table[0, (399 - back) // 16], head, (399 - back) % 16, d] = 0x7F
+        want[399 - back - first:, share * head:share * (head + 1), d] = True
+    for _ in range(30):
+        out, lse = s.attend(out=torch.full_like(clean, 3.0))
+        assert torch.equal(torch.isnan(out).cpu(), want)
+        assert torch.equal(out[~want.cuda()], clean[~want.cuda()]) and torch.equal(lse, clean_lse)
