@@ -193,6 +193,8 @@ KERNELS_PROTOTYPES = {
     "hcSynchronize": (C.c_int, [_vp]),
     "hcUseStream": (C.c_int, [_vp, _vp]),
     "hcUseOwnStream": (C.c_int, [_vp]),
+    "hcPushStream": (C.c_int, [_vp, _vp]),
+    "hcPopStream": (C.c_int, [_vp]),
     "hcLastError": (C.c_char_p, [_vp]),
     "hcLaunchCount": (_ll, [_vp]),
     "hcKernelStatus": (C.c_int, [_vp, C.POINTER(C.c_int)]),
@@ -590,6 +592,13 @@ class Context:
 
     def use_own_stream(self):
         self._check(self.lib.hcUseOwnStream(self.handle), "hcUseOwnStream")
+
+    def push_stream(self, stream: int):
+        """What this thread launches goes to this CUstream until :meth:`pop_stream`."""
+        self._check(self.lib.hcPushStream(self.handle, stream), "hcPushStream")
+
+    def pop_stream(self):
+        self._check(self.lib.hcPopStream(self.handle), "hcPopStream")
 
     def add_rms_norm(self, x, residual, summed, gain, out, scale_out, rows, cols, x_pitch,
                      residual_pitch, summed_pitch, out_pitch, scale_pitch, group, eps,

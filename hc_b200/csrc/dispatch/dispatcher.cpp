@@ -67,7 +67,7 @@ public:
 private:
   static void onMessage(void *self, OlSeverity sev, const char *text) {
     auto *c = static_cast<Context *>(self);
-    if (sev == OlSeverity::Error) {
+    if (sev == OlSeverity::Error && !c->handle) { // (of opening: later ones are hcLastError's)
       if (!c->errors.empty())
         c->errors += "; ";
       c->errors += text ? text : "";
@@ -658,20 +658,21 @@ void gemmW8A16(Context &ctx, py::handle a, py::handle w, py::handle scale, py::h
 }
 
 // ---- serving operators ------------------------------------------------------------------
-// Launches go to `stream` (a raw CUstream, 0 = the legacy default stream) for the
-// length of the scope, then to the context's own stream again; None: the own one.
+// This thread's launches go to `stream` (a raw CUstream, 0 = the legacy default stream)
+// for the length of the scope; None: to the context's own.  (Other threads may be inside
+// an entry point that runs without the interpreter lock: theirs stay where they were.)
 class StreamScope {
 public:
   StreamScope(Context &ctx, py::handle stream) {
     if (stream.is_none())
       return;
-    ctx.check(hcUseStream(ctx.get(), reinterpret_cast<void *>(stream.cast<uintptr_t>())),
-              "use_stream");
+    ctx.check(hcPushStream(ctx.get(), reinterpret_cast<void *>(stream.cast<uintptr_t>())),
+              "push_stream");
     held = ctx.get();
   }
   ~StreamScope() {
     if (held)
-      hcUseOwnStream(held);
+      hcPopStream(held);
   }
   StreamScope(const StreamScope &) = delete;
   StreamScope &operator=(const StreamScope &) = delete;

@@ -4,25 +4,56 @@
 
 #include "hc_b200_kernels.h"
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
 #include <map>
+#include <mutex>
 #include <string>
 #include <vector>
 
+// The last error's text: threads that share a context write it and read copies.
+class HcErrorText {
+public:
+  void operator=(const char *s) {
+    std::lock_guard<std::mutex> hold(lock);
+    text = s;
+  }
+  // Valid until the calling thread's next call.
+  const char *c_str() const {
+    static thread_local std::string copy;
+    std::lock_guard<std::mutex> hold(lock);
+    return (copy = text).c_str();
+  }
+
+private:
+  mutable std::mutex lock;
+  std::string text;
+};
+
+// One thread may be inside a host-buffer entry point (Python runs those without its
+// interpreter lock) while another launches through the same context: what both reach -
+// the tables of loaded images, the error's text, the count of launches - is guarded, and
+// which queue a launch goes to is a matter of the thread that launches.
 struct HcContextImpl {
   OlErrorCallback callback = nullptr;
   void *callbackCtx = nullptr;
   OlDevice device = nullptr;
-  OlQueue queue = nullptr;    // where launches go: ownQueue, or a borrowed one (hcUseStream)
   OlQueue ownQueue = nullptr;
+  OlQueue chosenQueue = nullptr; // ownQueue, or a borrowed one (hcUseStream)
+  // Where the calling thread's launches go: what it pushed last (hcPushStream,
+  // HcQueueScope), else chosenQueue.
+  OlQueue queue() const;
+  // The queue on a caller's stream, or null (with an error).
+  OlQueue borrowed(void *stream);
+  std::mutex tables; // guards the next three
   std::map<void *, OlQueue> borrowedQueues; // by the caller's stream handle
   std::vector<OlModule> modules; // one slot per image, loaded on first use
   std::map<std::string, OlKernel> kernels;
   int *statusWord = nullptr; // device
-  std::string lastError;
-  long long launches = 0;
+  HcErrorText lastError;
+  std::atomic<long long> launches{0};
   long long smCount = 0;
   long long ccMajor = 0;
   long long ccMinor = 0;
@@ -80,6 +111,19 @@ struct HcContextImpl {
                     void **args, size_t smem);
   // Scratch of the host-buffer entry points (host_api.cpp), released with the context.
   struct HostPipeline *hostPipeline = nullptr;
+};
+
+// Sends the calling thread's launches through `c` to `q` for the length of the scope,
+// whatever other threads choose meanwhile.
+class HcQueueScope {
+public:
+  HcQueueScope(HcContextImpl *c, OlQueue q);
+  ~HcQueueScope();
+  HcQueueScope(const HcQueueScope &) = delete;
+  HcQueueScope &operator=(const HcQueueScope &) = delete;
+
+private:
+  HcContextImpl *const context;
 };
 
 // Frees what the host-buffer entry points keep in a context (host_api.cpp).

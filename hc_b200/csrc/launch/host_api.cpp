@@ -61,9 +61,9 @@ void hcReleaseHostPipeline(HcContextImpl *c) {
   for (int s = 0; s < 2; ++s) {
     for (int k = 0; k < 2; ++k) {
       if (p->in[s][k].data)
-        olDeallocDevice(c->queue, p->in[s][k].data);
+        olDeallocDevice(c->ownQueue, p->in[s][k].data);
       if (p->out[s][k].data)
-        olDeallocDevice(c->queue, p->out[s][k].data);
+        olDeallocDevice(c->ownQueue, p->out[s][k].data);
     }
     olxReleaseEvent(c->device, p->uploaded[s]);
     olxReleaseEvent(c->device, p->kernelDone[s]);
@@ -71,7 +71,7 @@ void hcReleaseHostPipeline(HcContextImpl *c) {
   }
   olxReleaseEvent(c->device, p->start);
   if (p->resident.data)
-    olDeallocDevice(c->queue, p->resident.data);
+    olDeallocDevice(c->ownQueue, p->resident.data);
   if (p->up)
     olReleaseQueue(p->up);
   if (p->down)
@@ -111,12 +111,12 @@ int reserve(HcContextImpl *c, Slot &slot, size_t bytes) {
     return 0;
   if (slot.data) {
     // Nothing may still use the old buffer.
-    if (olSyncQueue(c->queue))
+    if (olSyncQueue(c->queue()))
       return 1;
-    olDeallocDevice(c->queue, slot.data);
+    olDeallocDevice(c->queue(), slot.data);
     slot = Slot{};
   }
-  slot.data = olAllocDevice(c->queue, bytes, 256);
+  slot.data = olAllocDevice(c->queue(), bytes, 256);
   if (!slot.data)
     return c->fail("host pipeline: device allocation of %zu bytes failed: %s", bytes,
                    c->lastError.c_str());
@@ -158,6 +158,7 @@ int streamRows(HcContextImpl *c, long long rows, long long chunkRows, const Stre
   HostPipeline *p = pipelineOf(c);
   if (!p)
     return 1;
+  const HcQueueScope one(c, c->queue()); // the whole call, whatever is chosen meanwhile
   chunkRows = std::max<long long>(1, std::min(chunkRows, rows));
   // Equal chunks rather than full ones and a short tail.
   const long long chunks = (rows + chunkRows - 1) / chunkRows;
@@ -171,7 +172,7 @@ int streamRows(HcContextImpl *c, long long rows, long long chunkRows, const Stre
         return 1;
   }
   // Whatever is already queued on the context's queue comes first.
-  int rc = olxRecordEvent(c->queue, p->start) || olxQueueWaitEvent(p->up, p->start) ||
+  int rc = olxRecordEvent(c->queue(), p->start) || olxQueueWaitEvent(p->up, p->start) ||
            olxQueueWaitEvent(p->down, p->start);
   bool used[2] = {false, false};
   long long index = 0;
@@ -184,15 +185,15 @@ int streamRows(HcContextImpl *c, long long rows, long long chunkRows, const Stre
       rc = copyRows(c, p->up, true, p->in[s][k].data, ins[k].host, r0, n, ins[k].rowBytes,
                     ins[k].pitchBytes);
     rc = rc || olxRecordEvent(p->up, p->uploaded[s]) ||
-         olxQueueWaitEvent(c->queue, p->uploaded[s]);
+         olxQueueWaitEvent(c->queue(), p->uploaded[s]);
     if (used[s]) // the download that read this slot's outputs two chunks ago
-      rc = rc || olxQueueWaitEvent(c->queue, p->downloaded[s]);
+      rc = rc || olxQueueWaitEvent(c->queue(), p->downloaded[s]);
     if (!rc) {
       void *inPtr[2] = {p->in[s][0].data, p->in[s][1].data};
       void *outPtr[2] = {p->out[s][0].data, p->out[s][1].data};
       rc = launch(inPtr, outPtr, r0, n);
     }
-    rc = rc || olxRecordEvent(c->queue, p->kernelDone[s]) ||
+    rc = rc || olxRecordEvent(c->queue(), p->kernelDone[s]) ||
          olxQueueWaitEvent(p->down, p->kernelDone[s]);
     for (int k = 0; k < nOut && !rc; ++k)
       rc = copyRows(c, p->down, false, p->out[s][k].data, outs[k].host, r0, n,
@@ -202,7 +203,7 @@ int streamRows(HcContextImpl *c, long long rows, long long chunkRows, const Stre
   }
   // The result is in host memory when the call returns - also after an error,
   // so that nothing is in flight on buffers the caller may free.
-  const int s1 = olSyncQueue(p->up), s2 = olSyncQueue(c->queue), s3 = olSyncQueue(p->down);
+  const int s1 = olSyncQueue(p->up), s2 = olSyncQueue(c->queue()), s3 = olSyncQueue(p->down);
   if (rc || s1 || s2 || s3)
     return c->fail("host pipeline failed: %s", c->lastError.c_str());
   return 0;
@@ -300,13 +301,14 @@ int hcGemmBf16Host(HcContext c, const void *aHost, const void *bHost, void *cHos
   HostPipeline *p = pipelineOf(c);
   if (!p)
     return 1;
+  const HcQueueScope one(c, c->queue());
   // B goes up whole, on the upload queue, ahead of the row blocks of A: every
   // product waits for its block of A, which follows B on that queue.  Device
   // rows are padded to 8 elements so that TMA can describe them.
   const long long kPad = (K + 7) / 8 * 8, nPad = (N + 7) / 8 * 8;
   if (reserve(c, p->resident, size_t(std::max<long long>(1, K)) * size_t(nPad) * 2))
     return 1;
-  if (olxRecordEvent(c->queue, p->start) || olxQueueWaitEvent(p->up, p->start))
+  if (olxRecordEvent(c->queue(), p->start) || olxQueueWaitEvent(p->up, p->start))
     return c->fail("hcGemmBf16Host: %s", c->lastError.c_str());
   if (K > 0 && copyRows(c, p->up, true, p->resident.data, const_cast<void *>(bHost), 0, K,
                         ldb == N && nPad == N ? N * 2 : N * 2, ldb * 2))

@@ -26,9 +26,11 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <iterator>
 #include <map>
 #include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
 // Loader-only export (gpu-runtime/loader/src/Loader.cpp:20-39 in the
@@ -196,7 +198,47 @@ constexpr int kRowHeldFillPercent = 90;
 
 } // namespace
 
+namespace {
+
+// What the calling thread has pushed, newest last.
+thread_local std::vector<std::pair<const HcContextImpl *, OlQueue>> pushed;
+
+bool popQueue(const HcContextImpl *c) {
+  for (auto it = pushed.rbegin(); it != pushed.rend(); ++it)
+    if (it->first == c) {
+      pushed.erase(std::next(it).base());
+      return true;
+    }
+  return false;
+}
+
+} // namespace
+
+OlQueue HcContextImpl::queue() const {
+  for (auto it = pushed.rbegin(); it != pushed.rend(); ++it)
+    if (it->first == this)
+      return it->second;
+  return chosenQueue;
+}
+
+OlQueue HcContextImpl::borrowed(void *stream) {
+  std::lock_guard<std::mutex> hold(tables);
+  auto it = borrowedQueues.find(stream);
+  if (it != borrowedQueues.end())
+    return it->second;
+  OlQueue q = olxCreateQueueOnStream(device, stream);
+  if (!q)
+    fail("no queue on the caller's stream: %s", lastError.c_str());
+  else
+    borrowedQueues[stream] = q;
+  return q;
+}
+
+HcQueueScope::HcQueueScope(HcContextImpl *c, OlQueue q) : context(c) { pushed.emplace_back(c, q); }
+HcQueueScope::~HcQueueScope() { popQueue(context); }
+
 OlKernel HcContextImpl::kernel(const char *name) {
+  std::lock_guard<std::mutex> hold(tables);
   auto it = kernels.find(name);
   if (it != kernels.end())
     return it->second;
@@ -231,7 +273,7 @@ int HcContextImpl::launch(const char *name, size_t gx, size_t gy, size_t gz, siz
     return 1;
   const size_t grid[3] = {gx, gy, gz};
   const size_t block[3] = {threads, 1, 1};
-  if (olLaunchKernel(queue, k, grid, block, 3, args, nArgs, smem))
+  if (olLaunchKernel(queue(), k, grid, block, 3, args, nArgs, smem))
     return fail("olLaunchKernel failed for %s: %s", name, lastError.c_str());
   ++launches;
   return 0;
@@ -244,7 +286,7 @@ int HcContextImpl::launchCluster(const char *name, size_t gx, size_t gy, size_t 
     return 1;
   const size_t grid[3] = {gx, gy, 1};
   const size_t clusters[3] = {1, cluster, 1};
-  if (olxLaunchCluster(queue, k, grid, threads, clusters, args, smem))
+  if (olxLaunchCluster(queue(), k, grid, threads, clusters, args, smem))
     return fail("olxLaunchCluster failed for %s: %s", name, lastError.c_str());
   ++launches;
   return 0;
@@ -304,8 +346,8 @@ HcContext hcCreateContext(const char *deviceDesc, OlErrorCallback errCallback,
   c->device = olCreateDevice(deviceDesc, &HcContextImpl::onBackendMessage, c.get());
   if (!c->device)
     return nullptr;
-  c->queue = c->ownQueue = olCreateQueue(c->device);
-  if (!c->queue) {
+  c->chosenQueue = c->ownQueue = olCreateQueue(c->device);
+  if (!c->ownQueue) {
     olReleaseDevice(c->device);
     return nullptr;
   }
@@ -314,9 +356,9 @@ HcContext hcCreateContext(const char *deviceDesc, OlErrorCallback errCallback,
   olxDeviceAttribute(c->device, OLX_DEVICE_CC_MINOR, &c->ccMinor);
   if (c->smCount <= 0)
     c->smCount = 1;
-  c->statusWord = static_cast<int *>(olAllocDevice(c->queue, 256, 256));
-  if (!c->statusWord || olxMemsetD8(c->queue, c->statusWord, 0, 256) ||
-      olSyncQueue(c->queue)) {
+  c->statusWord = static_cast<int *>(olAllocDevice(c->queue(), 256, 256));
+  if (!c->statusWord || olxMemsetD8(c->queue(), c->statusWord, 0, 256) ||
+      olSyncQueue(c->queue())) {
     hcReleaseContext(c.release());
     return nullptr;
   }
@@ -326,9 +368,9 @@ HcContext hcCreateContext(const char *deviceDesc, OlErrorCallback errCallback,
 void hcReleaseContext(HcContext c) {
   if (!c)
     return;
-  c->queue = c->ownQueue;
-  if (c->queue)
-    olSyncQueue(c->queue);
+  c->chosenQueue = c->ownQueue;
+  if (c->ownQueue)
+    olSyncQueue(c->ownQueue);
   for (auto &kv : c->borrowedQueues)
     olReleaseQueue(kv.second);
   for (auto &kv : c->kernels)
@@ -339,9 +381,9 @@ void hcReleaseContext(HcContext c) {
   hcReleaseHostPipeline(c);
   hcReleaseSpecialiser(c);
   if (c->statusWord)
-    olDeallocDevice(c->queue, c->statusWord);
-  if (c->queue)
-    olReleaseQueue(c->queue);
+    olDeallocDevice(c->ownQueue, c->statusWord);
+  if (c->ownQueue)
+    olReleaseQueue(c->ownQueue);
   if (c->device)
     olReleaseDevice(c->device);
   delete c;
@@ -356,27 +398,39 @@ void *hcContextStream(HcContext c) {
 int hcUseStream(HcContext c, void *stream) {
   if (!c)
     return 1;
-  OlQueue &q = c->borrowedQueues[stream];
+  OlQueue q = c->borrowed(stream);
   if (!q)
-    q = olxCreateQueueOnStream(c->device, stream);
-  if (!q) {
-    c->borrowedQueues.erase(stream);
-    return c->fail("hcUseStream: no queue on that stream: %s", c->lastError.c_str());
-  }
-  c->queue = q;
+    return 1;
+  c->chosenQueue = q;
   return 0;
 }
 
 int hcUseOwnStream(HcContext c) {
   if (!c)
     return 1;
-  c->queue = c->ownQueue;
+  c->chosenQueue = c->ownQueue;
   return 0;
 }
 
-int hcSynchronize(HcContext c) { return c ? olSyncQueue(c->queue) : 1; }
+int hcPushStream(HcContext c, void *stream) {
+  if (!c)
+    return 1;
+  OlQueue q = c->borrowed(stream);
+  if (!q)
+    return 1;
+  pushed.emplace_back(c, q);
+  return 0;
+}
+
+int hcPopStream(HcContext c) {
+  if (!c)
+    return 1;
+  return popQueue(c) ? 0 : c->fail("hcPopStream: this thread has pushed none");
+}
+
+int hcSynchronize(HcContext c) { return c ? olSyncQueue(c->queue()) : 1; }
 const char *hcLastError(HcContext c) { return c ? c->lastError.c_str() : ""; }
-long long hcLaunchCount(HcContext c) { return c ? c->launches : 0; }
+long long hcLaunchCount(HcContext c) { return c ? c->launches.load() : 0; }
 
 long long hcSpecialisedPrograms(HcContext c, int fromDisk) {
   return c ? hcSpecialiserCount(c, fromDisk ? 1 : 0) : 0;
@@ -388,12 +442,12 @@ int hcKernelStatus(HcContext c, int *statusRet) {
   if (!c || !statusRet)
     return 1;
   int value = 0;
-  if (olxMemcpyDtoH(c->queue, &value, c->statusWord, sizeof(int)) ||
-      olSyncQueue(c->queue))
+  if (olxMemcpyDtoH(c->queue(), &value, c->statusWord, sizeof(int)) ||
+      olSyncQueue(c->queue()))
     return c->fail("reading the kernel status word failed: %s",
                    c->lastError.c_str());
-  if (value != 0 && (olxMemsetD8(c->queue, c->statusWord, 0, sizeof(int)) ||
-                     olSyncQueue(c->queue)))
+  if (value != 0 && (olxMemsetD8(c->queue(), c->statusWord, 0, sizeof(int)) ||
+                     olSyncQueue(c->queue())))
     return 1;
   *statusRet = value;
   return 0;
@@ -406,17 +460,17 @@ int hcSelfTestWaitTimeout(HcContext c, unsigned long long limitNs, int *statusRe
   if (limitNs == 0 || limitNs > 1000000000ull)
     return c->fail("hcSelfTestWaitTimeout: limit must be between 1 ns and 1 s");
   // Scratch: [0] elapsed ns (8 bytes), [8..16) the two observed flags.
-  auto *scratch = static_cast<unsigned char *>(olAllocDevice(c->queue, 256, 256));
+  auto *scratch = static_cast<unsigned char *>(olAllocDevice(c->queue(), 256, 256));
   if (!scratch)
     return c->fail("hcSelfTestWaitTimeout: allocation failed: %s", c->lastError.c_str());
-  int rc = olxMemsetD8(c->queue, scratch, 0xff, 256);
+  int rc = olxMemsetD8(c->queue(), scratch, 0xff, 256);
   auto *elapsed = reinterpret_cast<unsigned long long *>(scratch);
   auto *observed = reinterpret_cast<int *>(scratch + 8);
   void *args[] = {&limitNs, &c->statusWord, &elapsed, &observed};
   rc = rc || c->launch("hc_selftest_wait_timeout", 1, 1, 1, 64, args, 4, 0);
   unsigned char host[16] = {0};
-  rc = rc || olxMemcpyDtoH(c->queue, host, scratch, sizeof(host)) || olSyncQueue(c->queue);
-  olDeallocDevice(c->queue, scratch);
+  rc = rc || olxMemcpyDtoH(c->queue(), host, scratch, sizeof(host)) || olSyncQueue(c->queue());
+  olDeallocDevice(c->queue(), scratch);
   if (rc)
     return c->fail("hcSelfTestWaitTimeout failed: %s", c->lastError.c_str());
   std::memcpy(elapsedNsRet, host, 8);
@@ -1394,7 +1448,7 @@ static int launchUmma(HcContext c, const void *a, const void *b,
     if (c->pairSlots == 0) {
       OlKernel k = c->kernel(name);
       int slots = 0;
-      if (!k || olxMaxActiveClusters(c->queue, k, kUmmaThreads, kUmmaSmemBytes, 2,
+      if (!k || olxMaxActiveClusters(c->queue(), k, kUmmaThreads, kUmmaSmemBytes, 2,
                                      &slots) || slots <= 0)
         return c->fail("cluster occupancy query failed: %s", c->lastError.c_str());
       c->pairSlots = slots;
@@ -1502,7 +1556,7 @@ int hcGemmF32Tensor(HcContext c, const void *a, const void *b, void *out, void *
     if (c->pairSlotsF32 == 0) {
       OlKernel k = c->kernel(name);
       int slots = 0;
-      if (!k || olxMaxActiveClusters(c->queue, k, 192, smem, 2, &slots) || slots <= 0)
+      if (!k || olxMaxActiveClusters(c->queue(), k, 192, smem, 2, &slots) || slots <= 0)
         return c->fail("cluster occupancy query failed: %s", c->lastError.c_str());
       c->pairSlotsF32 = slots;
     }
@@ -1876,7 +1930,7 @@ int hcGemmW8A16(HcContext c, const void *a, const void *w, const float *scale,
     if (c->pairSlotsW8 == 0) {
       OlKernel k = c->kernel(name);
       int slots = 0;
-      if (!k || olxMaxActiveClusters(c->queue, k, 480, smem, 2, &slots) || slots <= 0)
+      if (!k || olxMaxActiveClusters(c->queue(), k, 480, smem, 2, &slots) || slots <= 0)
         return c->fail("cluster occupancy query failed: %s", c->lastError.c_str());
       c->pairSlotsW8 = slots;
     }
@@ -1908,7 +1962,7 @@ int hcGemmW8A16(HcContext c, const void *a, const void *w, const float *scale,
     const size_t ringBytes = size_t(kBandSlots) * size_t(K) * kBandCols * 2;
     plan.converted = reinterpret_cast<unsigned *>(static_cast<char *>(workspace) + ringBytes);
     plan.consumed = plan.converted + plan.numBands;
-    if (olxMemsetD8(c->queue, plan.converted, 0, size_t(plan.numBands) * 2 * sizeof(unsigned)))
+    if (olxMemsetD8(c->queue(), plan.converted, 0, size_t(plan.numBands) * 2 * sizeof(unsigned)))
       return c->fail("hcGemmW8A16: clearing the band counters failed: %s", c->lastError.c_str());
     alignas(64) CUtensorMap mapA, mapB;
     if (olxEncodeTensorMap2D(c->device, &mapA, /*bf16*/ 0, a, size_t(M), size_t(K),
@@ -1922,7 +1976,7 @@ int hcGemmW8A16(HcContext c, const void *a, const void *w, const float *scale,
     if (c->pairSlotsBanded == 0) {
       OlKernel k = c->kernel(name);
       int slots = 0;
-      if (!k || olxMaxActiveClusters(c->queue, k, kUmmaThreads + 128, kUmmaSmemBytes, 2, &slots) ||
+      if (!k || olxMaxActiveClusters(c->queue(), k, kUmmaThreads + 128, kUmmaSmemBytes, 2, &slots) ||
           slots <= 0)
         return c->fail("cluster occupancy query failed: %s", c->lastError.c_str());
       c->pairSlotsBanded = slots;

@@ -364,7 +364,8 @@ const char *hcSpecialise(HcContextImpl *c, bool row, int dtype, const HcMapProgr
     return nullptr;
   OlModule module = olCreateModule(c->device, image.data(), image.size());
   if (!module) {
-    s.note = "olCreateModule failed for a specialised image: " + c->lastError;
+    s.note = "olCreateModule failed for a specialised image: ";
+    s.note += c->lastError.c_str();
     return nullptr;
   }
   // Every kernel of the image, under its name, beside those of the embedded images.
@@ -383,9 +384,10 @@ const char *hcSpecialise(HcContextImpl *c, bool row, int dtype, const HcMapProgr
     OlKernel k = olGetKernel(module, name);
     if (!k) {
       olReleaseModule(module);
-      s.note = std::string("a specialised image lacks ") + name + ": " + c->lastError;
+      s.note = std::string("a specialised image lacks ") + name + ": " + c->lastError.c_str();
       return nullptr;
     }
+    std::lock_guard<std::mutex> hold(c->tables);
     c->kernels[name] = k;
   }
   entry.tag = tag;
@@ -415,7 +417,8 @@ const char *hcSpecialiseItems(HcContextImpl *c, int dtype, const uint32_t *code,
     return nullptr;
   OlModule module = olCreateModule(c->device, image.data(), image.size());
   if (!module) {
-    s.note = "olCreateModule failed for a specialised image: " + c->lastError;
+    s.note = "olCreateModule failed for a specialised image: ";
+    s.note += c->lastError.c_str();
     return nullptr;
   }
   char name[96];
@@ -424,10 +427,13 @@ const char *hcSpecialiseItems(HcContextImpl *c, int dtype, const uint32_t *code,
   OlKernel k = olGetKernel(module, name);
   if (!k) {
     olReleaseModule(module);
-    s.note = std::string("a specialised image lacks ") + name + ": " + c->lastError;
+    s.note = std::string("a specialised image lacks ") + name + ": " + c->lastError.c_str();
     return nullptr;
   }
-  c->kernels[name] = k;
+  {
+    std::lock_guard<std::mutex> hold(c->tables);
+    c->kernels[name] = k;
+  }
   entry.tag = tag;
   entry.module = module;
   entry.failed = false;

@@ -95,8 +95,23 @@ struct ModuleState {
 struct KernelState {
   DeviceState *device = nullptr;
   CUfunction function = nullptr;
+  std::mutex smemLock; // two threads may launch a kernel
   int dynSmemLimit = 48 * 1024; // what the driver allows without opt-in
 };
+
+// Lets `k` use `bytes` of dynamic shared memory (the limit only grows).
+int allowSmem(KernelState *k, size_t bytes) {
+  std::lock_guard<std::mutex> hold(k->smemLock);
+  if (bytes <= size_t(k->dynSmemLimit))
+    return 0;
+  if (k->device->check("cuFuncSetAttribute",
+                       DriverApi::get().FuncSetAttribute(
+                           k->function, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                           static_cast<int>(bytes))))
+    return 1;
+  k->dynSmemLimit = static_cast<int>(bytes);
+  return 0;
+}
 
 struct QueueState {
   DeviceState *device = nullptr;
@@ -362,15 +377,8 @@ int olLaunchKernel(OlQueue queue, OlKernel kernel, const size_t *gridSizes,
   ContextScope scope(dev);
   if (!scope)
     return 1;
-  if (sharedMemSize > size_t(k->dynSmemLimit)) {
-    if (dev->check("cuFuncSetAttribute",
-                   cu.FuncSetAttribute(
-                       k->function,
-                       CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
-                       static_cast<int>(sharedMemSize))))
-      return 1;
-    k->dynSmemLimit = static_cast<int>(sharedMemSize);
-  }
+  if (allowSmem(k, sharedMemSize))
+    return 1;
   return dev->check(
       "cuLaunchKernel",
       cu.LaunchKernel(k->function, unsigned(gridSizes[0]),
@@ -397,14 +405,8 @@ int olxLaunchCluster(OlQueue queue, OlKernel kernel, const size_t *gridSizes, si
   ContextScope scope(dev);
   if (!scope)
     return 1;
-  if (sharedMemSize > size_t(k->dynSmemLimit)) {
-    if (dev->check("cuFuncSetAttribute",
-                   cu.FuncSetAttribute(k->function,
-                                       CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
-                                       static_cast<int>(sharedMemSize))))
-      return 1;
-    k->dynSmemLimit = static_cast<int>(sharedMemSize);
-  }
+  if (allowSmem(k, sharedMemSize))
+    return 1;
   CUlaunchAttribute attr{};
   attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
   attr.value.clusterDim.x = static_cast<unsigned>(clusterSizes[0]);
@@ -529,15 +531,8 @@ int olxMaxActiveClusters(OlQueue queue, OlKernel kernel, unsigned blockThreads,
   ContextScope scope(dev);
   if (!scope)
     return 1;
-  if (sharedMemSize > size_t(k->dynSmemLimit)) {
-    if (dev->check("cuFuncSetAttribute",
-                   cu.FuncSetAttribute(
-                       k->function,
-                       CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
-                       static_cast<int>(sharedMemSize))))
-      return 1;
-    k->dynSmemLimit = static_cast<int>(sharedMemSize);
-  }
+  if (allowSmem(k, sharedMemSize))
+    return 1;
   CUlaunchAttribute attr{};
   attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
   attr.value.clusterDim.x = clusterSize;

@@ -54,8 +54,10 @@ HC_B200_API int hcImageOfKernel(const char *kernelName);
  * py-runtime (GpuRuntime.cpp:23-39), but one per device description so that
  * several GPUs can be driven from one process.  Like the reference's runtime
  * (no locks anywhere, gpu-runtime/cuda-runtime/src/Runtime.cpp), a context is
- * not thread-safe: use it from one thread at a time.  Different contexts may
- * be used from different threads. */
+ * not thread-safe: use it from one thread at a time - but for the host-buffer
+ * entry points (below): while one thread waits in one of them, another may
+ * launch through the same context.  Different contexts may be used from
+ * different threads. */
 HC_B200_API HcContext hcCreateContext(const char *deviceDesc,
                                       OlErrorCallback errCallback, void *ctx);
 HC_B200_API void hcReleaseContext(HcContext c);
@@ -73,6 +75,10 @@ HC_B200_API int hcSynchronize(HcContext c);
  * own; hcSynchronize and hcKernelStatus wait for the stream in use. */
 HC_B200_API int hcUseStream(HcContext c, void *stream);
 HC_B200_API int hcUseOwnStream(HcContext c);
+/* The same for what the calling thread launches alone, until it pops it (pushes nest):
+ * other threads' work through the context stays where it was. */
+HC_B200_API int hcPushStream(HcContext c, void *stream);
+HC_B200_API int hcPopStream(HcContext c);
 HC_B200_API const char *hcLastError(HcContext c);
 /* Kernel launches issued through this context so far. */
 HC_B200_API long long hcLaunchCount(HcContext c);

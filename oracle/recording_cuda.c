@@ -18,10 +18,11 @@ struct launch {
   unsigned grid[3], block, smem;
   unsigned long long stream;
 };
-static struct launch launches[256];
-static int count;
+#define ROOM 65536 /* further launches overwrite the last one */
+static struct launch launches[ROOM];
+static int count; /* threads may launch at the same time */
 
-int recorded_launches(void) { return count; }
+int recorded_launches(void) { return count < ROOM ? count : ROOM; }
 void recorded_clear(void) { count = 0; }
 const struct launch *recorded_launch(int i) { return &launches[i]; }
 
@@ -85,7 +86,8 @@ int cuPointerGetAttribute(void *v, int what, unsigned long long p) { *(int *)v =
 int cuEventCreate(void **e, unsigned flags) { *e = (void *)0x20; return 0; }
 int cuLaunchKernel(void *f, unsigned gx, unsigned gy, unsigned gz, unsigned bx, unsigned by,
                    unsigned bz, unsigned smem, void *stream, void **params, void **extra) {
-  struct launch *l = &launches[count < 256 ? count++ : 255];
+  int at = __atomic_fetch_add(&count, 1, __ATOMIC_RELAXED);
+  struct launch *l = &launches[at < ROOM ? at : ROOM - 1];
   snprintf(l->name, sizeof l->name, "%s", (const char *)f);
   l->grid[0] = gx, l->grid[1] = gy, l->grid[2] = gz;
   l->block = bx * by * bz, l->smem = smem, l->stream = (unsigned long long)(uintptr_t)stream;

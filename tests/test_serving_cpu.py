@@ -420,6 +420,78 @@ def test_launches_go_to_the_stream_in_use(recording):
     """)
 
 
+def test_pushed_streams_nest_and_are_the_threads_own(recording):
+    recording("""
+    import threading
+    def go():
+        hc.softmax_rows(P, P + (1 << 20), 4, 64, 64, 64)
+        return launches()[0][4]
+    own = hc.stream
+    hc.push_stream(0x1000)
+    hc.push_stream(0x2000)
+    assert go() == 0x2000
+    seen = []
+    t = threading.Thread(target=lambda: seen.append(go()))
+    t.start(); t.join()
+    assert seen == [own]
+    hc.pop_stream()
+    assert go() == 0x1000
+    hc.use_stream(0x3000)  # the context's choice waits behind the thread's
+    assert go() == 0x1000
+    hc.pop_stream()
+    assert go() == 0x3000
+    hc.use_own_stream()
+    refused("pushed none", hc.pop_stream)
+    assert go() == own
+    hc.close()
+    """)
+
+
+def test_serving_calls_beside_a_host_buffer_call(recording):
+    """Two threads of one process, one context: the host-buffer call, which runs without
+    the interpreter lock, keeps its kernels on the context's stream, and the serving
+    calls go to theirs."""
+    recording("""
+    import threading
+    import numpy as np
+    from hc_b200._native import _dispatcher as d
+
+    class Dev:  # what the dispatcher reads of a device array
+        is_cuda = True
+        device = type("D", (), dict(index=0))
+        def __init__(self, *shape, dtype="torch.bfloat16"):
+            self.shape, self.dtype = shape, dtype
+        def data_ptr(self): return P
+        def element_size(self): return 2
+        def stride(self): return (64, 1)[-len(self.shape):]
+
+    ctx = d.Context("cuda:0")
+    x, gain, out = Dev(4, 64), Dev(64), Dev(4, 64)
+    big = np.empty((1 << 18, 1024), np.float32)  # 64 chunks
+    res = np.empty_like(big)
+    launches()
+    start = threading.Barrier(2)
+    done = []
+    def host():
+        start.wait()
+        for _ in range(50):
+            d.softmax_rows_host(ctx, big, res)
+        done.append(True)
+    t = threading.Thread(target=host)
+    t.start()
+    start.wait()
+    while not done:
+        d.add_rms_norm(ctx, x, gain, None, None, out, None, stream=0x1234000)
+    t.join()
+    got = launches()
+    names = ["softmax" in l[0] for l in got]
+    assert names.count(True) == 50 * 64 and names.count(False) > 100
+    assert sum(a != b for a, b in zip(names, names[1:])) > 100  # beside each other
+    for soft, l in zip(names, got):
+        assert l[4] == (ctx.stream if soft else 0x1234000), l
+    """)
+
+
 def test_every_serving_kernel_is_found_by_its_name():
     """The families that the launch code names lie in the images it says."""
     from hc_b200 import capi
