@@ -106,9 +106,9 @@ constexpr int kSlotBytes = 16 * 64;
 // activations in the order the lanes read them (piece (lane t, word j) at (4 j + t)
 // pieces), as f16 pairs (0,4) (1,5)/16 (2,6) (3,7)/16 or as bytes (0,2,4,6) (1,3,5,7);
 // then per segment of K (a span; Fine: 32) and column {sum of its activations in the
-// accumulator's unit, that unit times the activations' scale}; then per warp {scale,
-// zero} of its 16 weight rows and its groups; then the partial sums of two tiles per
-// warp; then 256 bytes of zeros that lanes without an activation row read.
+// accumulator's unit, that unit in the total's, times the activations' scale}; then per
+// warp {scale, zero} of its 16 weight rows and its groups; then the partial sums of two
+// tiles per warp; then 256 bytes of zeros that lanes without an activation row read.
 template <bool A8, bool Fine> struct Layout {
   static constexpr int pieceBytes = A8 ? 8 : 16;
   static constexpr int spanBytes = 16 * pieceBytes;
@@ -311,7 +311,7 @@ __device__ __forceinline__ void w4Body(const W4Params &p) {
         }
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
-          sum += e[b];
+          sum = fmaf(e[b], 0.001953125f, sum); // (2^-9: the sum of the largest overflows)
           top = fmaxf(top, fabsf(e[b]));
         }
 #pragma unroll
@@ -333,9 +333,10 @@ __device__ __forceinline__ void w4Body(const W4Params &p) {
         };
         *reinterpret_cast<uint4 *>(dst) =
             make_uint4(pair(e[0], e[4]), pair(e[1], e[5]), pair(e[2], e[6]), pair(e[3], e[7]));
-        // The accumulator counts in units of 2^-24 / up.
-        note.x = sum * up * 5.9604644775390625e-08f;
-        note.y = down * 16777216.0f;
+        // The accumulator counts in units of 2^-24 / up, the total in units of 2^-10: 2^14
+        // down is at most the segment's largest activation, so that no factor overflows.
+        note.x = sum * up * 3.0517578125e-05f; // 2^9 * 2^-24
+        note.y = down * 16384.0f;
       }
       if ((q & (kLanes - 1)) == 0)
         sAct[(span * L::segments + (Fine ? hi : 0)) * 8 + m] = note;
@@ -453,7 +454,9 @@ __device__ __forceinline__ void w4Body(const W4Params &p) {
         for (int w = 0; w < p.warpsK; ++w)
           sum += from[w * 128 + i];
         const int m = i >> 4, n = tile * 16 + (i & 15);
-        if (A8 && p.aGroup >= p.K && p.K > 0) // one scale per activation row
+        if constexpr (!A8)
+          sum *= 1024.0f;
+        else if (p.aGroup >= p.K && p.K > 0) // one scale per activation row
           sum *= p.aScale[(long long)m * p.ldas];
         if (n < p.N)
           p.out[(long long)m * p.ldc + n] = __float2bfloat16_rn(sum);

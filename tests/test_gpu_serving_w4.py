@@ -225,3 +225,31 @@ def test_single_rows_of_any_stride():
         w = c["w"][:1].clone().as_strided((1, (k + 1) // 2), (16, 1))
         one = {**c, "w": w, "scale": c["scale"][:1], "zero": c["zero"][:1]}
         assert torch.equal(serving.gemm_w4(**one), want[:, :1])
+
+
+@pytest.mark.parametrize("m", [1, 8, 40])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("power", [-100, -60, 100, 112, 118, 120])
+def test_activations_of_any_size(power, zeros, group, m):
+    """Far from 1 in either direction: the bounds are relative, nothing overflows or
+    vanishes on the way to a result that bfloat16 holds."""
+    c = _case(m, 130, 640, group, zeros)
+    c["a"] = (c["a"].float() * 2.0 ** power).bfloat16()
+    _check(c, serving.gemm_w4(**c))
+
+
+@pytest.mark.parametrize("m", [1, 8])
+@pytest.mark.parametrize("group", [32, 128])
+def test_the_largest_activations(group, m):
+    """Every activation of a segment at bfloat16's end: their sum is beyond float32, the
+    product with small weights is not."""
+    c = _case(m, 64, 256, group, True)
+    most = torch.finfo(torch.bfloat16).max
+    c["a"] = torch.full_like(c["a"], most)
+    c["a"][:, 1::2] = -most
+    c["scale"] = (c["scale"].float() * 2.0 ** -8).bfloat16()
+    _check(c, serving.gemm_w4(**c))
+    c["a"] = torch.full_like(c["a"], most)
+    c["scale"] = (c["scale"].float() * 2.0 ** -8).bfloat16()
+    _check(c, serving.gemm_w4(**c))
