@@ -313,7 +313,7 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
           packed;
     if (d == 0 && p.lse)
       p.lse[token * p.lseStride + qHead] =
-          sum == 0.0f ? kNegInf : (top + __log2f(sum)) * 0.693147180559945309f;
+          sum == 0.0f ? kNegInf : log2Of(top, sum) * 0.693147180559945309f;
   };
 
   int slot = 0; // of the warp's next piece
@@ -555,9 +555,7 @@ __device__ __forceinline__ void attend(const AttentionParams &p) {
       loadKeys(now);
       if (there) {
         // Scores in units of log2, masked; the largest one with its value scale.
-        float lsv = 0.0f;
-        if (sv > 0.0f && sv < INFINITY)
-          lsv = fmaxf(__log2f(sv), -96.0f);
+        const float lsv = logOfScale(sv);
         const bool whole = pos >= allLo && pos + 15 <= firstPos;
         float top[NT][2];
         bool grows = false;

@@ -537,7 +537,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
         Group g;
         g.key = kScale;
         g.value = vScale * kWeight;
-        g.logValue = vScale > 0.0f && vScale < INFINITY ? fmaxf(__log2f(vScale), -96.0f) : 0.0f;
+        g.logValue = logOfScale(vScale);
         g.there = page >= 0 ? 1.0f : 0.0f;
         const bool plain = __all_sync(
             0xffffffffu, lane >= S::groups || (page >= 0 && kScale >= 0.0f && p.scaleLog2 >= 0.0f));
@@ -858,7 +858,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     const int qi = queryOf(row0 + r), gh = row0 + r - qi * p.share;
     if (p.lse)
       p.lse[(long long)(span.row + qi) * p.lseStride + head * p.share + gh] =
-          sum == 0.0f ? kNegInf : (top + __log2f(sum)) * 0.693147180559945309f;
+          sum == 0.0f ? kNegInf : log2Of(top, sum) * 0.693147180559945309f;
   };
   const bool aborted = *abortFlag != 0;
   if (warp < 8 && !aborted) {

@@ -74,6 +74,25 @@ __device__ __forceinline__ float warpSum(float v) {
   return v;
 }
 
+// log2(2^top * sum) with the error of a logarithm of 1..2, however far top and the sum's
+// exponent are from 0: they cancel exactly.
+__device__ __forceinline__ float log2Of(float top, float sum) {
+  const uint32_t bits = __float_as_uint(sum), e = bits >> 23;
+  if (e == 0 || e >= 255) // subnormal or not finite
+    return top + __log2f(sum);
+  return (top + float(int(e) - 127)) +
+         __log2f(__uint_as_float((bits & 0x007fffffu) | 0x3f800000u));
+}
+
+// What a block's value scale adds to its scores where the reference of the exponentials
+// is chosen: exponential times scale then fits f16 whatever the scales are.  Scales below
+// 2^-96, and 0, count as that: their sums of exponentials stay below float32's end, and
+// blocks of zeros do not push the others' weights among f16's subnormals.
+__device__ __forceinline__ float logOfScale(float scale) {
+  const float s = fabsf(scale);
+  return s < INFINITY ? fmaxf(__log2f(s), -96.0f) : 0.0f;
+}
+
 // Maximum over aligned segments of `width` lanes (a power of two); NaN if any is.
 __device__ __forceinline__ float segmentMax(float v, int width) {
   for (int d = width >> 1; d > 0; d >>= 1)

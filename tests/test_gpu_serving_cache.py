@@ -465,3 +465,38 @@ def test_refusals():
     bad = serving.KvCache(odd, odd, ks[:4].contiguous(), ks[:4].contiguous())
     with pytest.raises(RuntimeError, match="multiple of 16"):
         call(cache=bad)
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("tiny", [-16, -30, -60])
+def test_attention_zeros_outweigh_small_values(store, tiny):
+    """Blocks of zeros that hold nearly all of the probability beside blocks of small
+    values: what little the output is has its full precision.  (More tiles than warps.)"""
+    lengths = [12000, 11000, 12000, 10000, 9000, 12000]
+    s = Setup(store, lengths, [1] * 6, one_each=True, dim=64, heads=2, share=2)
+    s.append()
+    # Keys along the query in the blocks of zeros alone: a score of 8 more, e^8 of the weight.
+    s.q = torch.zeros(6, 4, 64, dtype=torch.bfloat16, device="cuda")
+    s.q[:, :, 0] = 8
+    raw = 64 if store == "int8" else int(oracle.to_e4m3(np.array([64.0]))[0])
+    zeros = torch.zeros(s.pages, dtype=torch.bool, device="cuda")
+    for row in s.d_table:
+        zeros[row[row >= 0][::2].long()] = True
+    k = s.cache.k.view(torch.uint8)
+    k.zero_()
+    k[zeros, :, :, 0] = raw
+    s.cache.k_scale.fill_(2.0 ** -3)
+    s.cache.v_scale.fill_(2.0 ** tiny)
+    s.cache.v_scale[zeros] = 0
+    out, lse = s.attend()
+    values = [oracle.stored_values(b, store) for b in s.bytes()]
+    scales = [t.double().cpu().numpy() for t in (s.cache.k_scale, s.cache.v_scale)]
+    args = (s.q.double().cpu().numpy(), s.table.tolist(), s.spans(), 2, 64 ** -0.5, 0)
+    want, want_lse = oracle.kv_attention(values, scales, *args)
+    most, _ = oracle.kv_attention((values[0], np.abs(values[1])), scales, *args)
+    assert (most > 0).all() and most.max() < 448 * 2.0 ** (tiny - 10)
+    # The scores, 0 and 8, are exact in f16 and float32; the sums have up to 2^7 rounded
+    # partial sums per lane, 2^-17; probabilities round to f16.
+    room = 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16) * most
+    assert np.all(np.abs(out.double().cpu().numpy() - want) <= room)
+    assert np.all(np.abs(lse.double().cpu().numpy() - want_lse) <= 2.0 ** -16)

@@ -199,3 +199,9 @@ def test_rows_nan_values_where_rows_end_inside_a_warp(dim, fresh, share):
         out, lse = s.attend(out=torch.full_like(clean, 3.0))
         assert torch.equal(torch.isnan(out).cpu(), want)
         assert torch.equal(out[~want.cuda()], clean[~want.cuda()]) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("tiny", [-16, -30, -60])
+def test_rows_zeros_outweigh_small_values(store, tiny):
+    few.test_attention_zeros_outweigh_small_values(store, tiny)
