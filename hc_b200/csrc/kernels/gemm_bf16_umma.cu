@@ -1,5 +1,5 @@
 // Dense bf16 GEMM on the 5th-generation tensor cores:
-//   C[M, N] = bf16( (A[M, K] @ B[K, N]) (* scale[N]) ),  fp32 accumulation,
+//   C[M, N] = bf16( (A[M, K] @ B[K, N]) (* scale[N], or scale[M]) ),  fp32 accumulation,
 // A, B, C row-major with explicit row pitches.
 //
 // It computes what the reference's dot kernels compute (python/hckernel/tests/
@@ -21,7 +21,8 @@
 //              and is double-buffered so the epilogue of tile i overlaps the
 //              main loop of tile i+1.
 //   warps 2-5  epilogue: tcgen05.ld the accumulator, optional per-column
-//              scale, round to bf16 (nearest even), store clipped to M x N.
+//              (or per-row) scale, round to bf16 (nearest even), store clipped to
+//              M x N.
 //
 // PAIR = true runs two CTAs (a cluster of 2 neighbouring SMs) on one 256 x 256
 // tile with tcgen05.mma.cta_group::2: each CTA stages its own 128 rows of A
@@ -212,7 +213,8 @@ __device__ __forceinline__ void
 gemmUmma(const CUtensorMap *mapA, const CUtensorMap *mapB,
          __nv_bfloat16 *__restrict__ c, const float *__restrict__ scale,
          const Params &p, int *status, unsigned char *smemRaw,
-         const HcPeerDsts *peers = nullptr, const BandPlan *bp = nullptr) {
+         const HcPeerDsts *peers = nullptr, const BandPlan *bp = nullptr,
+         long long rowScaleStride = 0) {
   using Cfg = Config<PAIR>;
   // The swizzled stages need 1024-byte alignment.
   const uint32_t smemBase = (smemAddr(smemRaw) + 1023u) & ~1023u;
@@ -462,6 +464,14 @@ gemmUmma(const CUtensorMap *mapA, const CUtensorMap *mapB,
                   f[j] *= __ldg(scale + col + j);
             }
           }
+          if constexpr (!SCALED && !PEERS && !BANDED) {
+            if (scale) { // of the row (int8 activations as integers: hcGemmW4)
+              const float s = __ldg(scale + row * rowScaleStride);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                f[j] *= s;
+            }
+          }
           uint32_t w[16]; // the 32 values rounded to bf16, two per word
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
@@ -543,30 +553,38 @@ gemmUmma(const CUtensorMap *mapA, const CUtensorMap *mapB,
       long long ldc, int tilesM, int tilesN, int bandM, int vecStore,          \
       int *status
 
-#define HC_GEMM_BODY(PAIR, SCALED)                                             \
+#define HC_GEMM_SCALED_BODY(PAIR)                                              \
   extern __shared__ __align__(1024) unsigned char smemRaw[];                   \
   Params p{M, N, K, ldc, tilesM, tilesN, bandM, vecStore};                     \
-  gemmUmma<PAIR, SCALED>(&mapA, &mapB, c, scale, p, status, smemRaw);
+  gemmUmma<PAIR, true>(&mapA, &mapB, c, scale, p, status, smemRaw);
+
+// Without column scales: `scale` is null, or a scale per row.
+#define HC_GEMM_ROWS_BODY(PAIR)                                                \
+  extern __shared__ __align__(1024) unsigned char smemRaw[];                   \
+  Params p{M, N, K, ldc, tilesM, tilesN, bandM, vecStore};                     \
+  gemmUmma<PAIR, false>(&mapA, &mapB, c, scale, p, status, smemRaw, nullptr,   \
+                        nullptr, rowScaleStride);
 
 extern "C" __global__ void __launch_bounds__(NUM_THREADS, 1)
-    hc_gemm_bf16_umma(HC_GEMM_ARGS) {
-  HC_GEMM_BODY(false, false)
+    hc_gemm_bf16_umma(HC_GEMM_ARGS, long long rowScaleStride) {
+  HC_GEMM_ROWS_BODY(false)
 }
 
 extern "C" __global__ void __launch_bounds__(NUM_THREADS, 1)
     hc_gemm_bf16_umma_scaled(HC_GEMM_ARGS) {
-  HC_GEMM_BODY(false, true)
+  HC_GEMM_SCALED_BODY(false)
 }
 
 extern "C" __global__ void __cluster_dims__(2, 1, 1)
-    __launch_bounds__(NUM_THREADS, 1) hc_gemm_bf16_umma_pair(HC_GEMM_ARGS) {
-  HC_GEMM_BODY(true, false)
+    __launch_bounds__(NUM_THREADS, 1)
+        hc_gemm_bf16_umma_pair(HC_GEMM_ARGS, long long rowScaleStride) {
+  HC_GEMM_ROWS_BODY(true)
 }
 
 extern "C" __global__ void __cluster_dims__(2, 1, 1)
     __launch_bounds__(NUM_THREADS, 1)
         hc_gemm_bf16_umma_pair_scaled(HC_GEMM_ARGS) {
-  HC_GEMM_BODY(true, true)
+  HC_GEMM_SCALED_BODY(true)
 }
 
 // The dequantising GEMM that converts its weights inside the kernel, band by

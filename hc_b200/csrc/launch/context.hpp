@@ -129,6 +129,13 @@ private:
 // Frees what the host-buffer entry points keep in a context (host_api.cpp).
 void hcReleaseHostPipeline(HcContextImpl *c);
 
+// hcGemmBf16 on the tensor cores with row m of the product times rowScale[m *
+// rowScaleStride] before it is rounded (kernels_api.cpp).  Operands as TMA takes them.
+extern "C" int hcGemmBf16RowScaled(HcContextImpl *c, const void *a, const void *b,
+                                   const float *rowScale, long long rowScaleStride, void *out,
+                                   long long M, long long N, long long K, long long lda,
+                                   long long ldb, long long ldc);
+
 // Image of a serving kernel by its name, or null (serving_api.cpp).
 const char *hcServingImageOf(const char *kernel);
 

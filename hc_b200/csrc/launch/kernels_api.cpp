@@ -1412,11 +1412,13 @@ int hcGemmTiled(HcContext c, const void *a, const void *b, void *out,
                    args, 9, 0);
 }
 
-// Launches one of the tcgen05 kernels; `b` is bf16 [K, N].
+// Launches one of the tcgen05 kernels; `b` is bf16 [K, N].  scale: of the columns; or, with
+// neither that nor dsts, rowScale, one every rowScaleStride.
 static int launchUmma(HcContext c, const void *a, const void *b,
                       const float *scale, void *out, long long M, long long N,
                       long long K, long long lda, long long ldb, long long ldc,
-                      bool pair, const HcPeerOutputs *dsts = nullptr) {
+                      bool pair, const HcPeerOutputs *dsts = nullptr,
+                      const float *rowScale = nullptr, long long rowScaleStride = 0) {
   alignas(64) CUtensorMap mapA, mapB;
   if (olxEncodeTensorMap2D(c->device, &mapA, /*bf16*/ 0, a, size_t(M), size_t(K),
                            size_t(lda) * 2, kUmmaBM, kUmmaBK, 128) ||
@@ -1455,9 +1457,11 @@ static int launchUmma(HcContext c, const void *a, const void *b,
     }
     grid = 2 * std::min<long long>(tiles, c->pairSlots);
   }
-  void *args[] = {&mapA,   &mapB,   &out,   &scale,    &M,           &N,    &K,
-                  &ldc,    &tilesM, &tilesN, &bandM,   &vecStore, &c->statusWord, &peers};
-  return c->launch(name, size_t(grid), 1, 1, kUmmaThreads, args, dsts ? 14 : 13,
+  const float *scales = scale ? scale : rowScale;
+  void *last = dsts ? static_cast<void *>(&peers) : &rowScaleStride;
+  void *args[] = {&mapA,   &mapB,   &out,   &scales,   &M,           &N,    &K,
+                  &ldc,    &tilesM, &tilesN, &bandM,   &vecStore, &c->statusWord, last};
+  return c->launch(name, size_t(grid), 1, 1, kUmmaThreads, args, dsts || !scale ? 14 : 13,
                    kUmmaSmemBytes);
 }
 
@@ -1482,6 +1486,18 @@ int hcGemmBf16(HcContext c, const void *a, const void *b, void *out,
   // per 128 x 256 tile; it needs at least two row blocks to be worth a cluster.
   const bool pair = c->gemmVariant == 2 || (c->gemmVariant == 0 && M > kUmmaBM);
   return launchUmma(c, a, b, nullptr, out, M, N, K, lda, ldb, ldc, pair);
+}
+
+int hcGemmBf16RowScaled(HcContextImpl *c, const void *a, const void *b, const float *rowScale,
+                        long long rowScaleStride, void *out, long long M, long long N, long long K,
+                        long long lda, long long ldb, long long ldc) {
+  if (checkGemmShape(c, "hcGemmBf16RowScaled", a, b, out, M, N, K, lda, ldb, ldc))
+    return 1;
+  if (!ummaEligible(c, a, b, K, lda, ldb))
+    return c->fail("hcGemmBf16RowScaled: operands that TMA cannot describe");
+  const bool pair = c->gemmVariant == 2 || (c->gemmVariant == 0 && M > kUmmaBM);
+  return launchUmma(c, a, b, nullptr, out, M, N, K, lda, ldb, ldc, pair, nullptr, rowScale,
+                    rowScaleStride);
 }
 
 // ---- fp32 GEMM on the tensor cores (three tf32 products per fp32 product) ----------

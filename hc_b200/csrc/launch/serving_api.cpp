@@ -437,9 +437,10 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
     return c->fail("hcGemmW4: %lld rows need a 256-byte aligned workspace of %zu bytes, got %zu",
                    M, need, workspaceBytes);
   // The activations as bf16 rows that TMA can read.  A single scale per int8 row stays
-  // out of them (the integers are exact in bf16) where the epilogue can apply it.
+  // out of them (the integers are exact in bf16): the products' epilogues apply it.  (That
+  // of the CUDA-core product, which "gemm_variant" 3 forces, has none.)
   const bool fused = M <= kW4FusedRows;
-  const bool rowScaled = narrow && aGroup >= K && fused;
+  const bool rowScaled = narrow && aGroup >= K && (fused || c->gemmVariant != 3);
   long long pitchA = lda;
   if (!tmaRows) {
     void *rows = workspace;
@@ -508,6 +509,8 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
   if (c->launch("hc_dequant_w4_bf16", size_t(ceilDiv(N, 128)), size_t(ceilDiv(K, 128)), 1, 256,
                 args, 3, 0))
     return 1;
+  if (rowScaled)
+    return hcGemmBf16RowScaled(c, a, weights, aScale, ldas, out, M, N, K, pitchA, pitch, ldc);
   return hcGemmBf16(c, a, weights, out, M, N, K, pitchA, pitch, ldc);
 }
 

@@ -18,6 +18,7 @@ import pytest
 import torch
 
 from hc_b200 import serving
+from hc_b200.hckernel.kernel import get_context
 from oracle import serving as oracle
 
 pytestmark = pytest.mark.gpu
@@ -253,3 +254,38 @@ def test_the_largest_activations(group, m):
     c["a"] = torch.full_like(c["a"], most)
     c["scale"] = (c["scale"].float() * 2.0 ** -8).bfloat16()
     _check(c, serving.gemm_w4(**c))
+
+
+@pytest.mark.parametrize("m", [3, 8, 40, 1000, 1024, 1025, 1300])
+def test_int8_rows_with_one_scale_enter_exactly(m):
+    """Integer sums below 2^24 that cancel to little: exact, then one product with the row's
+    scale in float32 and one rounding.  (Scaled activations rounded to bfloat16 would leave
+    an error of the size of the terms.)"""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    dev = dict(device="cuda", generator=gen)
+    n, k = 72, 384
+    a = torch.randint(-40, 41, (m, k // 3, 3), dtype=torch.int8, **dev)
+    a[:, :, 2] = a[:, :, 0] + a[:, :, 1]
+    u = torch.tensor([9, 9, 7], dtype=torch.uint8, device="cuda").repeat(n, k // 3)
+    u[:, 0] = torch.randint(0, 16, (n,), dtype=torch.uint8, **dev)
+    w = u[:, 0::2] | u[:, 1::2] << 4
+    a, a_scale = a.view(m, k), torch.rand(m, 1, **dev) * 0.1 + 0.01
+    out = serving.gemm_w4(a, w, torch.ones(n, k // 32, device="cuda"), group=32, a_scale=a_scale)
+    want = a.double() @ (u.double() - 8).T
+    assert torch.equal(out, (want.float() * a_scale).bfloat16())
+
+
+@pytest.mark.parametrize("m", [2, 20, 1100])
+def test_row_scales_of_any_pitch_and_the_cuda_core_product(m):
+    c = _case(m, 96, 256, 64, True, a8=True)
+    want = serving.gemm_w4(**c)
+    wide = torch.full((m, 5), float("nan"), device="cuda")
+    wide[:, 2:3] = c["a_scale"]
+    assert torch.equal(serving.gemm_w4(**{**c, "a_scale": wide[:, 2:3]}), want)
+    ctx = get_context("cuda:0")
+    ctx.set_option("gemm_variant", 3)  # (has no place for a row's scale)
+    try:
+        _check(c, serving.gemm_w4(**c))
+        torch.cuda.synchronize()
+    finally:
+        ctx.set_option("gemm_variant", 0)
