@@ -44,7 +44,7 @@ struct W4UmmaParams {
   long long lds, ldz, rowScaleStride, ldc;
   int M, N, K;
   int group32;      // group / 32
-  uint32_t inverse; // ceil(2^32 / group32) for group32 > 1
+  uint32_t inverse; // 2^32 / group32, rounded down, for group32 > 1
   int groups;       // per row
   int cols;         // activation rows of a tile, a multiple of 16 up to 256
   int tilesM;
@@ -298,7 +298,13 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
 #pragma unroll
       for (int j = 0; j < kScales; ++j) {
         const uint32_t k32 = uint32_t(kb) * 4 + j;
-        const int gi = min(int(p.group32 == 1 ? k32 : __umulhi(k32, p.inverse)), p.groups - 1);
+        // The product's high word is the quotient or one less.
+        uint32_t g = k32;
+        if (p.group32 > 1) {
+          g = __umulhi(k32, p.inverse);
+          g += (g + 1) * uint32_t(p.group32) <= k32 ? 1 : 0;
+        }
+        const int gi = min(int(g), p.groups - 1);
         if constexpr (ScaleF32)
           scale[j] = __float_as_uint(__ldg(static_cast<const float *>(p.scale) + atScale + gi));
         else

@@ -468,7 +468,7 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
     u.lds = lds, u.ldz = ldz, u.ldc = ldc;
     u.M = p.M, u.N = p.N, u.K = p.K;
     u.group32 = int(group / 32);
-    u.inverse = u.group32 == 1 ? 0 : uint32_t((1ull << 32) / unsigned(u.group32) + 1);
+    u.inverse = u.group32 == 1 ? 0 : uint32_t((1ull << 32) / unsigned(u.group32));
     u.groups = int(groups);
     u.packed = group == 32 && lds % 4 == 0 && aligned(scale, 8) &&
                (!zero || (ldz % 4 == 0 && aligned(zero, 4)));

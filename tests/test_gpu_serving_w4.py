@@ -289,3 +289,38 @@ def test_row_scales_of_any_pitch_and_the_cuda_core_product(m):
         torch.cuda.synchronize()
     finally:
         ctx.set_option("gemm_variant", 0)
+
+
+@pytest.mark.parametrize("group,m", [(32, 7), (32, 8), (64, 7), (64, 8), (128, 8)])
+def test_eight_rows_of_the_deepest_that_fit(group, m):
+    """8 rows of K = 8192: in groups of 128 they fit in shared memory and weights enter
+    exactly; in finer groups fewer rows do, and the others take weights rounded to bf16
+    (worst case 2^-8 of the terms' sum)."""
+    c = _case(m, 96, 8192, group, True, seed=group)
+    out = serving.gemm_w4(**c).double()
+    w, a = _weights(c), c["a"].double()
+    room = ((8192 / 16 + 8) * 2.0 ** -22 + 2.0 ** -8) * (a.abs() @ w.abs().T)
+    assert ((out - a @ w.T).abs() <= 2.0 ** -8 * (a @ w.T).abs() + room).all()
+    if group == 128 or (group, m) == (64, 7):
+        _check(c, serving.gemm_w4(**c))
+
+
+@pytest.mark.parametrize("group", [65537 * 32, 65536 * 32 * 4])
+def test_groups_of_millions(group):
+    """The group of a column is found for every depth: the last 32 columns of the group
+    before a boundary belong to it."""
+    m, n, groups = 9, 16, 7
+    k = groups * group if group < 1 << 22 else 6 * group
+    groups = k // group
+    scale = torch.ones(n, groups, dtype=torch.bfloat16, device="cuda")
+    scale *= 2.0 ** torch.arange(groups, device="cuda")
+    w = torch.full((n, k // 2), 0x99, dtype=torch.uint8, device="cuda")
+    for g in range(1, groups):
+        a = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+        a[:, g * group - 32:g * group] = 1
+        out = serving.gemm_w4(a, w, scale, group=group)
+        assert torch.equal(out, torch.full_like(out, 32 * 2.0 ** (g - 1)))
+        a[:, g * group - 32:g * group] = 0
+        a[:, g * group:g * group + 32] = 1
+        out = serving.gemm_w4(a, w, scale, group=group)
+        assert torch.equal(out, torch.full_like(out, 32 * 2.0 ** g))
