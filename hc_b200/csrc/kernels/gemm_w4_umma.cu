@@ -199,7 +199,7 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
   auto filled = [&](uint64_t *bar, const RingAt &at, int code) {
     return mbarWait(smemAddr(&bar[at.stage]), at.parity, abortFlag, status, code);
   };
-  auto settle = [&]() { // after a wait gave up: copies may still be landing
+  auto settle = [&]() { // after a wait gave up: copies may still be landing, MMAs reading
     if (*abortFlag) {
       const unsigned long long t0 = globalTimerNs();
       while (globalTimerNs() - t0 < 1000000ull) {
@@ -263,6 +263,7 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
       }
       if (ok)
         ummaCommit(smemAddr(&bars.done));
+      settle();
     }
   } else if (warp >= 4) {
     // -------------------------------- converters -------------------------------
@@ -415,6 +416,19 @@ __device__ __forceinline__ void w4Umma(const CUtensorMap *mapB, const CUtensorMa
   if (warp == 1) {
     tcgen05FenceAfter();
     tmemFree<1>(tmemBase, uint32_t(p.tmemCols));
+  }
+  if (*abortFlag) {
+    // A wait was given up (nobody waits from here on): NaN instead of a tile, or of this
+    // rank's part of one, so that nothing that looks like a result is left.
+    const float nan = __uint_as_float(0x7fc00000u);
+    float *part = reinterpret_cast<float *>(smem);
+    for (int i = int(threadIdx.x); i < p.cols * 128; i += int(blockDim.x)) {
+      const int m = m0 + (i >> 7), n = n0 + (i & 127);
+      if (splits > 1)
+        part[i] = nan;
+      else if (m < p.M && n < p.N)
+        p.out[(long long)m * p.ldc + n] = __float2bfloat16_rn(nan);
+    }
   }
   if (splits > 1) {
     // Partial tiles, added in rank order; a rank finishes every splits-th row.

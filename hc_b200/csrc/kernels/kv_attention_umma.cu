@@ -938,10 +938,26 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
     tcgen05FenceAfter();
     tmemFree<1>(tmemBase, 512);
   }
+  // A wait that was given up must not leave rows that look like results: this unit's become
+  // NaN, or the part's share of the joint sums does.
+  const bool lost = *abortFlag != 0; // (nobody waits from here on)
   if (parts == 1) {
-    if (!aborted)
-      writeRows();
+    if (lost) {
+      const float nan = __uint_as_float(0x7fc00000u);
+      for (int i = tid; i < rowsHere * (DimCap / 4); i += kThreads)
+        keep(i / (DimCap / 4), i % (DimCap / 4) * 4, make_float4(nan, nan, nan, nan), 1.0f);
+      if (tid < rowsHere)
+        finishSum(tid, nan, nan);
+      __syncthreads();
+    }
+    writeRows();
     return;
+  }
+  if (lost && tid < 128) {
+    const HcKvPart none = hcKvLostPart();
+    float *slot = slotOf(int(blockIdx.y));
+    __stcg(slot + 128 * DimCap + tid, none.top);
+    __stcg(slot + 128 * DimCap + 128 + tid, none.sum);
   }
 
   // ---- the last part to finish joins them, in their order ------------------------------------
@@ -960,12 +976,12 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
       top = fmaxf(top, __ldcg(slotOf(x) + 128 * DimCap + tid));
     float sum = 0.0f;
     for (int x = 0; x < parts; ++x) {
-      const float part = __ldcg(slotOf(x) + 128 * DimCap + tid);
-      const float more = __ldcg(slotOf(x) + 128 * DimCap + 128 + tid);
       // (a part whose scores are NaN has a sum but no maximum)
-      const float f = part == kNegInf ? 0.0f : exp2Approx(part - top);
-      sum += part == kNegInf ? more : more * f;
-      sWeight[x * 128 + tid] = f;
+      const HcKvPart part{__ldcg(slotOf(x) + 128 * DimCap + tid),
+                          __ldcg(slotOf(x) + 128 * DimCap + 128 + tid)};
+      const float power = exp2Approx(part.top - top);
+      sum += hcKvPartSum(part, power);
+      sWeight[x * 128 + tid] = hcKvPartWeight(part, power);
     }
     sSum[0][tid] = sum;
     finishSum(tid, top, sum);

@@ -4,6 +4,7 @@
 // what comes out lies inside the buffers or is marked as not there.
 #pragma once
 
+#include <math.h>
 #include <stdint.h>
 
 #ifdef __CUDACC__
@@ -123,4 +124,26 @@ HC_KV_FN unsigned hcKvShareOf(const HcKvShares &s, unsigned x) {
   }
   const unsigned head = s.longer * (s.each + 1);
   return x < head ? x / (s.each + 1) : s.longer + (x - head) / s.each;
+}
+
+// ---- joining the parts of a unit -----------------------------------------------------
+// What a part of a unit's tokens leaves for a row: the sum of its exponentials and the
+// reference that they were taken against (-infinity: it saw nothing, or only NaN).
+struct HcKvPart {
+  float top, sum;
+};
+// A part whose CTA gave up a wait: nothing of its outputs is read, and the row's sum -
+// so its outputs and logarithm too - becomes NaN.
+HC_KV_FN HcKvPart hcKvLostPart() {
+  HcKvPart p;
+  p.top = -INFINITY;
+  p.sum = NAN;
+  return p;
+}
+// Its outputs' weight and its share of the sum; `power` is 2^(its top - the largest).
+HC_KV_FN float hcKvPartWeight(const HcKvPart &p, float power) {
+  return p.top == -INFINITY ? 0.0f : power;
+}
+HC_KV_FN float hcKvPartSum(const HcKvPart &p, float power) {
+  return p.top == -INFINITY ? p.sum : p.sum * power;
 }

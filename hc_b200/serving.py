@@ -9,6 +9,10 @@ straight on the stream that is current when they are called, so that a call
 costs one launch, is ordered with its neighbours by the stream alone and can
 be captured into a CUDA graph.  Call an operator once before capturing it: its
 kernel image is loaded at the first launch.
+
+The kernels on tcgen05 bound their waits; one that runs out (it never does while
+the GPU works) leaves NaN in place of what was not computed, and a code that the
+context's ``kernel_status()`` returns once the stream has been synchronised.
 """
 
 from __future__ import annotations

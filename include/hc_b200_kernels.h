@@ -84,7 +84,9 @@ HC_B200_API const char *hcLastError(HcContext c);
 HC_B200_API long long hcLaunchCount(HcContext c);
 /* Synchronizes, then returns in *statusRet the status word the tensor-core
  * kernels write when one of their bounded waits gives up (0 = none did) and
- * clears it. */
+ * clears it.  (It synchronizes the stream in use alone: wait for other streams
+ * that kernels were sent to first.)  The serving operators below leave NaN in
+ * place of what such a wait leaves uncomputed. */
 HC_B200_API int hcKernelStatus(HcContext c, int *statusRet);
 /* Runs a one-CTA kernel whose barrier wait can never be satisfied, with the
  * given time limit, waits for it and returns what happened: the status word
