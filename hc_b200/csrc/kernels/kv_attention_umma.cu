@@ -944,6 +944,7 @@ template <class Q, int DimCap> __device__ __forceinline__ void attendRows(const 
   if (parts == 1) {
     if (lost) {
       const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll 1
       for (int i = tid; i < rowsHere * (DimCap / 4); i += kThreads)
         keep(i / (DimCap / 4), i % (DimCap / 4) * 4, make_float4(nan, nan, nan, nan), 1.0f);
       if (tid < rowsHere)
