@@ -6,7 +6,8 @@
 //   out = y, or per group of columns  scale = max|y| / peak, out = round(y / scale)
 //
 // s, the sum of squares and y stay in fp32 (the sum that is written out is s rounded
-// to the input's type; the norm uses s itself), each value is rounded once.  peak is
+// to the input's type; the norm uses s itself), each value is rounded once.  Rows whose
+// squares overflow or vanish are scaled by a power of two and summed again.  peak is
 // 127 (int8) or 448 (e4m3).  A group that holds NaN gets the scale NaN, one that
 // holds an infinity the scale infinity: no value of such a group comes out finite.
 //
@@ -96,6 +97,17 @@ template <class Out> __device__ __forceinline__ float inverse(float most) {
   return most >= 3.0e-36f && most < __int_as_float(0x7f800000) ? Peak<Out>::value / most : 0.0f;
 }
 
+// A power of two for the values of a row whose squares leave float32, 1 for the others:
+// where their sum has overflowed (the values then reach 2^64 / sqrt(cols) at least), or is
+// so small that squares may have vanished and eps does not stand above them.
+__device__ __forceinline__ float rescale(float total, float eps) {
+  if (total == __int_as_float(0x7f800000))
+    return 1.3234889800848443e-23f; // 2^-76
+  if (total < 7.8886090522101181e-31f && eps < 5.2939559203393771e-23f) // 2^-100, 2^-74
+    return 1.2676506002282294e30f; // 2^100
+  return 1.0f;
+}
+
 template <class T> struct Same {};
 
 template <class T, class Out, int Threads, int V>
@@ -147,8 +159,21 @@ __device__ __forceinline__ void normRow(const NormParams &p) {
         storePacket(summed + row * p.summedPitch + c * 8, v[i]);
     }
   }
-  const float total = blockReduce<false>(squares, scratch[0]);
-  const float rms = __frsqrt_rn(total / float(p.cols) + p.eps);
+  float total = blockReduce<false>(squares, scratch[0]);
+  const float pre = rescale(total, p.eps);
+  if (pre != 1.0f) { // (the same for the whole CTA)
+    squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[i][k] *= pre;
+        squares = fmaf(v[i][k], v[i][k], squares);
+      }
+    __syncthreads();
+    total = blockReduce<false>(squares, scratch[0]);
+  }
+  const float rms = __frsqrt_rn(total / float(p.cols) + p.eps * pre * pre);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = i * Threads + tid;
@@ -232,11 +257,22 @@ __device__ __forceinline__ void normRowGeneric(const NormParams &p, int cached) 
       held[c] = s;
     squares = fmaf(s, s, squares);
   }
-  const float total = blockReduce<false>(squares, scratch[0]); // (a barrier: held is complete)
-  const float rms = __frsqrt_rn(total / float(p.cols) + p.eps);
+  float total = blockReduce<false>(squares, scratch[0]); // (a barrier: held is complete)
+  const float pre = rescale(total, p.eps);
+  if (pre != 1.0f) { // (the same for the whole CTA)
+    squares = 0.0f;
+    for (long long c = tid; c < p.cols; c += blockDim.x) {
+      const float s = value(c) * pre;
+      squares = fmaf(s, s, squares);
+    }
+    __syncthreads();
+    total = blockReduce<false>(squares, scratch[0]);
+  }
+  const float rms = __frsqrt_rn(total / float(p.cols) + p.eps * pre * pre);
+  auto norm = [&](long long c, float s) { return s * pre * rms * float(gain[c]); };
   auto put = [&](long long c, float inv) {
     const float s = value(c);
-    const float y = s * rms * float(gain[c]);
+    const float y = norm(c, s);
     if (summed)
       summed[c] = T(s);
     if constexpr (kSame)
@@ -250,7 +286,7 @@ __device__ __forceinline__ void normRowGeneric(const NormParams &p, int cached) 
   } else if (p.group == 0) {
     float top = 0.0f;
     for (long long c = tid; c < p.cols; c += blockDim.x)
-      top = hc::maxNan(top, fabsf(value(c) * rms * float(gain[c])));
+      top = hc::maxNan(top, fabsf(norm(c, value(c))));
     const float most = blockReduce<true>(top, scratch[1]);
     const float scale = most / Peak<Out>::value;
     const float inv = inverse<Out>(most);
@@ -265,7 +301,7 @@ __device__ __forceinline__ void normRowGeneric(const NormParams &p, int cached) 
       const long long end = min((g + 1) * p.group, p.cols);
       float top = 0.0f;
       for (long long c = g * p.group + lane; c < end; c += 32)
-        top = hc::maxNan(top, fabsf(value(c) * rms * float(gain[c])));
+        top = hc::maxNan(top, fabsf(norm(c, value(c))));
       const float most = segmentMax(top, 32);
       const float scale = most / Peak<Out>::value;
       const float inv = inverse<Out>(most);

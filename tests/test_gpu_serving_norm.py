@@ -165,3 +165,24 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="eps"):
         serving.add_rms_norm(x, gain, eps=-1.0)
     assert serving.add_rms_norm(x[:0], gain)[0].shape == (0, 64)
+
+
+@pytest.mark.parametrize("store", [None, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols,group", [(512, 0), (8192, 128), (1001, 0), (45000, 0),
+                                        (45000, 384)])
+@pytest.mark.parametrize("power", [-90, -70, 66, 120])
+def test_rows_whose_squares_leave_float32(power, cols, group, dtype, store):
+    """Finite rows whose squares overflow, or (eps = 0) vanish: y is what it is for others.
+    Rows of either kind among ordinary ones, and zeros."""
+    x, residual, gain = _inputs(5, cols, dtype, seed=power + 100)
+    by = torch.tensor([1.0, 2.0 ** power, 0.0, 2.0 ** power, 2.0 ** 30], device="cuda")[:, None]
+    x, residual = (x.float() * by).to(dtype), (residual.float() * by).to(dtype)
+    group = group if store is not None else 0
+    eps = 0.0 if power < 0 else 1e-5
+    out, scale, summed = serving.add_rms_norm(x, gain, residual, out_dtype=store, eps=eps,
+                                              group=group)
+    keep = [0, 1, 3, 4]
+    _check(x[keep], residual[keep], gain, out[keep], None if scale is None else scale[keep],
+           summed[keep], group, eps)
+    assert power < 0 or not out[2].float().any()
