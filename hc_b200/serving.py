@@ -13,6 +13,10 @@ kernel image is loaded at the first launch.
 The kernels on tcgen05 bound their waits; one that runs out (it never does while
 the GPU works) leaves NaN in place of what was not computed, and a code that the
 context's ``kernel_status()`` returns once the stream has been synchronised.
+
+No operator has a backward pass.  A call whose inputs require gradients is refused
+while gradients are recorded (call it under ``torch.no_grad()``): its results would
+be cut from the graph without a word.
 """
 
 from __future__ import annotations
@@ -23,6 +27,14 @@ from .hckernel.kernel import get_context
 
 _native = None
 _contexts = {}
+
+
+def _forward_only(name, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name}: no backward pass, but an argument requires gradients "
+                                   "(call it under torch.no_grad())")
 
 
 def _launcher(t):
@@ -53,6 +65,7 @@ def add_rms_norm(x, gain, residual=None, *, eps=1e-5, out_dtype=None, group=0, o
     and the sum in ``x``'s type, None without a residual.  ``out``, ``scale``
     and ``summed`` may be given; ``summed`` may be the residual itself.
     """
+    _forward_only("add_rms_norm", x, gain, residual, out, summed)
     native, ctx, stream = _launcher(x)
     if out is None:
         out = torch.empty_like(x, dtype=out_dtype)
@@ -84,6 +97,7 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     cores with the weights rounded to bfloat16.  Scratch memory is taken from
     torch's allocator for the length of the call.
     """
+    _forward_only("gemm_w4", a, scale, a_scale, out)
     native, ctx, stream = _launcher(a)
     m, k = a.shape
     n = w.shape[0]
@@ -111,6 +125,7 @@ class KvCache:
     """
 
     def __init__(self, k, v, k_scale, v_scale):
+        _forward_only("KvCache", k_scale, v_scale)
         native, ctx, _ = _launcher(k)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self._native = native.KvCache(ctx, k, v, k_scale, v_scale)
@@ -137,6 +152,7 @@ def kv_append(cache, k, v, table, lengths, starts=None, *, max_new=None):
     scale grows to what its new tokens need (earlier tokens are rounded
     again); pages that several sequences share must not be written.
     """
+    _forward_only("kv_append", k, v)
     native, ctx, stream = _launcher(k)
     native.kv_append(ctx, cache._native, k, v, table, lengths, starts,
                      -1 if max_new is None else max_new, stream)
@@ -173,6 +189,7 @@ def kv_attention(cache, q, table, lengths, starts=None, *, max_new=None, scale=N
     row's sum of exponentials, float32 [tokens, heads].  A row that sees
     nothing gives zeros and -inf; rows of no sequence are not written.
     """
+    _forward_only("kv_attention", q, out)
     native, ctx, stream = _launcher(q)
     if out is None:
         out = torch.empty_like(q)

@@ -193,6 +193,36 @@ def test_a_part_that_gave_up_shows_in_its_rows(tmp_path):
     assert np.isnan(total) and weights == [0, 1]
 
 
+def test_inputs_that_require_gradients_are_refused():
+    """There is no backward pass; under no_grad the call goes on (to the refusal of CPU
+    tensors, here)."""
+    from types import SimpleNamespace
+
+    from hc_b200 import serving
+
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    gain, rows = torch.zeros(64, dtype=torch.bfloat16), torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    w = torch.zeros(16, 32, dtype=torch.uint8)
+    scale, pages = torch.zeros(16, 2), torch.zeros(1, 1, 16, 64, dtype=torch.int8)
+    ints = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    cache = SimpleNamespace(_native=None, _root=1.0)
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: serving.add_rms_norm(grad(x), gain),
+             lambda: serving.add_rms_norm(x, grad(gain)),
+             lambda: serving.add_rms_norm(x, gain, grad(x)),
+             lambda: serving.gemm_w4(grad(x), w, scale, group=32),
+             lambda: serving.gemm_w4(x, w, grad(scale), group=32),
+             lambda: serving.kv_append(cache, grad(rows), rows, *ints),
+             lambda: serving.kv_append(cache, rows, grad(rows), *ints),
+             lambda: serving.kv_attention(cache, grad(rows), *ints),
+             lambda: serving.KvCache(pages, pages, grad(scale), scale)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA tensors"):
+            call()
+
+
 # ---- the C-ABI on a recording driver --------------------------------------------------------
 SCRIPT = """
 import ctypes as C
