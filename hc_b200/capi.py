@@ -265,6 +265,7 @@ KERNELS_PROTOTYPES = {
                   C.c_float, C.c_int, C.c_int]
     ),
     "hcGemmW4WorkspaceBytes": (_sz, [_ll, _ll, _ll, _ll, _ll, C.c_int]),
+    "hcGemmW4CallWorkspaceBytes": (_sz, [_vp, _ll, _ll, _ll, _ll, _ll, _ll, C.c_int]),
     "hcGemmW4": (
         C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _ll, _ll, _ll, _ll, _ll, _ll, _ll,
                   _ll, _ll, _ll, _ll, C.c_int, C.c_int]

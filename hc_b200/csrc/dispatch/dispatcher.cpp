@@ -1002,11 +1002,13 @@ PYBIND11_MODULE(_dispatcher, m) {
         py::arg("zero"), py::arg("out"), py::arg("group"), py::arg("a_scale") = py::none(),
         py::arg("a_group") = 0, py::arg("workspace") = py::none(), py::arg("stream") = py::none());
   m.def("w4_workspace_bytes",
-        [](long long rows, long long n, long long k, long long lda, long long ldw, bool int8) {
-          return hcGemmW4WorkspaceBytes(rows, n, k, lda, ldw, int8 ? HC_I8 : HC_BF16);
+        [](Context &c, long long rows, long long n, long long k, long long group, long long lda,
+           long long ldw, bool int8) {
+          return hcGemmW4CallWorkspaceBytes(c.get(), rows, n, k, group, lda, ldw,
+                                            int8 ? HC_I8 : HC_BF16);
         },
-        py::arg("m"), py::arg("n"), py::arg("k"), py::arg("lda"), py::arg("ldw"),
-        py::arg("int8") = false);
+        py::arg("ctx"), py::arg("m"), py::arg("n"), py::arg("k"), py::arg("group"),
+        py::arg("lda"), py::arg("ldw"), py::arg("int8") = false);
   py::class_<KvCache>(m, "KvCache")
       .def(py::init<Context &, py::object, py::object, py::object, py::object>(), py::arg("ctx"),
            py::arg("k"), py::arg("v"), py::arg("k_scale"), py::arg("v_scale"));

@@ -161,7 +161,12 @@ bool w4FitsFew(long long M, long long K, bool narrow, bool fine, long long group
   return M <= kW4FewRows && K <= (1 << 20) &&
          w4Few(M, K, narrow, fine, group).smem <= 227 * 1024;
 }
-
+// Whether groups are looked up per 128 columns.
+bool w4Coarse(long long K, long long group) { return group % 128 == 0 || group >= K; }
+// Which kernel a call of hcGemmW4 takes: the one for few rows or those of tcgen05.
+bool w4RunsFew(HcContext c, long long M, long long K, bool narrow, long long group) {
+  return c->w4Variant != 2 && w4FitsFew(M, K, narrow, !w4Coarse(K, group), group);
+}
 
 // Query rows (x head dimension) of a partial result in the attention's workspace, and
 // the CTAs per SM that can hold two of them each.
@@ -366,6 +371,13 @@ size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, long long l
   return w4RowBytes(M, K, aDtype != HC_I8 && lda % 8 == 0) + w4WeightBytes(M, N, K, ldw % 16 == 0);
 }
 
+size_t hcGemmW4CallWorkspaceBytes(HcContext c, long long M, long long N, long long K,
+                                  long long group, long long lda, long long ldw, int aDtype) {
+  if (!c || group <= 0 || w4RunsFew(c, M, K, aDtype == HC_I8, group))
+    return 0;
+  return hcGemmW4WorkspaceBytes(M, N, K, lda, ldw, aDtype);
+}
+
 int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, const void *scale,
              const void *zero, void *out, void *workspace, size_t workspaceBytes, long long M,
              long long N, long long K, long long group, long long aGroup, long long lda,
@@ -411,8 +423,8 @@ int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w, con
   const bool narrow = aDtype == HC_I8;
   p.vecA = narrow ? lda % 8 == 0 && aligned(a, 8) : lda % 8 == 0 && aligned(a, 16);
   char name[64];
-  const bool coarse = group % 128 == 0 || group >= K;
-  const bool few = c->w4Variant != 2 && w4FitsFew(M, K, narrow, !coarse, group);
+  const bool coarse = w4Coarse(K, group);
+  const bool few = w4RunsFew(c, M, K, narrow, group);
   if (c->w4Variant == 1 && !few)
     return c->fail("hcGemmW4: %lld rows of %lld do not fit the kernel for few rows", M, K);
   if (K == 0) // zeros

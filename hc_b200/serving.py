@@ -107,7 +107,7 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     # (A single row may report any stride; an unaligned array counts as one of odd pitch.)
     lda = 1 if a.data_ptr() % 16 else max(a.stride(0), k)
     ldw = 1 if w.data_ptr() % 16 else max(w.stride(0), (k + 1) // 2)
-    need = native.w4_workspace_bytes(m, n, k, lda, ldw, a.dtype == torch.int8)
+    need = native.w4_workspace_bytes(ctx, m, n, k, group, lda, ldw, a.dtype == torch.int8)
     if need:
         workspace = a.new_empty(need, dtype=torch.uint8)
     native.gemm_w4(ctx, a, w, scale, zero, out, group, a_scale, a_group, workspace, stream)

@@ -538,12 +538,16 @@ HC_B200_API int hcAddRmsNorm(HcContext c, const void *x, const void *residual, v
  * kernel that streams the weights as they are and need no workspace.  More rows run on
  * the tensor cores (tcgen05) with the weights rounded to bf16, once each: converted
  * inside that kernel up to 1024 rows, by a pass of their own for more.  workspace:
- * hcGemmW4WorkspaceBytes(M, N, K, lda, ldw, aDtype) bytes, 256-byte aligned, written by
- * the call (null where that is 0); an array that is not 16-byte aligned counts as one of
- * an odd pitch.  With few rows a non-finite activation makes its row of the
- * output NaN or infinite. */
+ * hcGemmW4CallWorkspaceBytes bytes, 256-byte aligned, written by the call (null where
+ * that is 0, as it is where the kernel for few rows runs; hcGemmW4WorkspaceBytes, which
+ * knows neither the groups nor the context's options, is never less); an array that is
+ * not 16-byte aligned counts as one of an odd pitch.  With few rows a non-finite
+ * activation makes its row of the output NaN or infinite. */
 HC_B200_API size_t hcGemmW4WorkspaceBytes(long long M, long long N, long long K, long long lda,
                                           long long ldw, int aDtype);
+HC_B200_API size_t hcGemmW4CallWorkspaceBytes(HcContext c, long long M, long long N,
+                                              long long K, long long group, long long lda,
+                                              long long ldw, int aDtype);
 HC_B200_API int hcGemmW4(HcContext c, const void *a, const float *aScale, const void *w,
                          const void *scale, const void *zero, void *out, void *workspace,
                          size_t workspaceBytes, long long M, long long N, long long K,

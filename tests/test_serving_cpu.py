@@ -399,6 +399,39 @@ def test_w4_refusals_and_choice(recording):
     """)
 
 
+def test_w4_workspace_of_a_call(recording):
+    """The kernel for few rows takes none, whatever the layout; others what the size that
+    knows the layout alone says."""
+    recording("""
+    from hc_b200._native import _dispatcher as d
+    def call(m, k, group, ws, lda, ldw, t):
+        hc.gemm_w4(P, P if t == capi.HC_I8 else None, P, P, None, P, P if ws else None, ws, m, 100,
+                   k, group, 0, lda, 1, ldw, 1 << 16, 0, 100, t)
+        return [l[0] for l in launches()]
+    layout = hc.lib.hcGemmW4WorkspaceBytes
+    need = hc.lib.hcGemmW4CallWorkspaceBytes
+    ctx = d.Context("cuda:0")
+    launches()
+    for t in (capi.HC_I8, capi.HC_BF16):
+        for m in (1, 3, 7, 8, 9, 40, 1100):
+            for k in (100, 4096, 4098, 8192, 30000):
+                for group in (32, 64, 128):
+                    for lda, ldw in ((k, (k + 1) // 2), (k + 7 & ~7, (k + 31) // 32 * 16)):
+                        ws = need(hc.handle, m, 100, k, group, lda, ldw, t)
+                        assert ws == d.w4_workspace_bytes(ctx, m, 100, k, group, lda, ldw,
+                                                          t == capi.HC_I8)
+                        names = call(m, k, group, ws, lda, ldw, t)
+                        few = "umma" not in names[-1]
+                        assert ws == (0 if few else layout(m, 100, k, lda, ldw, t)), (m, k, group)
+                        assert not few or m <= 8 and len(names) == 1
+                        if ws:
+                            refused("workspace", call, m, k, group, ws - 1, lda, ldw, t)
+    assert need(hc.handle, 3, 100, 4096, 128, 4096, 2048, capi.HC_I8) == 0
+    hc.set_option("w4_variant", 2)
+    assert need(hc.handle, 3, 100, 4096, 128, 4096, 2048, capi.HC_I8) == 3 * 8192
+    """)
+
+
 def test_cache_refusals_and_choice(recording):
     recording("""
     def cache(**kw):
