@@ -224,7 +224,7 @@ inline bool arrayFromExchange(py::handle obj, ArrayArg &a) {
   return true;
 }
 
-inline ArrayArg arrayFromPython(py::handle obj) {
+inline ArrayArg readArray(py::handle obj) {
   {
     ArrayArg a;
     if (arrayFromExchange(obj, a))
@@ -266,6 +266,19 @@ inline ArrayArg arrayFromPython(py::handle obj) {
     return arrayFromInterface(obj.attr("__array_interface__").cast<py::dict>(), false);
   throw std::runtime_error("Object is not an array (no data_ptr, __cuda_array_interface__ "
                            "or __array_interface__)");
+}
+
+inline ArrayArg arrayFromPython(py::handle obj) {
+  ArrayArg a = readArray(obj);
+  if (!a.data) {
+    bool empty = false;
+    for (int64_t n : a.shape)
+      empty = empty || n == 0;
+    if (!empty)
+      throw std::runtime_error("Array without memory of its own (a meta or fake tensor, or a "
+                               "wrapper of others)");
+  }
+  return a;
 }
 
 } // namespace hc

@@ -96,3 +96,41 @@ def test_get_kernel_failure_aborts_like_the_reference():
     assert proc.returncode == -6  # SIGABRT
     assert "Offload error: olCreateDevice failed" in proc.stderr
     assert "survived" not in proc.stdout
+
+
+def test_convert_kinds_of_torch_tensors(rt):
+    """Tensors are read through DLPack's exchange table where their type has one, and agree
+    with what data_ptr() says; those without memory of their own are refused."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    class Plain(torch.Tensor):
+        pass
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls):
+            return torch.Tensor._make_wrapper_subclass(cls, (3, 4), dtype=torch.float32)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError
+
+    d = _Desc2()
+    x = torch.zeros(3, 4)
+    for t in (x, torch.nn.Parameter(x), x.clone().requires_grad_(), x.as_subclass(Plain),
+              x.bool(), x.to(torch.float8_e4m3fn), x.to(torch.complex64), torch._neg_view(x),
+              torch.zeros(5, 9)[1:4, 2:6], torch.zeros(1, 4).expand(3, 4)):
+        assert rt.hcgpuConvertPyArray(None, t, 2, C.byref(d)) == 0
+        assert d.allocated == t.data_ptr()
+        assert list(d.sizes) == [3, 4] and list(d.strides) == list(t.stride())
+    for t in (torch.zeros(0, 4), torch.zeros(3, 0)):
+        assert rt.hcgpuConvertPyArray(None, t, 2, C.byref(d)) == 0
+        assert list(d.sizes) == list(t.shape)
+    with FakeTensorMode():
+        fake = torch.zeros(3, 4)
+    functional = []
+    torch.func.functionalize(lambda t: functional.append(
+        rt.hcgpuConvertPyArray(None, t, 2, C.byref(d))) or t + 1)(x)
+    assert functional == [1]
+    for t in (fake, Wrapper(), torch.zeros(3, 4, device="meta"), torch.eye(3, 4).to_sparse()):
+        assert rt.hcgpuConvertPyArray(None, t, 2, C.byref(d)) == 1
