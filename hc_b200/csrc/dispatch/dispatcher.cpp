@@ -17,10 +17,12 @@
 #include <pybind11/stl.h>
 
 #include <algorithm>
+#include <algorithm>
 #include <array>
 #include <charconv>
 #include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
 namespace py = pybind11;
@@ -798,6 +800,26 @@ void gemmW4(Context &ctx, py::handle a, py::handle w, py::handle scale, py::hand
             "gemm_w4");
 }
 
+// Whether elements of an array share memory (an expanded one, for instance): some stride
+// does not reach over what lies inside it.
+bool overlapping(const ArrayArg &a) {
+  std::vector<std::pair<int64_t, int64_t>> axes; // stride, extent
+  for (int d = 0; d < a.rank(); ++d) {
+    if (a.shape[d] == 0)
+      return false;
+    if (a.shape[d] > 1)
+      axes.emplace_back(a.strides[d], a.shape[d]);
+  }
+  std::sort(axes.begin(), axes.end());
+  int64_t span = 1;
+  for (const auto &[stride, extent] : axes) {
+    if (stride < span)
+      return true;
+    span += (extent - 1) * stride;
+  }
+  return false;
+}
+
 // The paged 8-bit cache: four arrays checked once and kept (with a reference to each).
 class KvCache {
 public:
@@ -829,6 +851,12 @@ public:
     cache.headStride = cache.heads > 1 ? K.strides[1] : 0;
     cache.pageStride = cache.pages > 1 ? K.strides[0] : 0;
     cache.scalePitch = pitch(KS);
+    shared = overlapping(K);
+  }
+  // (Reading pages that share memory is fine.)
+  void writable() const {
+    if (shared)
+      throw py::value_error("kv_append: elements of the cache share memory");
   }
   void on(const Context &ctx) const {
     if (ctx.ordinal != ordinal)
@@ -839,6 +867,7 @@ public:
 private:
   std::array<py::object, 4> arrays;
   int ordinal;
+  bool shared = false;
 };
 
 HcKvPlace kvPlace(Context &ctx, py::handle table, py::handle lengths, py::handle starts,
@@ -883,6 +912,7 @@ void rowsOfHeads(const ArrayArg &a, long long tokens, long long heads, long long
 void kvAppend(Context &ctx, KvCache &cache, py::handle k, py::handle v, py::handle table,
               py::handle lengths, py::handle starts, long long maxNew, py::handle stream) {
   cache.on(ctx);
+  cache.writable();
   ArrayArg K = deviceArray(ctx, k, "k", 3), V = deviceArray(ctx, v, "v", 3);
   rowsOfHeads(K, K.shape[0], cache.cache.heads, cache.cache.dim, "k");
   rowsOfHeads(V, K.shape[0], cache.cache.heads, cache.cache.dim, "v");
@@ -904,6 +934,8 @@ void kvAttention(Context &ctx, KvCache &cache, py::handle q, py::handle out, py:
                           std::to_string(cache.cache.heads) + " of the cache");
   rowsOfHeads(Q, Q.shape[0], heads, cache.cache.dim, "q");
   rowsOfHeads(O, Q.shape[0], heads, cache.cache.dim, "out");
+  if (overlapping(O))
+    throw py::value_error("out: its elements share memory");
   ArrayArg L, W = deviceArray(ctx, workspace, "workspace", 1);
   if (!lse.is_none()) {
     L = deviceArray(ctx, lse, "lse", 2);

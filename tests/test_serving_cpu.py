@@ -513,6 +513,68 @@ def test_cache_refusals_and_choice(recording):
     """)
 
 
+def test_arrays_that_are_written_to_have_memory_of_their_own(recording):
+    """Expanded caches and outputs: every layout without shared elements is taken."""
+    recording("""
+    from hc_b200._native import _dispatcher as d
+
+    class Dev:  # what the dispatcher reads of a device array
+        is_cuda = True
+        device = type("D", (), dict(index=0))
+        def __init__(self, dtype, shape, strides, size):
+            self.dtype, self.shape, self.strides, self.size = "torch." + dtype, shape, strides, size
+        def data_ptr(self): return P
+        def element_size(self): return self.size
+        def stride(self): return self.strides
+    def dense(dtype, size, *shape, order=None):
+        strides, at = [0] * len(shape), 1
+        for axis in reversed(order or range(len(shape))):
+            strides[axis], at = at, at * shape[axis]
+        return Dev(dtype, shape, tuple(strides), size)
+
+    ctx = d.Context("cuda:0")
+    scale = dense("float32", 4, 5, 2)
+    table, lengths = dense("int32", 4, 3, 2), dense("int32", 4, 3)
+    rows = dense("bfloat16", 2, 3, 2, 64)
+    ws = Dev("uint8", (d.kv_attention_workspace_bytes(ctx),), (1,), 1)
+    launches()
+    def append(pages):
+        d.kv_append(ctx, d.KvCache(ctx, pages, pages, scale, scale), rows, rows, table, lengths)
+        return len(launches())
+    def attend(pages, out):
+        cache = d.KvCache(ctx, pages, pages, scale, scale)
+        d.kv_attention(ctx, cache, dense("bfloat16", 2, 3, 4, 64), out, None, table, lengths, None,
+                       -1, 0.125, 0, ws)
+        return len(launches())
+    def no(match, call, *args):
+        try:
+            call(*args)
+        except ValueError as e:
+            assert match in str(e) and not launches(), str(e)
+            return
+        raise AssertionError("not refused")
+    out = dense("bfloat16", 2, 3, 4, 64)
+    for order in (None, (0, 2, 1, 3), (1, 0, 2, 3), (2, 0, 1, 3)):
+        pages = dense("int8", 1, 5, 2, 16, 64, order=order)
+        assert append(pages) == 1 and attend(pages, out) == 1
+    wide = Dev("int8", (5, 2, 16, 64), (2 * 2 * 16 * 80, 16 * 80, 80, 1), 1)
+    assert append(wide) == 1
+    one = Dev("int8", (5, 1, 16, 64), (16 * 64, 0, 64, 1), 1)  # an axis of one: any stride
+    single = dense("float32", 4, 5, 1)
+    d.kv_append(ctx, d.KvCache(ctx, one, one, single, single), dense("bfloat16", 2, 3, 1, 64),
+                dense("bfloat16", 2, 3, 1, 64), table, lengths)
+    assert len(launches()) == 1
+    for strides in ((0, 1024, 64, 1), (2048, 0, 64, 1), (1024, 1024, 64, 1), (2048, 512, 64, 1)):
+        pages = Dev("int8", (5, 2, 16, 64), strides, 1)
+        no("share memory", append, pages)
+        assert attend(pages, out) == 1
+    pages = dense("int8", 1, 5, 2, 16, 64)
+    assert attend(pages, dense("bfloat16", 2, 3, 4, 64, order=(1, 0, 2))) == 1
+    for strides in ((0, 64, 1), (256, 0, 1), (128, 64, 1), (64, 128, 1)):
+        no("share memory", attend, pages, Dev("bfloat16", (3, 4, 64), strides, 2))
+    """)
+
+
 def test_launches_go_to_the_stream_in_use(recording):
     recording("""
     def go():
