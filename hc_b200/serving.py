@@ -165,7 +165,11 @@ _COUNTER_BYTES = 4096  # HC_KV_COUNTER_BYTES of the C-ABI
 def _attention_workspace(native, ctx, device, stream):
     """Scratch of the attention, its counters zeroed: one per stream, and one of its own
     for every call that is being captured, so that graphs may run beside each other."""
-    capturing = torch.cuda.is_current_stream_capturing()
+    if torch.cuda.current_device() == device.index:
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(device):  # (the question is about the current device's stream)
+            capturing = torch.cuda.is_current_stream_capturing()
     key = (device.index, stream)
     buf = None if capturing else _scratch.get(key)
     if buf is None:

@@ -223,6 +223,44 @@ def test_inputs_that_require_gradients_are_refused():
             call()
 
 
+def test_a_capture_on_another_device_than_the_current_one(monkeypatch):
+    """The attention's workspace is a captured call's own where the stream of its device is
+    being captured, whichever device is the current one."""
+    from types import SimpleNamespace
+
+    from hc_b200 import serving
+
+    state = dict(current=0, capturing={0: False, 1: False})
+
+    class On:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, state["current"] = state["current"], self.index
+
+        def __exit__(self, *_):
+            state["current"] = self.before
+
+    empty = torch.empty
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing",
+                        lambda: state["capturing"][state["current"]])
+    monkeypatch.setattr(torch, "empty", lambda n, dtype, device: empty(n, dtype=dtype))
+    monkeypatch.setattr(serving, "_scratch", {})
+    native = SimpleNamespace(kv_attention_workspace_bytes=lambda ctx: 8192)
+    get = lambda i: serving._attention_workspace(  # noqa: E731
+        native, None, SimpleNamespace(index=i), 7)
+    kept = [get(0), get(1)]
+    assert get(0) is kept[0] and get(1) is kept[1] and kept[0] is not kept[1]
+    state["capturing"][1] = True
+    assert get(1) is not kept[1] and get(0) is kept[0]
+    state["capturing"] = {0: True, 1: False}
+    assert get(1) is kept[1] and get(0) is not kept[0]
+    assert state["current"] == 0
+
+
 # ---- the C-ABI on a recording driver --------------------------------------------------------
 SCRIPT = """
 import ctypes as C
