@@ -111,6 +111,7 @@ struct HcContextImpl {
                     void **args, size_t smem);
   // Scratch of the host-buffer entry points (host_api.cpp), released with the context.
   struct HostPipeline *hostPipeline = nullptr;
+  std::mutex hostCalls; // one of them at a time
 };
 
 // Sends the calling thread's launches through `c` to `q` for the length of the scope,

@@ -241,6 +241,7 @@ int hcSoftmaxRowsHost(HcContext c, const void *xHost, void *yHost, long long row
                       long long cols, long long xPitch, long long yPitch, int dtype) {
   if (!c)
     return 1;
+  std::lock_guard<std::mutex> turn(c->hostCalls);
   const int elem = elemBytesOf(dtype);
   if (!elem)
     return c->fail("hcSoftmaxRowsHost: unsupported dtype %d", dtype);
@@ -262,6 +263,7 @@ int hcReduceRowsHost(HcContext c, const void *xHost, void *sumHost, void *maxHos
                      long long rows, long long cols, long long pitch, int dtype) {
   if (!c)
     return 1;
+  std::lock_guard<std::mutex> turn(c->hostCalls);
   const int elem = elemBytesOf(dtype);
   if (!elem)
     return c->fail("hcReduceRowsHost: unsupported dtype %d", dtype);
@@ -292,6 +294,7 @@ int hcGemmBf16Host(HcContext c, const void *aHost, const void *bHost, void *cHos
                    long long ldc) {
   if (!c)
     return 1;
+  std::lock_guard<std::mutex> turn(c->hostCalls);
   if (M < 0 || N < 0 || K < 0 || lda < K || ldb < N || ldc < N)
     return c->fail("hcGemmBf16Host: invalid shape M=%lld N=%lld K=%lld", M, N, K);
   if (M == 0 || N == 0)

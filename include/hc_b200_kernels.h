@@ -55,9 +55,9 @@ HC_B200_API int hcImageOfKernel(const char *kernelName);
  * several GPUs can be driven from one process.  Like the reference's runtime
  * (no locks anywhere, gpu-runtime/cuda-runtime/src/Runtime.cpp), a context is
  * not thread-safe: use it from one thread at a time - but for the host-buffer
- * entry points (below): while one thread waits in one of them, another may
- * launch through the same context.  Different contexts may be used from
- * different threads. */
+ * entry points (below), which take turns when several threads call them, and
+ * beside which one other thread may launch through the same context.  Different
+ * contexts may be used from different threads. */
 HC_B200_API HcContext hcCreateContext(const char *deviceDesc,
                                       OlErrorCallback errCallback, void *ctx);
 HC_B200_API void hcReleaseContext(HcContext c);

@@ -7,6 +7,7 @@
  * the others.  Device addresses are made up and never dereferenced.  It is never
  * loaded in a process that uses a real GPU.
  */
+#include <pthread.h>
 #include <stddef.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -36,7 +37,6 @@ OK(cuFuncSetAttribute)
 OK(cuStreamDestroy_v2)
 OK(cuStreamSynchronize)
 OK(cuMemFree_v2)
-OK(cuMemcpyHtoDAsync_v2)
 OK(cuMemcpyDtoHAsync_v2)
 OK(cuMemsetD8Async)
 OK(cuTensorMapEncodeTiled)
@@ -46,6 +46,16 @@ OK(cuEventElapsedTime)
 OK(cuStreamWaitEvent)
 OK(cuMemHostRegister_v2)
 OK(cuMemHostUnregister)
+/* Uploads: which thread made each. */
+static unsigned long uploads[ROOM];
+static int uploaded;
+int recorded_uploads(void) { return uploaded < ROOM ? uploaded : ROOM; }
+unsigned long recorded_upload(int i) { return uploads[i]; }
+int cuMemcpyHtoDAsync_v2(unsigned long long dst, const void *src, size_t n, void *stream) {
+  int at = __atomic_fetch_add(&uploaded, 1, __ATOMIC_RELAXED);
+  uploads[at < ROOM ? at : ROOM - 1] = (unsigned long)pthread_self();
+  return 0;
+}
 int cuGetErrorName(int error, const char **name) {
   *name = "CUDA_ERROR_UNKNOWN";
   return 0;

@@ -706,6 +706,31 @@ def test_serving_calls_beside_a_host_buffer_call(recording):
     """)
 
 
+def test_host_buffer_calls_of_two_threads_take_turns(recording):
+    """They share the context's device slots: a call's chunks are its own from the first
+    to the last."""
+    recording("""
+    import threading
+    import numpy as np
+    from hc_b200._native import _dispatcher as d
+    fake.recorded_upload.restype = C.c_ulong
+    ctx = d.Context("cuda:0")
+    big = [np.empty((1 << 18, 1024), np.float32) for _ in range(2)]  # 64 chunks
+    start = threading.Barrier(2)
+    def host(x):
+        start.wait()
+        for _ in range(20):
+            d.reduce_rows_host(ctx, x, np.empty(1 << 18, np.float32), None)
+    threads = [threading.Thread(target=host, args=(x,)) for x in big]
+    for t in threads: t.start()
+    for t in threads: t.join()
+    who = [fake.recorded_upload(i) for i in range(fake.recorded_uploads())]
+    assert len(who) == 2 * 20 * 64 and len(set(who)) == 2
+    for i in range(0, len(who), 64):
+        assert len(set(who[i:i + 64])) == 1, i
+    """)
+
+
 def test_every_serving_kernel_is_found_by_its_name():
     """The families that the launch code names lie in the images it says."""
     from hc_b200 import capi
