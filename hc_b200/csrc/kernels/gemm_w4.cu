@@ -13,10 +13,9 @@
 // mma.sync (16 weight rows) and the activations the B operand (8 columns): a lane holds
 // two rows' 32 consecutive weights of 128 (one 16-byte load each), and since a sum does
 // not care about the order of its terms, K is permuted so that these are the very
-// elements the lane feeds to the MMAs.  Legacy mma.sync rather than tcgen05: one row
-// costs what eight do, the operand registers need no detour, and at up to 16 rows the
-// stream of weights is the bound (mma.sync measured 549 TFLOP/s in bf16 and 1127 TOP/s
-// in int8 on this GPU, against 13 and 26 needed per row at full bandwidth).
+// elements the lane feeds to the MMAs.  Legacy mma.sync rather than tcgen05: the operand
+// registers need no detour, and its rate is not the bound (mma.sync measured 549 TFLOP/s
+// in bf16 and 1127 TOP/s in int8 on this GPU; 8 rows at full bandwidth need 210).
 //   * bf16: the bits of a nibble ARE the f16 number u * 2^-24 (a subnormal, which the
 //     MMA takes as it is), and 16 u * 2^-24 one place further left: one AND per two
 //     weights and one shift per eight unpack them, exactly.  (The logic pipe has half
@@ -36,11 +35,19 @@
 //     tiles.
 //     The partial sums of a tile's warps meet in shared memory and are added in the
 //     order of K.
-// Measured, N = K = 8192 in groups of 128: 16.3 us with one row (2.1 TB/s of weights),
-// 19.6 with 4, 24.7 with 8, where the tcgen05 kernel (gemm_w4_umma.cu) takes 23.5 whatever
-// the rows; N = K = 4096: 6.3 / 8.4 / 11.1 against 11.2; groups of 32 at 8192: 27.5 / 30.4
-// against 26.  What bounds it is the instructions that unpack (all of a warp's 32 lanes
-// work for 8 columns, of which one row uses one) and, at 4096, the start of the stream.
+// Measured with weights from HBM, us, for 1 / 4 / 8 rows of bf16 (6 where 8 do not fit), and
+// the tcgen05 kernel (gemm_w4_umma.cu) whatever the rows:
+//                  groups of 128           64                      32
+//   8192 x 8192    16.2 / 19.5 / 24.7, 23  20.5 / 23.5 / 25.8, 26  23.2 / 26.3 / 29.0, 25
+//   4096 x 4096     6.6 /  8.4 / 11.2, 12   8.0 /  9.7 / 12.3, 12   8.4 / 10.1 / 12.8, 11
+//   14336 x 4096   16.5 / 18.5 / 22.0, 23  21.6 / 23.3 / 26.6, 26  23.7 / 25.2 / 28.3, 25
+//   1024 x 8192     6.5 /  9.6 / 14.0, 12   7.6 / 10.4 / 12.5, 12   8.2 / 11.1 / 13.1, 12
+// and int8 14.3 / 17.2 / 22.3 against 26 at 8192 x 8192 in groups of 128.  So with six to
+// eight rows the other kernel is up to a sixth faster; this one is taken all the same
+// wherever the rows fit, because its weights are not rounded: one to eight rows are one
+// accuracy class.  What bounds it (2.1 TB/s of weights with one row) is the instructions
+// that unpack (all of a warp's 32 lanes work for 8 columns, of which one row uses one) and,
+// at 4096, the start of the stream.
 #include "serving_math.cuh"
 
 #include <type_traits>

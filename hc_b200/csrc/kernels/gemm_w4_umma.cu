@@ -22,11 +22,17 @@
 //   * Where the tiles alone do not fill the GPU a cluster of CTAs shares the K of a tile;
 //     the partial tiles meet through distributed shared memory, added in rank order.
 // Few columns are bound by the stream of weights and its conversion, many by the tensor
-// pipe.  Measured, N = K = 8192, groups of 128: 23 us for 16 and 32 rows (1.5 TB/s of packed
-// weights), 26 for 64 (the last with two CTAs per SM: 128 take 35), 44 for 256, 64 for 512
-// (1.07 PFLOP/s); a launch costs 6.7 us before the first weight arrives.  Above 512 rows
-// the row tiles come in two waves (122 us for 1024), from 1025 on converting first is as
-// fast (1024 rows that way: 140 us).  Waits are bounded as in the other tcgen05 kernels (hc_ptx.cuh).
+// pipe.  Measured, N = K = 8192, groups of 128: 24 us for 16 and 32 rows (1.5 TB/s of packed
+// weights), 26 for 64 (the last with two CTAs per SM: 128 take 35), 45 for 256, 64 for 512
+// (1.07 PFLOP/s); a launch costs 6.7 us before the first weight arrives.  Up to 1024 rows
+// run here, more are converted first (gemm_w4.cu, gemm_bf16_umma.cu); us, here / converted
+// first, groups of 128:
+//   rows           512       1024        1280        1536        2048        4096
+//   8192 x 8192    64 / 98   122 / 137   178 / 182   179 / 182   240 / 229   506 / 435
+//   4096 x 4096    31 / 49    39 /  41    71 /  60    72 /  60    73 /  61   141 / 106
+//   14336 x 4096   73 / 95   139 / 133   141 / 137   176 / 159   241 / 201   459 / 349
+// Waits are bounded as in the other tcgen05 kernels (hc_ptx.cuh); one that is given up
+// leaves NaN.
 #include "serving_math.cuh"
 
 #include <cooperative_groups.h>

@@ -21,8 +21,8 @@
 //     2^-14 of the row's largest element; the block's key scale multiplies the fp32
 //     scores; its value scale goes into the probabilities before they are rounded to
 //     f16: w = 2^11 * exp2(x - m) * vScale, where m follows the running maximum of
-//     x + log2(vScale) and is at most 4 behind it, so w <= 2^15 whatever the scales are
-//     and the outputs are rescaled a few times per sequence only.  The sum of
+//     x + log2(vScale) and is at most 4 behind it (a scale below 2^-96, or 0, counts as
+//     that), so w <= 2^15 whatever the scales are and the outputs are rescaled a few times per sequence only.  The sum of
 //     exp2(x - m), the maxima and the output are fp32; rounding w costs 2^-12 of a term
 //     (terms below 2^-25 of the largest lose more, by at most 2^-36 of it).
 //   * The tiles (16 tokens) of all (sequence, head, row tile) units stand in one line

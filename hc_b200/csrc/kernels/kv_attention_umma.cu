@@ -20,8 +20,9 @@
 // three run beside each other.  Reading the cache is small beside that (32 KiB a tile,
 // mostly from L2).
 // Measured: 512 new tokens of 32 heads (8 for keys and values, dim 128) at 16384 tokens in
-// 198 us with int8 and 188 with e4m3, 690 and 720 TFLOP/s, against 1143 and 1020 us with
-// kv_attention.cu; dim 64 166 us, dim 256 424.  Counters show half of the issue slots
+// 196 us with int8 and 198 to 201 with e4m3 (690 TFLOP/s; the compiler's order of the same
+// code moves either by 5 %), against 1143 and 1020 us with kv_attention.cu; dim 64 168 us,
+// dim 256 408.  Eight whole prompts of 2048: 670.  Counters show half of the issue slots
 // taken (8600 instructions per tile, half of them conversion), the tensor pipe at a
 // quarter and no single pipe full: what is left are the latencies of the hand-overs
 // between the roles.

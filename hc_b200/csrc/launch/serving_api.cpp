@@ -127,7 +127,7 @@ long long roundUp(long long a, long long b) { return ceilDiv(a, b) * b; }
 // shared memory beside the scales of its 16 warps.
 constexpr long long kW4FewRows = 8; // (both sides measured: gemm_w4.cu)
 // Up to this many the weights are converted inside the tcgen05 kernel, for more by a pass
-// of their own in front of hcGemmBf16.
+// of their own in front of the bf16 product (both sides measured: gemm_w4_umma.cu).
 constexpr long long kW4FusedRows = 1024;
 
 // The parts of hcGemmW4's workspace: the activations in bf16 (int8 ones, and bf16 ones

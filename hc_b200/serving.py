@@ -93,9 +93,12 @@ def gemm_w4(a, w, scale, zero=None, *, group, a_scale=None, a_group=0, out=None)
     :func:`add_rms_norm` returns them (``a_group``: its ``group``).  Returns
     ``out`` bfloat16 [M, N].
 
-    Up to 8 rows stream the weights as they are; more rows run on the tensor
-    cores with the weights rounded to bfloat16.  Scratch memory is taken from
-    torch's allocator for the length of the call.
+    Up to 8 rows that fit in shared memory (``include/hc_b200_kernels.h``:
+    at ``K`` = 8192 in bfloat16 6 to 8, by ``group``) stream the weights as
+    they are; more rows run on the tensor cores with the weights rounded to
+    bfloat16, and int8 activations with several scales per row (``a_group``)
+    too.  Scratch memory is taken from torch's allocator for the length of
+    the call.
     """
     _forward_only("gemm_w4", a, scale, a_scale, out)
     native, ctx, stream = _launcher(a)

@@ -534,9 +534,13 @@ HC_B200_API int hcAddRmsNorm(HcContext c, const void *x, const void *residual, v
  * (z = 8 throughout).  `group` is a multiple of 32.  a is HC_BF16 (aScale null, as = 1)
  * or HC_I8 with float aScale [M, ceil(K/aGroup)], pitch ldas - what hcAddRmsNorm
  * writes; aGroup is 0 (one scale per row) or a multiple of `group`.  out is bf16.
- * Up to 8 rows that fit in shared memory (8 rows of K = 8192 in bf16 do) run on the
- * kernel that streams the weights as they are and need no workspace.  More rows run on
- * the tensor cores (tcgen05) with the weights rounded to bf16, once each: converted
+ * Up to 8 rows that fit in shared memory run on the kernel that streams the weights as
+ * they are and need no workspace.  (All 8 fit up to K = 6144 in bf16 and 8192 in int8; at
+ * K = 8192 in bf16 8 in groups that are multiples of 128, 7 in groups of 64 and 96, 6 of
+ * 32; at K = 16384 3, 2 and 1.)  More rows, or deeper ones, run on the tensor cores
+ * (tcgen05) with two more roundings: of the weights (u - z) * s to bf16, once each; and
+ * of int8 activations with several scales per row, a * as, to bf16 (with one scale per
+ * row the integers enter exactly and the scale multiplies the sum).  They are converted
  * inside that kernel up to 1024 rows, by a pass of their own for more.  workspace:
  * hcGemmW4CallWorkspaceBytes bytes, 256-byte aligned, written by the call (null where
  * that is 0, as it is where the kernel for few rows runs; hcGemmW4WorkspaceBytes, which
