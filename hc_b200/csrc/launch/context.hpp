@@ -20,11 +20,11 @@ public:
     std::lock_guard<std::mutex> hold(lock);
     text = s;
   }
-  // Valid until the calling thread's next call.
+  // The calling thread's copy of this context's text, valid until it asks again.
   const char *c_str() const {
-    static thread_local std::string copy;
+    static thread_local std::map<const HcErrorText *, std::string> copies;
     std::lock_guard<std::mutex> hold(lock);
-    return (copy = text).c_str();
+    return (copies[this] = text).c_str();
   }
 
 private:

@@ -368,6 +368,8 @@ HcContext hcCreateContext(const char *deviceDesc, OlErrorCallback errCallback,
 void hcReleaseContext(HcContext c) {
   if (!c)
     return;
+  while (popQueue(c)) { // (an address that another context may get)
+  }
   c->chosenQueue = c->ownQueue;
   if (c->ownQueue)
     olSyncQueue(c->ownQueue);

@@ -657,6 +657,27 @@ def test_pushed_streams_nest_and_are_the_threads_own(recording):
     """)
 
 
+def test_errors_and_pushed_streams_are_a_contexts_own(recording):
+    """Two contexts' last errors side by side; a context opened where one with a pushed
+    stream was released starts on its own."""
+    recording("""
+    other = capi.Context("cuda:0")
+    last = hc.lib.hcLastError
+    last.restype = C.c_void_p
+    assert hc.lib.hcSetOption(hc.handle, b"no such option", 1)
+    assert other.lib.hcReportError(other.handle, b"of the other")
+    a, b = last(hc.handle), last(other.handle)
+    assert b"no such option" in C.string_at(a) and C.string_at(b) == b"of the other"
+    for _ in range(20):
+        c = capi.Context("cuda:0")
+        c.softmax_rows(P, P + (1 << 20), 4, 64, 64, 64)
+        assert launches()[0][4] == c.stream
+        c.push_stream(0x5000)
+        c.push_stream(0x6000)
+        c.close()
+    """)
+
+
 def test_serving_calls_beside_a_host_buffer_call(recording):
     """Two threads of one process, one context: the host-buffer call, which runs without
     the interpreter lock, keeps its kernels on the context's stream, and the serving
