@@ -500,3 +500,61 @@ def test_attention_zeros_outweigh_small_values(store, tiny):
     room = 2.0 ** -8 * np.abs(want) + (2.0 ** -11 + 2.0 ** -16) * most
     assert np.all(np.abs(out.double().cpu().numpy() - want) <= room)
     assert np.all(np.abs(lse.double().cpu().numpy() - want_lse) <= 2.0 ** -16)
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-6])
+def test_attention_scales_of_any_sign(store, scale):
+    s = Setup(store, [300, 17, 90], [1, 3, 2], block=32, share=3, dim=64)
+    s.append()
+    for window in (0, 20):
+        out, lse = s.attend(window, scale=scale)
+        want, want_lse = oracle.kv_attention(
+            [oracle.stored_values(b, store) for b in s.bytes()],
+            [t.double().cpu().numpy() for t in (s.cache.k_scale, s.cache.v_scale)],
+            s.q.double().cpu().numpy(), s.table.tolist(), s.spans(), 3, scale, window)
+        top = np.abs(want).max() * 4
+        # |scale| up to the default's, so the default's bound on the scores' error (2^-9 at these
+        # magnitudes, as in check_attention) holds.
+        assert np.all(np.abs(out.double().cpu().numpy() - want) <=
+                      2.0 ** -8 * np.abs(want) + 2.0 ** -9 * top)
+        assert np.all(np.abs(lse.double().cpu().numpy() - want_lse) <= 2.0 ** -9)
+
+
+def test_threads_with_a_stream_each():
+    """A step in each of three threads at once: streams and workspaces are each one's own."""
+    import threading
+
+    setups = [Setup(store, lengths, fresh, share=share, dim=64, seed=i)
+              for i, (store, lengths, fresh, share) in enumerate((
+                  ("int8", [2000, 40], [1, 1], 2), ("e4m3", [700], [60], 4),
+                  ("int8", [300, 9, 64], [5, 9, 1], 3)))]
+    w = torch.randint(0, 256, (128, 32), dtype=torch.uint8, device="cuda")
+    scale, gain = torch.rand(128, 2, device="cuda"), torch.rand(64, device="cuda").bfloat16()
+
+    def step(s):
+        out, lse = s.attend()
+        h, a_scale, _ = serving.add_rms_norm(out.view(-1, 64), gain, out_dtype=torch.int8)
+        return out, lse, serving.gemm_w4(h, w, scale, group=32, a_scale=a_scale)
+
+    for s in setups:
+        s.append()
+    want = [step(s) for s in setups]
+    torch.cuda.synchronize()
+    got = [[] for _ in setups]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = [step(setups[i]) for _ in range(50)]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(3):
+        assert len(got[i]) == 50
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))

@@ -205,3 +205,13 @@ def test_rows_nan_values_where_rows_end_inside_a_warp(dim, fresh, share):
 @pytest.mark.parametrize("tiny", [-16, -30, -60])
 def test_rows_zeros_outweigh_small_values(store, tiny):
     few.test_attention_zeros_outweigh_small_values(store, tiny)
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-6])
+def test_rows_scales_of_any_sign(store, scale):
+    few.test_attention_scales_of_any_sign(store, scale)
+
+
+def test_rows_threads_with_a_stream_each():
+    few.test_threads_with_a_stream_each()
