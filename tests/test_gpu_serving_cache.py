@@ -558,3 +558,35 @@ def test_threads_with_a_stream_each():
         assert len(got[i]) == 50
         for outs in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
+@pytest.mark.parametrize("store", STORES)
+def test_caches_beyond_four_gigabytes(store):
+    """The same step in a small cache and in one whose pages lie beyond 2^32 bytes (and at
+    both ends of it): the same bytes and outputs."""
+    pages, heads, block, dim = 70000, 8, 64, 128
+    small = serving.KvCache.empty(40, heads, block, dim, TORCH[store])
+    large = serving.KvCache.empty(pages, heads, block, dim, TORCH[store])
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rows = lambda *shape: torch.randn(*shape, device="cuda", generator=gen).bfloat16()  # noqa: E731
+    lengths = torch.tensor([600, 900, 130], dtype=torch.int32, device="cuda")
+    table = torch.full((3, 15), -1, dtype=torch.int32, device="cuda")
+    order = torch.randperm(40, device="cuda", generator=gen).int()
+    table[0, :10], table[1], table[2, :3] = order[:10], order[10:25], order[25:28]
+    far = torch.where(table < 0, table, torch.where(table % 2 == 0, table, pages - 1 - table))
+    starts = torch.tensor([0, 600, 1500, 1630], dtype=torch.int32, device="cuda")
+    k, v, q = rows(1630, heads, dim), rows(1630, heads, dim), rows(1630, 2 * heads, dim)
+    for cache, at in ((small, table), (large, far)):
+        serving.kv_append(cache, k, v, at, lengths, starts, max_new=900)
+    for a, b, sa, sb in ((small.k, large.k, small.k_scale, large.k_scale),
+                         (small.v, large.v, small.v_scale, large.v_scale)):
+        used, there = table[table >= 0].long(), far[table >= 0].long()
+        assert torch.equal(a.view(torch.uint8)[used], b.view(torch.uint8)[there])
+        assert torch.equal(sa[used], sb[there])
+    few = torch.tensor([0, 1, 3, 8], dtype=torch.int32, device="cuda")
+    for new, at in ((starts, 900), (few, 5)):
+        tokens = int(new[-1])
+        outs = [serving.kv_attention(c, q[:tokens], t, lengths, new, max_new=at, return_lse=True)
+                for c, t in ((small, table), (large, far))]
+        assert torch.isfinite(outs[0][1]).all()
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
